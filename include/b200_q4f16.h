@@ -456,6 +456,74 @@ B200_API int b200_silu_mul(const void* gu, void* out, int64_t B, int64_t I, void
 /* The same in its early-release form (see b200_rmsnorm_early_release). */
 B200_API int b200_silu_mul_early_release(const void* gu, void* out, int64_t B, int64_t I, void* cuda_stream);
 
+/* ---- sequences of different lengths over a paged key-value cache --------------------------------
+ * The reference has no attention op and no cache (its op list ends at softmax, python/tvm/relax/transform/legalize_ops.py:378-381,
+ * 506-514); the values are the composition of its elementwise ops, statistics in fp32, one rounding at each output.
+ *
+ * Keys and values live in pages: [pages, kv_heads, page_size, head_dim], the last three contiguous, so that one head's share of a
+ * page is one piece of memory.  Row b of the page table names the pages of sequence b in order; entries that no token of the
+ * sequence has reached are never used, whatever they hold, and neither is what the slots behind its last token hold.
+ *   lengths[b]  tokens of sequence b in the cache, those of this call among them
+ *   starts      [batch + 1], starts[0] = 0, starts[batch] = tokens: rows starts[b] .. starts[b + 1] - 1 are the newest tokens of sequence
+ *               b, at positions lengths[b] - (their number) .. lengths[b] - 1.  NULL: one row for each sequence (tokens = batch)
+ *   max_query   no sequence has more rows in this call (chooses kernel and grid; a larger number costs time only)
+ * Lengths and page numbers are held inside the table and the pool as they are read; a row whose position is negative has no place:
+ * nothing is appended for it and its results are zeros.
+ * All sizes are in elements.  page_size 16, 32, 64 or 128; head_dim 64 or 128; 16-byte aligned pages, page strides multiples of 8. */
+#define B200_F16 0
+#define B200_BF16 1
+#define B200_F32 2 /* logits only */
+typedef struct {
+  int32_t dtype; /* of the pages and of the rows: B200_F16 or B200_BF16 */
+  int32_t kv_heads, head_dim, page_size;
+  int64_t pages, k_page_stride, v_page_stride;
+  void* k_pages; void* v_pages;
+  int32_t batch, table_width, max_query;
+  int64_t table_stride, tokens;
+  const void* page_table; /* int32 [batch, table_width] */
+  const void* lengths;    /* int32 [batch] */
+  const void* starts;     /* int32 [batch + 1] or NULL */
+} B200PagedCache;
+
+/* Rotary positions for q and k, then k and v go to the pages.  qkv [tokens, (heads + 2 kv_heads) * head_dim] = q | k | v, rows qkv_stride
+ * apart; q_out [tokens, heads, head_dim].  The first `rotary` values of a head are turned (a multiple of 16, at most head_dim), the others
+ * kept: pairs (i, i + rotary / 2), with `interleaved` (2 i, 2 i + 1), by tables cos and sin, fp32 [table_rows, rotary / 2], at the
+ * token's position, or at positions[row] (int32) where that is given: (a cos - b sin, b cos + a sin) in fp32, rounded once.  Table rows
+ * are held inside the table as they are read.  qkv, q_out and the tables 16-byte aligned, qkv_stride a multiple of 8. */
+B200_API int b200_paged_rope_append(const B200PagedCache* cache, const void* qkv, int64_t qkv_stride, int32_t heads, const void* cos_t,
+                                    const void* sin_t, int64_t table_rows, int32_t rotary, int32_t interleaved, const void* positions,
+                                    void* q_out, void* cuda_stream);
+
+/* out[row, h] = sum_j softmax_j(s_j) v_j over the visible keys j of the row's sequence, of key head h / (heads / kv_heads):
+ *   s = scale * q . k;  cap > 0: s = cap * tanh(s / cap);  slopes: s -= slopes[h] * |position - j|
+ *   visible: j < lengths[b], and (causal = 0; or j < prefix[b]; or j <= position and (window = 0 or position - j < window))
+ * A row without a visible key gets zeros.  A key that no row of a sequence sees may hold anything; every value that some row sees has to be finite.
+ * The weights of the sum are rounded to the cache's type, as the operands of the tensor cores are.
+ * scratch: b200_paged_attention_scratch_bytes() bytes of device memory, zeroed once by the caller and left zeroed where it matters by
+ * every call; calls that share it must be ordered (one stream).  Allocates nothing.  heads <= 128 * kv_heads. */
+typedef struct {
+  const void* q;       /* [tokens, heads, head_dim], rows q_stride apart, 16-byte aligned, q_stride a multiple of 8 */
+  int64_t q_stride;
+  void* out;           /* [tokens, heads, head_dim], 16-byte aligned */
+  int32_t heads, causal, window;
+  float scale, cap;
+  const void* slopes;  /* fp32 [heads] or NULL */
+  const void* prefix;  /* int32 [batch] or NULL */
+} B200PagedAttention;
+B200_API int64_t b200_paged_attention_scratch_bytes(void);
+B200_API int b200_paged_attention(const B200PagedCache* cache, const B200PagedAttention* args, void* scratch, int64_t scratch_bytes,
+                                  void* cuda_stream);
+
+/* ---- what the logits of a row say ----------------------------------------------------------------
+ * p = softmax(logits[row, 0..V)), statistics in fp32:
+ *   logprob[row] = log p[tokens[row]], fp32 (a token outside 0..V-1: -inf);  entropy[row] = -sum p log p, fp32 (0 log 0 = 0)
+ *   top_token[row, i], top_logprob[row, i], i < top: the likeliest entries, equal ones by index; int32, fp32 (top = 0: both may be NULL)
+ * A logit of -inf is an excluded entry: probability 0.  A row of nothing else has logprob -inf and entropy 0; one with a NaN or +inf
+ * has NaN everywhere and tokens 0 .. top - 1.  dtype B200_F16, B200_BF16 or B200_F32; rows `stride` elements apart (any alignment of the type's
+ * size; 16 bytes are faster); logprob and entropy may be NULL (tokens too, without logprob).  0 <= top <= 32, top <= V < 2^31.  One launch, no scratch. */
+B200_API int b200_token_logprobs(const void* logits, int32_t dtype, int64_t stride, const void* tokens, void* logprob, void* entropy,
+                                 void* top_logprob, void* top_token, int64_t rows, int64_t V, int32_t top, void* cuda_stream);
+
 /* ---- introspection used by tests and the benchmark --------------------------------------- */
 
 /* Number of kernels this library has launched on the calling thread since the last reset. */

@@ -83,6 +83,32 @@ class DecodeLayer(ctypes.Structure):
     ]
 
 
+F16, BF16, F32 = 0, 1, 2   # B200_F16, B200_BF16, B200_F32
+
+
+class PagedCache(ctypes.Structure):
+    """B200PagedCache of include/b200_q4f16.h."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("page_size", ctypes.c_int32),
+        ("pages", ctypes.c_int64), ("k_page_stride", ctypes.c_int64), ("v_page_stride", ctypes.c_int64),
+        ("k_pages", ctypes.c_void_p), ("v_pages", ctypes.c_void_p),
+        ("batch", ctypes.c_int32), ("table_width", ctypes.c_int32), ("max_query", ctypes.c_int32),
+        ("table_stride", ctypes.c_int64), ("tokens", ctypes.c_int64),
+        ("page_table", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("starts", ctypes.c_void_p),
+    ]
+
+
+class PagedAttention(ctypes.Structure):
+    """B200PagedAttention of include/b200_q4f16.h."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("out", ctypes.c_void_p),
+        ("heads", ctypes.c_int32), ("causal", ctypes.c_int32), ("window", ctypes.c_int32),
+        ("scale", ctypes.c_float), ("cap", ctypes.c_float), ("slopes", ctypes.c_void_p), ("prefix", ctypes.c_void_p),
+    ]
+
+
 # name -> (restype, argtypes); one entry per prototype in include/b200_q4f16.h
 _vp, _i64, _ci = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
 _dlp = ctypes.POINTER(DLTensor)
@@ -144,6 +170,11 @@ PROTOTYPES = {
     "b200_embed_rows_stats": (_ci, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "b200_embed_rows": (_ci, [_vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "b200_advance_pos": (_ci, [_vp, _i64, _vp]),
+    "b200_paged_rope_append": (_ci, [ctypes.POINTER(PagedCache), _vp, _i64, ctypes.c_int32, _vp, _vp, _i64, ctypes.c_int32, ctypes.c_int32, _vp,
+                                     _vp, _vp]),
+    "b200_paged_attention_scratch_bytes": (_i64, []),
+    "b200_paged_attention": (_ci, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedAttention), _vp, _i64, _vp]),
+    "b200_token_logprobs": (_ci, [_vp, ctypes.c_int32, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, ctypes.c_int32, _vp]),
     "b200_launch_count": (_i64, []),
     "b200_reset_launch_count": (None, []),
     "b200_device_error_flags": (_ci, []),

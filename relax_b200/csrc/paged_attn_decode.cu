@@ -1,0 +1,524 @@
+// Attention of a few rows (query heads of one key head x new tokens) over a paged key-value cache, split over the length and joined.
+//
+// Work: the rows of a sequence that share a key head are cut into tiles of R = 8 or 16.  The keys that a tile can see (a prefix and
+// a range behind it) are units of 16 tokens; a tile with more than c units is cut into chunks of about c, one CTA each, c chosen on the
+// device from all lengths so that the chunks fill the GPU once.  So sequences of any mixture of lengths are balanced, and what the
+// host knows is a bound only.  A tile that was cut leaves partial sums in scratch memory, and the CTA that arrives last adds them up in
+// the order of the chunks (the same bits whoever comes last).
+//
+// A warp takes one unit (head_dim 64: two) at a time, straight from global memory into the registers of mma.sync operands, with no
+// shared memory between: scores^T [16 tokens x 8 rows] = K q^T, out^T [head_dim x 8 rows] += V^T p.  The dims of a k-step and the rows of
+// an output tile are in an order of our own, the one in which a lane's 16-byte load holds what it needs:
+//   K    lane (g, t): tokens g and g + 8, dims 32 j + 8 t .. + 7 (two k-steps of 16)
+//   V    lane (g, t): tokens 2 t, 2 t + 1, 8 + 2 t, 9 + 2 t, dims 8 g .. + 7 and 64 + 8 g .. + 7: byte permutes pair two tokens of a dim
+//   p    from the scores' accumulator by two 8x8 transposes a unit
+// The next unit's keys and values are requested as soon as this one's are used.  The running maximum is raised only where a score
+// is above it by more than 8 (in the exponent of 2), so the usual unit needs a vote instead of a reduction over lanes; weights
+// stay below 2^8, fp32 sums take that.  Weights are rounded to the cache's type for the product with V.
+#include "paged_common.cuh"
+
+namespace b200 {
+
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kUnit = 16;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kSlack = 8.f;                  // how far above the running maximum a score may lie, log2
+
+struct DecodeParams {
+  PagedParams c;
+  const void* q;
+  void* out;
+  int64_t q_stride;
+  int heads, group, causal, window;
+  float scale, cap;
+  const float* slopes;
+  const int* prefix;
+  float* partial;              // [chunk of a cut tile][R][D], then the maxima and sums of all of them
+  float* partial_ml;           // [chunk of a cut tile][2][R]
+  int* arrived;                // [cut tile]
+  int slots;                   // CTAs that run at once
+};
+
+__device__ __forceinline__ void mma(__half, float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma(__nv_bfloat16, float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint4 load16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Units of 16 tokens that some row of a tile sees: those below `pre`, then those of [low, high).
+struct Range {
+  int pre, low, high;          // tokens; low >= 0
+  int pre_units, second, units;
+  __device__ __forceinline__ void set(const DecodeParams& p, const Sequence& s, int b, int first_token, int last_token) {
+    const int base = s.length - s.rows;
+    pre = p.causal ? (p.prefix ? min(max(p.prefix[b], 0), s.length) : 0) : s.length;
+    high = max(min(s.length, base + last_token + 1), 0);
+    low = p.window ? max(base + first_token - p.window + 1, 0) : 0;
+    if (high == 0) pre = 0;                     // (no row has a position)
+    pre_units = (pre + kUnit - 1) / kUnit;
+    second = max(pre_units, low / kUnit);
+    units = pre_units + max((high + kUnit - 1) / kUnit - second, 0);
+  }
+  __device__ __forceinline__ int unit(int u) const { return u < pre_units ? u : u - pre_units + second; }
+};
+
+__device__ __forceinline__ int64_t warp_sum64(int64_t v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ int warp_scan(int v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += t;
+  }
+  return v;
+}
+
+template <typename T, int D, int NT, bool kExtra>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
+paged_decode_kernel(const DecodeParams p) {
+  constexpr int R = 8 * NT;                     // rows of a tile
+  constexpr int SUB = 128 / D;                  // units a warp takes at a time
+  constexpr int KC = D / 32, VC = D / 64, MT = D / 16;
+  __shared__ __align__(16) float sm_o[kWarps][R][D + 4];
+  __shared__ float sm_m[kWarps][R], sm_l[kWarps][R];
+  __shared__ int sm_last;
+  ptx::pdl_wait();
+  ptx::pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int h = blockIdx.x % p.c.kv_heads, item = blockIdx.x / p.c.kv_heads;
+
+  // ---- which tile and chunk: every warp adds up all sequences' units, then looks for its item --------------------------
+  int b, tile, chunk, chunks, cut_tile, cut_chunk;
+  Sequence s;
+  {
+    auto units_of = [&](int i, int& tiles) {    // of one tile (a bound where several tiles differ), and the tiles
+      const Sequence x = sequence_of(p.c, i);
+      tiles = (x.rows * p.group + R - 1) / R;
+      Range r;
+      r.set(p, x, i, 0, x.rows - 1);
+      return tiles > 0 ? r.units : 0;
+    };
+    int64_t total = 0;
+    for (int i = lane; i < p.c.batch; i += 32) {
+      int tiles;
+      const int u = units_of(i, tiles);
+      total += (int64_t)u * tiles;
+    }
+    total = warp_sum64(total) * p.c.kv_heads;
+    constexpr int kStep = kWarps * SUB;         // units of one trip of the CTA's warps
+    const int64_t even = (total + p.slots - 1) / p.slots;
+    const int c = (int)((max(even, (int64_t)1) + kStep - 1) / kStep) * kStep;
+    int before = 0, cut_tiles = 0, cut_chunks = 0;
+    b = -1;
+    for (int base = 0; base < p.c.batch; base += 32) {
+      int tiles = 0, n = 1;
+      if (base + lane < p.c.batch) {
+        const int u = units_of(base + lane, tiles);
+        n = max((u + c - 1) / c, 1);
+      }
+      const int mine = tiles * n, cut = n > 1 ? tiles : 0, cutc = n > 1 ? mine : 0;
+      const int upto = warp_scan(mine, lane), cut_upto = warp_scan(cut, lane), cutc_upto = warp_scan(cutc, lane);
+      const unsigned hit = __ballot_sync(0xffffffffu, before + upto > item);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        const int in = item - before - __shfl_sync(0xffffffffu, upto - mine, l);
+        chunks = __shfl_sync(0xffffffffu, n, l);
+        b = base + l;
+        tile = in / chunks;
+        chunk = in - tile * chunks;
+        cut_tile = cut_tiles + __shfl_sync(0xffffffffu, cut_upto - cut, l) + tile;
+        cut_chunk = cut_chunks + __shfl_sync(0xffffffffu, cutc_upto - cutc, l) + in;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+      cut_tiles += __shfl_sync(0xffffffffu, cut_upto, 31);
+      cut_chunks += __shfl_sync(0xffffffffu, cutc_upto, 31);
+    }
+    if (b < 0) return;                          // (the grid is a bound)
+    s = sequence_of(p.c, b);
+  }
+  const int rows = s.rows * p.group, row0 = tile * R, nrows = min(rows - row0, R);
+  const int token0 = row0 / p.group, token1 = (row0 + nrows - 1) / p.group;
+  const int base = s.length - s.rows;
+  Range range;
+  range.set(p, s, b, token0, token1);
+  const int u_begin = (int)((int64_t)range.units * chunk / chunks), u_end = (int)((int64_t)range.units * (chunk + 1) / chunks);
+
+  // ---- queries: the B operand's row g of a tile of eight -----------------------------------------------------------------
+  uint4 qf[NT][KC];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int r = row0 + 8 * n + g;
+    const T* src = static_cast<const T*>(p.q) + (int64_t)(s.first + r / p.group) * p.q_stride + (int64_t)(h * p.group + r % p.group) * D;
+#pragma unroll
+    for (int j = 0; j < KC; ++j) qf[n][j] = 8 * n + g < nrows ? load16(src + 32 * j + 8 * t) : make_uint4(0, 0, 0, 0);
+  }
+  // this lane's rows in the accumulators: 8 n + 2 t + e
+  int position[NT][2];
+  float slope[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = row0 + 8 * n + 2 * t + e;
+      position[n][e] = r < rows ? base + r / p.group : -1;
+      slope[n][e] = kExtra && p.slopes && r < rows ? p.slopes[h * p.group + r % p.group] * kLog2e : 0.f;
+    }
+  const int position0 = base + token0, position1 = base + token1;
+  const int window = p.window ? p.window : 0x7fffffff;
+  const float to_log2 = p.scale * kLog2e;
+  const float cap_in = kExtra && p.cap > 0.f ? 2.f * p.scale / p.cap * kLog2e : 0.f, cap_log2 = p.cap * kLog2e;
+
+  const int page = 1 << p.c.page_log2;
+  const T* kbase = static_cast<const T*>(p.c.k) + (int64_t)h * page * D + 8 * t;
+  const T* vbase = static_cast<const T*>(p.c.v) + (int64_t)h * page * D + 8 * g;
+  // units of step i of this warp; past the end the last one stands in and is masked
+  auto unit_at = [&](int i, int sub) { return range.unit(min(u_begin + i * SUB + sub, u_end - 1)); };
+  auto page_at = [&](int i, int sub) { return page_of(p.c, b, unit_at(i, sub) >> (p.c.page_log2 - 4)); };
+  uint4 kr[SUB][2][KC], vr[SUB][4][VC];
+  auto load_k = [&](int i, const int (&id)[SUB]) {
+#pragma unroll
+    for (int x = 0; x < SUB; ++x) {
+      const T* src = kbase + id[x] * p.c.k_stride + (int64_t)((unit_at(i, x) * kUnit) & (page - 1)) * D;
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int j = 0; j < KC; ++j) kr[x][r][j] = load16(src + (g + 8 * r) * D + 32 * j);
+    }
+  };
+  auto load_v = [&](int i, const int (&id)[SUB]) {
+#pragma unroll
+    for (int x = 0; x < SUB; ++x) {
+      const T* src = vbase + id[x] * p.c.v_stride + (int64_t)((unit_at(i, x) * kUnit) & (page - 1)) * D;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < VC; ++j) vr[x][r][j] = load16(src + (2 * t + (r & 1) + 8 * (r >> 1)) * D + 64 * j);
+    }
+  };
+
+  float m[NT][2], l[NT][2], acc[NT][MT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) { m[n][e] = -INFINITY; l[n][e] = 0.f; }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[n][i][j] = 0.f;
+  }
+
+  const int steps = (u_end - u_begin + SUB - 1) / SUB;
+  int id[SUB], id_next[SUB];
+  if (warp < steps) {
+#pragma unroll
+    for (int x = 0; x < SUB; ++x) id[x] = page_at(warp, x);
+    load_k(warp, id);
+    load_v(warp, id);
+#pragma unroll
+    for (int x = 0; x < SUB; ++x) id[x] = warp + kWarps < steps ? page_at(warp + kWarps, x) : 0;
+  }
+  for (int i = warp; i < steps; i += kWarps) {
+    const bool more = i + kWarps < steps;
+#pragma unroll
+    for (int x = 0; x < SUB; ++x) id_next[x] = i + 2 * kWarps < steps ? page_at(i + 2 * kWarps, x) : 0;
+    // scores of tokens g (0, 1) and g + 8 (2, 3), rows 2 t (0, 2) and 2 t + 1 (1, 3)
+    float sc[SUB][NT][4];
+#pragma unroll
+    for (int x = 0; x < SUB; ++x)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sc[x][n][j] = 0.f;
+#pragma unroll
+        for (int j = 0; j < KC; ++j) {
+          mma(T(), sc[x][n], kr[x][0][j].x, kr[x][1][j].x, kr[x][0][j].y, kr[x][1][j].y, qf[n][j].x, qf[n][j].y);
+          mma(T(), sc[x][n], kr[x][0][j].z, kr[x][1][j].z, kr[x][0][j].w, kr[x][1][j].w, qf[n][j].z, qf[n][j].w);
+        }
+      }
+    if (more) load_k(i + kWarps, id);
+    bool above = false;
+#pragma unroll
+    for (int x = 0; x < SUB; ++x) {
+      const int first = unit_at(i, x) * kUnit;
+      const bool there = u_begin + i * SUB + x < u_end;
+      // every row sees the whole unit (rows past the tile's end come out as something finite that nobody stores)
+      const bool whole = there && position0 >= 0 &&
+                         (first + kUnit <= range.pre || (first + kUnit - 1 <= position0 && position1 - first < window));
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int token = first + g + 8 * (j >> 1), at = position[n][j & 1];
+          float v = sc[x][n][j];
+          if (kExtra && p.cap > 0.f) v = cap_log2 * (1.f - __fdividef(2.f, exp2_approx(v * cap_in) + 1.f));
+          else v *= to_log2;
+          if (kExtra) v -= slope[n][j & 1] * fabsf((float)(at - token));
+          if (!whole) {
+            const bool seen = there && at >= 0 && (token < range.pre || (token <= at && at - token < window));
+            if (!seen) v = -INFINITY;
+          }
+          sc[x][n][j] = v;
+          above |= v > m[n][j & 1] + kSlack;
+        }
+      if (!whole) {                             // what nobody sees may be anything, and 0 * NaN is NaN
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int token = first + 2 * t + (r & 1) + 8 * (r >> 1);
+          if (!(there && (token < range.pre || (token >= range.low && token < range.high))))
+#pragma unroll
+            for (int j = 0; j < VC; ++j) vr[x][r][j] = make_uint4(0, 0, 0, 0);
+        }
+      }
+    }
+    if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float v = m[n][e];
+#pragma unroll
+          for (int x = 0; x < SUB; ++x) v = fmaxf(v, fmaxf(sc[x][n][e], sc[x][n][e + 2]));
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+          const float f = v == -INFINITY ? 1.f : exp2_approx(m[n][e] - v);
+          m[n][e] = v;
+          l[n][e] *= f;
+#pragma unroll
+          for (int k = 0; k < MT; ++k) { acc[n][k][e] *= f; acc[n][k][e + 2] *= f; }
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < SUB; ++x) {
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          w[j] = sc[x][n][j] == -INFINITY ? 0.f : exp2_approx(sc[x][n][j] - m[n][j & 1]);
+          l[n][j & 1] += w[j];
+        }
+        pb[n][0] = transpose8x8(pack2(T(), w[0], w[1]));
+        pb[n][1] = transpose8x8(pack2(T(), w[2], w[3]));
+      }
+#pragma unroll
+      for (int k = 0; k < MT; ++k) {
+        // row g of the tile: dim 8 g + k, row g + 8: dim 64 + 8 g + k (head_dim 64: 8 g + 4 + k)
+        const int k1 = D == 128 ? k : k + 4, j1 = VC - 1;
+        const unsigned s0 = k & 1 ? 0x7632 : 0x5410, s1 = k1 & 1 ? 0x7632 : 0x5410;
+        const uint32_t a0 = __byte_perm(word(vr[x][0][0], k / 2), word(vr[x][1][0], k / 2), s0);
+        const uint32_t a1 = __byte_perm(word(vr[x][0][j1], k1 / 2), word(vr[x][1][j1], k1 / 2), s1);
+        const uint32_t a2 = __byte_perm(word(vr[x][2][0], k / 2), word(vr[x][3][0], k / 2), s0);
+        const uint32_t a3 = __byte_perm(word(vr[x][2][j1], k1 / 2), word(vr[x][3][j1], k1 / 2), s1);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma(T(), acc[n][k], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+      }
+    }
+    if (more) load_v(i + kWarps, id);
+#pragma unroll
+    for (int x = 0; x < SUB; ++x) id[x] = id_next[x];
+  }
+
+  // ---- the CTA's warps ----------------------------------------------------------------------------------------------------
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o);
+      const int r = 8 * n + 2 * t + e;
+      if (g == 0) { sm_m[warp][r] = m[n][e]; sm_l[warp][r] = l[n][e]; }
+#pragma unroll
+      for (int k = 0; k < MT; k += 4) {
+        *reinterpret_cast<float4*>(&sm_o[warp][r][8 * g + k]) =
+            make_float4(acc[n][k][e], acc[n][k + 1][e], acc[n][k + 2][e], acc[n][k + 3][e]);
+        const int d1 = D == 128 ? 64 + 8 * g + k : 8 * g + 4 + k;
+        *reinterpret_cast<float4*>(&sm_o[warp][r][d1]) =
+            make_float4(acc[n][k][e + 2], acc[n][k + 1][e + 2], acc[n][k + 2][e + 2], acc[n][k + 3][e + 2]);
+      }
+    }
+  __syncthreads();
+  constexpr int kQuads = R * D / 4;
+  auto row_out = [&](int r) {
+    const int x = row0 + r;
+    return static_cast<T*>(p.out) + ((int64_t)(s.first + x / p.group) * p.heads + h * p.group + x % p.group) * D;
+  };
+  auto store = [&](int r, int d, const float (&v)[4], float sum) {
+    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;       // (NaN stays)
+    if (r < nrows) *reinterpret_cast<uint2*>(row_out(r) + d) = make_uint2(pack2(T(), v[0] * inv, v[1] * inv), pack2(T(), v[2] * inv, v[3] * inv));
+  };
+  const int64_t part = (int64_t)cut_chunk * p.c.kv_heads + h, first_part = part - (int64_t)chunk * p.c.kv_heads;
+#pragma unroll
+  for (int q0 = 0; q0 < kQuads; q0 += kWarps * 32) {
+    const int q = q0 + threadIdx.x, r = q / (D / 4), d = (q % (D / 4)) * 4;
+    float M = -INFINITY, L = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm_m[w][r]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = sm_m[w][r] == -INFINITY ? 0.f : exp2_approx(sm_m[w][r] - M);
+      const float4 a = *reinterpret_cast<const float4*>(&sm_o[w][r][d]);
+      if (f == 0.f && sm_l[w][r] == 0.f) continue;
+      L += sm_l[w][r] * f;
+      v[0] += a.x * f; v[1] += a.y * f; v[2] += a.z * f; v[3] += a.w * f;
+    }
+    if (chunks == 1) {
+      store(r, d, v, L);
+    } else {
+      *reinterpret_cast<float4*>(p.partial + part * (R * D) + r * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+      if (d == 0) { p.partial_ml[part * 2 * R + r] = M; p.partial_ml[part * 2 * R + R + r] = L; }
+    }
+  }
+  if (chunks == 1) return;
+
+  // ---- the chunks of a cut tile: the last CTA adds them up -------------------------------------------------------------------
+  __threadfence();
+  __syncthreads();
+  int* counter = p.arrived + (int64_t)cut_tile * p.c.kv_heads + h;
+  if (threadIdx.x == 0) {
+    const int n = atomicAdd(counter, 1);
+    sm_last = n == chunks - 1;
+    if (sm_last) *counter = 0;                  // (as the next launch expects it)
+  }
+  __syncthreads();
+  if (!sm_last) return;
+  __threadfence();
+#pragma unroll
+  for (int q0 = 0; q0 < kQuads; q0 += kWarps * 32) {
+    const int q = q0 + threadIdx.x, r = q / (D / 4), d = (q % (D / 4)) * 4;
+    float M = -INFINITY, L = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < chunks; ++k) M = fmaxf(M, __ldcg(p.partial_ml + (first_part + (int64_t)k * p.c.kv_heads) * 2 * R + r));
+    for (int k = 0; k < chunks; ++k) {
+      const int64_t x = first_part + (int64_t)k * p.c.kv_heads;
+      const float mk = __ldcg(p.partial_ml + x * 2 * R + r), lk = __ldcg(p.partial_ml + x * 2 * R + R + r);
+      const float f = mk == -INFINITY ? 0.f : exp2_approx(mk - M);
+      const float4 a = __ldcg(reinterpret_cast<const float4*>(p.partial + x * (R * D) + r * D + d));
+      if (f == 0.f && lk == 0.f) continue;
+      L += lk * f;
+      v[0] += a.x * f; v[1] += a.y * f; v[2] += a.z * f; v[3] += a.w * f;
+    }
+    store(r, d, v, L);
+  }
+}
+
+constexpr int kCtasPerSm1 = 3, kCtasPerSm2 = 2;
+constexpr int kMaxSms = 256;
+constexpr int64_t kCounters = kMaxSms * kCtasPerSm1;              // cut tiles: each has more than a slot's share of the units
+constexpr int64_t kParts8 = 2 * kMaxSms * kCtasPerSm1, kParts16 = 2 * kMaxSms * kCtasPerSm2;   // their chunks, twice as many at most
+constexpr int64_t kCounterBytes = kCounters * 4;
+constexpr int64_t kMlBytes = (kParts8 * 16 > kParts16 * 32 ? kParts8 * 16 : kParts16 * 32) * 4;
+constexpr int64_t kPartBytes = (kParts8 * 8 > kParts16 * 16 ? kParts8 * 8 : kParts16 * 16) * 128 * 4;
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+int launch_decode(const char* who, const B200PagedCache* c, DecodeParams p, cudaStream_t stream) {
+  const int64_t most = (int64_t)c->max_query * p.group;          // rows of a sequence that share a key head
+  const bool narrow = most <= 8;
+  const int R = narrow ? 8 : 16;
+  if (sm_count() > kMaxSms) return fail(B200_ENODEVICE, "%s: more than %d SMs", who, kMaxSms);
+  p.slots = sm_count() * (narrow ? kCtasPerSm1 : kCtasPerSm2);
+  // tiles of all sequences, at most; each may have one chunk more than its share of the slots
+  const int64_t tiles = (c->tokens * p.group + R - 1) / R + c->batch;
+  const int64_t grid = (tiles + p.slots / p.c.kv_heads + 1) * p.c.kv_heads;
+  if (grid > 0x7fffffffLL) return fail(B200_EINVAL, "%s: too many rows", who);
+  auto launch = [&](auto kern) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = options().gemv_pdl ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+    if (e != cudaSuccess) return fail(B200_ELAUNCH, "%s launch: %s", who, cudaGetErrorString(e));
+    count_launch();
+    return B200_OK;
+  };
+  const bool extra = p.cap > 0.f || p.slopes;
+  auto by_form = [&](auto type, auto dim) {
+    using T = decltype(type);
+    constexpr int D = decltype(dim)::value;
+    if (narrow) return extra ? launch(paged_decode_kernel<T, D, 1, true>) : launch(paged_decode_kernel<T, D, 1, false>);
+    return extra ? launch(paged_decode_kernel<T, D, 2, true>) : launch(paged_decode_kernel<T, D, 2, false>);
+  };
+  auto by_dim = [&](auto type) {
+    return c->head_dim == 128 ? by_form(type, std::integral_constant<int, 128>()) : by_form(type, std::integral_constant<int, 64>());
+  };
+  return c->dtype == B200_F16 ? by_dim(__half()) : by_dim(__nv_bfloat16());
+}
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" {
+
+int64_t b200_paged_attention_scratch_bytes(void) { return kCounterBytes + kMlBytes + kPartBytes; }
+
+int b200_paged_attention(const B200PagedCache* cache, const B200PagedAttention* a, void* scratch, int64_t scratch_bytes, void* stream) {
+  const char* who = "paged_attention";
+  DecodeParams p = {};
+  int rc = paged_params(who, cache, &p.c);
+  if (rc) return rc;
+  if (!a) return fail(B200_EINVAL, "%s: null argument descriptor", who);
+  if (a->heads <= 0 || a->heads % cache->kv_heads || a->heads / cache->kv_heads > 128)
+    return fail(B200_EINVAL, "%s: heads is a multiple of kv_heads, up to 128 times as many; got %d and %d", who, a->heads, cache->kv_heads);
+  if (a->window < 0 || (a->window && !a->causal)) return fail(B200_EINVAL, "%s: a window is positive and needs causal", who);
+  if (!(a->scale == a->scale) || !(a->cap >= 0.f)) return fail(B200_EINVAL, "%s: scale is a number, cap a number >= 0", who);
+  if (cache->tokens == 0) return B200_OK;
+  if (cache->batch == 0 || cache->max_query == 0) return fail(B200_EINVAL, "%s: rows without sequences", who);
+  if (a->q_stride < (int64_t)a->heads * cache->head_dim || a->q_stride % 8)
+    return fail(B200_EINVAL, "%s: q_stride is a multiple of 8 and at least a row", who);
+  if (!a->q || !a->out || !aligned16(a->q) || !aligned16(a->out)) return fail(B200_EINVAL, "%s: q and out must be non-null and 16-byte aligned", who);
+  if (!scratch || !aligned16(scratch) || scratch_bytes < b200_paged_attention_scratch_bytes())
+    return fail(B200_EINVAL, "%s: scratch is 16-byte aligned memory of %lld bytes", who, (long long)b200_paged_attention_scratch_bytes());
+  if ((rc = ensure_device())) return rc;
+  p.q = a->q;
+  p.out = a->out;
+  p.q_stride = a->q_stride;
+  p.heads = a->heads;
+  p.group = a->heads / cache->kv_heads;
+  p.causal = a->causal != 0;
+  p.window = a->window;
+  p.scale = a->scale;
+  p.cap = a->cap;
+  p.slopes = static_cast<const float*>(a->slopes);
+  p.prefix = static_cast<const int*>(a->prefix);
+  char* at = static_cast<char*>(scratch);
+  p.arrived = reinterpret_cast<int*>(at);
+  p.partial_ml = reinterpret_cast<float*>(at + kCounterBytes);
+  p.partial = reinterpret_cast<float*>(at + kCounterBytes + kMlBytes);
+  return launch_decode(who, cache, p, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

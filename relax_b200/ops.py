@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import importlib.util
+import typing
 
 import torch
 
@@ -155,7 +156,8 @@ def _torch_call():
         else:
             L = _lib.lib()
             module.bind(*(ctypes.cast(fn, ctypes.c_void_p).value
-                          for fn in (L.b200_set_stream, L.b200_q4f16_matmul, L.b200_q4f16_matmul_layout, L.b200_q4f16_dequantize)))
+                          for fn in (L.b200_set_stream, L.b200_q4f16_matmul, L.b200_q4f16_matmul_layout, L.b200_q4f16_dequantize,
+                                     L.b200_paged_rope_append, L.b200_paged_attention, L.b200_token_logprobs)))
             _native = module
     return _native
 
@@ -246,6 +248,185 @@ def q4f16_dequantize(wq: torch.Tensor, scales: torch.Tensor, out: torch.Tensor |
         vw, vs, vo = (_DLView(t) for t in (wq, scales, out))
         _lib.check(L.b200_q4f16_dequantize_dl(vw.ptr(), vs.ptr(), vo.ptr()))
     return out
+
+
+# ---------------------------------------------------------------------------------------------- paged key-value cache
+_CACHE_TYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_LOGIT_TYPES = {**_CACHE_TYPES, torch.float32: _lib.F32}
+
+
+def _same_device(device, **tensors):
+    if device.type != "cuda":
+        raise ValueError("the tensors must be on a CUDA device: there is no host implementation")
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, other arguments on {device}")
+
+
+def _index(name, t, shape):
+    if t is None:
+        return None
+    if t.dtype is not torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _paged_cache(rows, k_pages, v_pages, page_table, lengths, starts, max_query) -> _lib.PagedCache:
+    """The descriptor of a call over `rows` (whose first dimension is the tokens of the call), its tensors checked."""
+    if k_pages.dtype not in _CACHE_TYPES or v_pages.dtype is not k_pages.dtype:
+        raise ValueError(f"pages are fp16 or bf16, both alike: got {k_pages.dtype} and {v_pages.dtype}")
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+        raise ValueError(f"pages are [pages, kv_heads, page_size, head_dim], both alike: got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+    pages, kv_heads, page_size, head_dim = k_pages.shape
+    inner = (page_size * head_dim, head_dim, 1)
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        if t.stride()[1:] != inner:
+            raise ValueError(f"the heads of a page of {name} must be contiguous: strides {t.stride()}")
+    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError("page_table is an int32 tensor [batch, pages of the longest sequence] with contiguous rows")
+    batch, width = page_table.shape
+    tokens = rows.shape[0]
+    if starts is None:
+        max_query = 1
+        if tokens != batch:
+            raise ValueError(f"{tokens} rows of {batch} sequences: without starts every sequence has one row")
+    elif max_query is None:
+        max_query = tokens
+    stride = page_table.stride(0) if batch > 1 else width
+    return _lib.PagedCache(_CACHE_TYPES[k_pages.dtype], kv_heads, head_dim, page_size, pages, k_pages.stride(0), v_pages.stride(0),
+                           k_pages.data_ptr(), v_pages.data_ptr(), batch, width, int(max_query), stride, tokens, page_table.data_ptr(),
+                           _index("lengths", lengths, (batch,)), _index("starts", starts, (batch + 1,)))
+
+
+def paged_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                      page_table: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor | None = None, interleaved: bool = False,
+                      positions: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Turns q and k of qkv [tokens, (heads + 2 kv_heads) * head_dim] by their positions, stores k and v in the pages and returns
+    q [tokens, heads, head_dim].
+
+    ``lengths`` [batch] counts the tokens of every sequence with the new ones; rows ``starts[b] .. starts[b + 1] - 1`` are the newest of
+    sequence b (None: one row each).  cos and sin, fp32 [positions, r / 2], turn the first r values of a head: pairs (i, i + r / 2), or
+    (2 i, 2 i + 1) with ``interleaved``; ``positions`` (int32 [tokens]) names other rows of the tables than the tokens' places."""
+    native = _native or _torch_call()
+    if native:
+        q = native.paged_rope_append(qkv, cos, sin, k_pages, v_pages, page_table, lengths, starts, interleaved, positions, out)
+        if q is not None:
+            return q
+    cache = _paged_cache(qkv, k_pages, v_pages, page_table, lengths, starts, 1)
+    kv, dim = cache.kv_heads, cache.head_dim
+    if qkv.dtype is not k_pages.dtype or qkv.dim() != 2 or (qkv.shape[1] > 1 and qkv.stride(1) != 1) or qkv.shape[1] % dim:
+        raise ValueError(f"qkv is [tokens, (heads + 2 kv_heads) * {dim}] of the pages' type with contiguous rows")
+    heads = qkv.shape[1] // dim - 2 * kv
+    if heads <= 0:
+        raise ValueError(f"qkv of {qkv.shape[1]} columns has no query heads beside {kv} key and value heads of {dim}")
+    for name, t in (("cos", cos), ("sin", sin)):
+        if t.dtype is not torch.float32 or t.dim() != 2 or not t.is_contiguous() or t.shape != cos.shape:
+            raise ValueError(f"{name} is a contiguous fp32 table [positions, rotary / 2], both alike")
+    if out is None:
+        out = torch.empty((qkv.shape[0], heads, dim), dtype=qkv.dtype, device=qkv.device)
+    elif out.dtype is not qkv.dtype or out.shape != (qkv.shape[0], heads, dim) or not out.is_contiguous():
+        raise ValueError(f"out is a contiguous [tokens, {heads}, {dim}] of qkv's type")
+    _same_device(qkv.device, k_pages=k_pages, v_pages=v_pages, page_table=page_table, lengths=lengths, starts=starts, cos=cos, sin=sin,
+                 positions=positions, out=out)
+    stride = qkv.stride(0) if qkv.shape[0] > 1 else qkv.shape[1]
+    with _on(qkv.device):
+        _lib.check(_lib.lib().b200_paged_rope_append(
+            ctypes.byref(cache), qkv.data_ptr(), stride, heads, cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1],
+            int(interleaved), _index("positions", positions, (qkv.shape[0],)), out.data_ptr(), _stream_ptr(qkv.device)))
+    return out
+
+
+_scratch: dict = {}     # (device, stream) -> memory of paged_attention calls on that stream
+
+
+def paged_attention_scratch(device) -> torch.Tensor:
+    """Memory that paged_attention calls of one stream may share (``scratch=``): where several streams or captured graphs make such
+    calls at the same time, each needs its own."""
+    return torch.zeros((int(_lib.lib().b200_paged_attention_scratch_bytes()),), dtype=torch.uint8, device=device)
+
+
+def _stream_scratch(device) -> torch.Tensor:
+    if torch._C._cuda_isCurrentStreamCapturing():       # a graph may be replayed beside anything: it has memory of its own
+        return paged_attention_scratch(device)
+    key = (device.index, torch._C._cuda_getCurrentRawStream(device.index))
+    found = _scratch.get(key)
+    if found is None:
+        found = _scratch[key] = paged_attention_scratch(device)
+    return found
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                    starts: torch.Tensor | None = None, max_query: int | None = None, scale: float | None = None, causal: bool = True,
+                    window: int = 0, cap: float = 0.0, slopes: torch.Tensor | None = None, prefix: torch.Tensor | None = None,
+                    out: torch.Tensor | None = None, scratch: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the rows q [tokens, heads, head_dim] over the keys and values of their sequences in the pages.
+
+    ``lengths``, ``starts`` and the rows of a sequence as in :func:`paged_rope_append`, which has stored their keys before;
+    ``max_query``: no sequence has more rows (None: the number of tokens).  A row at position t sees key j where j < prefix[b], or j <= t and
+    (``window`` = 0 or t - j < window); ``causal`` = False: every key of its sequence.  Scores are scale * q.k (scale: 1 / sqrt(head_dim)),
+    with ``cap`` > 0 cap * tanh(score / cap), with ``slopes`` (fp32 [heads]) less slopes[h] * |t - j|.  A row that sees nothing gets zeros.
+    ``scratch``: see :func:`paged_attention_scratch`; None takes memory that belongs to the current stream."""
+    native = _native or _torch_call()
+    if native and q.is_cuda and torch._C._cuda_getDevice() == q.device.index:
+        if scratch is None:
+            scratch = _stream_scratch(q.device)
+        result = native.paged_attention(q, k_pages, v_pages, page_table, lengths, starts, max_query, scale, causal, window, cap, slopes,
+                                        prefix, out, scratch)
+        if result is not None:
+            return result
+    cache = _paged_cache(q, k_pages, v_pages, page_table, lengths, starts, max_query)
+    kv, dim = cache.kv_heads, cache.head_dim
+    if q.dtype is not k_pages.dtype or q.dim() != 3 or q.shape[2] != dim or (q.shape[0] and q.stride()[1:] != (dim, 1)):
+        raise ValueError(f"q is [tokens, heads, {dim}] of the pages' type, a token's heads contiguous")
+    heads = q.shape[1]
+    if slopes is not None and (slopes.dtype is not torch.float32 or slopes.shape != (heads,) or not slopes.is_contiguous()):
+        raise ValueError(f"slopes are a contiguous fp32 tensor of {heads} values")
+    if out is None:
+        out = torch.empty((q.shape[0], heads, dim), dtype=q.dtype, device=q.device)
+    elif out.dtype is not q.dtype or out.shape != q.shape or not out.is_contiguous():
+        raise ValueError("out is a contiguous tensor of q's shape and type")
+    _same_device(q.device, k_pages=k_pages, v_pages=v_pages, page_table=page_table, lengths=lengths, starts=starts, slopes=slopes,
+                 prefix=prefix, out=out, scratch=scratch)
+    with _on(q.device):
+        if scratch is None:
+            scratch = _stream_scratch(q.device)
+        args = _lib.PagedAttention(q.data_ptr(), q.stride(0) if q.shape[0] > 1 else heads * dim, out.data_ptr(), heads, int(causal), int(window),
+                                   dim ** -0.5 if scale is None else scale, cap, None if slopes is None else slopes.data_ptr(),
+                                   _index("prefix", prefix, (cache.batch,)))
+        _lib.check(_lib.lib().b200_paged_attention(ctypes.byref(cache), ctypes.byref(args), scratch.data_ptr(),
+                                                   scratch.numel() * scratch.element_size(), _stream_ptr(q.device)))
+    return out
+
+
+class TokenLogprobs(typing.NamedTuple):
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    top_logprob: torch.Tensor | None
+    top_token: torch.Tensor | None
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
+    """Of every row of logits [rows, V] (fp16, bf16 or fp32): the log probability of tokens[row] (int32), the entropy of the
+    distribution and its ``top`` likeliest entries (at most 32; equal ones by index), all in fp32.  A logit of -inf is an excluded entry."""
+    native = _native or _torch_call()
+    if native:
+        found = native.token_logprobs(logits, tokens, top)
+        if found is not None:
+            return TokenLogprobs(*found)
+    if logits.dtype not in _LOGIT_TYPES or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits are an fp16, bf16 or fp32 tensor [rows, V] with contiguous rows")
+    rows, V = logits.shape
+    at = _index("tokens", tokens, (rows,))
+    _same_device(logits.device, tokens=tokens)
+    fp32 = dict(dtype=torch.float32, device=logits.device)
+    logprob, entropy = torch.empty(rows, **fp32), torch.empty(rows, **fp32)
+    best = torch.empty((rows, top), **fp32) if top else None
+    best_token = torch.empty((rows, top), dtype=torch.int32, device=logits.device) if top else None
+    with _on(logits.device):
+        _lib.check(_lib.lib().b200_token_logprobs(
+            logits.data_ptr(), _LOGIT_TYPES[logits.dtype], logits.stride(0) if rows > 1 else V, at, logprob.data_ptr(), entropy.data_ptr(),
+            best.data_ptr() if top else None, best_token.data_ptr() if top else None, rows, V, top, _stream_ptr(logits.device)))
+    return TokenLogprobs(logprob, entropy, best, best_token)
 
 
 def launch_count() -> int:
