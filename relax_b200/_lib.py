@@ -84,6 +84,7 @@ class DecodeLayer(ctypes.Structure):
 
 
 F16, BF16, F32 = 0, 1, 2   # B200_F16, B200_BF16, B200_F32
+PAGED_ZEROED_BYTES = 16384   # B200_PAGED_ZEROED_BYTES
 
 
 class PagedCache(ctypes.Structure):

@@ -95,13 +95,15 @@ int launch_lm_head(const __half* x, const float* stats, const __half* norm_w, fl
 int64_t lm_head_scratch_bytes();
 int launch_argmax_rows(const __half* logits, int* tokens, int64_t B, int64_t V, cudaStream_t stream);
 
-// Reads and clears the per-kernel device error words (bit 0-7: skinny pipeline, 8-15: tensor-core GEMM, 16-23: weight-stationary GEMM,
+// Reads and clears the per-kernel device error words (bit 0-7: skinny pipeline, 8-15: tensor-core GEMM and (bit 14) attention of many
+// rows, 16-23: weight-stationary GEMM,
 // 24-30: decoder-layer kernel).
 int device_error_flags_read_and_clear();
 int gemv_pipe_error_read_and_clear();
 int gemm_error_read_and_clear();
 int gemm_ws_error_read_and_clear();
 int layer_error_read_and_clear();
+int paged_prompt_error_read_and_clear();
 
 // Lets `kern` be launched with `bytes` of dynamic shared memory on the current device (`limit`: that kernel's own).
 int raise_smem_limit(SmemLimit& limit, const void* kern, size_t bytes, const char* who);

@@ -23,24 +23,6 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kUnit = 16;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kSlack = 8.f;                  // how far above the running maximum a score may lie, log2
-
-struct DecodeParams {
-  PagedParams c;
-  const void* q;
-  void* out;
-  int64_t q_stride;
-  int heads, group, causal, window;
-  float scale, cap;
-  const float* slopes;
-  const int* prefix;
-  float* partial;              // [chunk of a cut tile][R][D], then the maxima and sums of all of them
-  float* partial_ml;           // [chunk of a cut tile][2][R]
-  int* arrived;                // [cut tile]
-  int slots;                   // CTAs that run at once
-};
-
 __device__ __forceinline__ void mma(__half, float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -62,46 +44,9 @@ __device__ __forceinline__ uint4 load16(const void* p) {
   return v;
 }
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Units of 16 tokens that some row of a tile sees: those below `pre`, then those of [low, high).
-struct Range {
-  int pre, low, high;          // tokens; low >= 0
-  int pre_units, second, units;
-  __device__ __forceinline__ void set(const DecodeParams& p, const Sequence& s, int b, int first_token, int last_token) {
-    const int base = s.length - s.rows;
-    pre = p.causal ? (p.prefix ? min(max(p.prefix[b], 0), s.length) : 0) : s.length;
-    high = max(min(s.length, base + last_token + 1), 0);
-    low = p.window ? max(base + first_token - p.window + 1, 0) : 0;
-    if (high == 0) pre = 0;                     // (no row has a position)
-    pre_units = (pre + kUnit - 1) / kUnit;
-    second = max(pre_units, low / kUnit);
-    units = pre_units + max((high + kUnit - 1) / kUnit - second, 0);
-  }
-  __device__ __forceinline__ int unit(int u) const { return u < pre_units ? u : u - pre_units + second; }
-};
-
-__device__ __forceinline__ int64_t warp_sum64(int64_t v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-__device__ __forceinline__ int warp_scan(int v, int lane) {
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int t = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += t;
-  }
-  return v;
-}
-
 template <typename T, int D, int NT, bool kExtra>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
-paged_decode_kernel(const DecodeParams p) {
+paged_decode_kernel(const PagedAttnParams p) {
   constexpr int R = 8 * NT;                     // rows of a tile
   constexpr int SUB = 128 / D;                  // units a warp takes at a time
   constexpr int KC = D / 32, VC = D / 64, MT = D / 16;
@@ -111,62 +56,23 @@ paged_decode_kernel(const DecodeParams p) {
   ptx::pdl_wait();
   ptx::pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int h = blockIdx.x % p.c.kv_heads, item = blockIdx.x / p.c.kv_heads;
+  const int h = blockIdx.x % p.c.kv_heads, index = blockIdx.x / p.c.kv_heads;
 
-  // ---- which tile and chunk: every warp adds up all sequences' units, then looks for its item --------------------------
-  int b, tile, chunk, chunks, cut_tile, cut_chunk;
-  Sequence s;
+  // ---- which tile and chunk: c units a chunk fill the slots once, in whole trips of the CTA's warps -----------------------
+  Item item;
   {
-    auto units_of = [&](int i, int& tiles) {    // of one tile (a bound where several tiles differ), and the tiles
-      const Sequence x = sequence_of(p.c, i);
-      tiles = (x.rows * p.group + R - 1) / R;
-      Range r;
-      r.set(p, x, i, 0, x.rows - 1);
-      return tiles > 0 ? r.units : 0;
-    };
-    int64_t total = 0;
-    for (int i = lane; i < p.c.batch; i += 32) {
-      int tiles;
-      const int u = units_of(i, tiles);
-      total += (int64_t)u * tiles;
-    }
-    total = warp_sum64(total) * p.c.kv_heads;
-    constexpr int kStep = kWarps * SUB;         // units of one trip of the CTA's warps
-    const int64_t even = (total + p.slots - 1) / p.slots;
+    auto tiles_of = [&](const Sequence& x) { return (x.rows * p.group + R - 1) / R; };
+    constexpr int kStep = kWarps * SUB;
+    const int64_t even = (total_units<kUnit>(p, lane, tiles_of) + p.slots - 1) / p.slots;
     const int c = (int)((max(even, (int64_t)1) + kStep - 1) / kStep) * kStep;
-    int before = 0, cut_tiles = 0, cut_chunks = 0;
-    b = -1;
-    for (int base = 0; base < p.c.batch; base += 32) {
-      int tiles = 0, n = 1;
-      if (base + lane < p.c.batch) {
-        const int u = units_of(base + lane, tiles);
-        n = max((u + c - 1) / c, 1);
-      }
-      const int mine = tiles * n, cut = n > 1 ? tiles : 0, cutc = n > 1 ? mine : 0;
-      const int upto = warp_scan(mine, lane), cut_upto = warp_scan(cut, lane), cutc_upto = warp_scan(cutc, lane);
-      const unsigned hit = __ballot_sync(0xffffffffu, before + upto > item);
-      if (hit) {
-        const int l = __ffs(hit) - 1;
-        const int in = item - before - __shfl_sync(0xffffffffu, upto - mine, l);
-        chunks = __shfl_sync(0xffffffffu, n, l);
-        b = base + l;
-        tile = in / chunks;
-        chunk = in - tile * chunks;
-        cut_tile = cut_tiles + __shfl_sync(0xffffffffu, cut_upto - cut, l) + tile;
-        cut_chunk = cut_chunks + __shfl_sync(0xffffffffu, cutc_upto - cutc, l) + in;
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, upto, 31);
-      cut_tiles += __shfl_sync(0xffffffffu, cut_upto, 31);
-      cut_chunks += __shfl_sync(0xffffffffu, cutc_upto, 31);
-    }
-    if (b < 0) return;                          // (the grid is a bound)
-    s = sequence_of(p.c, b);
+    if (!find_item<kUnit>(p, index, c, lane, tiles_of, item)) return;       // (the grid is a bound)
   }
-  const int rows = s.rows * p.group, row0 = tile * R, nrows = min(rows - row0, R);
+  const int b = item.b, chunk = item.chunk, chunks = item.chunks;
+  const Sequence s = sequence_of(p.c, b);
+  const int rows = s.rows * p.group, row0 = item.tile * R, nrows = min(rows - row0, R);
   const int token0 = row0 / p.group, token1 = (row0 + nrows - 1) / p.group;
   const int base = s.length - s.rows;
-  Range range;
+  Range<kUnit> range;
   range.set(p, s, b, token0, token1);
   const int u_begin = (int)((int64_t)range.units * chunk / chunks), u_end = (int)((int64_t)range.units * (chunk + 1) / chunks);
 
@@ -374,7 +280,7 @@ paged_decode_kernel(const DecodeParams p) {
     const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;       // (NaN stays)
     if (r < nrows) *reinterpret_cast<uint2*>(row_out(r) + d) = make_uint2(pack2(T(), v[0] * inv, v[1] * inv), pack2(T(), v[2] * inv, v[3] * inv));
   };
-  const int64_t part = (int64_t)cut_chunk * p.c.kv_heads + h, first_part = part - (int64_t)chunk * p.c.kv_heads;
+  const int64_t part = (int64_t)item.cut_chunk * p.c.kv_heads + h, first_part = part - (int64_t)chunk * p.c.kv_heads;
 #pragma unroll
   for (int q0 = 0; q0 < kQuads; q0 += kWarps * 32) {
     const int q = q0 + threadIdx.x, r = q / (D / 4), d = (q % (D / 4)) * 4;
@@ -401,7 +307,7 @@ paged_decode_kernel(const DecodeParams p) {
   // ---- the chunks of a cut tile: the last CTA adds them up -------------------------------------------------------------------
   __threadfence();
   __syncthreads();
-  int* counter = p.arrived + (int64_t)cut_tile * p.c.kv_heads + h;
+  int* counter = p.arrived + (int64_t)item.cut_tile * p.c.kv_heads + h;
   if (threadIdx.x == 0) {
     const int n = atomicAdd(counter, 1);
     sm_last = n == chunks - 1;
@@ -429,20 +335,12 @@ paged_decode_kernel(const DecodeParams p) {
 }
 
 constexpr int kCtasPerSm1 = 3, kCtasPerSm2 = 2;
-constexpr int kMaxSms = 256;
-constexpr int64_t kCounters = kMaxSms * kCtasPerSm1;              // cut tiles: each has more than a slot's share of the units
-constexpr int64_t kParts8 = 2 * kMaxSms * kCtasPerSm1, kParts16 = 2 * kMaxSms * kCtasPerSm2;   // their chunks, twice as many at most
-constexpr int64_t kCounterBytes = kCounters * 4;
-constexpr int64_t kMlBytes = (kParts8 * 16 > kParts16 * 32 ? kParts8 * 16 : kParts16 * 32) * 4;
-constexpr int64_t kPartBytes = (kParts8 * 8 > kParts16 * 16 ? kParts8 * 8 : kParts16 * 16) * 128 * 4;
-
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-int launch_decode(const char* who, const B200PagedCache* c, DecodeParams p, cudaStream_t stream) {
+int launch_decode(const char* who, const B200PagedCache* c, PagedAttnParams p, cudaStream_t stream) {
   const int64_t most = (int64_t)c->max_query * p.group;          // rows of a sequence that share a key head
   const bool narrow = most <= 8;
   const int R = narrow ? 8 : 16;
-  if (sm_count() > kMaxSms) return fail(B200_ENODEVICE, "%s: more than %d SMs", who, kMaxSms);
   p.slots = sm_count() * (narrow ? kCtasPerSm1 : kCtasPerSm2);
   // tiles of all sequences, at most; each may have one chunk more than its share of the slots
   const int64_t tiles = (c->tokens * p.group + R - 1) / R + c->batch;
@@ -483,11 +381,18 @@ using namespace b200;
 
 extern "C" {
 
-int64_t b200_paged_attention_scratch_bytes(void) { return kCounterBytes + kMlBytes + kPartBytes; }
+// The counters; then, of twice as many chunks as there are slots (a cut tile has more than a slot's share of the units, its chunks at least half
+// of that), the maxima and sums and the partial results: 256 rows of the many-rows kernel are the most.
+static int64_t scratch_rows() { return (int64_t)2 * sm_count() * 256; }
+
+int64_t b200_paged_attention_scratch_bytes(void) {
+  if (ensure_device()) return -1;
+  return B200_PAGED_ZEROED_BYTES + scratch_rows() * (2 + 128) * (int64_t)sizeof(float);
+}
 
 int b200_paged_attention(const B200PagedCache* cache, const B200PagedAttention* a, void* scratch, int64_t scratch_bytes, void* stream) {
   const char* who = "paged_attention";
-  DecodeParams p = {};
+  PagedAttnParams p = {};
   int rc = paged_params(who, cache, &p.c);
   if (rc) return rc;
   if (!a) return fail(B200_EINVAL, "%s: null argument descriptor", who);
@@ -500,9 +405,10 @@ int b200_paged_attention(const B200PagedCache* cache, const B200PagedAttention* 
   if (a->q_stride < (int64_t)a->heads * cache->head_dim || a->q_stride % 8)
     return fail(B200_EINVAL, "%s: q_stride is a multiple of 8 and at least a row", who);
   if (!a->q || !a->out || !aligned16(a->q) || !aligned16(a->out)) return fail(B200_EINVAL, "%s: q and out must be non-null and 16-byte aligned", who);
-  if (!scratch || !aligned16(scratch) || scratch_bytes < b200_paged_attention_scratch_bytes())
-    return fail(B200_EINVAL, "%s: scratch is 16-byte aligned memory of %lld bytes", who, (long long)b200_paged_attention_scratch_bytes());
+  if (!scratch || !aligned16(scratch)) return fail(B200_EINVAL, "%s: scratch must be non-null and 16-byte aligned", who);
   if ((rc = ensure_device())) return rc;
+  if (scratch_bytes < b200_paged_attention_scratch_bytes() || sm_count() * kCtasPerSm1 * 4 > B200_PAGED_ZEROED_BYTES)
+    return fail(B200_EINVAL, "%s: scratch of %lld bytes is less than b200_paged_attention_scratch_bytes()", who, (long long)scratch_bytes);
   p.q = a->q;
   p.out = a->out;
   p.q_stride = a->q_stride;
@@ -516,9 +422,12 @@ int b200_paged_attention(const B200PagedCache* cache, const B200PagedAttention* 
   p.prefix = static_cast<const int*>(a->prefix);
   char* at = static_cast<char*>(scratch);
   p.arrived = reinterpret_cast<int*>(at);
-  p.partial_ml = reinterpret_cast<float*>(at + kCounterBytes);
-  p.partial = reinterpret_cast<float*>(at + kCounterBytes + kMlBytes);
-  return launch_decode(who, cache, p, static_cast<cudaStream_t>(stream));
+  p.partial_ml = reinterpret_cast<float*>(at + B200_PAGED_ZEROED_BYTES);
+  p.partial = p.partial_ml + 2 * scratch_rows();
+  // Rows of a sequence that share a key head: up to 16 are two operand tiles of the few-rows kernel; more are cut into tiles that
+  // each read the keys again, where the kernel for many rows reads them once for 256.
+  if ((int64_t)cache->max_query * p.group <= 16) return launch_decode(who, cache, p, static_cast<cudaStream_t>(stream));
+  return launch_paged_prompt(who, cache, p, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

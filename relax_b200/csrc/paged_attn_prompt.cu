@@ -1,0 +1,647 @@
+// Attention of many rows (prompts, chunks of them, several new tokens of many heads) over a paged key-value cache, on the tensor cores.
+//
+// A tile is up to 128 rows: all query heads of a key head for as many tokens as fit, so every key and value that is fetched serves the
+// whole group.  One CTA per SM works on a pair of neighbouring tiles with the same ring of key and value blocks (128 tokens each): while the
+// tensor cores multiply for one tile, the other's scores go through the softmax.
+//     S = Q K^T   tcgen05.mma, both operands in shared memory, 128 x 128 fp32 in tensor memory
+//     P           a thread has a row: maximum, 2^(s - m), sum, rounded to the cache's type, stored over S as the next operand
+//     O += P V    tcgen05.mma, P in tensor memory, V [token][dim] in shared memory (rows along N)
+// O stays in tensor memory; it is multiplied only when a row's maximum has grown by more than 2^8 since it was last set, by the softmax
+// warps themselves: S of a block complete means that O of the block before is, since the MMAs of a CTA complete in order.
+//
+// Warps: 0 TMA (the pages of a block: one load per page and 64 dims; a page behind the last token lies outside the tensor map, which
+// gives zeros), 1 MMA, 2 zeroes the values of a block that nobody sees, 3 hands out the work, 4..7 and 8..11 the rows of the two tiles.
+#include <atomic>
+#include <type_traits>
+
+#include "paged_common.cuh"
+#include "tmap.h"
+
+namespace b200 {
+
+namespace {
+
+using namespace ptx;
+
+constexpr int kRows = 128;                     // of a tile
+constexpr int kBlock = 128;                    // tokens of a block of keys
+constexpr int kThreads = 384;
+constexpr int kHalfBytes = kBlock * 128;       // 64 dims of a block
+constexpr int kReady = 4;                      // value blocks between the zeroing warp and the MMA warp
+constexpr int kWorks = 2;                      // work descriptors in flight
+constexpr uint64_t kWaitNs = 4000000000ull;
+constexpr int kAuxRegs = 72, kRowRegs = 216, kLaunchRegs = 168;       // 128 x 72 + 256 x 216 = 384 x 168
+__device__ int g_prompt_error = 0;
+
+struct PromptParams {
+  CUtensorMap tm_q;                            // {D, heads, tokens}, box {64, group, tokens of a tile}, SWIZZLE_128B
+  CUtensorMap tm_k, tm_v;                      // {D, page, kv_heads, pages}, box {64, page, 1, 1}, SWIZZLE_128B
+  PagedAttnParams a;
+  int tile_tokens;
+};
+
+struct Work {
+  int b, h;                                    // b < 0: no more
+  int first, rows, base, length;               // of the sequence: first row, rows, position of the first, tokens in the cache
+  int token;                                   // the pair's first
+  int u0, u1;                                  // its chunk of blocks
+  Range<kBlock> range;
+  int low[2], high[2], last[2];                // of each tile: the keys it sees beside the prefix, its last block (u) or -1
+  int chunk, chunks, cut_tile, part, part_step;
+};
+// Whether a tile sees anything of block u.
+struct Sight {
+  Range<kBlock> range;
+  int low, high;
+  bool any;
+  __device__ __forceinline__ Sight(const Work& w, int t) : range(w.range), low(w.low[t]), high(w.high[t]), any(w.last[t] >= 0) {}
+  __device__ __forceinline__ bool operator()(int u) const {
+    const int from = range.unit(u) * kBlock;
+    return any && (from < range.pre || (from < high && from + kBlock > low));
+  }
+};
+
+template <int D>
+struct Smem {
+  static constexpr int kStages = D == 128 ? 5 : 8;
+  static constexpr int kBlockBytes = kHalfBytes * (D / 64);
+  unsigned char q[2][kBlockBytes];
+  unsigned char ring[kStages][kBlockBytes];
+  uint64_t q_full, q_empty;
+  uint64_t full[kStages], empty[kStages], ready[kReady];
+  uint64_t s_full[2], p_ready[2], o_full[2], o_empty[2];
+  uint64_t work_full[kWorks], work_empty[kWorks];
+  Work work[kWorks];
+  uint32_t tmem_base;
+  int abort_flag;
+  int last_here[2];
+};
+
+// Bounded wait; false: it ran out, here or in another warp, and the kernel ends.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int code) {
+  if (mbar_try_wait(bar, parity)) return true;
+  if (*abort_flag) return false;
+  if (mbar_wait_ns(bar, parity, kWaitNs)) return true;
+  *abort_flag = 1;
+  atomicExch(&g_prompt_error, code);
+  return false;
+}
+__device__ __forceinline__ bool wait_relaxed(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int code) {
+  if (*abort_flag) return false;
+  if (mbar_wait_ns_relaxed(bar, parity, kWaitNs)) return true;
+  *abort_flag = 1;
+  atomicExch(&g_prompt_error, code);
+  return false;
+}
+
+__device__ __forceinline__ unsigned long long pair64(float a, float b) {
+  return (unsigned long long)__float_as_uint(b) << 32 | __float_as_uint(a);
+}
+__device__ __forceinline__ void fma2(float& x, float& y, float ax, float ay, float bx, float by, float cx, float cy) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(pair64(ax, ay)), "l"(pair64(bx, by)), "l"(pair64(cx, cy)));
+  x = __uint_as_float((uint32_t)d);
+  y = __uint_as_float((uint32_t)(d >> 32));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float ax, float ay) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair64(x, y)), "l"(pair64(ax, ay)));
+  x = __uint_as_float((uint32_t)d);
+  y = __uint_as_float((uint32_t)(d >> 32));
+}
+
+template <typename T, int D, bool kExtra>
+__global__ void __launch_bounds__(kThreads, 1)
+paged_prompt_kernel(const __grid_constant__ PromptParams p) {
+  using Shared = Smem<D>;
+  constexpr int kStages = Shared::kStages, kBlockBytes = Shared::kBlockBytes, kHalves = D / 64;
+  constexpr uint32_t kIdescS = umma_idesc_16bit_f32(kRows, kBlock, std::is_same<T, __nv_bfloat16>::value, false);
+  constexpr uint32_t kIdescO = umma_idesc_16bit_f32(kRows, D, std::is_same<T, __nv_bfloat16>::value, true);
+  extern __shared__ unsigned char smem_unaligned[];
+  Shared& sm = *reinterpret_cast<Shared*>(smem_unaligned + ((1024u - (smem_u32(smem_unaligned) & 1023u)) & 1023u));
+  volatile int* abort_flag = &sm.abort_flag;
+  const PagedAttnParams& a = p.a;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    sm.abort_flag = 0;
+    mbar_init(&sm.q_full, 1);
+    mbar_init(&sm.q_empty, 1);
+    for (int i = 0; i < kStages; ++i) { mbar_init(&sm.full[i], 1); mbar_init(&sm.empty[i], 1); }
+    for (int i = 0; i < kReady; ++i) mbar_init(&sm.ready[i], 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&sm.s_full[t], 1);
+      mbar_init(&sm.p_ready[t], 4);
+      mbar_init(&sm.o_full[t], 1);
+      mbar_init(&sm.o_empty[t], 4);
+    }
+    for (int i = 0; i < kWorks; ++i) { mbar_init(&sm.work_full[i], 1); mbar_init(&sm.work_empty[i], 11); }
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&sm.tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = sm.tmem_base;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // the next work descriptor; null: there is none, or a wait ran out.  It stays until it is handed back.
+  uint32_t works = 0;
+  auto next_work = [&]() -> const Work* {
+    if (!wait(&sm.work_full[works % kWorks], (works / kWorks) & 1, abort_flag, 1)) return nullptr;
+    const Work* w = &sm.work[works % kWorks];
+    return w->b >= 0 ? w : nullptr;
+  };
+  auto work_done = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sm.work_empty[works % kWorks]);
+    ++works;
+  };
+
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kAuxRegs));
+  if (warp == 0) {
+    // ---------------------------------------------------------------------- TMA
+    const int per_page = 7 - a.c.page_log2, pages = 1 << per_page;       // of a block
+    uint32_t pos = 0, items = 0;
+    for (const Work* wp; (wp = next_work()) != nullptr; work_done()) {
+      const Work& w = *wp;
+      if (w.u1 == w.u0) continue;
+      if (items > 0 && !wait_relaxed(&sm.q_empty, (items - 1) & 1, abort_flag, 2)) break;
+      ++items;
+      const int tiles = w.token + p.tile_tokens < w.rows ? 2 : 1;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&sm.q_full, (uint32_t)(tiles * kHalves * p.tile_tokens * a.group * 128));
+        for (int t = 0; t < tiles; ++t)
+          for (int i = 0; i < kHalves; ++i)
+            tma_load_3d(sm.q[t] + i * kHalfBytes, &p.tm_q, i * 64, w.h * a.group, w.first + w.token + t * p.tile_tokens, &sm.q_full);
+      }
+      // lane: page lane % pages of the block, dims 64 * (lane / pages); the page numbers a block ahead
+      const int in_block = lane & (pages - 1), half = lane >> per_page;
+      const int used = (w.length + (1 << a.c.page_log2) - 1) >> a.c.page_log2;
+      const Range<kBlock> range = w.range;
+      const int b = w.b, h = w.h, u1 = w.u1;
+      auto page_at = [&](int u) {
+        const int i = range.unit(u) * pages + in_block;
+        return i < used ? page_of(a.c, b, i) : a.c.pages;                 // (behind the last page: outside the map)
+      };
+      int id = page_at(w.u0);
+      bool ok = true;
+      for (int u = w.u0; ok && u < u1; ++u) {
+        const int id_next = u + 1 < u1 ? page_at(u + 1) : 0;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const uint32_t slot = pos % kStages, round = pos / kStages;
+          if (round > 0 && !wait_relaxed(&sm.empty[slot], (round - 1) & 1, abort_flag, 3)) { ok = false; break; }
+          if (lane == 0) mbar_arrive_expect_tx(&sm.full[slot], kBlockBytes);
+          __syncwarp();
+          if (half < kHalves)
+            tma_load_4d(sm.ring[slot] + half * kHalfBytes + (in_block << (a.c.page_log2 + 7)), kv ? &p.tm_v : &p.tm_k, half * 64, 0, h, id,
+                        &sm.full[slot]);
+          ++pos;
+        }
+        id = id_next;
+      }
+      if (!ok) break;
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------------- MMA
+    const uint64_t dq = umma_desc_k128(smem_u32(sm.q[0]));
+    const uint64_t dk = umma_desc_k128(smem_u32(sm.ring[0]));
+    const uint64_t dv = umma_desc_mn128(smem_u32(sm.ring[0]), kHalfBytes);
+    constexpr uint32_t kStep = kBlockBytes >> 4, kHalfStep = kHalfBytes >> 4;
+    uint32_t pos = 0, vblocks = 0, items = 0, n_p[2] = {0, 0}, n_o[2] = {0, 0};
+    auto scores = [&](int t, uint32_t slot) {
+#pragma unroll
+      for (int i = 0; i < kHalves; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          umma_f16_ss(tmem + t * 128, dq + t * kStep + i * kHalfStep + 2 * k, dk + (uint64_t)(slot * kStep) + i * kHalfStep + 2 * k, kIdescS,
+                      i + k > 0);
+      umma_commit(&sm.s_full[t]);
+    };
+    bool ok = true;
+    for (const Work* wp; ok && (wp = next_work()) != nullptr; work_done()) {
+      const int u0 = wp->u0, u1 = wp->u1, last[2] = {wp->last[0], wp->last[1]};
+      const Sight sees[2] = {Sight(*wp, 0), Sight(*wp, 1)};
+      if (u1 == u0) continue;
+      if (!wait(&sm.q_full, items & 1, abort_flag, 4)) break;
+      ++items;
+      bool begun[2] = {false, false};
+      uint32_t slot = pos % kStages;
+      if (!wait(&sm.full[slot], (pos / kStages) & 1, abort_flag, 5)) break;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (sees[t](u0)) scores(t, slot);
+      umma_commit(&sm.empty[slot]);
+      if (u1 - u0 == 1) umma_commit(&sm.q_empty);
+      ++pos;
+      for (int u = u0; ok && u < u1; ++u) {
+        const uint32_t vslot = pos % kStages;
+        ++pos;
+        const bool more = u + 1 < u1;
+        const uint32_t kslot = pos % kStages, kround = pos / kStages;
+        bool keys = false;
+        ok = wait(&sm.ready[vblocks % kReady], (vblocks / kReady) & 1, abort_flag, 6);
+        ++vblocks;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (ok && sees[t](u)) {
+            if (!begun[t] && n_o[t] > 0) ok = wait(&sm.o_empty[t], (n_o[t] - 1) & 1, abort_flag, 7);
+            ok = ok && wait(&sm.p_ready[t], n_p[t] & 1, abort_flag, 8);
+            if (ok) {
+              ++n_p[t];
+              tc_fence_after_sync();
+#pragma unroll
+              for (int k = 0; k < kBlock / 16; ++k)
+                umma_f16_ts(tmem + 256 + t * D, tmem + t * 128 + 8 * k, dv + (uint64_t)(vslot * kStep) + k * (2048 >> 4), kIdescO, begun[t] || k > 0);
+              begun[t] = true;
+              if (u == last[t]) {
+                umma_commit(&sm.o_full[t]);
+                ++n_o[t];
+              }
+            }
+          }
+          if (ok && more && sees[t](u + 1)) {
+            if (!keys) ok = wait(&sm.full[kslot], kround & 1, abort_flag, 9);
+            keys = true;
+            if (ok) scores(t, kslot);
+          }
+        }
+        if (ok && more && !keys) ok = wait(&sm.full[kslot], kround & 1, abort_flag, 9);
+        if (!ok) break;
+        umma_commit(&sm.empty[vslot]);
+        if (more) {
+          umma_commit(&sm.empty[kslot]);
+          if (u + 2 == u1) umma_commit(&sm.q_empty);
+          ++pos;
+        }
+      }
+    }
+  } else if (warp == 2) {
+    // ---------------------------------------------------------------------- values that nobody sees: 0 * NaN is NaN
+    uint32_t pos = 0, vblocks = 0;
+    bool ok = true;
+    for (const Work* wp; ok && (wp = next_work()) != nullptr; work_done()) {
+      const Range<kBlock> range = wp->range;
+      const int u1 = wp->u1;
+      for (int u = wp->u0; u < u1; ++u, pos += 2) {
+        const uint32_t slot = (pos + 1) % kStages, round = (pos + 1) / kStages;
+        if (!wait_relaxed(&sm.full[slot], round & 1, abort_flag, 10)) { ok = false; break; }
+        const int from = range.unit(u) * kBlock;
+        const bool whole = from + kBlock <= range.pre || (from >= range.low && from + kBlock <= range.high);
+        if (!whole) {
+          for (int i = lane; i < kBlock * 8 * kHalves; i += 32) {
+            const int token = from + ((i >> 3) & (kBlock - 1));
+            if (!(token < range.pre || (token >= range.low && token < range.high)))
+              reinterpret_cast<uint4*>(sm.ring[slot])[i] = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(&sm.ready[vblocks % kReady]);
+        ++vblocks;
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------------- the work, longest tiles of a sequence first
+    const int pair_tokens = 2 * p.tile_tokens;
+    auto tiles_of = [&](const Sequence& s) { return (s.rows + pair_tokens - 1) / pair_tokens; };
+    const int64_t even = (total_units<kBlock>(a, lane, tiles_of) + a.slots - 1) / a.slots;
+    const int c = (int)max(even, (int64_t)8);
+    for (uint32_t i = 0;; ++i) {
+      const uint32_t slot = i % kWorks, round = i / kWorks;
+      if (round > 0 && !wait_relaxed(&sm.work_empty[slot], (round - 1) & 1, abort_flag, 11)) break;
+      const int64_t index = (int64_t)i * gridDim.x + ((i & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+      Item item;
+      Work w;
+      w.b = -1;
+      if (index / a.c.kv_heads < 0x7fffffff && find_item<kBlock>(a, (int)(index / a.c.kv_heads), c, lane, tiles_of, item)) {
+        const Sequence s = sequence_of(a.c, item.b);
+        const int tile = tiles_of(s) - 1 - item.tile;
+        w.b = item.b;
+        w.h = (int)(index % a.c.kv_heads);
+        w.first = s.first;
+        w.rows = s.rows;
+        w.base = s.length - s.rows;
+        w.length = s.length;
+        w.token = tile * pair_tokens;
+        w.range.set(a, s, item.b, w.token, min(w.token + pair_tokens, s.rows) - 1);
+        w.u0 = (int)((int64_t)w.range.units * item.chunk / item.chunks);
+        w.u1 = (int)((int64_t)w.range.units * (item.chunk + 1) / item.chunks);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int from = w.token + t * p.tile_tokens;
+          const bool there = from < s.rows;
+          Range<kBlock> r;
+          r.set(a, s, item.b, from, min(from + p.tile_tokens, s.rows) - 1);
+          w.low[t] = r.low;
+          w.high[t] = r.high;
+          w.last[t] = there && r.high > 0 ? 0 : -1;
+          int last = -1;
+          const Sight sees(w, t);
+          for (int u = w.u0 + lane; u < w.u1; u += 32)
+            if (sees(u)) last = u;
+          w.last[t] = __reduce_max_sync(0xffffffffu, last);
+        }
+        w.chunk = item.chunk;
+        w.chunks = item.chunks;
+        w.cut_tile = (item.cut_tile * a.c.kv_heads + w.h) * 2;
+        w.part = item.cut_chunk * a.c.kv_heads + w.h;
+        w.part_step = a.c.kv_heads;
+      }
+      if (lane == 0) {
+        sm.work[slot] = w;
+        mbar_arrive(&sm.work_full[slot]);
+      }
+      if (w.b < 0) break;
+    }
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegs));
+    // ---------------------------------------------------------------------- the rows
+    const int t = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
+    const uint32_t s_at = tmem + t * 128 + ((uint32_t)((warp & 3) * 32) << 16), o_at = s_at - t * 128 + 256 + t * D;
+    uint32_t n_s = 0, n_o = 0;
+    bool ok = true;
+    auto tile_barrier = [&]() {
+      if (t == 0) bar_sync(1, 128);
+      else bar_sync(2, 128);
+    };
+    const int token_in_tile = r / a.group, head_in_group = r - token_in_tile * a.group;
+    const float scale_log2 = kExtra ? 1.f : a.scale * kLog2e;
+    const float cap_in = kExtra && a.cap > 0.f ? 2.f * a.scale / a.cap * kLog2e : 0.f, cap_log2 = a.cap * kLog2e;
+    for (const Work* wp; ok && (wp = next_work()) != nullptr; work_done()) {
+      const Work& w = *wp;
+      const Sight sees(w, t);
+      const Range<kBlock>& range = sees.range;
+      const int u0 = w.u0, u1 = w.u1;
+      const int token = w.token + t * p.tile_tokens + token_in_tile;
+      const bool mine = token_in_tile < p.tile_tokens && token < w.rows;
+      const int at = mine ? w.base + token : -1;
+      const int head = w.h * a.group + head_in_group;
+      const int tile_first = w.base + w.token + t * p.tile_tokens;
+      const int tile_last = w.base + min(w.token + (t + 1) * p.tile_tokens, w.rows) - 1;
+      const int window = a.window ? a.window : 0x7fffffff;
+      const float slope = kExtra && a.slopes && mine ? a.slopes[head] * kLog2e : 0.f;
+      float m = -INFINITY, l0 = 0.f, l1 = 0.f;
+      bool begun = false;
+      for (int u = u0; u < u1; ++u) {
+        if (!sees(u)) continue;
+        if (!wait(&sm.s_full[t], n_s & 1, abort_flag, 12)) { ok = false; break; }
+        ++n_s;
+        tc_fence_after_sync();
+        uint32_t raw[4][32];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(s_at + 32 * i, raw[i]);
+        tmem_ld_wait();
+        auto s = [&](int i) { return __uint_as_float(raw[i >> 5][i & 31]); };
+        const int from = range.unit(u) * kBlock;
+        if (kExtra) {
+#pragma unroll
+          for (int i = 0; i < kBlock; ++i) {
+            float v = s(i);
+            if (a.cap > 0.f) v = cap_log2 * (1.f - __fdividef(2.f, exp2_approx(v * cap_in) + 1.f));
+            else v *= a.scale * kLog2e;
+            v -= slope * fabsf((float)(at - (from + i)));
+            raw[i >> 5][i & 31] = __float_as_uint(v);
+          }
+        }
+        const bool whole = from + kBlock <= range.pre || (from + kBlock - 1 <= tile_first && tile_last - from < window && tile_first >= 0);
+        if (!whole) {
+          // columns [0, prefix) and [first, end) are seen
+          const int prefix = at >= 0 ? range.pre - from : 0;
+          const int end = at >= 0 ? at - from + 1 : 0, first = at - from >= window ? at - from - window + 1 : 0;
+#pragma unroll
+          for (int i = 0; i < kBlock; ++i)
+            if (!(i < prefix || (i >= first && i < end))) raw[i >> 5][i & 31] = 0xff800000u;
+        }
+        float top = s(0);
+#pragma unroll
+        for (int i = 1; i < kBlock; ++i) top = fmaxf(top, s(i));
+        top *= scale_log2;
+        const bool above = top > m + kSlack;
+        if (__any_sync(0xffffffffu, above)) {
+          const float to = fmaxf(m, top), f = to == -INFINITY ? 1.f : exp2_approx(m - to);
+          m = to;
+          l0 *= f;
+          l1 *= f;
+          if (begun) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(o_at + 16 * i, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              tmem_st_32x32b_x16(o_at + 16 * i, o);
+            }
+          }
+        }
+        begun = true;
+        const float minus = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t packed[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            float x, y;
+            fma2(x, y, s(64 * i + 2 * j), s(64 * i + 2 * j + 1), scale_log2, scale_log2, minus, minus);
+            x = exp2_approx(x);
+            y = exp2_approx(y);
+            add2(l0, l1, x, y);
+            packed[j] = pack2(T(), x, y);
+          }
+          tmem_st_32x32b_x32(s_at + 32 * i, packed);
+        }
+        tmem_st_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_ready[t]);
+      }
+      if (!ok) break;
+      // ---- the tile's result -------------------------------------------------------------------------------------------------
+      const float l = l0 + l1;
+      const bool any = w.last[t] >= 0;
+      if (any) {
+        if (!wait(&sm.o_full[t], n_o & 1, abort_flag, 13)) break;
+        ++n_o;
+        tc_fence_after_sync();
+      }
+      if (w.chunks == 1) {
+        const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+        T* out = static_cast<T*>(a.out) + ((int64_t)(w.first + token) * a.heads + head) * D;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          uint32_t o[32];
+          if (any) {
+            tmem_ld_32x32b_x32(o_at + 32 * i, o);
+            tmem_ld_wait();
+          }
+          if (mine) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint32_t v[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                v[k] = any && l != 0.f ? pack2(T(), __uint_as_float(o[8 * j + 2 * k]) * inv, __uint_as_float(o[8 * j + 2 * k + 1]) * inv) : 0u;
+              reinterpret_cast<uint4*>(out)[4 * i + j] = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+          }
+        }
+      } else {
+        const int64_t row = ((int64_t)w.part * 2 + t) * kRows + r;
+        a.partial_ml[row * 2] = m;
+        a.partial_ml[row * 2 + 1] = l;
+        float* to = a.partial + row * D;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          uint32_t o[32];
+          if (any) {
+            tmem_ld_32x32b_x32(o_at + 32 * i, o);
+            tmem_ld_wait();
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            reinterpret_cast<uint4*>(to)[8 * i + j] =
+                any && l != 0.f ? make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]) : make_uint4(0, 0, 0, 0);
+        }
+      }
+      if (any) {
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.o_empty[t]);
+      }
+      if (w.chunks == 1) continue;
+      // ---- a tile that was cut: the CTA that comes last adds up, in the order of the chunks -------------------------------------
+      __threadfence();
+      tile_barrier();
+      if (r == 0) {
+        int* counter = a.arrived + w.cut_tile + t;
+        const int n = atomicAdd(counter, 1);
+        sm.last_here[t] = n == w.chunks - 1;
+        if (n == w.chunks - 1) *counter = 0;
+      }
+      tile_barrier();
+      const bool last = sm.last_here[t] != 0;
+      tile_barrier();
+      if (!last) continue;
+      __threadfence();
+      const int64_t part0 = (int64_t)w.part - (int64_t)w.chunk * w.part_step;
+      constexpr int kQuads = D / 4;
+      for (int i = r; i < kRows * kQuads; i += 128) {
+        const int row = i / kQuads, d = (i % kQuads) * 4;
+        const int tok_in = row / a.group, tok = w.token + t * p.tile_tokens + tok_in;
+        if (tok_in >= p.tile_tokens || tok >= w.rows) break;
+        float M = -INFINITY, L = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < w.chunks; ++k) M = fmaxf(M, __ldcg(a.partial_ml + (((part0 + (int64_t)k * w.part_step) * 2 + t) * kRows + row) * 2));
+        for (int k = 0; k < w.chunks; ++k) {
+          const int64_t x = ((part0 + (int64_t)k * w.part_step) * 2 + t) * kRows + row;
+          const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.partial_ml + x * 2));
+          const float4 o = __ldcg(reinterpret_cast<const float4*>(a.partial + x * D + d));
+          if (ml.x == -INFINITY && ml.y == 0.f) continue;
+          const float f = exp2_approx(ml.x - M);
+          L += ml.y * f;
+          v[0] += o.x * f; v[1] += o.y * f; v[2] += o.z * f; v[3] += o.w * f;
+        }
+        const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
+        T* out = static_cast<T*>(a.out) + ((int64_t)(w.first + tok) * a.heads + w.h * a.group + row - tok_in * a.group) * D + d;
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack2(T(), v[0] * inv, v[1] * inv), pack2(T(), v[2] * inv, v[3] * inv));
+      }
+    }
+  }
+
+  if (*abort_flag) {
+    // loads and products may still be under way into this CTA's memory: let them land before it is released
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace
+
+int launch_paged_prompt(const char* who, const B200PagedCache* c, PagedAttnParams a, cudaStream_t stream) {
+  PromptParams p;
+  p.tile_tokens = kRows / a.group;
+  const uint32_t page = (uint32_t)c->page_size, group = (uint32_t)a.group;
+  const CUtensorMapDataType type = c->dtype == B200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const uint64_t D = (uint64_t)c->head_dim;
+  int rc;
+  {
+    const uint64_t d[3] = {D, (uint64_t)a.heads, (uint64_t)c->tokens};
+    const uint64_t s[2] = {D * 2, (uint64_t)a.q_stride * 2};
+    const uint32_t b[3] = {64, group, (uint32_t)p.tile_tokens};
+    if ((rc = make_tmap(&p.tm_q, type, 3, a.q, d, s, b, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
+  }
+  for (int v = 0; v < 2; ++v) {
+    const uint64_t d[4] = {D, page, (uint64_t)c->kv_heads, (uint64_t)c->pages};
+    const uint64_t s[3] = {D * 2, (uint64_t)page * D * 2, (uint64_t)(v ? c->v_page_stride : c->k_page_stride) * 2};
+    const uint32_t b[4] = {64, page, 1, 1};
+    if ((rc = make_tmap(v ? &p.tm_v : &p.tm_k, type, 4, v ? c->v_pages : c->k_pages, d, s, b, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
+  }
+  a.slots = sm_count();
+  p.a = a;
+  // pairs of tiles of all sequences, at most, and as many chunks more as there are slots
+  const int64_t pairs = (c->tokens + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens) + c->batch;
+  const int64_t most = pairs * c->kv_heads + a.slots;
+  if (most > 0x3fffffffLL) return fail(B200_EINVAL, "%s: too many rows", who);
+  auto launch = [&](auto kern, size_t bytes, SmemLimit& limit, std::atomic<int>& regs) {
+    const size_t smem = bytes + 1024;
+    int e = raise_smem_limit(limit, reinterpret_cast<const void*>(kern), smem, who);
+    if (e) return e;
+    // the register split asks for what the launch has: a kernel that was built with fewer would wait for ever
+    if (regs.load(std::memory_order_relaxed) == 0) {
+      cudaFuncAttributes attr;
+      if (cudaFuncGetAttributes(&attr, kern) != cudaSuccess) return fail(B200_ELAUNCH, "%s: cudaFuncGetAttributes", who);
+      regs.store(attr.numRegs, std::memory_order_relaxed);
+    }
+    if (regs.load(std::memory_order_relaxed) < kLaunchRegs)
+      return fail(B200_ELAUNCH, "%s: built with %d registers a thread, %d are needed", who, regs.load(), kLaunchRegs);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(most < a.slots ? most : a.slots));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = options().gemv_pdl ? 1 : 0;
+    const cudaError_t r = cudaLaunchKernelEx(&cfg, kern, p);
+    if (r != cudaSuccess) return fail(B200_ELAUNCH, "%s launch: %s", who, cudaGetErrorString(r));
+    count_launch();
+    return B200_OK;
+  };
+  const bool extra = a.cap > 0.f || a.slopes || !(a.scale > 0.f);
+  auto by_form = [&](auto type_, auto dim) {
+    using T = decltype(type_);
+    constexpr int N = decltype(dim)::value;
+    static SmemLimit limit[2];
+    static std::atomic<int> regs[2];
+    return extra ? launch(paged_prompt_kernel<T, N, true>, sizeof(Smem<N>), limit[1], regs[1])
+                 : launch(paged_prompt_kernel<T, N, false>, sizeof(Smem<N>), limit[0], regs[0]);
+  };
+  auto by_dim = [&](auto type_) {
+    return c->head_dim == 128 ? by_form(type_, std::integral_constant<int, 128>()) : by_form(type_, std::integral_constant<int, 64>());
+  };
+  return c->dtype == B200_F16 ? by_dim(__half()) : by_dim(__nv_bfloat16());
+}
+
+int paged_prompt_error_read_and_clear() {
+  int v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_prompt_error, sizeof(int)) != cudaSuccess) return 0xff;
+  if (v) cudaMemcpyToSymbol(g_prompt_error, &zero, sizeof(int));
+  return v;
+}
+
+}  // namespace b200

@@ -51,6 +51,119 @@ __device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// What both attention kernels get.
+struct PagedAttnParams {
+  PagedParams c;
+  const void* q;
+  void* out;
+  int64_t q_stride;
+  int heads, group, causal, window;
+  float scale, cap;
+  const float* slopes;
+  const int* prefix;
+  float* partial;              // [chunk of a cut tile][rows][D], and the maxima and sums of all of them
+  float* partial_ml;           // [chunk of a cut tile][2][rows]
+  int* arrived;                // [cut tile]
+  int slots;                   // CTAs that run at once
+};
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kSlack = 8.f;  // how far above the running maximum a score may lie, log2
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Units of kUnit tokens that some row of a tile sees: those below `pre`, then those of [low, high).
+template <int kUnit>
+struct Range {
+  int pre, low, high;          // tokens; low >= 0
+  int pre_units, second, units;
+  __device__ __forceinline__ void set(const PagedAttnParams& p, const Sequence& s, int b, int first_token, int last_token) {
+    const int base = s.length - s.rows;
+    pre = p.causal ? (p.prefix ? min(max(p.prefix[b], 0), s.length) : 0) : s.length;
+    high = max(min(s.length, base + last_token + 1), 0);
+    low = p.window ? max(base + first_token - p.window + 1, 0) : 0;
+    if (high == 0) pre = 0;                     // (no row has a position)
+    pre_units = (pre + kUnit - 1) / kUnit;
+    second = max(pre_units, low / kUnit);
+    units = pre_units + max((high + kUnit - 1) / kUnit - second, 0);
+  }
+  __device__ __forceinline__ int unit(int u) const { return u < pre_units ? u : u - pre_units + second; }
+};
+
+__device__ __forceinline__ int64_t warp_sum64(int64_t v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ int warp_scan(int v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += t;
+  }
+  return v;
+}
+
+// The split of all sequences into tiles of rows (tiles_of: how many a sequence has) and of a tile's units into chunks, as every warp works
+// it out for itself.  A sequence of more than c units is cut, all its tiles into the same number of chunks.
+struct Item {
+  int b, tile, chunk, chunks;
+  int cut_tile, cut_chunk;     // of those that are cut, for their place in scratch memory
+};
+template <int kUnit, class Tiles>
+__device__ __forceinline__ int units_of(const PagedAttnParams& p, int b, Tiles tiles_of, int& tiles) {
+  const Sequence s = sequence_of(p.c, b);
+  tiles = tiles_of(s);
+  Range<kUnit> r;
+  r.set(p, s, b, 0, s.rows - 1);
+  return tiles > 0 ? r.units : 0;               // (of one tile; a bound where several differ)
+}
+template <int kUnit, class Tiles>
+__device__ __forceinline__ int64_t total_units(const PagedAttnParams& p, int lane, Tiles tiles_of) {
+  int64_t total = 0;
+  for (int i = lane; i < p.c.batch; i += 32) {
+    int tiles;
+    const int u = units_of<kUnit>(p, i, tiles_of, tiles);
+    total += (int64_t)u * tiles;
+  }
+  return warp_sum64(total) * p.c.kv_heads;
+}
+template <int kUnit, class Tiles>
+__device__ __forceinline__ bool find_item(const PagedAttnParams& p, int index, int c, int lane, Tiles tiles_of, Item& item) {
+  int before = 0, cut_tiles = 0, cut_chunks = 0;
+  for (int base = 0; base < p.c.batch; base += 32) {
+    int tiles = 0, n = 1;
+    if (base + lane < p.c.batch) {
+      const int u = units_of<kUnit>(p, base + lane, tiles_of, tiles);
+      n = max((u + c - 1) / c, 1);
+    }
+    const int mine = tiles * n, cut = n > 1 ? tiles : 0, cutc = n > 1 ? mine : 0;
+    const int upto = warp_scan(mine, lane), cut_upto = warp_scan(cut, lane), cutc_upto = warp_scan(cutc, lane);
+    const unsigned hit = __ballot_sync(0xffffffffu, before + upto > index);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      const int in = index - before - __shfl_sync(0xffffffffu, upto - mine, l);
+      item.chunks = __shfl_sync(0xffffffffu, n, l);
+      item.b = base + l;
+      item.tile = in / item.chunks;
+      item.chunk = in - item.tile * item.chunks;
+      item.cut_tile = cut_tiles + __shfl_sync(0xffffffffu, cut_upto - cut, l) + item.tile;
+      item.cut_chunk = cut_chunks + __shfl_sync(0xffffffffu, cutc_upto - cutc, l) + in;
+      return true;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+    cut_tiles += __shfl_sync(0xffffffffu, cut_upto, 31);
+    cut_chunks += __shfl_sync(0xffffffffu, cutc_upto, 31);
+  }
+  return false;
+}
+
+// The kernel for many rows (paged_attn_prompt.cu).
+int launch_paged_prompt(const char* who, const B200PagedCache* c, PagedAttnParams p, cudaStream_t stream);
+
 // Launch parameters of a checked descriptor; `who` names the entry point in messages.
 int paged_params(const char* who, const B200PagedCache* c, PagedParams* out);
 

@@ -163,6 +163,21 @@ __device__ __forceinline__ void tma_load_2d_hint(void* smem_dst, const void* tma
       "l"(tmap), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "l"(policy)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const void* tmap, int32_t c0, int32_t c1, int32_t c2, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(tmap), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(void* smem_dst, const void* tmap, int32_t c0, int32_t c1, int32_t c2, int32_t c3,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(tmap), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
 __device__ __forceinline__ void tma_load_3d_hint(void* smem_dst, const void* tmap, int32_t c0, int32_t c1, int32_t c2,
                                                  uint64_t* bar, uint64_t policy) {
   asm volatile(
@@ -317,6 +332,14 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
       "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
@@ -334,12 +357,22 @@ __device__ __forceinline__ uint64_t umma_desc_k128(uint32_t smem_addr) {
   d |= (uint64_t)2 << 61;
   return d;
 }
+// The same for an operand whose rows of 128 bytes run along M or N (64 16-bit values) and follow each other along K: the leading byte
+// offset is the step to the next 64 values of M or N, the stride byte offset (1024) that to the next 8 rows.
+__device__ __forceinline__ uint64_t umma_desc_mn128(uint32_t smem_addr, uint32_t next64_bytes) {
+  return (umma_desc_k128(smem_addr) & ~((uint64_t)0x3fff << 16)) | (uint64_t)((next64_bytes >> 4) & 0x3fffu) << 16;
+}
 // Instruction descriptor, kind::f16: D fp32, A and B fp16, both K-major, shape M x N.
 //   bits 4-5 D format (1 = f32)   7-9 A format (0 = f16)   10-12 B format (0 = f16)
 //   bit 15 A major (0 = K)   bit 16 B major (0 = K)   17-22 N >> 3   24-28 M >> 4
 __host__ __device__ constexpr uint32_t umma_idesc_f16_f32(int m, int n) {
   return (1u << 4) | (0u << 7) | (0u << 10) | (0u << 15) | (0u << 16) | ((uint32_t)(n >> 3) << 17) |
          ((uint32_t)(m >> 4) << 24);
+}
+
+// The same with A and B in bf16, or with a B whose rows run along N (umma_desc_mn128).
+__host__ __device__ constexpr uint32_t umma_idesc_16bit_f32(int m, int n, bool bf16, bool b_along_n) {
+  return umma_idesc_f16_f32(m, n) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_along_n ? 1u << 16 : 0u);
 }
 
 // The same wait for barriers that other CTAs of the cluster arrive on.

@@ -342,7 +342,13 @@ _scratch: dict = {}     # (device, stream) -> memory of paged_attention calls on
 def paged_attention_scratch(device) -> torch.Tensor:
     """Memory that paged_attention calls of one stream may share (``scratch=``): where several streams or captured graphs make such
     calls at the same time, each needs its own."""
-    return torch.zeros((int(_lib.lib().b200_paged_attention_scratch_bytes()),), dtype=torch.uint8, device=device)
+    with _on(device):
+        size = int(_lib.lib().b200_paged_attention_scratch_bytes())
+        if size < 0:
+            _lib.check(_lib.ENODEVICE)
+        scratch = torch.empty((size,), dtype=torch.uint8, device=device)
+        scratch[:_lib.PAGED_ZEROED_BYTES].zero_()
+    return scratch
 
 
 def _stream_scratch(device) -> torch.Tensor:
