@@ -11,7 +11,6 @@
 //
 // Warps: 0 TMA (the pages of a block: one load per page and 64 dims; a page behind the last token lies outside the tensor map, which
 // gives zeros), 1 MMA, 2 zeroes the values of a block that nobody sees, 3 hands out the work, 4..7 and 8..11 the rows of the two tiles.
-#include <atomic>
 #include <type_traits>
 
 #include "paged_common.cuh"
@@ -30,7 +29,6 @@ constexpr int kHalfBytes = kBlock * 128;       // 64 dims of a block
 constexpr int kReady = 4;                      // value blocks between the zeroing warp and the MMA warp
 constexpr int kWorks = 2;                      // work descriptors in flight
 constexpr uint64_t kWaitNs = 4000000000ull;
-constexpr int kAuxRegs = 72, kRowRegs = 216, kLaunchRegs = 168;       // 128 x 72 + 256 x 216 = 384 x 168
 __device__ int g_prompt_error = 0;
 
 struct PromptParams {
@@ -161,8 +159,6 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
     ++works;
   };
 
-  if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kAuxRegs));
   if (warp == 0) {
     // ---------------------------------------------------------------------- TMA
     const int per_page = 7 - a.c.page_log2, pages = 1 << per_page;       // of a block
@@ -306,7 +302,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         ++vblocks;
       }
     }
-  } else {
+  } else if (warp == 3) {
     // ---------------------------------------------------------------------- the work, longest tiles of a sequence first
     const int pair_tokens = 2 * p.tile_tokens;
     auto tiles_of = [&](const Sequence& s) { return (s.rows + pair_tokens - 1) / pair_tokens; };
@@ -359,9 +355,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       }
       if (w.b < 0) break;
     }
-  }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegs));
     // ---------------------------------------------------------------------- the rows
     const int t = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t s_at = tmem + t * 128 + ((uint32_t)((warp & 3) * 32) << 16), o_at = s_at - t * 128 + 256 + t * D;
@@ -372,7 +366,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       else bar_sync(2, 128);
     };
     const int token_in_tile = r / a.group, head_in_group = r - token_in_tile * a.group;
-    const float scale_log2 = kExtra ? 1.f : a.scale * kLog2e;
+    const float to_log2 = a.scale * kLog2e, scale_log2 = kExtra ? 1.f : to_log2;
     const float cap_in = kExtra && a.cap > 0.f ? 2.f * a.scale / a.cap * kLog2e : 0.f, cap_log2 = a.cap * kLog2e;
     for (const Work* wp; ok && (wp = next_work()) != nullptr; work_done()) {
       const Work& w = *wp;
@@ -387,48 +381,78 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       const int tile_last = w.base + min(w.token + (t + 1) * p.tile_tokens, w.rows) - 1;
       const int window = a.window ? a.window : 0x7fffffff;
       const float slope = kExtra && a.slopes && mine ? a.slopes[head] * kLog2e : 0.f;
-      float m = -INFINITY, l0 = 0.f, l1 = 0.f;
+      float m = -INFINITY, l[4] = {0.f, 0.f, 0.f, 0.f};
       bool begun = false;
       for (int u = u0; u < u1; ++u) {
         if (!sees(u)) continue;
         if (!wait(&sm.s_full[t], n_s & 1, abort_flag, 12)) { ok = false; break; }
         ++n_s;
         tc_fence_after_sync();
-        uint32_t raw[4][32];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(s_at + 32 * i, raw[i]);
-        tmem_ld_wait();
-        auto s = [&](int i) { return __uint_as_float(raw[i >> 5][i & 31]); };
+        // First pass: the maximum, 32 columns at a time, the next ones on their way; scores that a cap, a bias or a mask changes go
+        // back to tensor memory.  Second pass: the weights.  (All 128 scores in registers spilled, and with this much shared memory a
+        // spilled value comes from L2.)
         const int from = range.unit(u) * kBlock;
-        if (kExtra) {
+        const bool whole = from + kBlock <= range.pre || (from + kBlock - 1 <= tile_first && tile_last - from < window && tile_first >= 0);
+        uint32_t raw[2][32];
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};      // (four chains: one would be 128 dependent steps)
+        auto highest = [&](const uint32_t(&x)[32]) {
 #pragma unroll
-          for (int i = 0; i < kBlock; ++i) {
-            float v = s(i);
-            if (a.cap > 0.f) v = cap_log2 * (1.f - __fdividef(2.f, exp2_approx(v * cap_in) + 1.f));
-            else v *= a.scale * kLog2e;
-            v -= slope * fabsf((float)(at - (from + i)));
-            raw[i >> 5][i & 31] = __float_as_uint(v);
+          for (int j = 0; j < 32; ++j) tops[j & 3] = fmaxf(tops[j & 3], __uint_as_float(x[j]));
+        };
+        if (kExtra || !whole) {
+          // columns [0, prefix) and [first, end) are seen
+          int prefix = at >= 0 ? range.pre - from : 0, end = at >= 0 ? at - from + 1 : 0;
+          int first = at - from >= window ? at - from - window + 1 : 0;
+          if (whole) prefix = kBlock;
+          float distance = (float)(at - from);
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i) {
+            uint32_t(&x)[32] = raw[0];
+            tmem_ld_32x32b_x32(s_at + 32 * i, x);
+            tmem_ld_wait();
+            if (kExtra) {
+              if (a.cap > 0.f) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  x[j] = __float_as_uint(cap_log2 * (1.f - __fdividef(2.f, exp2_approx(__uint_as_float(x[j]) * cap_in) + 1.f)));
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * to_log2);
+              }
+              if (a.slopes) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(fmaf(-slope, fabsf(distance - (float)j), __uint_as_float(x[j])));
+              }
+              distance -= 32.f;
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (!(j < prefix || (j >= first && j < end))) x[j] = 0xff800000u;
+            prefix -= 32;
+            first -= 32;
+            end -= 32;
+            tmem_st_32x32b_x32(s_at + 32 * i, x);
+            highest(x);
+          }
+          tmem_st_wait();
+        } else {
+          tmem_ld_32x32b_x32(s_at, raw[0]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            tmem_ld_wait();
+            if (i < 3) tmem_ld_32x32b_x32(s_at + 32 * (i + 1), raw[(i + 1) & 1]);
+            highest(raw[i & 1]);
           }
         }
-        const bool whole = from + kBlock <= range.pre || (from + kBlock - 1 <= tile_first && tile_last - from < window && tile_first >= 0);
-        if (!whole) {
-          // columns [0, prefix) and [first, end) are seen
-          const int prefix = at >= 0 ? range.pre - from : 0;
-          const int end = at >= 0 ? at - from + 1 : 0, first = at - from >= window ? at - from - window + 1 : 0;
-#pragma unroll
-          for (int i = 0; i < kBlock; ++i)
-            if (!(i < prefix || (i >= first && i < end))) raw[i >> 5][i & 31] = 0xff800000u;
-        }
-        float top = s(0);
-#pragma unroll
-        for (int i = 1; i < kBlock; ++i) top = fmaxf(top, s(i));
+        tmem_ld_32x32b_x32(s_at, raw[0]);
+        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         top *= scale_log2;
         const bool above = top > m + kSlack;
         if (__any_sync(0xffffffffu, above)) {
           const float to = fmaxf(m, top), f = to == -INFINITY ? 1.f : exp2_approx(m - to);
           m = to;
-          l0 *= f;
-          l1 *= f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) l[i] *= f;
           if (begun) {
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
@@ -444,18 +468,21 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         begun = true;
         const float minus = m == -INFINITY ? 0.f : -m;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t packed[32];
+        for (int i = 0; i < 4; ++i) {             // (weights 32 i .. go over scores 16 i .., which have been read)
+          const uint32_t(&x)[32] = raw[i & 1];
+          tmem_ld_wait();
+          if (i < 3) tmem_ld_32x32b_x32(s_at + 32 * (i + 1), raw[(i + 1) & 1]);
+          uint32_t packed[16];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            float x, y;
-            fma2(x, y, s(64 * i + 2 * j), s(64 * i + 2 * j + 1), scale_log2, scale_log2, minus, minus);
-            x = exp2_approx(x);
-            y = exp2_approx(y);
-            add2(l0, l1, x, y);
-            packed[j] = pack2(T(), x, y);
+          for (int j = 0; j < 16; ++j) {
+            float v, w;
+            fma2(v, w, __uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]), scale_log2, scale_log2, minus, minus);
+            v = exp2_approx(v);
+            w = exp2_approx(w);
+            add2(l[2 * (j & 1)], l[2 * (j & 1) + 1], v, w);
+            packed[j] = pack2(T(), v, w);
           }
-          tmem_st_32x32b_x32(s_at + 32 * i, packed);
+          tmem_st_32x32b_x16(s_at + 16 * i, packed);
         }
         tmem_st_wait();
         tc_fence_before_sync();
@@ -464,7 +491,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       }
       if (!ok) break;
       // ---- the tile's result -------------------------------------------------------------------------------------------------
-      const float l = l0 + l1;
+      const float sum = (l[0] + l[1]) + (l[2] + l[3]);
       const bool any = w.last[t] >= 0;
       if (any) {
         if (!wait(&sm.o_full[t], n_o & 1, abort_flag, 13)) break;
@@ -472,9 +499,9 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         tc_fence_after_sync();
       }
       if (w.chunks == 1) {
-        const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+        const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
         T* out = static_cast<T*>(a.out) + ((int64_t)(w.first + token) * a.heads + head) * D;
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < D / 32; ++i) {
           uint32_t o[32];
           if (any) {
@@ -487,7 +514,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
               uint32_t v[4];
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                v[k] = any && l != 0.f ? pack2(T(), __uint_as_float(o[8 * j + 2 * k]) * inv, __uint_as_float(o[8 * j + 2 * k + 1]) * inv) : 0u;
+                v[k] = any && sum != 0.f ? pack2(T(), __uint_as_float(o[8 * j + 2 * k]) * inv, __uint_as_float(o[8 * j + 2 * k + 1]) * inv) : 0u;
               reinterpret_cast<uint4*>(out)[4 * i + j] = make_uint4(v[0], v[1], v[2], v[3]);
             }
           }
@@ -495,9 +522,9 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       } else {
         const int64_t row = ((int64_t)w.part * 2 + t) * kRows + r;
         a.partial_ml[row * 2] = m;
-        a.partial_ml[row * 2 + 1] = l;
+        a.partial_ml[row * 2 + 1] = sum;
         float* to = a.partial + row * D;
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < D / 32; ++i) {
           uint32_t o[32];
           if (any) {
@@ -507,7 +534,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             reinterpret_cast<uint4*>(to)[8 * i + j] =
-                any && l != 0.f ? make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]) : make_uint4(0, 0, 0, 0);
+                any && sum != 0.f ? make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]) : make_uint4(0, 0, 0, 0);
         }
       }
       if (any) {
@@ -595,18 +622,10 @@ int launch_paged_prompt(const char* who, const B200PagedCache* c, PagedAttnParam
   const int64_t pairs = (c->tokens + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens) + c->batch;
   const int64_t most = pairs * c->kv_heads + a.slots;
   if (most > 0x3fffffffLL) return fail(B200_EINVAL, "%s: too many rows", who);
-  auto launch = [&](auto kern, size_t bytes, SmemLimit& limit, std::atomic<int>& regs) {
+  auto launch = [&](auto kern, size_t bytes, SmemLimit& limit) {
     const size_t smem = bytes + 1024;
     int e = raise_smem_limit(limit, reinterpret_cast<const void*>(kern), smem, who);
     if (e) return e;
-    // the register split asks for what the launch has: a kernel that was built with fewer would wait for ever
-    if (regs.load(std::memory_order_relaxed) == 0) {
-      cudaFuncAttributes attr;
-      if (cudaFuncGetAttributes(&attr, kern) != cudaSuccess) return fail(B200_ELAUNCH, "%s: cudaFuncGetAttributes", who);
-      regs.store(attr.numRegs, std::memory_order_relaxed);
-    }
-    if (regs.load(std::memory_order_relaxed) < kLaunchRegs)
-      return fail(B200_ELAUNCH, "%s: built with %d registers a thread, %d are needed", who, regs.load(), kLaunchRegs);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(most < a.slots ? most : a.slots));
     cfg.blockDim = dim3(kThreads);
@@ -627,9 +646,8 @@ int launch_paged_prompt(const char* who, const B200PagedCache* c, PagedAttnParam
     using T = decltype(type_);
     constexpr int N = decltype(dim)::value;
     static SmemLimit limit[2];
-    static std::atomic<int> regs[2];
-    return extra ? launch(paged_prompt_kernel<T, N, true>, sizeof(Smem<N>), limit[1], regs[1])
-                 : launch(paged_prompt_kernel<T, N, false>, sizeof(Smem<N>), limit[0], regs[0]);
+    return extra ? launch(paged_prompt_kernel<T, N, true>, sizeof(Smem<N>), limit[1])
+                 : launch(paged_prompt_kernel<T, N, false>, sizeof(Smem<N>), limit[0]);
   };
   auto by_dim = [&](auto type_) {
     return c->head_dim == 128 ? by_form(type_, std::integral_constant<int, 128>()) : by_form(type_, std::integral_constant<int, 64>());
