@@ -11,6 +11,7 @@
 //
 // Warps: 0 TMA (the pages of a block: one load per page and 64 dims; a page behind the last token lies outside the tensor map, which
 // gives zeros), 1 MMA, 2 zeroes the values of a block that nobody sees, 3 hands out the work, 4..7 and 8..11 the rows of the two tiles.
+#include <atomic>
 #include <type_traits>
 
 #include "paged_common.cuh"
@@ -29,6 +30,7 @@ constexpr int kHalfBytes = kBlock * 128;       // 64 dims of a block
 constexpr int kReady = 4;                      // value blocks between the zeroing warp and the MMA warp
 constexpr int kWorks = 2;                      // work descriptors in flight
 constexpr uint64_t kWaitNs = 4000000000ull;
+constexpr int kAuxRegs = 72, kRowRegs = 216, kLaunchRegs = 168;      // 128 x 72 + 256 x 216 = 384 x 168
 __device__ int g_prompt_error = 0;
 
 struct PromptParams {
@@ -159,6 +161,8 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
     ++works;
   };
 
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kAuxRegs));
   if (warp == 0) {
     // ---------------------------------------------------------------------- TMA
     const int per_page = 7 - a.c.page_log2, pages = 1 << per_page;       // of a block
@@ -302,7 +306,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         ++vblocks;
       }
     }
-  } else if (warp == 3) {
+  } else {
     // ---------------------------------------------------------------------- the work, longest tiles of a sequence first
     const int pair_tokens = 2 * p.tile_tokens;
     auto tiles_of = [&](const Sequence& s) { return (s.rows + pair_tokens - 1) / pair_tokens; };
@@ -355,7 +359,9 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       }
       if (w.b < 0) break;
     }
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegs));
     // ---------------------------------------------------------------------- the rows
     const int t = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t s_at = tmem + t * 128 + ((uint32_t)((warp & 3) * 32) << 16), o_at = s_at - t * 128 + 256 + t * D;
@@ -467,22 +473,26 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         }
         begun = true;
         const float minus = m == -INFINITY ? 0.f : -m;
+        // (weights 32 i .. go over scores 16 i .., which have been read; unrolled further, the sums wait for the end in registers)
+#pragma unroll 1
+        for (int i = 0; i < 4; i += 2) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {             // (weights 32 i .. go over scores 16 i .., which have been read)
-          const uint32_t(&x)[32] = raw[i & 1];
-          tmem_ld_wait();
-          if (i < 3) tmem_ld_32x32b_x32(s_at + 32 * (i + 1), raw[(i + 1) & 1]);
-          uint32_t packed[16];
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t(&x)[32] = raw[h];
+            tmem_ld_wait();
+            if (i + h < 3) tmem_ld_32x32b_x32(s_at + 32 * (i + h + 1), raw[h ^ 1]);
+            uint32_t packed[16];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            float v, w;
-            fma2(v, w, __uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]), scale_log2, scale_log2, minus, minus);
-            v = exp2_approx(v);
-            w = exp2_approx(w);
-            add2(l[2 * (j & 1)], l[2 * (j & 1) + 1], v, w);
-            packed[j] = pack2(T(), v, w);
+            for (int j = 0; j < 16; ++j) {
+              float v, w;
+              fma2(v, w, __uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]), scale_log2, scale_log2, minus, minus);
+              v = exp2_approx(v);
+              w = exp2_approx(w);
+              add2(l[2 * (j & 1)], l[2 * (j & 1) + 1], v, w);
+              packed[j] = pack2(T(), v, w);
+            }
+            tmem_st_32x32b_x16(s_at + 16 * (i + h), packed);
           }
-          tmem_st_32x32b_x16(s_at + 16 * i, packed);
         }
         tmem_st_wait();
         tc_fence_before_sync();
@@ -559,12 +569,16 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       __threadfence();
       const int64_t part0 = (int64_t)w.part - (int64_t)w.chunk * w.part_step;
       constexpr int kQuads = D / 4;
-      for (int i = r; i < kRows * kQuads; i += 128) {
+      int i0 = r;
+      asm volatile("" : "+r"(i0));               // (else what follows from it is worked out once and held in registers all along)
+#pragma unroll 1
+      for (int i = i0; i < kRows * kQuads; i += 128) {
         const int row = i / kQuads, d = (i % kQuads) * 4;
         const int tok_in = row / a.group, tok = w.token + t * p.tile_tokens + tok_in;
         if (tok_in >= p.tile_tokens || tok >= w.rows) break;
         float M = -INFINITY, L = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
         for (int k = 0; k < w.chunks; ++k) M = fmaxf(M, __ldcg(a.partial_ml + (((part0 + (int64_t)k * w.part_step) * 2 + t) * kRows + row) * 2));
+#pragma unroll 1
         for (int k = 0; k < w.chunks; ++k) {
           const int64_t x = ((part0 + (int64_t)k * w.part_step) * 2 + t) * kRows + row;
           const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.partial_ml + x * 2));
@@ -622,10 +636,18 @@ int launch_paged_prompt(const char* who, const B200PagedCache* c, PagedAttnParam
   const int64_t pairs = (c->tokens + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens) + c->batch;
   const int64_t most = pairs * c->kv_heads + a.slots;
   if (most > 0x3fffffffLL) return fail(B200_EINVAL, "%s: too many rows", who);
-  auto launch = [&](auto kern, size_t bytes, SmemLimit& limit) {
+  auto launch = [&](auto kern, size_t bytes, SmemLimit& limit, std::atomic<int>& regs) {
     const size_t smem = bytes + 1024;
     int e = raise_smem_limit(limit, reinterpret_cast<const void*>(kern), smem, who);
     if (e) return e;
+    // the register split asks for what the launch has: a kernel that was built with fewer would wait for ever
+    if (regs.load(std::memory_order_relaxed) == 0) {
+      cudaFuncAttributes attr;
+      if (cudaFuncGetAttributes(&attr, kern) != cudaSuccess) return fail(B200_ELAUNCH, "%s: cudaFuncGetAttributes", who);
+      regs.store(attr.numRegs, std::memory_order_relaxed);
+    }
+    if (regs.load(std::memory_order_relaxed) < kLaunchRegs)
+      return fail(B200_ELAUNCH, "%s: built with %d registers a thread, %d are needed", who, regs.load(), kLaunchRegs);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(most < a.slots ? most : a.slots));
     cfg.blockDim = dim3(kThreads);
@@ -646,8 +668,9 @@ int launch_paged_prompt(const char* who, const B200PagedCache* c, PagedAttnParam
     using T = decltype(type_);
     constexpr int N = decltype(dim)::value;
     static SmemLimit limit[2];
-    return extra ? launch(paged_prompt_kernel<T, N, true>, sizeof(Smem<N>), limit[1])
-                 : launch(paged_prompt_kernel<T, N, false>, sizeof(Smem<N>), limit[0]);
+    static std::atomic<int> regs[2];
+    return extra ? launch(paged_prompt_kernel<T, N, true>, sizeof(Smem<N>), limit[1], regs[1])
+                 : launch(paged_prompt_kernel<T, N, false>, sizeof(Smem<N>), limit[0], regs[0]);
   };
   auto by_dim = [&](auto type_) {
     return c->head_dim == 128 ? by_form(type_, std::integral_constant<int, 128>()) : by_form(type_, std::integral_constant<int, 64>());
