@@ -46,19 +46,14 @@ struct Work {
   int token;                                   // the pair's first
   int u0, u1;                                  // its chunk of blocks
   Range<kBlock> range;
-  int low[2], high[2], last[2];                // of each tile: the keys it sees beside the prefix, its last block (u) or -1
+  int first_u[2], last[2];                     // of each tile: its first block (u) behind the prefix, its last one or -1
   int chunk, chunks, cut_tile, part, part_step;
 };
 // Whether a tile sees anything of block u.
 struct Sight {
-  Range<kBlock> range;
-  int low, high;
-  bool any;
-  __device__ __forceinline__ Sight(const Work& w, int t) : range(w.range), low(w.low[t]), high(w.high[t]), any(w.last[t] >= 0) {}
-  __device__ __forceinline__ bool operator()(int u) const {
-    const int from = range.unit(u) * kBlock;
-    return any && (from < range.pre || (from < high && from + kBlock > low));
-  }
+  int pre, first, last;
+  __device__ __forceinline__ Sight(const Work& w, int t) : pre(w.range.pre_units), first(w.first_u[t]), last(w.last[t]) {}
+  __device__ __forceinline__ bool operator()(int u) const { return u <= last && (u >= first || u < pre); }
 };
 
 template <int D>
@@ -76,6 +71,54 @@ struct Smem {
   int abort_flag;
   int last_here[2];
 };
+
+// Four MMAs along K under one election; the descriptors advance by 32 bytes (operands with rows along K), the address of an A in tensor
+// memory by 8 columns and a B with rows along N by 2048 bytes (16 rows).
+__device__ __forceinline__ void mma4_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p, t, e;\n"
+      ".reg .b64 a1, a2, a3, b1, b2, b3;\n"
+      "elect.sync _|e, 0xffffffff;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "setp.eq.b32 t, 0, 0;\n"
+      "add.s64 a1, %1, 2;\n"
+      "add.s64 b1, %2, 2;\n"
+      "add.s64 a2, %1, 4;\n"
+      "add.s64 b2, %2, 4;\n"
+      "add.s64 a3, %1, 6;\n"
+      "add.s64 b3, %2, 6;\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, t;\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n"
+      "}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma4_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p, t, e;\n"
+      ".reg .b32 a1, a2, a3;\n"
+      ".reg .b64 b1, b2, b3;\n"
+      "elect.sync _|e, 0xffffffff;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "setp.eq.b32 t, 0, 0;\n"
+      "add.s32 a1, %1, 8;\n"
+      "add.s64 b1, %2, 128;\n"
+      "add.s32 a2, %1, 16;\n"
+      "add.s64 b2, %2, 256;\n"
+      "add.s32 a3, %1, 24;\n"
+      "add.s64 b3, %2, 384;\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, t;\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, t;\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, t;\n"
+      "}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 
 // Bounded wait; false: it ran out, here or in another warp, and the kernel ends.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int code) {
@@ -109,6 +152,62 @@ __device__ __forceinline__ void add2(float& x, float& y, float ax, float ay) {
   x = __uint_as_float((uint32_t)d);
   y = __uint_as_float((uint32_t)(d >> 32));
 }
+
+// 2^x of two values without the special-function unit: x = n + f with n the nearest whole number (by adding 1.5 * 2^23, whose sum has n
+// in its low bits), a polynomial of degree kDegree for 2^f on [-1/2, 1/2] (least largest relative error, found by the exchange
+// algorithm: 7.5e-5 for degree 3, 2.6e-6 for degree 4; a weight is rounded to 2^-12 or worse right after), n added to the exponent.
+// x from -126 on, below that 2^-126.
+constexpr int kDegree = 4;
+__device__ __forceinline__ void exp2_poly(float& x, float& y) {
+  constexpr float c3[4] = {0.99992806f, 0.69326097f, 0.24261113f, 0.05517167f};
+  constexpr float c4[5] = {0.9999993f, 0.6931218f, 0.24024744f, 0.05591786f, 0.009570102f};
+  auto c = [&](int i) { return kDegree == 3 ? c3[i & 3] : c4[i]; };
+  constexpr float kMagic = 12582912.f;
+  const float u = fmaxf(x, -126.f), v = fmaxf(y, -126.f);
+  float tu = u, tv = v, nu, nv, fu, fv, pu = c(kDegree), pv = pu;
+  add2(tu, tv, kMagic, kMagic);
+  nu = tu;
+  nv = tv;
+  add2(nu, nv, -kMagic, -kMagic);
+  fma2(fu, fv, nu, nv, -1.f, -1.f, u, v);
+#pragma unroll
+  for (int i = kDegree - 1; i >= 0; --i) fma2(pu, pv, pu, pv, fu, fv, c(i), c(i));
+  x = __uint_as_float(__float_as_uint(pu) + (__float_as_uint(tu) << 23));
+  y = __uint_as_float(__float_as_uint(pv) + (__float_as_uint(tv) << 23));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+constexpr int kPolyOfEight = 2;                 // pairs of weights of eight that go that way
+
+__device__ __forceinline__ void mul2(float& x, float& y, float ax, float ay) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair64(x, y)), "l"(pair64(ax, ay)));
+  x = __uint_as_float((uint32_t)d);
+  y = __uint_as_float((uint32_t)(d >> 32));
+}
+// cap * tanh(scale * x / cap) in the exponent of 2, of two scores.  Small: |scale * x / cap| <= 0.4, where tanh's Taylor series to the
+// ninth power is 1e-6 off; nearly all scores are, and the other form takes two special functions for each.
+struct Cap {
+  float per_cap, to_log2, twice_log2, cap_log2;
+  __device__ __forceinline__ Cap(float scale, float cap)
+      : per_cap(cap > 0.f ? scale / cap : 0.f), to_log2(scale * kLog2e), twice_log2(2.f * per_cap * kLog2e), cap_log2(cap * kLog2e) {}
+  __device__ __forceinline__ void small(float& x, float& y) const {
+    float u = x, v = y;
+    mul2(u, v, per_cap, per_cap);
+    mul2(u, v, u, v);
+    float pu = 62.f / 2835.f, pv = pu;
+    fma2(pu, pv, pu, pv, u, v, -17.f / 315.f, -17.f / 315.f);
+    fma2(pu, pv, pu, pv, u, v, 2.f / 15.f, 2.f / 15.f);
+    fma2(pu, pv, pu, pv, u, v, -1.f / 3.f, -1.f / 3.f);
+    fma2(pu, pv, pu, pv, u, v, 1.f, 1.f);
+    mul2(x, y, to_log2, to_log2);
+    mul2(x, y, pu, pv);
+  }
+  __device__ __forceinline__ float any(float x) const { return cap_log2 * (1.f - __fdividef(2.f, exp2_approx(x * twice_log2) + 1.f)); }
+};
 
 template <typename T, int D, bool kExtra>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -217,10 +316,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
     auto scores = [&](int t, uint32_t slot) {
 #pragma unroll
       for (int i = 0; i < kHalves; ++i)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          umma_f16_ss(tmem + t * 128, dq + t * kStep + i * kHalfStep + 2 * k, dk + (uint64_t)(slot * kStep) + i * kHalfStep + 2 * k, kIdescS,
-                      i + k > 0);
+        mma4_ss(tmem + t * 128, dq + t * kStep + i * kHalfStep, dk + (uint64_t)(slot * kStep) + i * kHalfStep, kIdescS, i > 0);
       umma_commit(&sm.s_full[t]);
     };
     bool ok = true;
@@ -256,8 +352,8 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
               ++n_p[t];
               tc_fence_after_sync();
 #pragma unroll
-              for (int k = 0; k < kBlock / 16; ++k)
-                umma_f16_ts(tmem + 256 + t * D, tmem + t * 128 + 8 * k, dv + (uint64_t)(vslot * kStep) + k * (2048 >> 4), kIdescO, begun[t] || k > 0);
+              for (int k = 0; k < 2; ++k)
+                mma4_ts(tmem + 256 + t * D, tmem + t * 128 + 32 * k, dv + (uint64_t)(vslot * kStep) + k * 512, kIdescO, begun[t] || k > 0);
               begun[t] = true;
               if (u == last[t]) {
                 umma_commit(&sm.o_full[t]);
@@ -335,17 +431,15 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const int from = w.token + t * p.tile_tokens;
-          const bool there = from < s.rows;
           Range<kBlock> r;
           r.set(a, s, item.b, from, min(from + p.tile_tokens, s.rows) - 1);
-          w.low[t] = r.low;
-          w.high[t] = r.high;
-          w.last[t] = there && r.high > 0 ? 0 : -1;
-          int last = -1;
-          const Sight sees(w, t);
-          for (int u = w.u0 + lane; u < w.u1; u += 32)
-            if (sees(u)) last = u;
-          w.last[t] = __reduce_max_sync(0xffffffffu, last);
+          // its own blocks begin where the pair's do, or later, and end where the pair's do, or earlier
+          const int end = w.range.pre_units + (r.high + kBlock - 1) / kBlock - w.range.second;
+          w.first_u[t] = w.range.pre_units + max(r.low / kBlock - w.range.second, 0);
+          w.last[t] = min(end > w.range.pre_units ? end : w.range.pre_units, w.u1) - 1;
+          if (from >= s.rows || r.high == 0 || w.last[t] < w.u0 || (w.last[t] < w.first_u[t] && w.u0 >= w.range.pre_units)) w.last[t] = -1;
+          // (no block of its own, but the prefix's)
+          else if (w.last[t] < w.first_u[t]) w.last[t] = min(w.range.pre_units, w.u1) - 1;
         }
         w.chunk = item.chunk;
         w.chunks = item.chunks;
@@ -373,11 +467,11 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
     };
     const int token_in_tile = r / a.group, head_in_group = r - token_in_tile * a.group;
     const float to_log2 = a.scale * kLog2e, scale_log2 = kExtra ? 1.f : to_log2;
-    const float cap_in = kExtra && a.cap > 0.f ? 2.f * a.scale / a.cap * kLog2e : 0.f, cap_log2 = a.cap * kLog2e;
+    const Cap cap(a.scale, a.cap);
     for (const Work* wp; ok && (wp = next_work()) != nullptr; work_done()) {
       const Work& w = *wp;
       const Sight sees(w, t);
-      const Range<kBlock>& range = sees.range;
+      const Range<kBlock> range = w.range;
       const int u0 = w.u0, u1 = w.u1;
       const int token = w.token + t * p.tile_tokens + token_in_tile;
       const bool mine = token_in_tile < p.tile_tokens && token < w.rows;
@@ -403,13 +497,12 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};      // (four chains: one would be 128 dependent steps)
         auto highest = [&](const uint32_t(&x)[32]) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) tops[j & 3] = fmaxf(tops[j & 3], __uint_as_float(x[j]));
+          for (int j = 0; j < 16; ++j) tops[j & 3] = max3(tops[j & 3], __uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]));
         };
         if (kExtra || !whole) {
           // columns [0, prefix) and [first, end) are seen
           int prefix = at >= 0 ? range.pre - from : 0, end = at >= 0 ? at - from + 1 : 0;
           int first = at - from >= window ? at - from - window + 1 : 0;
-          if (whole) prefix = kBlock;
           float distance = (float)(at - from);
 #pragma unroll 1
           for (int i = 0; i < 4; ++i) {
@@ -418,22 +511,42 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
             tmem_ld_wait();
             if (kExtra) {
               if (a.cap > 0.f) {
+                float most = 0.f;
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  x[j] = __float_as_uint(cap_log2 * (1.f - __fdividef(2.f, exp2_approx(__uint_as_float(x[j]) * cap_in) + 1.f)));
+                for (int j = 0; j < 32; ++j) most = fmaxf(most, fabsf(__uint_as_float(x[j])));
+                if (__any_sync(0xffffffffu, most * fabsf(cap.per_cap) > 0.4f)) {
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(cap.any(__uint_as_float(x[j])));
+                } else {
+#pragma unroll
+                  for (int j = 0; j < 32; j += 2) {
+                    float v = __uint_as_float(x[j]), w = __uint_as_float(x[j + 1]);
+                    cap.small(v, w);
+                    x[j] = __float_as_uint(v);
+                    x[j + 1] = __float_as_uint(w);
+                  }
+                }
               } else {
 #pragma unroll
                 for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * to_log2);
               }
               if (a.slopes) {
+                // -slope * |distance - j|; at or before the row itself, as nearly everywhere, one multiply-add
+                const bool past = __all_sync(0xffffffffu, distance >= 31.f);
+                const float base = -slope * distance;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(fmaf(-slope, fabsf(distance - (float)j), __uint_as_float(x[j])));
+                for (int j = 0; j < 32; ++j) {
+                  const float v = __uint_as_float(x[j]);
+                  x[j] = __float_as_uint(past ? fmaf(slope, (float)j, v + base) : fmaf(-slope, fabsf(distance - (float)j), v));
+                }
               }
               distance -= 32.f;
             }
+            if (!whole) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (!(j < prefix || (j >= first && j < end))) x[j] = 0xff800000u;
+              for (int j = 0; j < 32; ++j)
+                if (!(j < prefix || (j >= first && j < end))) x[j] = 0xff800000u;
+            }
             prefix -= 32;
             first -= 32;
             end -= 32;
@@ -486,8 +599,12 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
             for (int j = 0; j < 16; ++j) {
               float v, w;
               fma2(v, w, __uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]), scale_log2, scale_log2, minus, minus);
-              v = exp2_approx(v);
-              w = exp2_approx(w);
+              if ((j & 7) < kPolyOfEight) {
+                exp2_poly(v, w);
+              } else {
+                v = exp2_approx(v);
+                w = exp2_approx(w);
+              }
               add2(l[2 * (j & 1)], l[2 * (j & 1) + 1], v, w);
               packed[j] = pack2(T(), v, w);
             }
@@ -501,7 +618,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       }
       if (!ok) break;
       // ---- the tile's result -------------------------------------------------------------------------------------------------
-      const float sum = (l[0] + l[1]) + (l[2] + l[3]);
+      const float sum = m == -INFINITY ? 0.f : (l[0] + l[1]) + (l[2] + l[3]);   // (a row that saw nothing: 2^-126 of every key)
       const bool any = w.last[t] >= 0;
       if (any) {
         if (!wait(&sm.o_full[t], n_o & 1, abort_flag, 13)) break;
@@ -512,20 +629,20 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
         T* out = static_cast<T*>(a.out) + ((int64_t)(w.first + token) * a.heads + head) * D;
 #pragma unroll 1
-        for (int i = 0; i < D / 32; ++i) {
-          uint32_t o[32];
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t o[16];
           if (any) {
-            tmem_ld_32x32b_x32(o_at + 32 * i, o);
+            tmem_ld_32x32b_x16(o_at + 16 * i, o);
             tmem_ld_wait();
           }
           if (mine) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 2; ++j) {
               uint32_t v[4];
 #pragma unroll
               for (int k = 0; k < 4; ++k)
                 v[k] = any && sum != 0.f ? pack2(T(), __uint_as_float(o[8 * j + 2 * k]) * inv, __uint_as_float(o[8 * j + 2 * k + 1]) * inv) : 0u;
-              reinterpret_cast<uint4*>(out)[4 * i + j] = make_uint4(v[0], v[1], v[2], v[3]);
+              reinterpret_cast<uint4*>(out)[2 * i + j] = make_uint4(v[0], v[1], v[2], v[3]);
             }
           }
         }
@@ -535,15 +652,15 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         a.partial_ml[row * 2 + 1] = sum;
         float* to = a.partial + row * D;
 #pragma unroll 1
-        for (int i = 0; i < D / 32; ++i) {
-          uint32_t o[32];
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t o[16];
           if (any) {
-            tmem_ld_32x32b_x32(o_at + 32 * i, o);
+            tmem_ld_32x32b_x16(o_at + 16 * i, o);
             tmem_ld_wait();
           }
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            reinterpret_cast<uint4*>(to)[8 * i + j] =
+          for (int j = 0; j < 4; ++j)
+            reinterpret_cast<uint4*>(to)[4 * i + j] =
                 any && sum != 0.f ? make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]) : make_uint4(0, 0, 0, 0);
         }
       }
