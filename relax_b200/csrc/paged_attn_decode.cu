@@ -381,9 +381,9 @@ using namespace b200;
 
 extern "C" {
 
-// The counters; then, of twice as many chunks as there are slots (a cut tile has more than a slot's share of the units, its chunks at least half
-// of that), the maxima and sums and the partial results: 256 rows of the many-rows kernel are the most.
-static int64_t scratch_rows() { return (int64_t)2 * sm_count() * 256; }
+// The counters, the maxima and sums of chunks, their partial results.  Here a cut tile has more than a slot's share of the units and its
+// chunks at least half of that: fewer cut tiles than slots, twice as many chunks at most, of 16 rows.  The many-rows kernel needs more.
+static int64_t scratch_rows() { return (int64_t)kPartsOfSlots * sm_count() * 256; }
 
 int64_t b200_paged_attention_scratch_bytes(void) {
   if (ensure_device()) return -1;
@@ -407,7 +407,7 @@ int b200_paged_attention(const B200PagedCache* cache, const B200PagedAttention* 
   if (!a->q || !a->out || !aligned16(a->q) || !aligned16(a->out)) return fail(B200_EINVAL, "%s: q and out must be non-null and 16-byte aligned", who);
   if (!scratch || !aligned16(scratch)) return fail(B200_EINVAL, "%s: scratch must be non-null and 16-byte aligned", who);
   if ((rc = ensure_device())) return rc;
-  if (scratch_bytes < b200_paged_attention_scratch_bytes() || sm_count() * kCtasPerSm1 * 4 > B200_PAGED_ZEROED_BYTES)
+  if (scratch_bytes < b200_paged_attention_scratch_bytes() || sm_count() * kCtasPerSm1 > kCutTiles)
     return fail(B200_EINVAL, "%s: scratch of %lld bytes is less than b200_paged_attention_scratch_bytes()", who, (long long)scratch_bytes);
   p.q = a->q;
   p.out = a->out;

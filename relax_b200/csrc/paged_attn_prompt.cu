@@ -29,6 +29,7 @@ constexpr int kThreads = 384;
 constexpr int kHalfBytes = kBlock * 128;       // 64 dims of a block
 constexpr int kReady = 4;                      // value blocks between the zeroing warp and the MMA warp
 constexpr int kWorks = 2;                      // work descriptors in flight
+constexpr int kKept = 64;                      // sequences whose sizes the scheduling warp keeps
 constexpr uint64_t kWaitNs = 4000000000ull;
 constexpr int kAuxRegs = 72, kRowRegs = 216, kLaunchRegs = 168;      // 128 x 72 + 256 x 216 = 384 x 168
 __device__ int g_prompt_error = 0;
@@ -38,6 +39,8 @@ struct PromptParams {
   CUtensorMap tm_k, tm_v;                      // {D, page, kv_heads, pages}, box {64, page, 1, 1}, SWIZZLE_128B
   PagedAttnParams a;
   int tile_tokens;
+  unsigned long long per_pair;                 // 2^40 / (tokens of a pair), rounded up: n of them divided exactly up to 2^32
+  int* next;                                   // the next item, CTAs that are through
 };
 
 struct Work {
@@ -49,6 +52,166 @@ struct Work {
   int first_u[2], last[2];                     // of each tile: its first block (u) behind the prefix, its last one or -1
   int chunk, chunks, cut_tile, part, part_step;
 };
+// The work of a launch, the same for every CTA: pairs of tiles in the order of the blocks they see, most first, each with all its key
+// heads; a sequence of many blocks may have its pairs cut into chunks.  CTAs take the next one from a counter.
+struct Plan {
+  int c;                                       // a sequence of more blocks than this is cut
+  struct Seq {
+    int base, rows, most, first;               // position of the first row, rows, blocks of the last pair; first row
+  };
+  Seq* kept;                                   // of the first kKept sequences: a load from global memory is a trip to L2 here
+  __device__ __forceinline__ static int blocks(int tokens) { return max((tokens + kBlock - 1) / kBlock, 1); }
+  __device__ __forceinline__ static Seq load(const PromptParams& p, int b) {
+    const PagedAttnParams& a = p.a;
+    const Sequence s = sequence_of(a.c, b);
+    Seq q = {s.length - s.rows, s.rows, blocks(s.length), s.first};
+    if (a.causal && a.window) q.most = min(q.most, (a.window + 2 * p.tile_tokens) / kBlock + 2 + (a.prefix ? max(a.prefix[b], 0) / kBlock : 0));
+    return q;
+  }
+  __device__ __forceinline__ Seq sequence(const PromptParams& p, int b) const { return b < kKept ? kept[b] : load(p, b); }
+  __device__ __forceinline__ int chunks(const Seq& q) const { return q.most > c ? (q.most + c - 1) / c : 1; }
+  // Pairs of tiles that hold so many tokens.  (A division by a variable takes this warp longer than the rest of its search.)
+  __device__ __forceinline__ static int pairs_of(const PromptParams& p, int tokens) {
+    return (int)((unsigned long long)(unsigned)(tokens + 2 * p.tile_tokens - 1) * p.per_pair >> 40);
+  }
+  __device__ __forceinline__ static int pairs(const PromptParams& p, const Seq& q) { return pairs_of(p, q.rows); }
+  // Pairs of a sequence with x blocks or more (the number of blocks grows with the pair's place).
+  __device__ __forceinline__ static int at_least(const PromptParams& p, const Seq& q, int x) {
+    const int all = pairs(p, q), need = (x - 1) * kBlock + 1 - q.base;
+    if (x > q.most) return 0;
+    if (x <= 1 || !p.a.causal || need <= 0) return all;
+    return max(all - (pairs_of(p, need) - 1), 0);
+  }
+  // Several ways to cut, one a lane: the longest pairs into 1, 2, ... chunks, all others into chunks no longer.  What a way costs: its rounds of items over the
+  // CTAs times an item's average length, 3 blocks of time for its beginning and end and 6 more for partial results; or the longest item.
+  __device__ __forceinline__ Plan(const PromptParams& p, int lane, Seq* memory) : c(0x3fffffff), kept(memory) {
+    const PagedAttnParams& a = p.a;
+    int64_t total = 0;
+    int longest = 1;
+#pragma unroll 1
+    for (int b = lane; b < a.c.batch; b += 32) {
+      const Seq q = load(p, b);
+      if (b < kKept) kept[b] = q;
+      const int first = a.causal ? min(blocks(q.base + 2 * p.tile_tokens), q.most) : q.most, n = pairs(p, q);
+      total += (int64_t)n * (first + q.most);
+      if (n) longest = max(longest, q.most);
+    }
+    __syncwarp();
+    total = warp_sum64(total) * a.c.kv_heads / 2;
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    if (a.c.batch > kKept) {                   // (looking at all ways would take longer than it saves)
+      const int share = (int)((total + a.slots - 1) / a.slots);
+      if (longest > 2 * share) c = max(share, 8);
+      return;
+    }
+    const int mine = max((longest + lane) / (lane + 1), 4);
+    int items = 0, parts = 0, cut = 0;
+#pragma unroll 1
+    for (int b = 0; b < a.c.batch; ++b) {
+      const Seq q = kept[b];
+      const int tiles = pairs(p, q) * a.c.kv_heads, n = q.most > mine ? (q.most + mine - 1) / mine : 1;
+      items += tiles * n;
+      if (n > 1) {
+        parts += tiles * n;
+        cut += tiles;
+      }
+    }
+    int cost = 0x7fffffff;
+    if (items > 0 && parts <= kPartsOfSlots * a.slots && cut * 2 <= kCutTiles) {
+      const float rounds = (float)((items + a.slots - 1) / a.slots);
+      cost = (int)fmaxf(fminf(rounds * ((float)total * 4.f / (float)items + (parts ? 36.f : 12.f)), 1e9f), (float)(min(mine, longest) * 4 + 12));
+    }
+    const int best = __reduce_min_sync(0xffffffffu, cost);
+    c = __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, cost == best)) - 1);
+  }
+  // Item `index` into w; w.b stays -1 where there is none.
+  __device__ __forceinline__ void find(const PromptParams& p, int index, int lane, Work& w) const {
+    const PagedAttnParams& a = p.a;
+    const int h = index % a.c.kv_heads, rank = index / a.c.kv_heads;
+    // the largest x such that more than `rank` chunks belong to pairs with x blocks or more
+    int x = 0, above = (int)((int64_t)a.c.table_width << a.c.page_log2) / kBlock + 2, in = rank;
+#pragma unroll 1
+    while (above - x > 1) {
+      const int mid = (x + above) >> 1;
+      int n = 0;
+#pragma unroll 1
+      for (int b = lane; b < a.c.batch; b += 32) {
+        const Seq q = sequence(p, b);
+        n += at_least(p, q, mid) * chunks(q);
+      }
+      n = (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
+      if (n > rank) {
+        x = mid;
+      } else {
+        above = mid;
+        in = rank - n;
+      }
+    }
+    if (x == 0) return;
+#pragma unroll 1
+    for (int b0 = 0;; b0 += 32) {              // (ends: there are more than `in` of them)
+      Seq q = {};
+      int level = 0;
+      if (b0 + lane < a.c.batch) {
+        q = sequence(p, b0 + lane);
+        level = (at_least(p, q, x) - at_least(p, q, x + 1)) * chunks(q);
+      }
+      const int upto = warp_scan(level, lane);
+      const unsigned hit = __ballot_sync(0xffffffffu, upto > in);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        in -= __shfl_sync(0xffffffffu, upto - level, l);
+        w.b = b0 + l;
+        break;
+      }
+      in -= __shfl_sync(0xffffffffu, upto, 31);
+      if (b0 + 32 >= a.c.batch) return;
+    }
+    const Seq q = sequence(p, w.b);
+    const Sequence s = {q.first, q.rows, q.base + q.rows};
+    const int n = chunks(q), tile = pairs(p, q) - at_least(p, q, x + 1) - 1 - in / n;
+    // place in scratch memory: behind the cut pairs of the sequences in front
+    int cut = 0, parts = 0;
+    if (n > 1)
+#pragma unroll 1
+      for (int b = lane; b < w.b; b += 32) {
+        const Seq o = sequence(p, b);
+        if (chunks(o) > 1) {
+          cut += pairs(p, o);
+          parts += pairs(p, o) * chunks(o);
+        }
+      }
+    cut = (int)__reduce_add_sync(0xffffffffu, (unsigned)cut);
+    parts = (int)__reduce_add_sync(0xffffffffu, (unsigned)parts);
+    w.h = h;
+    w.first = s.first;
+    w.rows = s.rows;
+    w.base = q.base;
+    w.length = s.length;
+    w.token = tile * 2 * p.tile_tokens;
+    w.chunks = n;
+    w.chunk = in % n;
+    w.cut_tile = ((cut + tile) * a.c.kv_heads + h) * 2;
+    w.part = (parts + tile * n + w.chunk) * a.c.kv_heads + h;
+    w.part_step = a.c.kv_heads;
+    w.range.set(a, s, w.b, w.token, min(w.token + 2 * p.tile_tokens, s.rows) - 1);
+    w.u0 = (int)((int64_t)w.range.units * w.chunk / w.chunks);
+    w.u1 = (int)((int64_t)w.range.units * (w.chunk + 1) / w.chunks);
+#pragma unroll 1
+    for (int t = 0; t < 2; ++t) {
+      const int from = w.token + t * p.tile_tokens;
+      Range<kBlock> r;
+      r.set(a, s, w.b, from, min(from + p.tile_tokens, s.rows) - 1);
+      // its own blocks begin where the pair's do, or later, and end where the pair's do, or earlier
+      const int end = w.range.pre_units + (r.high + kBlock - 1) / kBlock - w.range.second;
+      w.first_u[t] = w.range.pre_units + max(r.low / kBlock - w.range.second, 0);
+      w.last[t] = min(max(end, w.range.pre_units), w.u1) - 1;
+      if (w.last[t] < w.first_u[t]) w.last[t] = min(w.range.pre_units, w.u1) - 1;       // (none of its own: the prefix's)
+      if (from >= s.rows || r.high == 0 || w.last[t] < w.u0) w.last[t] = -1;
+    }
+  }
+};
+
 // Whether a tile sees anything of block u.
 struct Sight {
   int pre, first, last;
@@ -65,11 +228,12 @@ struct Smem {
   uint64_t q_full, q_empty;
   uint64_t full[kStages], empty[kStages], ready[kReady];
   uint64_t s_full[2], p_ready[2], o_full[2], o_empty[2];
-  uint64_t work_full[kWorks], work_empty[kWorks];
+  uint64_t work_full[kWorks], work_empty[kWorks], issued;
   Work work[kWorks];
   uint32_t tmem_base;
   int abort_flag;
   int last_here[2];
+  Plan::Seq kept[kKept];
 };
 
 // Four MMAs along K under one election; the descriptors advance by 32 bytes (operands with rows along K), the address of an A in tensor
@@ -175,11 +339,18 @@ __device__ __forceinline__ void exp2_poly(float& x, float& y) {
   x = __uint_as_float(__float_as_uint(pu) + (__float_as_uint(tu) << 23));
   y = __uint_as_float(__float_as_uint(pv) + (__float_as_uint(tv) << 23));
 }
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+// What happens to a score before the softmax: a scale > 0; that and a cap; that and a bias by distance; anything.
+constexpr int kPlain = 0, kCapped = 1, kSloped = 2, kGeneral = 3;
 constexpr int kPolyOfEight = 2;                 // pairs of weights of eight that go that way
 
 __device__ __forceinline__ void mul2(float& x, float& y, float ax, float ay) {
@@ -209,7 +380,7 @@ struct Cap {
   __device__ __forceinline__ float any(float x) const { return cap_log2 * (1.f - __fdividef(2.f, exp2_approx(x * twice_log2) + 1.f)); }
 };
 
-template <typename T, int D, bool kExtra>
+template <typename T, int D, int kForm>
 __global__ void __launch_bounds__(kThreads, 1)
 paged_prompt_kernel(const __grid_constant__ PromptParams p) {
   using Shared = Smem<D>;
@@ -233,6 +404,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       mbar_init(&sm.o_full[t], 1);
       mbar_init(&sm.o_empty[t], 4);
     }
+    mbar_init(&sm.issued, 1);
     for (int i = 0; i < kWorks; ++i) { mbar_init(&sm.work_full[i], 1); mbar_init(&sm.work_empty[i], 11); }
     mbar_fence_init();
   }
@@ -266,7 +438,11 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
     // ---------------------------------------------------------------------- TMA
     const int per_page = 7 - a.c.page_log2, pages = 1 << per_page;       // of a block
     uint32_t pos = 0, items = 0;
-    for (const Work* wp; (wp = next_work()) != nullptr; work_done()) {
+    auto issued = [&]() {
+      if (lane == 0) mbar_arrive(&sm.issued);
+      work_done();
+    };
+    for (const Work* wp; (wp = next_work()) != nullptr; issued()) {
       const Work& w = *wp;
       if (w.u1 == w.u0) continue;
       if (items > 0 && !wait_relaxed(&sm.q_empty, (items - 1) & 1, abort_flag, 2)) break;
@@ -403,55 +579,30 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       }
     }
   } else {
-    // ---------------------------------------------------------------------- the work, longest tiles of a sequence first
-    const int pair_tokens = 2 * p.tile_tokens;
-    auto tiles_of = [&](const Sequence& s) { return (s.rows + pair_tokens - 1) / pair_tokens; };
-    const int64_t even = (total_units<kBlock>(a, lane, tiles_of) + a.slots - 1) / a.slots;
-    const int c = (int)max(even, (int64_t)8);
+    // ---------------------------------------------------------------------- the work, longest tiles first
+    const Plan plan(p, lane, sm.kept);
     for (uint32_t i = 0;; ++i) {
       const uint32_t slot = i % kWorks, round = i / kWorks;
       if (round > 0 && !wait_relaxed(&sm.work_empty[slot], (round - 1) & 1, abort_flag, 11)) break;
-      const int64_t index = (int64_t)i * gridDim.x + ((i & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-      Item item;
+      // the next item is taken when this one's loads are all on their way, two or three blocks before its end: taken earlier, the CTA with
+      // the longest item would get one of the second longest too
+      if (i > 0 && !wait_relaxed(&sm.issued, (i - 1) & 1, abort_flag, 15)) break;
+      int index = 0;
+      if (lane == 0) index = atomicAdd(p.next, 1);
+      index = __shfl_sync(0xffffffffu, index, 0);
       Work w;
       w.b = -1;
-      if (index / a.c.kv_heads < 0x7fffffff && find_item<kBlock>(a, (int)(index / a.c.kv_heads), c, lane, tiles_of, item)) {
-        const Sequence s = sequence_of(a.c, item.b);
-        const int tile = tiles_of(s) - 1 - item.tile;
-        w.b = item.b;
-        w.h = (int)(index % a.c.kv_heads);
-        w.first = s.first;
-        w.rows = s.rows;
-        w.base = s.length - s.rows;
-        w.length = s.length;
-        w.token = tile * pair_tokens;
-        w.range.set(a, s, item.b, w.token, min(w.token + pair_tokens, s.rows) - 1);
-        w.u0 = (int)((int64_t)w.range.units * item.chunk / item.chunks);
-        w.u1 = (int)((int64_t)w.range.units * (item.chunk + 1) / item.chunks);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int from = w.token + t * p.tile_tokens;
-          Range<kBlock> r;
-          r.set(a, s, item.b, from, min(from + p.tile_tokens, s.rows) - 1);
-          // its own blocks begin where the pair's do, or later, and end where the pair's do, or earlier
-          const int end = w.range.pre_units + (r.high + kBlock - 1) / kBlock - w.range.second;
-          w.first_u[t] = w.range.pre_units + max(r.low / kBlock - w.range.second, 0);
-          w.last[t] = min(end > w.range.pre_units ? end : w.range.pre_units, w.u1) - 1;
-          if (from >= s.rows || r.high == 0 || w.last[t] < w.u0 || (w.last[t] < w.first_u[t] && w.u0 >= w.range.pre_units)) w.last[t] = -1;
-          // (no block of its own, but the prefix's)
-          else if (w.last[t] < w.first_u[t]) w.last[t] = min(w.range.pre_units, w.u1) - 1;
-        }
-        w.chunk = item.chunk;
-        w.chunks = item.chunks;
-        w.cut_tile = (item.cut_tile * a.c.kv_heads + w.h) * 2;
-        w.part = item.cut_chunk * a.c.kv_heads + w.h;
-        w.part_step = a.c.kv_heads;
-      }
+      plan.find(p, index, lane, w);
       if (lane == 0) {
         sm.work[slot] = w;
         mbar_arrive(&sm.work_full[slot]);
       }
       if (w.b < 0) break;
+    }
+    // the CTA that comes last leaves the counters as the next launch expects them
+    if (lane == 0 && atomicAdd(p.next + 1, 1) == (int)gridDim.x - 1) {
+      p.next[0] = 0;
+      p.next[1] = 0;
     }
   }
   } else {
@@ -466,7 +617,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       else bar_sync(2, 128);
     };
     const int token_in_tile = r / a.group, head_in_group = r - token_in_tile * a.group;
-    const float to_log2 = a.scale * kLog2e, scale_log2 = kExtra ? 1.f : to_log2;
+    const float to_log2 = a.scale * kLog2e;
     const Cap cap(a.scale, a.cap);
     for (const Work* wp; ok && (wp = next_work()) != nullptr; work_done()) {
       const Work& w = *wp;
@@ -480,7 +631,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       const int tile_first = w.base + w.token + t * p.tile_tokens;
       const int tile_last = w.base + min(w.token + (t + 1) * p.tile_tokens, w.rows) - 1;
       const int window = a.window ? a.window : 0x7fffffff;
-      const float slope = kExtra && a.slopes && mine ? a.slopes[head] * kLog2e : 0.f;
+      const float slope = (kForm == kSloped || kForm == kGeneral) && a.slopes && mine ? a.slopes[head] * kLog2e : 0.f;
       float m = -INFINITY, l[4] = {0.f, 0.f, 0.f, 0.f};
       bool begun = false;
       for (int u = u0; u < u1; ++u) {
@@ -494,52 +645,72 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         const int from = range.unit(u) * kBlock;
         const bool whole = from + kBlock <= range.pre || (from + kBlock - 1 <= tile_first && tile_last - from < window && tile_first >= 0);
         uint32_t raw[2][32];
-        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};      // (four chains: one would be 128 dependent steps)
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};      // (four chains: one would be 64 dependent steps)
+        float top;
         auto highest = [&](const uint32_t(&x)[32]) {
 #pragma unroll
           for (int j = 0; j < 16; ++j) tops[j & 3] = max3(tops[j & 3], __uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]));
         };
-        if (kExtra || !whole) {
-          // columns [0, prefix) and [first, end) are seen
+        auto all_tops = [&]() { return fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])); };
+        const float bias = kForm == kSloped ? -slope * (float)(at - from) : 0.f;       // of the block's first key, which lies before the row
+        bool direct = whole && kForm != kGeneral && (kForm != kSloped || from + kBlock - 1 <= tile_first);
+        if (direct) {
+          float lows[2] = {INFINITY, INFINITY};
+          tmem_ld_32x32b_x32(s_at, raw[0]);
+#pragma unroll 1
+          for (int i = 0; i < 4; i += 2) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t(&x)[32] = raw[h];
+              tmem_ld_wait();
+              if (i + h < 3) tmem_ld_32x32b_x32(s_at + 32 * (i + h + 1), raw[h ^ 1]);
+              if (kForm == kSloped) {
+                const float at_i = fmaf(slope, (float)(32 * (i + h)), bias);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                  float v, w, bv, bw;
+                  fma2(bv, bw, (float)(2 * j), (float)(2 * j + 1), slope, slope, at_i, at_i);
+                  fma2(v, w, __uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]), to_log2, to_log2, bv, bw);
+                  tops[j & 3] = max3(tops[j & 3], v, w);
+                }
+              } else {
+                highest(x);
+              }
+              if (kForm == kCapped)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) lows[j & 1] = min3(lows[j & 1], __uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]));
+            }
+          }
+          top = all_tops();
+          if (kForm == kCapped) {
+            direct = __all_sync(0xffffffffu, fmaxf(fabsf(top), fabsf(fminf(lows[0], lows[1]))) * cap.per_cap <= 0.4f);
+            top = cap.any(top);
+          } else if (kForm == kPlain) {
+            top *= to_log2;
+          }
+        }
+        if (!direct) {
+          // Scores that a cap, a bias or a mask changes go back to tensor memory.  Columns [0, prefix) and [first, end) are seen.
           int prefix = at >= 0 ? range.pre - from : 0, end = at >= 0 ? at - from + 1 : 0;
           int first = at - from >= window ? at - from - window + 1 : 0;
           float distance = (float)(at - from);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tops[i] = -INFINITY;
 #pragma unroll 1
           for (int i = 0; i < 4; ++i) {
             uint32_t(&x)[32] = raw[0];
             tmem_ld_32x32b_x32(s_at + 32 * i, x);
             tmem_ld_wait();
-            if (kExtra) {
-              if (a.cap > 0.f) {
-                float most = 0.f;
+            if (kForm == kCapped || (kForm == kGeneral && a.cap > 0.f)) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) most = fmaxf(most, fabsf(__uint_as_float(x[j])));
-                if (__any_sync(0xffffffffu, most * fabsf(cap.per_cap) > 0.4f)) {
+              for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(cap.any(__uint_as_float(x[j])));
+            } else if (kForm != kPlain) {
 #pragma unroll
-                  for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(cap.any(__uint_as_float(x[j])));
-                } else {
+              for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * to_log2);
+            }
+            if (kForm == kSloped || (kForm == kGeneral && a.slopes)) {
 #pragma unroll
-                  for (int j = 0; j < 32; j += 2) {
-                    float v = __uint_as_float(x[j]), w = __uint_as_float(x[j + 1]);
-                    cap.small(v, w);
-                    x[j] = __float_as_uint(v);
-                    x[j + 1] = __float_as_uint(w);
-                  }
-                }
-              } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * to_log2);
-              }
-              if (a.slopes) {
-                // -slope * |distance - j|; at or before the row itself, as nearly everywhere, one multiply-add
-                const bool past = __all_sync(0xffffffffu, distance >= 31.f);
-                const float base = -slope * distance;
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                  const float v = __uint_as_float(x[j]);
-                  x[j] = __float_as_uint(past ? fmaf(slope, (float)j, v + base) : fmaf(-slope, fabsf(distance - (float)j), v));
-                }
-              }
+              for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(fmaf(-slope, fabsf(distance - (float)j), __uint_as_float(x[j])));
               distance -= 32.f;
             }
             if (!whole) {
@@ -554,18 +725,9 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
             highest(x);
           }
           tmem_st_wait();
-        } else {
-          tmem_ld_32x32b_x32(s_at, raw[0]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            tmem_ld_wait();
-            if (i < 3) tmem_ld_32x32b_x32(s_at + 32 * (i + 1), raw[(i + 1) & 1]);
-            highest(raw[i & 1]);
-          }
+          top = all_tops() * (kForm == kPlain ? to_log2 : 1.f);
         }
         tmem_ld_32x32b_x32(s_at, raw[0]);
-        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-        top *= scale_log2;
         const bool above = top > m + kSlack;
         if (__any_sync(0xffffffffu, above)) {
           const float to = fmaxf(m, top), f = to == -INFINITY ? 1.f : exp2_approx(m - to);
@@ -587,30 +749,47 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         begun = true;
         const float minus = m == -INFINITY ? 0.f : -m;
         // (weights 32 i .. go over scores 16 i .., which have been read; unrolled further, the sums wait for the end in registers)
+        auto weights = [&](auto changed) {
+          const float scale_log2 = kForm == kPlain || (kForm == kSloped && !changed) ? to_log2 : 1.f;
 #pragma unroll 1
-        for (int i = 0; i < 4; i += 2) {
+          for (int i = 0; i < 4; i += 2) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t(&x)[32] = raw[h];
-            tmem_ld_wait();
-            if (i + h < 3) tmem_ld_32x32b_x32(s_at + 32 * (i + h + 1), raw[h ^ 1]);
-            uint32_t packed[16];
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t(&x)[32] = raw[h];
+              tmem_ld_wait();
+              if (i + h < 3) tmem_ld_32x32b_x32(s_at + 32 * (i + h + 1), raw[h ^ 1]);
+              const float at_i = fmaf(slope, (float)(32 * (i + h)), bias + minus);
+              uint32_t packed[16];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              float v, w;
-              fma2(v, w, __uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]), scale_log2, scale_log2, minus, minus);
-              if ((j & 7) < kPolyOfEight) {
-                exp2_poly(v, w);
-              } else {
-                v = exp2_approx(v);
-                w = exp2_approx(w);
+              for (int j = 0; j < 16; ++j) {
+                float v = __uint_as_float(x[2 * j]), w = __uint_as_float(x[2 * j + 1]);
+                if (kForm == kSloped && !changed) {
+                  float bv, bw;
+                  fma2(bv, bw, (float)(2 * j), (float)(2 * j + 1), slope, slope, at_i, at_i);
+                  fma2(v, w, v, w, scale_log2, scale_log2, bv, bw);
+                } else if (kForm == kCapped && !changed) {
+                  cap.small(v, w);
+                  add2(v, w, minus, minus);
+                } else if (kForm == kPlain) {
+                  fma2(v, w, v, w, scale_log2, scale_log2, minus, minus);
+                } else {
+                  add2(v, w, minus, minus);
+                }
+                if ((j & 7) < kPolyOfEight) {
+                  exp2_poly(v, w);
+                } else {
+                  v = exp2_approx(v);
+                  w = exp2_approx(w);
+                }
+                add2(l[2 * (j & 1)], l[2 * (j & 1) + 1], v, w);
+                packed[j] = pack2(T(), v, w);
               }
-              add2(l[2 * (j & 1)], l[2 * (j & 1) + 1], v, w);
-              packed[j] = pack2(T(), v, w);
+              tmem_st_32x32b_x16(s_at + 16 * (i + h), packed);
             }
-            tmem_st_32x32b_x16(s_at + 16 * (i + h), packed);
           }
-        }
+        };
+        if (kForm == kPlain || direct) weights(std::false_type());
+        else weights(std::true_type());
         tmem_st_wait();
         tc_fence_before_sync();
         __syncwarp();
@@ -748,10 +927,12 @@ int launch_paged_prompt(const char* who, const B200PagedCache* c, PagedAttnParam
     if ((rc = make_tmap(v ? &p.tm_v : &p.tm_k, type, 4, v ? c->v_pages : c->k_pages, d, s, b, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
   }
   a.slots = sm_count();
+  p.per_pair = ((1ull << 40) + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
+  p.next = a.arrived + kCutTiles;
   p.a = a;
-  // pairs of tiles of all sequences, at most, and as many chunks more as there are slots
+  // pairs of tiles of all sequences, at most, and their chunks
   const int64_t pairs = (c->tokens + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens) + c->batch;
-  const int64_t most = pairs * c->kv_heads + a.slots;
+  const int64_t most = pairs * c->kv_heads + (int64_t)kPartsOfSlots * a.slots;
   if (most > 0x3fffffffLL) return fail(B200_EINVAL, "%s: too many rows", who);
   auto launch = [&](auto kern, size_t bytes, SmemLimit& limit, std::atomic<int>& regs) {
     const size_t smem = bytes + 1024;
@@ -766,7 +947,7 @@ int launch_paged_prompt(const char* who, const B200PagedCache* c, PagedAttnParam
     if (regs.load(std::memory_order_relaxed) < kLaunchRegs)
       return fail(B200_ELAUNCH, "%s: built with %d registers a thread, %d are needed", who, regs.load(), kLaunchRegs);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(most < a.slots ? most : a.slots));
+    cfg.gridDim = dim3((unsigned)a.slots);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -780,14 +961,15 @@ int launch_paged_prompt(const char* who, const B200PagedCache* c, PagedAttnParam
     count_launch();
     return B200_OK;
   };
-  const bool extra = a.cap > 0.f || a.slopes || !(a.scale > 0.f);
+  const int form = !(a.scale > 0.f) || (a.cap > 0.f && a.slopes) ? kGeneral : a.cap > 0.f ? kCapped : a.slopes ? kSloped : kPlain;
   auto by_form = [&](auto type_, auto dim) {
     using T = decltype(type_);
     constexpr int N = decltype(dim)::value;
-    static SmemLimit limit[2];
-    static std::atomic<int> regs[2];
-    return extra ? launch(paged_prompt_kernel<T, N, true>, sizeof(Smem<N>), limit[1], regs[1])
-                 : launch(paged_prompt_kernel<T, N, false>, sizeof(Smem<N>), limit[0], regs[0]);
+    static SmemLimit limit[4];
+    static std::atomic<int> regs[4];
+    auto kern = form == kPlain ? paged_prompt_kernel<T, N, kPlain> : form == kCapped ? paged_prompt_kernel<T, N, kCapped>
+              : form == kSloped ? paged_prompt_kernel<T, N, kSloped> : paged_prompt_kernel<T, N, kGeneral>;
+    return launch(kern, sizeof(Smem<N>), limit[form], regs[form]);
   };
   auto by_dim = [&](auto type_) {
     return c->head_dim == 128 ? by_form(type_, std::integral_constant<int, 128>()) : by_form(type_, std::integral_constant<int, 64>());

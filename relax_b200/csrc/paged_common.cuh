@@ -161,6 +161,11 @@ __device__ __forceinline__ bool find_item(const PagedAttnParams& p, int index, i
   return false;
 }
 
+// Scratch memory: counters of cut tiles, two more of the many-rows kernel's, and partial results.  Partial results of the many-rows kernel are 256
+// rows; of its items at most so many times as there are slots are cut.
+constexpr int kCutTiles = 2048, kPartsOfSlots = 4;
+static_assert((kCutTiles + 2) * 4 <= B200_PAGED_ZEROED_BYTES, "the counters");
+
 // The kernel for many rows (paged_attn_prompt.cu).
 int launch_paged_prompt(const char* who, const B200PagedCache* c, PagedAttnParams p, cudaStream_t stream);
 
