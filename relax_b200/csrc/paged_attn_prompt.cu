@@ -56,6 +56,7 @@ struct Work {
 // heads; a sequence of many blocks may have its pairs cut into chunks.  CTAs take the next one from a counter.
 struct Plan {
   int c;                                       // a sequence of more blocks than this is cut
+  int level, behind;                           // the blocks of the last item's pair (at first the most there are), and how many chunks have more
   struct Seq {
     int base, rows, most, first;               // position of the first row, rows, blocks of the last pair; first row
   };
@@ -99,6 +100,8 @@ struct Plan {
     __syncwarp();
     total = warp_sum64(total) * a.c.kv_heads / 2;
     longest = __reduce_max_sync(0xffffffffu, longest);
+    level = longest;
+    behind = 0;
     if (a.c.batch > kKept) {                   // (looking at all ways would take longer than it saves)
       const int share = (int)((total + a.slots - 1) / a.slots);
       if (longest > 2 * share) c = max(share, 8);
@@ -124,43 +127,50 @@ struct Plan {
     const int best = __reduce_min_sync(0xffffffffu, cost);
     c = __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, cost == best)) - 1);
   }
-  // Item `index` into w; w.b stays -1 where there is none.
-  __device__ __forceinline__ void find(const PromptParams& p, int index, int lane, Work& w) const {
+  // Item `index`, which is larger than the one before, into w; w.b stays -1 where there is none.
+  __device__ __forceinline__ void find(const PromptParams& p, int index, int lane, Work& w) {
     const PagedAttnParams& a = p.a;
     const int h = index % a.c.kv_heads, rank = index / a.c.kv_heads;
-    // the largest x such that more than `rank` chunks belong to pairs with x blocks or more
-    int x = 0, above = (int)((int64_t)a.c.table_width << a.c.page_log2) / kBlock + 2, in = rank;
-#pragma unroll 1
-    while (above - x > 1) {
-      const int mid = (x + above) >> 1;
+    // the largest x such that more than `rank` chunks belong to pairs with x blocks or more; ranks only grow, so it only falls: from the last
+    // one downwards in growing steps, then between
+    auto count = [&](int at) {
       int n = 0;
 #pragma unroll 1
       for (int b = lane; b < a.c.batch; b += 32) {
         const Seq q = sequence(p, b);
-        n += at_least(p, q, mid) * chunks(q);
+        n += at_least(p, q, at) * chunks(q);
       }
-      n = (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
+      return (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
+    };
+    int x = 0, above = level + 1, step = 1;
+#pragma unroll 1
+    while (above - x > 1) {
+      const int mid = x > 0 || step > above ? (x + above) >> 1 : max(above - step, 1);
+      const int n = count(mid);
+      step *= 2;
       if (n > rank) {
         x = mid;
       } else {
         above = mid;
-        in = rank - n;
+        behind = n;
       }
     }
     if (x == 0) return;
+    level = x;
+    int in = rank - behind;
 #pragma unroll 1
     for (int b0 = 0;; b0 += 32) {              // (ends: there are more than `in` of them)
       Seq q = {};
-      int level = 0;
+      int here = 0;
       if (b0 + lane < a.c.batch) {
         q = sequence(p, b0 + lane);
-        level = (at_least(p, q, x) - at_least(p, q, x + 1)) * chunks(q);
+        here = (at_least(p, q, x) - at_least(p, q, x + 1)) * chunks(q);
       }
-      const int upto = warp_scan(level, lane);
+      const int upto = warp_scan(here, lane);
       const unsigned hit = __ballot_sync(0xffffffffu, upto > in);
       if (hit) {
         const int l = __ffs(hit) - 1;
-        in -= __shfl_sync(0xffffffffu, upto - level, l);
+        in -= __shfl_sync(0xffffffffu, upto - here, l);
         w.b = b0 + l;
         break;
       }
@@ -227,7 +237,7 @@ struct Smem {
   unsigned char ring[kStages][kBlockBytes];
   uint64_t q_full, q_empty;
   uint64_t full[kStages], empty[kStages], ready[kReady];
-  uint64_t s_full[2], p_ready[2], o_full[2], o_empty[2];
+  uint64_t s_full[2], p_ready[2][2], o_full[2], o_empty[2];       // [tile][half of a block]
   uint64_t work_full[kWorks], work_empty[kWorks], issued;
   Work work[kWorks];
   uint32_t tmem_base;
@@ -362,9 +372,8 @@ __device__ __forceinline__ void mul2(float& x, float& y, float ax, float ay) {
 // cap * tanh(scale * x / cap) in the exponent of 2, of two scores.  Small: |scale * x / cap| <= 0.4, where tanh's Taylor series to the
 // ninth power is 1e-6 off; nearly all scores are, and the other form takes two special functions for each.
 struct Cap {
-  float per_cap, to_log2, twice_log2, cap_log2;
-  __device__ __forceinline__ Cap(float scale, float cap)
-      : per_cap(cap > 0.f ? scale / cap : 0.f), to_log2(scale * kLog2e), twice_log2(2.f * per_cap * kLog2e), cap_log2(cap * kLog2e) {}
+  float per_cap, to_log2;
+  __device__ __forceinline__ Cap(float scale, float cap) : per_cap(cap > 0.f ? scale / cap : 0.f), to_log2(scale * kLog2e) {}
   __device__ __forceinline__ void small(float& x, float& y) const {
     float u = x, v = y;
     mul2(u, v, per_cap, per_cap);
@@ -377,7 +386,9 @@ struct Cap {
     mul2(x, y, to_log2, to_log2);
     mul2(x, y, pu, pv);
   }
-  __device__ __forceinline__ float any(float x) const { return cap_log2 * (1.f - __fdividef(2.f, exp2_approx(x * twice_log2) + 1.f)); }
+  __device__ __forceinline__ float any(float x, float cap) const {
+    return cap * kLog2e * (1.f - __fdividef(2.f, exp2_approx(x * (2.f * kLog2e * per_cap)) + 1.f));
+  }
 };
 
 template <typename T, int D, int kForm>
@@ -400,7 +411,8 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
     for (int i = 0; i < kReady; ++i) mbar_init(&sm.ready[i], 1);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sm.s_full[t], 1);
-      mbar_init(&sm.p_ready[t], 4);
+      mbar_init(&sm.p_ready[t][0], 4);
+      mbar_init(&sm.p_ready[t][1], 4);
       mbar_init(&sm.o_full[t], 1);
       mbar_init(&sm.o_empty[t], 4);
     }
@@ -523,18 +535,18 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         for (int t = 0; t < 2; ++t) {
           if (ok && sees[t](u)) {
             if (!begun[t] && n_o[t] > 0) ok = wait(&sm.o_empty[t], (n_o[t] - 1) & 1, abort_flag, 7);
-            ok = ok && wait(&sm.p_ready[t], n_p[t] & 1, abort_flag, 8);
-            if (ok) {
-              ++n_p[t];
-              tc_fence_after_sync();
 #pragma unroll
-              for (int k = 0; k < 2; ++k)
-                mma4_ts(tmem + 256 + t * D, tmem + t * 128 + 32 * k, dv + (uint64_t)(vslot * kStep) + k * 512, kIdescO, begun[t] || k > 0);
-              begun[t] = true;
-              if (u == last[t]) {
-                umma_commit(&sm.o_full[t]);
-                ++n_o[t];
-              }
+            for (int h = 0; h < 2; ++h) {         // (the first half's products run beside the second half's weights)
+              ok = ok && wait(&sm.p_ready[t][h], n_p[t] & 1, abort_flag, 8);
+              if (!ok) break;
+              tc_fence_after_sync();
+              mma4_ts(tmem + 256 + t * D, tmem + t * 128 + 32 * h, dv + (uint64_t)(vslot * kStep) + h * 512, kIdescO, begun[t] || h > 0);
+            }
+            begun[t] = true;
+            ++n_p[t];
+            if (ok && u == last[t]) {
+              umma_commit(&sm.o_full[t]);
+              ++n_o[t];
             }
           }
           if (ok && more && sees[t](u + 1)) {
@@ -580,16 +592,18 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
     }
   } else {
     // ---------------------------------------------------------------------- the work, longest tiles first
-    const Plan plan(p, lane, sm.kept);
+    Plan plan(p, lane, sm.kept);
     for (uint32_t i = 0;; ++i) {
       const uint32_t slot = i % kWorks, round = i / kWorks;
       if (round > 0 && !wait_relaxed(&sm.work_empty[slot], (round - 1) & 1, abort_flag, 11)) break;
       // the next item is taken when this one's loads are all on their way, two or three blocks before its end: taken earlier, the CTA with
       // the longest item would get one of the second longest too
       if (i > 0 && !wait_relaxed(&sm.issued, (i - 1) & 1, abort_flag, 15)) break;
-      int index = 0;
-      if (lane == 0) index = atomicAdd(p.next, 1);
-      index = __shfl_sync(0xffffffffu, index, 0);
+      int index = blockIdx.x;
+      if (i > 0) {
+        if (lane == 0) index = gridDim.x + atomicAdd(p.next, 1);
+        index = __shfl_sync(0xffffffffu, index, 0);
+      }
       Work w;
       w.b = -1;
       plan.find(p, index, lane, w);
@@ -684,7 +698,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
           top = all_tops();
           if (kForm == kCapped) {
             direct = __all_sync(0xffffffffu, fmaxf(fabsf(top), fabsf(fminf(lows[0], lows[1]))) * cap.per_cap <= 0.4f);
-            top = cap.any(top);
+            top = cap.any(top, a.cap);
           } else if (kForm == kPlain) {
             top *= to_log2;
           }
@@ -703,7 +717,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
             tmem_ld_wait();
             if (kForm == kCapped || (kForm == kGeneral && a.cap > 0.f)) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(cap.any(__uint_as_float(x[j])));
+              for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(cap.any(__uint_as_float(x[j]), a.cap));
             } else if (kForm != kPlain) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * to_log2);
@@ -786,14 +800,14 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
               }
               tmem_st_32x32b_x16(s_at + 16 * (i + h), packed);
             }
+            tmem_st_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.p_ready[t][i >> 1]);
           }
         };
         if (kForm == kPlain || direct) weights(std::false_type());
         else weights(std::true_type());
-        tmem_st_wait();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.p_ready[t]);
       }
       if (!ok) break;
       // ---- the tile's result -------------------------------------------------------------------------------------------------
@@ -807,21 +821,26 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       if (w.chunks == 1) {
         const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
         T* out = static_cast<T*>(a.out) + ((int64_t)(w.first + token) * a.heads + head) * D;
+        const bool some = any && sum != 0.f;
+        uint32_t o[2][16];
+        if (any) tmem_ld_32x32b_x16(o_at, o[0]);
 #pragma unroll 1
-        for (int i = 0; i < D / 16; ++i) {
-          uint32_t o[16];
-          if (any) {
-            tmem_ld_32x32b_x16(o_at + 16 * i, o);
-            tmem_ld_wait();
-          }
-          if (mine) {
+        for (int i = 0; i < D / 16; i += 2) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              uint32_t v[4];
+          for (int h = 0; h < 2; ++h) {
+            if (any) {
+              tmem_ld_wait();
+              if (i + h + 1 < D / 16) tmem_ld_32x32b_x16(o_at + 16 * (i + h + 1), o[h ^ 1]);
+            }
+            if (mine) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                v[k] = any && sum != 0.f ? pack2(T(), __uint_as_float(o[8 * j + 2 * k]) * inv, __uint_as_float(o[8 * j + 2 * k + 1]) * inv) : 0u;
-              reinterpret_cast<uint4*>(out)[2 * i + j] = make_uint4(v[0], v[1], v[2], v[3]);
+              for (int j = 0; j < 2; ++j) {
+                uint32_t v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  v[k] = some ? pack2(T(), __uint_as_float(o[h][8 * j + 2 * k]) * inv, __uint_as_float(o[h][8 * j + 2 * k + 1]) * inv) : 0u;
+                reinterpret_cast<uint4*>(out)[2 * (i + h) + j] = make_uint4(v[0], v[1], v[2], v[3]);
+              }
             }
           }
         }
