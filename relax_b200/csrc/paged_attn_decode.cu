@@ -23,6 +23,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kUnit = 16;
+constexpr int kCtasPerSm1 = 3, kCtasPerSm2 = 2;       // of tiles of 8 rows, of 16
 __device__ __forceinline__ void mma(__half, float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -44,297 +45,407 @@ __device__ __forceinline__ uint4 load16(const void* p) {
   return v;
 }
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+// A tile's part of a warp that is not the whole tile.
+struct Piece {
+  int64_t first;                                // the tile's first unit, counted over everything
+  int b, tile, h, units;                        // units < 0: no piece
+};
+
 template <typename T, int D, int NT, bool kExtra>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kCtasPerSm1 : kCtasPerSm2)
 paged_decode_kernel(const PagedAttnParams p) {
   constexpr int R = 8 * NT;                     // rows of a tile
   constexpr int SUB = 128 / D;                  // units a warp takes at a time
   constexpr int KC = D / 32, VC = D / 64, MT = D / 16;
-  __shared__ __align__(16) float sm_o[kWarps][R][D + 4];
-  __shared__ float sm_m[kWarps][R], sm_l[kWarps][R];
+  constexpr int kPitch = D + 4;
+  extern __shared__ __align__(16) float sm_o[];           // [2 kWarps][R][kPitch]: a warp's first piece and its last
+  __shared__ float sm_m[2 * kWarps][R], sm_l[2 * kWarps][R];
+  __shared__ Piece sm_piece[2 * kWarps];
   __shared__ int sm_last;
   ptx::pdl_wait();
   ptx::pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int h = blockIdx.x % p.c.kv_heads, index = blockIdx.x / p.c.kv_heads;
+  const int kv = p.c.kv_heads;
+  auto tiles_of = [&](const Sequence& x) { return (x.rows * p.group + R - 1) / R; };
 
-  // ---- which tile and chunk: c units a chunk fill the slots once, in whole trips of the CTA's warps -----------------------
-  Item item;
-  {
-    auto tiles_of = [&](const Sequence& x) { return (x.rows * p.group + R - 1) / R; };
-    constexpr int kStep = kWarps * SUB;
-    const int64_t even = (total_units<kUnit>(p, lane, tiles_of) + p.slots - 1) / p.slots;
-    const int c = (int)((max(even, (int64_t)1) + kStep - 1) / kStep) * kStep;
-    if (!find_item<kUnit>(p, index, c, lane, tiles_of, item)) return;       // (the grid is a bound)
+  // ---- the units of all sequences, in the order sequence, tile, key head, unit; every warp gets an equal part of them ----------
+  auto units_of = [&](int i, int& per_tile) {
+    const Sequence x = sequence_of(p.c, i);
+    const int tiles = tiles_of(x);
+    Range<kUnit> r;
+    r.set(p, x, i, 0, x.rows - 1);
+    per_tile = tiles > 0 ? max(r.units, 1) : 0;           // (rows that see nothing have a result too)
+    return (int64_t)per_tile * tiles * kv;
+  };
+  int64_t mine = 0;
+  int per_tile0 = 0;                            // of sequence `lane`
+  int64_t units0 = 0;
+#pragma unroll 1
+  for (int i = lane; i < p.c.batch; i += 32) {
+    int u;
+    const int64_t n = units_of(i, u);
+    if (i == lane) { per_tile0 = u; units0 = n; }
+    mine += n;
   }
-  const int b = item.b, chunk = item.chunk, chunks = item.chunks;
-  const Sequence s = sequence_of(p.c, b);
-  const int rows = s.rows * p.group, row0 = item.tile * R, nrows = min(rows - row0, R);
-  const int token0 = row0 / p.group, token1 = (row0 + nrows - 1) / p.group;
-  const int base = s.length - s.rows;
-  Range<kUnit> range;
-  range.set(p, s, b, token0, token1);
-  const int u_begin = (int)((int64_t)range.units * chunk / chunks), u_end = (int)((int64_t)range.units * (chunk + 1) / chunks);
+  const int64_t total = warp_sum64(mine);
+  const int active = (int)min(max(total / kWarps, (int64_t)1), (int64_t)gridDim.x), warps = active * kWarps;
+  if ((int)blockIdx.x >= active) return;
+  const bool small = total * warps <= 0xffffffffLL;       // (a 32-bit division is a good deal shorter)
+  auto share = [&](int i) { return small ? (int64_t)((unsigned)total * (unsigned)i / (unsigned)warps) : total * i / warps; };
+  int64_t at = share(blockIdx.x * kWarps + warp);
+  const int64_t end = share(blockIdx.x * kWarps + warp + 1);
+  if (lane == 0) sm_piece[2 * warp].units = sm_piece[2 * warp + 1].units = -1;
 
-  // ---- queries: the B operand's row g of a tile of eight -----------------------------------------------------------------
-  uint4 qf[NT][KC];
+  // the sequence of unit `at`, and how many units lie before it
+  int b = 0, per_tile = 0;
+  int64_t before = 0, seq_units = 0;
+  if (at < end) {
+#pragma unroll 1
+    for (int base = 0; base < p.c.batch; base += 32) {
+      int u = per_tile0;
+      int64_t n = units0;
+      if (base > 0) {
+        n = 0;
+        if (base + lane < p.c.batch) n = units_of(base + lane, u);
+      }
+      int64_t upto = n;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int r = row0 + 8 * n + g;
-    const T* src = static_cast<const T*>(p.q) + (int64_t)(s.first + r / p.group) * p.q_stride + (int64_t)(h * p.group + r % p.group) * D;
-#pragma unroll
-    for (int j = 0; j < KC; ++j) qf[n][j] = 8 * n + g < nrows ? load16(src + 32 * j + 8 * t) : make_uint4(0, 0, 0, 0);
-  }
-  // this lane's rows in the accumulators: 8 n + 2 t + e
-  int position[NT][2];
-  float slope[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = row0 + 8 * n + 2 * t + e;
-      position[n][e] = r < rows ? base + r / p.group : -1;
-      slope[n][e] = kExtra && p.slopes && r < rows ? p.slopes[h * p.group + r % p.group] * kLog2e : 0.f;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + upto > at);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        b = base + l;
+        before += __shfl_sync(0xffffffffu, upto - n, l);
+        seq_units = __shfl_sync(0xffffffffu, n, l);
+        per_tile = __shfl_sync(0xffffffffu, u, l);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
     }
-  const int position0 = base + token0, position1 = base + token1;
+  }
+  const int page = 1 << p.c.page_log2;
   const int window = p.window ? p.window : 0x7fffffff;
   const float to_log2 = p.scale * kLog2e;
   const float cap_in = kExtra && p.cap > 0.f ? 2.f * p.scale / p.cap * kLog2e : 0.f, cap_log2 = p.cap * kLog2e;
 
-  const int page = 1 << p.c.page_log2;
-  const T* kbase = static_cast<const T*>(p.c.k) + (int64_t)h * page * D + 8 * t;
-  const T* vbase = static_cast<const T*>(p.c.v) + (int64_t)h * page * D + 8 * g;
-  // units of step i of this warp; past the end the last one stands in and is masked
-  auto unit_at = [&](int i, int sub) { return range.unit(min(u_begin + i * SUB + sub, u_end - 1)); };
-  auto page_at = [&](int i, int sub) { return page_of(p.c, b, unit_at(i, sub) >> (p.c.page_log2 - 4)); };
-  uint4 kr[SUB][2][KC], vr[SUB][4][VC];
-  auto load_k = [&](int i, const int (&id)[SUB]) {
-#pragma unroll
-    for (int x = 0; x < SUB; ++x) {
-      const T* src = kbase + id[x] * p.c.k_stride + (int64_t)((unit_at(i, x) * kUnit) & (page - 1)) * D;
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int j = 0; j < KC; ++j) kr[x][r][j] = load16(src + (g + 8 * r) * D + 32 * j);
-    }
-  };
-  auto load_v = [&](int i, const int (&id)[SUB]) {
-#pragma unroll
-    for (int x = 0; x < SUB; ++x) {
-      const T* src = vbase + id[x] * p.c.v_stride + (int64_t)((unit_at(i, x) * kUnit) & (page - 1)) * D;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int j = 0; j < VC; ++j) vr[x][r][j] = load16(src + (2 * t + (r & 1) + 8 * (r >> 1)) * D + 64 * j);
-    }
-  };
+  int pieces = 0;
+  while (at < end) {
+    // ---- a part of one tile: units [u_begin, u_end) of per_tile ---------------------------------------------------------------
+    const Sequence s = sequence_of(p.c, b);
+    const int in_seq = (int)(at - before), index = in_seq / per_tile, u_begin = in_seq - index * per_tile;
+    const int u_end = (int)min((int64_t)per_tile, u_begin + (end - at));
+    const int tile = index / kv, h = index - tile * kv;
+    const int rows = s.rows * p.group, row0 = tile * R, nrows = min(rows - row0, R);
+    const int base = s.length - s.rows;
+    const int position0 = base + row0 / p.group, position1 = base + (row0 + nrows - 1) / p.group;
+    Range<kUnit> range;
+    range.set(p, s, b, 0, s.rows - 1);
 
-  float m[NT][2], l[NT][2], acc[NT][MT][4];
+    const T* kbase = static_cast<const T*>(p.c.k) + (int64_t)h * page * D + 8 * t;
+    const T* vbase = static_cast<const T*>(p.c.v) + (int64_t)h * page * D + 8 * g;
+    // units of step i; past the end the last one stands in and is masked
+    auto unit_at = [&](int i, int sub) { return range.unit(min(u_begin + i * SUB + sub, u_end - 1)); };
+    auto page_at = [&](int i, int sub) { return page_of(p.c, b, unit_at(i, sub) >> (p.c.page_log2 - 4)); };
+    uint4 kr[SUB][2][KC], vr[SUB][4][VC];
+    auto load_k = [&](int i, const int (&id)[SUB]) {
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
+      for (int x = 0; x < SUB; ++x) {
+        const T* src = kbase + id[x] * p.c.k_stride + (int64_t)((unit_at(i, x) * kUnit) & (page - 1)) * D;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) { m[n][e] = -INFINITY; l[n][e] = 0.f; }
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[n][i][j] = 0.f;
-  }
-
-  const int steps = (u_end - u_begin + SUB - 1) / SUB;
-  int id[SUB], id_next[SUB];
-  if (warp < steps) {
-#pragma unroll
-    for (int x = 0; x < SUB; ++x) id[x] = page_at(warp, x);
-    load_k(warp, id);
-    load_v(warp, id);
-#pragma unroll
-    for (int x = 0; x < SUB; ++x) id[x] = warp + kWarps < steps ? page_at(warp + kWarps, x) : 0;
-  }
-  for (int i = warp; i < steps; i += kWarps) {
-    const bool more = i + kWarps < steps;
-#pragma unroll
-    for (int x = 0; x < SUB; ++x) id_next[x] = i + 2 * kWarps < steps ? page_at(i + 2 * kWarps, x) : 0;
-    // scores of tokens g (0, 1) and g + 8 (2, 3), rows 2 t (0, 2) and 2 t + 1 (1, 3)
-    float sc[SUB][NT][4];
-#pragma unroll
-    for (int x = 0; x < SUB; ++x)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sc[x][n][j] = 0.f;
-#pragma unroll
-        for (int j = 0; j < KC; ++j) {
-          mma(T(), sc[x][n], kr[x][0][j].x, kr[x][1][j].x, kr[x][0][j].y, kr[x][1][j].y, qf[n][j].x, qf[n][j].y);
-          mma(T(), sc[x][n], kr[x][0][j].z, kr[x][1][j].z, kr[x][0][j].w, kr[x][1][j].w, qf[n][j].z, qf[n][j].w);
-        }
+          for (int j = 0; j < KC; ++j) kr[x][r][j] = load16(src + (g + 8 * r) * D + 32 * j);
       }
-    if (more) load_k(i + kWarps, id);
-    bool above = false;
+    };
+    auto load_v = [&](int i, const int (&id)[SUB]) {
 #pragma unroll
-    for (int x = 0; x < SUB; ++x) {
-      const int first = unit_at(i, x) * kUnit;
-      const bool there = u_begin + i * SUB + x < u_end;
-      // every row sees the whole unit (rows past the tile's end come out as something finite that nobody stores)
-      const bool whole = there && position0 >= 0 &&
-                         (first + kUnit <= range.pre || (first + kUnit - 1 <= position0 && position1 - first < window));
+      for (int x = 0; x < SUB; ++x) {
+        const T* src = vbase + id[x] * p.c.v_stride + (int64_t)((unit_at(i, x) * kUnit) & (page - 1)) * D;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int token = first + g + 8 * (j >> 1), at = position[n][j & 1];
-          float v = sc[x][n][j];
-          if (kExtra && p.cap > 0.f) v = cap_log2 * (1.f - __fdividef(2.f, exp2_approx(v * cap_in) + 1.f));
-          else v *= to_log2;
-          if (kExtra) v -= slope[n][j & 1] * fabsf((float)(at - token));
-          if (!whole) {
-            const bool seen = there && at >= 0 && (token < range.pre || (token <= at && at - token < window));
-            if (!seen) v = -INFINITY;
+          for (int j = 0; j < VC; ++j) vr[x][r][j] = load16(src + (2 * t + (r & 1) + 8 * (r >> 1)) * D + 64 * j);
+      }
+    };
+    const int steps = (u_end - u_begin + SUB - 1) / SUB;
+    int id[SUB];
+#pragma unroll
+    for (int x = 0; x < SUB; ++x) id[x] = page_at(0, x);
+    // queries: the B operand's row g of a tile of eight
+    uint4 qf[NT][KC];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = row0 + 8 * n + g;
+      const T* src = static_cast<const T*>(p.q) + (int64_t)(s.first + r / p.group) * p.q_stride + (int64_t)(h * p.group + r % p.group) * D;
+#pragma unroll
+      for (int j = 0; j < KC; ++j) qf[n][j] = 8 * n + g < nrows ? load16(src + 32 * j + 8 * t) : make_uint4(0, 0, 0, 0);
+    }
+    load_k(0, id);
+    load_v(0, id);
+#pragma unroll
+    for (int x = 0; x < SUB; ++x) id[x] = 1 < steps ? page_at(1, x) : 0;
+    // this lane's rows in the accumulators: 8 n + 2 t + e
+    int position[NT][2];
+    float slope[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = row0 + 8 * n + 2 * t + e;
+        position[n][e] = r < rows ? base + r / p.group : -1;
+        slope[n][e] = kExtra && p.slopes && r < rows ? p.slopes[h * p.group + r % p.group] * kLog2e : 0.f;
+      }
+    float m[NT][2], l[NT][2], acc[NT][MT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) { m[n][e] = -INFINITY; l[n][e] = 0.f; }
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[n][i][j] = 0.f;
+    }
+#pragma unroll 1
+    for (int i = 0; i < steps; ++i) {
+      const bool more = i + 1 < steps;
+      int id_next[SUB];
+#pragma unroll
+      for (int x = 0; x < SUB; ++x) id_next[x] = i + 2 < steps ? page_at(i + 2, x) : 0;
+      // scores of tokens g (0, 1) and g + 8 (2, 3), rows 2 t (0, 2) and 2 t + 1 (1, 3)
+      float sc[SUB][NT][4];
+#pragma unroll
+      for (int x = 0; x < SUB; ++x)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[x][n][j] = 0.f;
+#pragma unroll
+          for (int j = 0; j < KC; ++j) {
+            mma(T(), sc[x][n], kr[x][0][j].x, kr[x][1][j].x, kr[x][0][j].y, kr[x][1][j].y, qf[n][j].x, qf[n][j].y);
+            mma(T(), sc[x][n], kr[x][0][j].z, kr[x][1][j].z, kr[x][0][j].w, kr[x][1][j].w, qf[n][j].z, qf[n][j].w);
           }
-          sc[x][n][j] = v;
-          above |= v > m[n][j & 1] + kSlack;
         }
-      if (!whole) {                             // what nobody sees may be anything, and 0 * NaN is NaN
+      if (more) load_k(i + 1, id);
+      bool above = false;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int token = first + 2 * t + (r & 1) + 8 * (r >> 1);
-          if (!(there && (token < range.pre || (token >= range.low && token < range.high))))
+      for (int x = 0; x < SUB; ++x) {
+        const int first = unit_at(i, x) * kUnit;
+        const bool there = u_begin + i * SUB + x < u_end;
+        // every row sees the whole unit (rows past the tile's end come out as something finite that nobody stores)
+        const bool whole = there && position0 >= 0 &&
+                           (first + kUnit <= range.pre || (first + kUnit - 1 <= position0 && position1 - first < window));
 #pragma unroll
-            for (int j = 0; j < VC; ++j) vr[x][r][j] = make_uint4(0, 0, 0, 0);
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int token = first + g + 8 * (j >> 1), at = position[n][j & 1];
+            float v = sc[x][n][j];
+            if (kExtra && p.cap > 0.f) v = cap_log2 * (1.f - __fdividef(2.f, exp2_approx(v * cap_in) + 1.f));
+            else v *= to_log2;
+            if (kExtra) v -= slope[n][j & 1] * fabsf((float)(at - token));
+            if (!whole) {
+              const bool seen = there && at >= 0 && (token < range.pre || (token <= at && at - token < window));
+              if (!seen) v = -INFINITY;
+            }
+            sc[x][n][j] = v;
+            above |= v > m[n][j & 1] + kSlack;
+          }
+        if (!whole) {                             // what nobody sees may be anything, and 0 * NaN is NaN
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int token = first + 2 * t + (r & 1) + 8 * (r >> 1);
+            if (!(there && (token < range.pre || (token >= range.low && token < range.high))))
+#pragma unroll
+              for (int j = 0; j < VC; ++j) vr[x][r][j] = make_uint4(0, 0, 0, 0);
+          }
         }
       }
-    }
-    if (__any_sync(0xffffffffu, above)) {
+      if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float v = m[n][e];
+          for (int e = 0; e < 2; ++e) {
+            float v = m[n][e];
 #pragma unroll
-          for (int x = 0; x < SUB; ++x) v = fmaxf(v, fmaxf(sc[x][n][e], sc[x][n][e + 2]));
+            for (int x = 0; x < SUB; ++x) v = fmaxf(v, fmaxf(sc[x][n][e], sc[x][n][e + 2]));
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-          const float f = v == -INFINITY ? 1.f : exp2_approx(m[n][e] - v);
-          m[n][e] = v;
-          l[n][e] *= f;
+            for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+            const float f = v == -INFINITY ? 1.f : exp2_approx(m[n][e] - v);
+            m[n][e] = v;
+            l[n][e] *= f;
 #pragma unroll
-          for (int k = 0; k < MT; ++k) { acc[n][k][e] *= f; acc[n][k][e + 2] *= f; }
-        }
-    }
-#pragma unroll
-    for (int x = 0; x < SUB; ++x) {
-      uint32_t pb[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          w[j] = sc[x][n][j] == -INFINITY ? 0.f : exp2_approx(sc[x][n][j] - m[n][j & 1]);
-          l[n][j & 1] += w[j];
-        }
-        pb[n][0] = transpose8x8(pack2(T(), w[0], w[1]));
-        pb[n][1] = transpose8x8(pack2(T(), w[2], w[3]));
+            for (int k = 0; k < MT; ++k) { acc[n][k][e] *= f; acc[n][k][e + 2] *= f; }
+          }
       }
 #pragma unroll
-      for (int k = 0; k < MT; ++k) {
-        // row g of the tile: dim 8 g + k, row g + 8: dim 64 + 8 g + k (head_dim 64: 8 g + 4 + k)
-        const int k1 = D == 128 ? k : k + 4, j1 = VC - 1;
-        const unsigned s0 = k & 1 ? 0x7632 : 0x5410, s1 = k1 & 1 ? 0x7632 : 0x5410;
-        const uint32_t a0 = __byte_perm(word(vr[x][0][0], k / 2), word(vr[x][1][0], k / 2), s0);
-        const uint32_t a1 = __byte_perm(word(vr[x][0][j1], k1 / 2), word(vr[x][1][j1], k1 / 2), s1);
-        const uint32_t a2 = __byte_perm(word(vr[x][2][0], k / 2), word(vr[x][3][0], k / 2), s0);
-        const uint32_t a3 = __byte_perm(word(vr[x][2][j1], k1 / 2), word(vr[x][3][j1], k1 / 2), s1);
+      for (int x = 0; x < SUB; ++x) {
+        uint32_t pb[NT][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma(T(), acc[n][k], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+        for (int n = 0; n < NT; ++n) {
+          float w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            w[j] = sc[x][n][j] == -INFINITY ? 0.f : exp2_approx(sc[x][n][j] - m[n][j & 1]);
+            l[n][j & 1] += w[j];
+          }
+          pb[n][0] = transpose8x8(pack2(T(), w[0], w[1]));
+          pb[n][1] = transpose8x8(pack2(T(), w[2], w[3]));
+        }
+#pragma unroll
+        for (int k = 0; k < MT; ++k) {
+          // row g of the tile: dim 8 g + k, row g + 8: dim 64 + 8 g + k (head_dim 64: 8 g + 4 + k)
+          const int k1 = D == 128 ? k : k + 4, j1 = VC - 1;
+          const unsigned s0 = k & 1 ? 0x7632 : 0x5410, s1 = k1 & 1 ? 0x7632 : 0x5410;
+          const uint32_t a0 = __byte_perm(word(vr[x][0][0], k / 2), word(vr[x][1][0], k / 2), s0);
+          const uint32_t a1 = __byte_perm(word(vr[x][0][j1], k1 / 2), word(vr[x][1][j1], k1 / 2), s1);
+          const uint32_t a2 = __byte_perm(word(vr[x][2][0], k / 2), word(vr[x][3][0], k / 2), s0);
+          const uint32_t a3 = __byte_perm(word(vr[x][2][j1], k1 / 2), word(vr[x][3][j1], k1 / 2), s1);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma(T(), acc[n][k], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+        }
       }
-    }
-    if (more) load_v(i + kWarps, id);
+      if (more) load_v(i + 1, id);
 #pragma unroll
-    for (int x = 0; x < SUB; ++x) id[x] = id_next[x];
+      for (int x = 0; x < SUB; ++x) id[x] = id_next[x];
+    }
+    // ---- the warp's rows: a whole tile goes out, a part of one to shared memory -------------------------------------------------
+    const bool all = u_begin == 0 && u_end == per_tile;
+    const int slot = 2 * warp + (pieces > 0);
+    if (!all && lane == 0) sm_piece[slot] = {at - u_begin, b, tile, h, per_tile};
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o);
+        const int r = 8 * n + 2 * t + e;
+        // dims 8 g .. + 7 and 64 + 8 g .. + 7 (head_dim 64: 8 g .. + 7)
+        if (all) {
+          const float sum = l[n][e], inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;       // (NaN stays)
+          if (r < nrows) {
+            const int x = row0 + r;
+            T* out = static_cast<T*>(p.out) + ((int64_t)(s.first + x / p.group) * p.heads + h * p.group + x % p.group) * D + 8 * g;
+            uint32_t v[2][4];
+#pragma unroll
+            for (int k = 0; k < MT; k += 2) {
+              v[0][(k / 2) & 3] = pack2(T(), acc[n][k][e] * inv, acc[n][k + 1][e] * inv);
+              if (D == 128) v[1][k / 2] = pack2(T(), acc[n][k][e + 2] * inv, acc[n][k + 1][e + 2] * inv);
+              else v[0][2 + k / 2] = pack2(T(), acc[n][k][e + 2] * inv, acc[n][k + 1][e + 2] * inv);
+            }
+            *reinterpret_cast<uint4*>(out) = make_uint4(v[0][0], v[0][1], v[0][2], v[0][3]);
+            if (D == 128) *reinterpret_cast<uint4*>(out + 64) = make_uint4(v[1][0], v[1][1], v[1][2], v[1][3]);
+          }
+        } else {
+          if (g == 0) { sm_m[slot][r] = m[n][e]; sm_l[slot][r] = l[n][e]; }
+          float* to = sm_o + (slot * R + r) * kPitch;
+#pragma unroll
+          for (int k = 0; k < MT; k += 4) {
+            *reinterpret_cast<float4*>(to + 8 * g + k) = make_float4(acc[n][k][e], acc[n][k + 1][e], acc[n][k + 2][e], acc[n][k + 3][e]);
+            *reinterpret_cast<float4*>(to + (D == 128 ? 64 + 8 * g + k : 8 * g + 4 + k)) =
+                make_float4(acc[n][k][e + 2], acc[n][k + 1][e + 2], acc[n][k + 2][e + 2], acc[n][k + 3][e + 2]);
+          }
+        }
+      }
+    pieces += !all;
+    at += u_end - u_begin;
+    if (at < end && at - before == seq_units) {           // the next sequence that has rows
+      before += seq_units;
+      do {
+        ++b;
+        seq_units = units_of(b, per_tile);
+      } while (seq_units == 0);
+    }
   }
 
-  // ---- the CTA's warps ----------------------------------------------------------------------------------------------------
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o);
-      const int r = 8 * n + 2 * t + e;
-      if (g == 0) { sm_m[warp][r] = m[n][e]; sm_l[warp][r] = l[n][e]; }
-#pragma unroll
-      for (int k = 0; k < MT; k += 4) {
-        *reinterpret_cast<float4*>(&sm_o[warp][r][8 * g + k]) =
-            make_float4(acc[n][k][e], acc[n][k + 1][e], acc[n][k + 2][e], acc[n][k + 3][e]);
-        const int d1 = D == 128 ? 64 + 8 * g + k : 8 * g + 4 + k;
-        *reinterpret_cast<float4*>(&sm_o[warp][r][d1]) =
-            make_float4(acc[n][k][e + 2], acc[n][k + 1][e + 2], acc[n][k + 2][e + 2], acc[n][k + 3][e + 2]);
-      }
-    }
+  // ---- pieces of the same tile in this CTA, then those of different CTAs: the one that comes last adds them up --------------------
   __syncthreads();
   constexpr int kQuads = R * D / 4;
-  auto row_out = [&](int r) {
-    const int x = row0 + r;
-    return static_cast<T*>(p.out) + ((int64_t)(s.first + x / p.group) * p.heads + h * p.group + x % p.group) * D;
+  auto put = [&](const Piece& w, int r, int d, const float (&v)[4], float sum) {
+    const Sequence s = sequence_of(p.c, w.b);
+    const int x = w.tile * R + r;
+    if (x >= s.rows * p.group) return;
+    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+    T* out = static_cast<T*>(p.out) + ((int64_t)(s.first + x / p.group) * p.heads + w.h * p.group + x % p.group) * D + d;
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack2(T(), v[0] * inv, v[1] * inv), pack2(T(), v[2] * inv, v[3] * inv));
   };
-  auto store = [&](int r, int d, const float (&v)[4], float sum) {
-    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;       // (NaN stays)
-    if (r < nrows) *reinterpret_cast<uint2*>(row_out(r) + d) = make_uint2(pack2(T(), v[0] * inv, v[1] * inv), pack2(T(), v[2] * inv, v[3] * inv));
-  };
-  const int64_t part = (int64_t)item.cut_chunk * p.c.kv_heads + h, first_part = part - (int64_t)chunk * p.c.kv_heads;
-#pragma unroll
-  for (int q0 = 0; q0 < kQuads; q0 += kWarps * 32) {
-    const int q = q0 + threadIdx.x, r = q / (D / 4), d = (q % (D / 4)) * 4;
-    float M = -INFINITY, L = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm_m[w][r]);
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = sm_m[w][r] == -INFINITY ? 0.f : exp2_approx(sm_m[w][r] - M);
-      const float4 a = *reinterpret_cast<const float4*>(&sm_o[w][r][d]);
-      if (f == 0.f && sm_l[w][r] == 0.f) continue;
-      L += sm_l[w][r] * f;
-      v[0] += a.x * f; v[1] += a.y * f; v[2] += a.z * f; v[3] += a.w * f;
+  const int64_t cta_begin = share(blockIdx.x * kWarps), cta_end = share(blockIdx.x * kWarps + kWarps);
+  int left[2] = {-1, -1};                       // pieces' slots of tiles that other CTAs share: begun before this one, ended after it
+#pragma unroll 1
+  for (int s0 = 0; s0 < 2 * kWarps;) {
+    if (sm_piece[s0].units < 0) { ++s0; continue; }
+    const Piece w = sm_piece[s0];
+    int s1 = s0 + 1;                            // slots [s0, s1) are of this tile, or empty
+    while (s1 < 2 * kWarps && (sm_piece[s1].units < 0 || sm_piece[s1].first == w.first)) ++s1;
+    const bool whole = w.first >= cta_begin && w.first + w.units <= cta_end;
+    const int part = 2 * blockIdx.x + (w.first >= cta_begin);
+    if (!whole) left[w.first >= cta_begin] = s0;
+#pragma unroll 1
+    for (int q = threadIdx.x; q < kQuads; q += kWarps * 32) {
+      const int r = q / (D / 4), d = (q % (D / 4)) * 4;
+      float M = -INFINITY, L = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int x = s0; x < s1; ++x)
+        if (sm_piece[x].units >= 0) M = fmaxf(M, sm_m[x][r]);
+      for (int x = s0; x < s1; ++x) {
+        if (sm_piece[x].units < 0 || (sm_m[x][r] == -INFINITY && sm_l[x][r] == 0.f)) continue;
+        const float f = sm_m[x][r] == -INFINITY ? 0.f : exp2_approx(sm_m[x][r] - M);
+        const float4 o = *reinterpret_cast<const float4*>(sm_o + (x * R + r) * kPitch + d);
+        L += sm_l[x][r] * f;
+        v[0] += o.x * f; v[1] += o.y * f; v[2] += o.z * f; v[3] += o.w * f;
+      }
+      if (whole) {
+        put(w, r, d, v, L);
+      } else {
+        *reinterpret_cast<float4*>(p.partial + ((int64_t)part * R + r) * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+        if (d == 0) *reinterpret_cast<float2*>(p.partial_ml + 2 * (part * R + r)) = make_float2(M, L);
+      }
     }
-    if (chunks == 1) {
-      store(r, d, v, L);
-    } else {
-      *reinterpret_cast<float4*>(p.partial + part * (R * D) + r * D + d) = make_float4(v[0], v[1], v[2], v[3]);
-      if (d == 0) { p.partial_ml[part * 2 * R + r] = M; p.partial_ml[part * 2 * R + R + r] = L; }
-    }
+    s0 = s1;
   }
-  if (chunks == 1) return;
-
-  // ---- the chunks of a cut tile: the last CTA adds them up -------------------------------------------------------------------
+  if (left[0] < 0 && left[1] < 0) return;
   __threadfence();
-  __syncthreads();
-  int* counter = p.arrived + (int64_t)item.cut_tile * p.c.kv_heads + h;
-  if (threadIdx.x == 0) {
-    const int n = atomicAdd(counter, 1);
-    sm_last = n == chunks - 1;
-    if (sm_last) *counter = 0;                  // (as the next launch expects it)
-  }
-  __syncthreads();
-  if (!sm_last) return;
-  __threadfence();
-#pragma unroll
-  for (int q0 = 0; q0 < kQuads; q0 += kWarps * 32) {
-    const int q = q0 + threadIdx.x, r = q / (D / 4), d = (q % (D / 4)) * 4;
-    float M = -INFINITY, L = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < chunks; ++k) M = fmaxf(M, __ldcg(p.partial_ml + (first_part + (int64_t)k * p.c.kv_heads) * 2 * R + r));
-    for (int k = 0; k < chunks; ++k) {
-      const int64_t x = first_part + (int64_t)k * p.c.kv_heads;
-      const float mk = __ldcg(p.partial_ml + x * 2 * R + r), lk = __ldcg(p.partial_ml + x * 2 * R + R + r);
-      const float f = mk == -INFINITY ? 0.f : exp2_approx(mk - M);
-      const float4 a = __ldcg(reinterpret_cast<const float4*>(p.partial + x * (R * D) + r * D + d));
-      if (f == 0.f && lk == 0.f) continue;
-      L += lk * f;
-      v[0] += a.x * f; v[1] += a.y * f; v[2] += a.z * f; v[3] += a.w * f;
+#pragma unroll 1
+  for (int side = 0; side < 2; ++side) {
+    if (left[side] < 0) continue;
+    const Piece w = sm_piece[left[side]];
+    // the CTAs from that of the tile's first unit to that of its last; its counter is the first one's
+    auto owner = [&](int64_t unit) {
+      const int64_t n = (unit + 1) * warps - 1;
+      return (int)(small ? (unsigned)n / (unsigned)total : n / total) / kWarps;
+    };
+    const int first = owner(w.first), last = owner(w.first + w.units - 1);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const int n = atomicAdd(p.arrived + first, 1);
+      sm_last = n == last - first;
+      if (sm_last) p.arrived[first] = 0;        // (as the next launch expects it)
     }
-    store(r, d, v, L);
+    __syncthreads();
+    if (!sm_last) continue;
+    __threadfence();
+#pragma unroll 1
+    for (int q = threadIdx.x; q < kQuads; q += kWarps * 32) {
+      const int r = q / (D / 4), d = (q % (D / 4)) * 4;
+      float M = -INFINITY, L = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+      auto part_of = [&](int c) { return 2 * c + (c == first); };
+#pragma unroll 4
+      for (int c = first; c <= last; ++c) M = fmaxf(M, __ldcg(p.partial_ml + 2 * (part_of(c) * R + r)));
+#pragma unroll 4
+      for (int c = first; c <= last; ++c) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.partial_ml + 2 * (part_of(c) * R + r)));
+        const float4 o = __ldcg(reinterpret_cast<const float4*>(p.partial + ((int64_t)part_of(c) * R + r) * D + d));
+        const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - M);
+        if (ml.x == -INFINITY && ml.y == 0.f) continue;
+        L += ml.y * f;
+        v[0] += o.x * f; v[1] += o.y * f; v[2] += o.z * f; v[3] += o.w * f;
+      }
+      put(w, r, d, v, L);
+    }
   }
 }
 
-constexpr int kCtasPerSm1 = 3, kCtasPerSm2 = 2;
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 int launch_decode(const char* who, const B200PagedCache* c, PagedAttnParams p, cudaStream_t stream) {
@@ -342,14 +453,14 @@ int launch_decode(const char* who, const B200PagedCache* c, PagedAttnParams p, c
   const bool narrow = most <= 8;
   const int R = narrow ? 8 : 16;
   p.slots = sm_count() * (narrow ? kCtasPerSm1 : kCtasPerSm2);
-  // tiles of all sequences, at most; each may have one chunk more than its share of the slots
-  const int64_t tiles = (c->tokens * p.group + R - 1) / R + c->batch;
-  const int64_t grid = (tiles + p.slots / p.c.kv_heads + 1) * p.c.kv_heads;
-  if (grid > 0x7fffffffLL) return fail(B200_EINVAL, "%s: too many rows", who);
-  auto launch = [&](auto kern) {
+  auto launch = [&](auto kern, SmemLimit& limit) {
+    const size_t smem = (size_t)2 * kWarps * R * (c->head_dim + 4) * sizeof(float);
+    int rc = raise_smem_limit(limit, reinterpret_cast<const void*>(kern), smem, who);
+    if (rc) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)grid);
+    cfg.gridDim = dim3((unsigned)p.slots);
     cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -365,8 +476,9 @@ int launch_decode(const char* who, const B200PagedCache* c, PagedAttnParams p, c
   auto by_form = [&](auto type, auto dim) {
     using T = decltype(type);
     constexpr int D = decltype(dim)::value;
-    if (narrow) return extra ? launch(paged_decode_kernel<T, D, 1, true>) : launch(paged_decode_kernel<T, D, 1, false>);
-    return extra ? launch(paged_decode_kernel<T, D, 2, true>) : launch(paged_decode_kernel<T, D, 2, false>);
+    static SmemLimit limit[4];
+    if (narrow) return extra ? launch(paged_decode_kernel<T, D, 1, true>, limit[3]) : launch(paged_decode_kernel<T, D, 1, false>, limit[2]);
+    return extra ? launch(paged_decode_kernel<T, D, 2, true>, limit[1]) : launch(paged_decode_kernel<T, D, 2, false>, limit[0]);
   };
   auto by_dim = [&](auto type) {
     return c->head_dim == 128 ? by_form(type, std::integral_constant<int, 128>()) : by_form(type, std::integral_constant<int, 64>());
