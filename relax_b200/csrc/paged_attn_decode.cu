@@ -48,7 +48,7 @@ __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 
 // A tile's part of a warp that is not the whole tile.
 struct Piece {
   int64_t first;                                // the tile's first unit, counted over everything
-  int b, tile, h, units;                        // units < 0: no piece
+  int row, tile, h, units, rows;                // the sequence's first row; rows of the tile, 0: no piece
 };
 
 template <typename T, int D, int NT, bool kExtra>
@@ -61,7 +61,7 @@ paged_decode_kernel(const PagedAttnParams p) {
   extern __shared__ __align__(16) float sm_o[];           // [2 kWarps][R][kPitch]: a warp's first piece and its last
   __shared__ float sm_m[2 * kWarps][R], sm_l[2 * kWarps][R];
   __shared__ Piece sm_piece[2 * kWarps];
-  __shared__ int sm_last;
+  __shared__ int sm_first[2], sm_parts[2];
   ptx::pdl_wait();
   ptx::pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -94,7 +94,7 @@ paged_decode_kernel(const PagedAttnParams p) {
   auto share = [&](int i) { return small ? (int64_t)((unsigned)total * (unsigned)i / (unsigned)warps) : total * i / warps; };
   int64_t at = share(blockIdx.x * kWarps + warp);
   const int64_t end = share(blockIdx.x * kWarps + warp + 1);
-  if (lane == 0) sm_piece[2 * warp].units = sm_piece[2 * warp + 1].units = -1;
+  if (lane == 0) sm_piece[2 * warp].rows = sm_piece[2 * warp + 1].rows = 0;
 
   // the sequence of unit `at`, and how many units lie before it
   int b = 0, per_tile = 0;
@@ -314,7 +314,7 @@ paged_decode_kernel(const PagedAttnParams p) {
     // ---- the warp's rows: a whole tile goes out, a part of one to shared memory -------------------------------------------------
     const bool all = u_begin == 0 && u_end == per_tile;
     const int slot = 2 * warp + (pieces > 0);
-    if (!all && lane == 0) sm_piece[slot] = {at - u_begin, b, tile, h, per_tile};
+    if (!all && lane == 0) sm_piece[slot] = {at - u_begin, s.first, tile, h, per_tile, nrows};
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -361,87 +361,141 @@ paged_decode_kernel(const PagedAttnParams p) {
   }
 
   // ---- pieces of the same tile in this CTA, then those of different CTAs: the one that comes last adds them up --------------------
+  // A warp takes a row at a time, a lane four of its dims (head_dim 64: two), and a part's maximum and sum in a lane of its own.
   __syncthreads();
-  constexpr int kQuads = R * D / 4;
-  auto put = [&](const Piece& w, int r, int d, const float (&v)[4], float sum) {
-    const Sequence s = sequence_of(p.c, w.b);
+  constexpr int kDims = D / 32;
+  float v[kDims];
+  auto add = [&](float f, const float* from) {
+    if (kDims == 4) {
+      const float4 o = *reinterpret_cast<const float4*>(from + 4 * lane);
+      v[0] = fmaf(f, o.x, v[0]); v[1] = fmaf(f, o.y, v[1]); v[kDims - 2] = fmaf(f, o.z, v[kDims - 2]); v[kDims - 1] = fmaf(f, o.w, v[kDims - 1]);
+    } else {
+      const float2 o = *reinterpret_cast<const float2*>(from + 2 * lane);
+      v[0] = fmaf(f, o.x, v[0]); v[1] = fmaf(f, o.y, v[1]);
+    }
+  };
+  auto store = [&](float* to) {
+    if (kDims == 4) *reinterpret_cast<float4*>(to + 4 * lane) = make_float4(v[0], v[1], v[kDims - 2], v[kDims - 1]);
+    else *reinterpret_cast<float2*>(to + 2 * lane) = make_float2(v[0], v[1]);
+  };
+  auto put = [&](const Piece& w, int r, float sum) {
     const int x = w.tile * R + r;
-    if (x >= s.rows * p.group) return;
     const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-    T* out = static_cast<T*>(p.out) + ((int64_t)(s.first + x / p.group) * p.heads + w.h * p.group + x % p.group) * D + d;
-    *reinterpret_cast<uint2*>(out) = make_uint2(pack2(T(), v[0] * inv, v[1] * inv), pack2(T(), v[2] * inv, v[3] * inv));
+    T* out = static_cast<T*>(p.out) + ((int64_t)(w.row + x / p.group) * p.heads + w.h * p.group + x % p.group) * D + kDims * lane;
+    if (kDims == 4) *reinterpret_cast<uint2*>(out) = make_uint2(pack2(T(), v[0] * inv, v[1] * inv), pack2(T(), v[kDims - 2] * inv, v[kDims - 1] * inv));
+    else *reinterpret_cast<uint32_t*>(out) = pack2(T(), v[0] * inv, v[1] * inv);
+  };
+  auto warp_max = [&](float x) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
+  };
+  auto warp_add = [&](float x) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
   };
   const int64_t cta_begin = share(blockIdx.x * kWarps), cta_end = share(blockIdx.x * kWarps + kWarps);
-  int left[2] = {-1, -1};                       // pieces' slots of tiles that other CTAs share: begun before this one, ended after it
+  int left[2] = {-1, -1};                       // slots of tiles that other CTAs share: begun before this one's part, ended behind it
 #pragma unroll 1
   for (int s0 = 0; s0 < 2 * kWarps;) {
-    if (sm_piece[s0].units < 0) { ++s0; continue; }
+    if (sm_piece[s0].rows == 0) { ++s0; continue; }
     const Piece w = sm_piece[s0];
     int s1 = s0 + 1;                            // slots [s0, s1) are of this tile, or empty
-    while (s1 < 2 * kWarps && (sm_piece[s1].units < 0 || sm_piece[s1].first == w.first)) ++s1;
-    const bool whole = w.first >= cta_begin && w.first + w.units <= cta_end;
-    const int part = 2 * blockIdx.x + (w.first >= cta_begin);
-    if (!whole) left[w.first >= cta_begin] = s0;
+    while (s1 < 2 * kWarps && (sm_piece[s1].rows == 0 || sm_piece[s1].first == w.first)) ++s1;
+    const bool begun = w.first >= cta_begin, whole = begun && w.first + w.units <= cta_end;
+    const int part = (2 * blockIdx.x + begun) * R;
+    if (!whole) left[begun] = s0;
 #pragma unroll 1
-    for (int q = threadIdx.x; q < kQuads; q += kWarps * 32) {
-      const int r = q / (D / 4), d = (q % (D / 4)) * 4;
-      float M = -INFINITY, L = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int x = s0; x < s1; ++x)
-        if (sm_piece[x].units >= 0) M = fmaxf(M, sm_m[x][r]);
-      for (int x = s0; x < s1; ++x) {
-        if (sm_piece[x].units < 0 || (sm_m[x][r] == -INFINITY && sm_l[x][r] == 0.f)) continue;
-        const float f = sm_m[x][r] == -INFINITY ? 0.f : exp2_approx(sm_m[x][r] - M);
-        const float4 o = *reinterpret_cast<const float4*>(sm_o + (x * R + r) * kPitch + d);
-        L += sm_l[x][r] * f;
-        v[0] += o.x * f; v[1] += o.y * f; v[2] += o.z * f; v[3] += o.w * f;
+    for (int r = warp; r < w.rows; r += kWarps) {
+      const int x = s0 + lane;
+      const bool there = x < s1 && sm_piece[x < 2 * kWarps ? x : 0].rows > 0;
+      const float m = there ? sm_m[x][r] : -INFINITY, M = warp_max(m);
+      const float f = m == -INFINITY ? 0.f : exp2_approx(m - M);
+      const float L = warp_add(there ? sm_l[x][r] * f : 0.f);
+#pragma unroll
+      for (int i = 0; i < kDims; ++i) v[i] = 0.f;
+#pragma unroll 1
+      for (int y = s0; y < s1; ++y) {
+        const float fy = __shfl_sync(0xffffffffu, f, y - s0);
+        if (fy != 0.f) add(fy, sm_o + (y * R + r) * kPitch);
       }
       if (whole) {
-        put(w, r, d, v, L);
+        put(w, r, L);
       } else {
-        *reinterpret_cast<float4*>(p.partial + ((int64_t)part * R + r) * D + d) = make_float4(v[0], v[1], v[2], v[3]);
-        if (d == 0) *reinterpret_cast<float2*>(p.partial_ml + 2 * (part * R + r)) = make_float2(M, L);
+        store(p.partial + (int64_t)(part + r) * D);
+        if (lane == 0) *reinterpret_cast<float2*>(p.partial_ml + 2 * (part + r)) = make_float2(M, L);
       }
     }
     s0 = s1;
   }
   if (left[0] < 0 && left[1] < 0) return;
-  __threadfence();
-#pragma unroll 1
-  for (int side = 0; side < 2; ++side) {
-    if (left[side] < 0) continue;
-    const Piece w = sm_piece[left[side]];
-    // the CTAs from that of the tile's first unit to that of its last; its counter is the first one's
+  // the CTAs from that of a tile's first unit to that of its last; its counter is the first one's
+  __syncthreads();
+  if (threadIdx.x < 2 && left[threadIdx.x] >= 0) {
+    const Piece w = sm_piece[left[threadIdx.x]];
+    __threadfence();                            // (of everybody's stores: the barrier has put them before it)
     auto owner = [&](int64_t unit) {
       const int64_t n = (unit + 1) * warps - 1;
       return (int)(small ? (unsigned)n / (unsigned)total : n / total) / kWarps;
     };
     const int first = owner(w.first), last = owner(w.first + w.units - 1);
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      const int n = atomicAdd(p.arrived + first, 1);
-      sm_last = n == last - first;
-      if (sm_last) p.arrived[first] = 0;        // (as the next launch expects it)
-    }
-    __syncthreads();
-    if (!sm_last) continue;
+    const int n = atomicAdd(p.arrived + first, 1);
+    if (n == last - first) p.arrived[first] = 0;          // (as the next launch expects it)
     __threadfence();
+    sm_first[threadIdx.x] = first;
+    sm_parts[threadIdx.x] = n == last - first ? n + 1 : 0;
+  }
+  __syncthreads();
 #pragma unroll 1
-    for (int q = threadIdx.x; q < kQuads; q += kWarps * 32) {
-      const int r = q / (D / 4), d = (q % (D / 4)) * 4;
-      float M = -INFINITY, L = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-      auto part_of = [&](int c) { return 2 * c + (c == first); };
-#pragma unroll 4
-      for (int c = first; c <= last; ++c) M = fmaxf(M, __ldcg(p.partial_ml + 2 * (part_of(c) * R + r)));
-#pragma unroll 4
-      for (int c = first; c <= last; ++c) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.partial_ml + 2 * (part_of(c) * R + r)));
-        const float4 o = __ldcg(reinterpret_cast<const float4*>(p.partial + ((int64_t)part_of(c) * R + r) * D + d));
-        const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - M);
-        if (ml.x == -INFINITY && ml.y == 0.f) continue;
-        L += ml.y * f;
-        v[0] += o.x * f; v[1] += o.y * f; v[2] += o.z * f; v[3] += o.w * f;
+  for (int side = 0; side < 2; ++side) {
+    if (left[side] < 0 || sm_parts[side] == 0) continue;
+    const Piece w = sm_piece[left[side]];
+    const int first = sm_first[side], parts = sm_parts[side];
+    auto row_of = [&](int c, int r) { return (2 * (first + c) + (c == 0)) * R + r; };
+#pragma unroll 1
+    for (int r = warp; r < w.rows; r += kWarps) {
+      float M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int i = 0; i < kDims; ++i) v[i] = 0.f;
+#pragma unroll 1
+      for (int c0 = 0; c0 < parts; c0 += 32) {
+        const int n = min(32, parts - c0);
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (lane < n) ml = __ldcg(reinterpret_cast<const float2*>(p.partial_ml + 2 * row_of(c0 + lane, r)));
+        float f = 0.f;
+#pragma unroll 1
+        for (int y0 = 0; y0 < n; y0 += 8) {
+          float o[8][kDims];
+#pragma unroll
+          for (int y = 0; y < 8; ++y) {         // (behind the end the last one again, with weight 0)
+            const float* from = p.partial + (int64_t)row_of(c0 + min(y0 + y, n - 1), r) * D + kDims * lane;
+            if (kDims == 4) {
+              const float4 q = __ldcg(reinterpret_cast<const float4*>(from));
+              o[y][0] = q.x; o[y][1] = q.y; o[y][kDims - 2] = q.z; o[y][kDims - 1] = q.w;
+            } else {
+              const float2 q = __ldcg(reinterpret_cast<const float2*>(from));
+              o[y][0] = q.x; o[y][1] = q.y;
+            }
+          }
+          if (y0 == 0) {                        // (behind the loads: the maximum of these parts and those before)
+            const float to = fmaxf(M, warp_max(ml.x)), old = M == -INFINITY ? 0.f : exp2_approx(M - to);
+            M = to;
+            f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - M);
+            L = L * old + ml.y * f;
+#pragma unroll
+            for (int i = 0; i < kDims; ++i) v[i] *= old;
+          }
+#pragma unroll
+          for (int y = 0; y < 8; ++y) {
+            const float fy = __shfl_sync(0xffffffffu, f, (y0 + y) & 31);
+            if (y0 + y < n)
+#pragma unroll
+              for (int i = 0; i < kDims; ++i) v[i] = fmaf(fy, o[y][i], v[i]);
+          }
+        }
       }
-      put(w, r, d, v, L);
+      put(w, r, warp_add(L));
     }
   }
 }
