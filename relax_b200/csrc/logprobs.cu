@@ -6,7 +6,8 @@
 //
 // The likeliest k without a second pass over everything: the maxima of groups of four threads bound the k-th largest value from below
 // (k of the groups have an element at or above the k-th largest group maximum), and only threads whose own maximum reaches that
-// bound look through their part again, which is in cache.  What they find, a few more than k, is put in order by counting.
+// bound saw anything that counts: their parts, which are in cache, are looked through again by all.  What is found, a few more than k, is put
+// in order by counting.
 // Equal values go by index; where more elements equal the bound than the list holds, their lowest indices are found by a scan in order.
 //
 // A row is one CTA of 256 threads; few rows are spread over a cluster of up to 8, joined through shared memory.
@@ -106,9 +107,10 @@ token_logprobs_kernel(const LogprobParams p) {
   constexpr int N = Vec<T>::N;
   constexpr int U = 4;                          // loads in flight
   __shared__ Stats sm_stats[kWarps];
-  __shared__ uint32_t sm_group[kGroups];
+  __shared__ __align__(16) uint32_t sm_group[kGroups];
   __shared__ uint32_t sm_bound;
-  __shared__ int sm_above, sm_equal, sm_count;
+  __shared__ int sm_above, sm_equal, sm_count, sm_hots;
+  __shared__ uint8_t sm_hot[kThreads];
   __shared__ unsigned long long sm_list[kList];         // key << 32 | ~index
   __shared__ int sm_equal_at[kList];
   __shared__ unsigned long long sm_best[kMaxTop];       // this CTA's, in order
@@ -183,20 +185,20 @@ token_logprobs_kernel(const LogprobParams p) {
     gk = max(gk, __shfl_xor_sync(0xffffffffu, gk, 1));
     gk = max(gk, __shfl_xor_sync(0xffffffffu, gk, 2));
     if ((lane & 3) == 0) sm_group[tid >> 2] = gk;
-    if (tid == 0) sm_above = sm_equal = sm_count = 0;
+    if (tid == 0) sm_above = sm_equal = sm_count = sm_hots = 0;
     if (tid < k) sm_best[tid] = 0;
     __syncthreads();
-    if (warp == 0) {                                    // the k-th largest of the 64 groups
-      uint32_t a = sm_group[lane], b = sm_group[lane + 32];
-      if (a < b) { const uint32_t t = a; a = b; b = t; }
-      uint32_t bound = 0;
-      for (int j = 0; j < k; ++j) {
-        bound = __reduce_max_sync(0xffffffffu, a);
-        const unsigned who = __ballot_sync(0xffffffffu, a == bound);
-        if (lane == __ffs(who) - 1) { a = b; b = 0; }
+    if (tid < kGroups) {                                // the k-th largest of the 64 groups, by counting
+      const uint32_t key = sm_group[tid];
+      int r = 0;
+#pragma unroll
+      for (int j = 0; j < kGroups; j += 4) {
+        const uint4 o = *reinterpret_cast<const uint4*>(sm_group + j);
+        r += (o.x > key || (o.x == key && j < tid)) + (o.y > key || (o.y == key && j + 1 < tid)) + (o.z > key || (o.z == key && j + 2 < tid)) +
+             (o.w > key || (o.w == key && j + 3 < tid));
       }
       // -inf (an excluded entry, or a group without elements): nothing but real values is collected
-      if (lane == 0) sm_bound = max(bound, kKeyNegInf);
+      if (r == k - 1) sm_bound = max(key, kKeyNegInf);
     }
     __syncthreads();
     const uint32_t bound = sm_bound;
@@ -210,15 +212,26 @@ token_logprobs_kernel(const LogprobParams p) {
         if (n < kList) sm_equal_at[n] = at;
       }
     };
-    if (mine >= bound) {
+    // The threads that saw such an element; all of them look through those threads' vectors together.
+    const bool hot = mine >= bound;
+    if (hot) {
       for (int j = begin + tid; j < body; j += kThreads) look(to_float(x[j]), j);
-      for (int j = tid; j < vecs; j += kThreads) {
-        float f[N];
-        unpack<T>(__ldg(xv + j), f);
-#pragma unroll
-        for (int u = 0; u < N; ++u) look(f[u], body + j * N + u);
-      }
       for (int j = tail + tid; j < end; j += kThreads) look(to_float(x[j]), j);
+      sm_hot[atomicAdd(&sm_hots, 1)] = tid;
+    }
+    __syncthreads();
+    const int rounds = (vecs + kThreads - 1) / kThreads, hots = sm_hots;
+    for (int j = tid; j < hots * rounds; j += kThreads) {
+      const int who = j / rounds, i = sm_hot[who] + (j - who * rounds) * kThreads;
+      if (i >= vecs) continue;
+      float f[N];
+      unpack<T>(__ldg(xv + i), f);
+      float top = f[0];
+#pragma unroll
+      for (int u = 1; u < N; ++u) top = fmaxf(top, f[u]);
+      if (key_of(top) < bound) continue;
+#pragma unroll
+      for (int u = 0; u < N; ++u) look(f[u], body + i * N + u);
     }
     __syncthreads();
     const int above = sm_above, equal = sm_equal;

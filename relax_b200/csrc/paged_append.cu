@@ -10,7 +10,9 @@ namespace b200 {
 
 namespace {
 
-constexpr int kThreads = 256;
+// Threads of a block; heads and copies that a thread has under way at a time.  7.9k tokens of 48 heads, 209 MB, us: 64 x 2 45.8, 128 x 1 43.1,
+// 128 x 2 40.4 (5.2 TB/s; a copy of as much 32), 128 x 3 54, 192 x 2 57, 256 x 2 51.7, 512 x 2 120; 64 tokens 3.0 with 128 x 2, 2.7 with 256 x 2.
+constexpr int kThreads = 128, kBatch = 2;
 
 struct AppendParams {
   PagedParams c;
@@ -28,57 +30,86 @@ __global__ void __launch_bounds__(kThreads)
 paged_append_kernel(const AppendParams p) {
   ptx::pdl_wait();
   ptx::pdl_launch_dependents();
+  const int kv = p.c.kv_heads, page = 1 << p.c.page_log2;
   const int row = blockIdx.x;
-  const int kv = p.c.kv_heads;
-  // the sequence of this row: the last one that starts at or before it
-  int b = row;
-  if (p.c.starts) {
-    int lo = 0, hi = p.c.batch;                 // starts[lo] <= row < starts[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (p.c.starts[mid] <= row) lo = mid; else hi = mid;
-    }
-    b = lo;
-  }
-  const Sequence s = sequence_of(p.c, b);
-  const int place = row - s.first;
-  const int position = s.length - s.rows + place;
-  const bool placed = position >= 0 && place >= 0 && place < s.rows;
   const T* in = static_cast<const T*>(p.qkv) + (int64_t)row * p.qkv_stride;
   T* q = static_cast<T*>(p.q_out) + (int64_t)row * p.heads * D;
-  if (!placed) {
-    for (int i = threadIdx.x; i < p.heads * D / 8; i += kThreads) reinterpret_cast<uint4*>(q)[i] = make_uint4(0, 0, 0, 0);
-    return;
-  }
-  const int page = 1 << p.c.page_log2;
-  const int64_t id = page_of(p.c, b, position >> p.c.page_log2);
-  const int64_t slot = (int64_t)(position & (page - 1)) * D;
-  T* kp = static_cast<T*>(p.c.k) + id * p.c.k_stride + slot;
-  T* vp = static_cast<T*>(p.c.v) + id * p.c.v_stride + slot;
-  const int64_t head_step = (int64_t)page * D;
-  auto target = [&](int head) { return head < p.heads ? q + head * D : kp + (head - p.heads) * head_step; };
-
   const int half = p.rotary / 2;
-  int64_t at = p.positions ? p.positions[row] : position;
-  at = at < 0 ? 0 : at >= p.table_rows ? p.table_rows - 1 : at;
   const int pairs = p.rotary / 16;              // chunk pairs of a head's rotated part
   const int c = threadIdx.x % pairs, first = threadIdx.x / pairs, step = kThreads / pairs;
-  if (first < step) {
-    float cs[8], sn[8];
-    const float4* cp = reinterpret_cast<const float4*>(p.cos_t + at * half + c * 8);
-    const float4* sp = reinterpret_cast<const float4*>(p.sin_t + at * half + c * 8);
+  const int o0 = kInterleaved ? 16 * c : 8 * c, o1 = kInterleaved ? o0 + 8 : half + 8 * c;
+  const int kept = (D - p.rotary) / 8;          // chunks of a q or k head that are not turned
+  const int turned = first < step ? p.heads + kv : 0, values = kv * (D / 8), copies = values + kept * (p.heads + kv);
+  T *kp = nullptr, *vp = nullptr;
+  bool placed = false, known = false;
+  float cs[8], sn[8];
+  // The values are asked for before it is known where they go: that takes a chain of loads of its own.
+  int head0 = first, copy0 = threadIdx.x;
+  do {
+    uint4 x[kBatch], y[kBatch], z[kBatch];
+    int from[kBatch];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const float4 x = cp[j], y = sp[j];
-      cs[4 * j] = x.x; cs[4 * j + 1] = x.y; cs[4 * j + 2] = x.z; cs[4 * j + 3] = x.w;
-      sn[4 * j] = y.x; sn[4 * j + 1] = y.y; sn[4 * j + 2] = y.z; sn[4 * j + 3] = y.w;
+    for (int k = 0; k < kBatch; ++k) {
+      const int head = head0 + k * step, i = copy0 + k * kThreads;
+      if (head < turned) {
+        x[k] = *reinterpret_cast<const uint4*>(in + head * D + o0);
+        y[k] = *reinterpret_cast<const uint4*>(in + head * D + o1);
+      }
+      from[k] = -1;
+      if (i < values) {
+        from[k] = (p.heads + kv) * D + i * 8;
+      } else if (i < copies) {
+        const int j = i - values, h = j / kept;
+        from[k] = h * D + p.rotary + (j - h * kept) * 8;
+      }
+      if (from[k] >= 0) z[k] = *reinterpret_cast<const uint4*>(in + from[k]);
     }
-    const int o0 = kInterleaved ? 16 * c : 8 * c, o1 = kInterleaved ? o0 + 8 : half + 8 * c;
-    for (int head = first; head < p.heads + kv; head += step) {
-      const T* src = in + head * D;
-      T* dst = target(head);
-      const uint4 x = *reinterpret_cast<const uint4*>(src + o0), y = *reinterpret_cast<const uint4*>(src + o1);
-      const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+    if (!known) {
+      known = true;
+      // the sequence of this row: the last one that starts at or before it
+      int b = row;
+      if (p.c.starts) {
+        int lo = 0, hi = p.c.batch;             // starts[lo] <= row < starts[hi]
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (p.c.starts[mid] <= row) lo = mid; else hi = mid;
+        }
+        b = lo;
+      }
+      const Sequence s = sequence_of(p.c, b);
+      const int place = row - s.first, position = s.length - s.rows + place;
+      placed = position >= 0 && place >= 0 && place < s.rows;
+      if (!placed) break;
+      const int64_t id = page_of(p.c, b, position >> p.c.page_log2);
+      const int64_t slot = (int64_t)(position & (page - 1)) * D;
+      kp = static_cast<T*>(p.c.k) + id * p.c.k_stride + slot;
+      vp = static_cast<T*>(p.c.v) + id * p.c.v_stride + slot;
+      if (turned) {
+        int64_t at = p.positions ? p.positions[row] : position;
+        at = at < 0 ? 0 : at >= p.table_rows ? p.table_rows - 1 : at;
+        const float4* cp = reinterpret_cast<const float4*>(p.cos_t + at * half + c * 8);
+        const float4* sp = reinterpret_cast<const float4*>(p.sin_t + at * half + c * 8);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float4 u = cp[j], w = sp[j];
+          cs[4 * j] = u.x; cs[4 * j + 1] = u.y; cs[4 * j + 2] = u.z; cs[4 * j + 3] = u.w;
+          sn[4 * j] = w.x; sn[4 * j + 1] = w.y; sn[4 * j + 2] = w.z; sn[4 * j + 3] = w.w;
+        }
+      }
+    }
+    const int64_t head_step = (int64_t)page * D;
+    // where element `e` of the row goes
+    auto target = [&](int e) {
+      const int h = e / D, o = e - h * D;
+      return h < p.heads ? q + e : h < p.heads + kv ? kp + (h - p.heads) * head_step + o : vp + (h - p.heads - kv) * head_step + o;
+    };
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int head = head0 + k * step;
+      if (from[k] >= 0) *reinterpret_cast<uint4*>(target(from[k])) = z[k];
+      if (head >= turned) continue;
+      T* dst = target(head * D);
+      const uint32_t xw[4] = {x[k].x, x[k].y, x[k].z, x[k].w}, yw[4] = {y[k].x, y[k].y, y[k].z, y[k].w};
       uint32_t xo[4], yo[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -94,17 +125,11 @@ paged_append_kernel(const AppendParams p) {
       *reinterpret_cast<uint4*>(dst + o0) = make_uint4(xo[0], xo[1], xo[2], xo[3]);
       *reinterpret_cast<uint4*>(dst + o1) = make_uint4(yo[0], yo[1], yo[2], yo[3]);
     }
-  }
-  const int kept = (D - p.rotary) / 8;          // chunks of a q or k head that are not turned
-  for (int i = threadIdx.x; i < kept * (p.heads + kv); i += kThreads) {
-    const int head = i / kept, o = p.rotary + (i - head * kept) * 8;
-    *reinterpret_cast<uint4*>(target(head) + o) = *reinterpret_cast<const uint4*>(in + head * D + o);
-  }
-  const T* v = in + (int64_t)(p.heads + kv) * D;
-  for (int i = threadIdx.x; i < kv * (D / 8); i += kThreads) {
-    const int head = i / (D / 8), o = (i % (D / 8)) * 8;
-    *reinterpret_cast<uint4*>(vp + head * head_step + o) = *reinterpret_cast<const uint4*>(v + head * D + o);
-  }
+    head0 += kBatch * step;
+    copy0 += kBatch * kThreads;
+  } while (head0 < turned || copy0 < copies);
+  if (!placed)
+    for (int i = threadIdx.x; i < p.heads * D / 8; i += kThreads) reinterpret_cast<uint4*>(q)[i] = make_uint4(0, 0, 0, 0);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
