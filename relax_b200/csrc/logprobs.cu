@@ -14,6 +14,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "internal.h"
 #include "sm100_ptx.cuh"
 
@@ -21,7 +23,7 @@ namespace b200 {
 
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kCtasPerSm = 5;
 constexpr int kMaxTop = 32, kMaxCluster = 8;
 constexpr int kGroups = 64;                     // of four neighbouring threads
 constexpr int kList = 512;                      // elements above the bound, elements equal to it
@@ -102,7 +104,7 @@ struct Stats {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 6)
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
 token_logprobs_kernel(const LogprobParams p) {
   constexpr int N = Vec<T>::N;
   constexpr int U = 4;                          // loads in flight
@@ -115,6 +117,7 @@ token_logprobs_kernel(const LogprobParams p) {
   __shared__ int sm_equal_at[kList];
   __shared__ unsigned long long sm_best[kMaxTop];       // this CTA's, in order
   __shared__ Stats in_stats[kMaxCluster];               // of the cluster, in CTA 0
+  __shared__ int in_count[kMaxCluster];                 // how many of its likeliest a CTA has
   __shared__ unsigned long long in_best[kMaxCluster * kMaxTop];
   ptx::pdl_wait();
   ptx::pdl_launch_dependents();
@@ -137,24 +140,75 @@ token_logprobs_kernel(const LogprobParams p) {
     s.raise(v);
     if (s.m > -INFINITY || v != v) s.add(v);
   };
-  auto many = [&](const uint4& v) {
-    float f[N];
-    unpack<T>(v, f);
-    float top = f[0];
+  // Several vectors at a time: one maximum.  Where it is not near the type's lowest value, entries below kFloor, excluded ones among them,
+  // count as kFloor: weight 0, and 0 times a number instead of 0 times infinity.  Then four operations an entry beside the special
+  // function, two entries an instruction.
+  constexpr float kFloor = std::is_same<T, __half>::value ? -65504.f : -1e30f, kFar = std::is_same<T, __half>::value ? -65000.f : -1e29f;
+  auto many = [&](auto& v) {                            // uint4 [n]
+    constexpr int n = sizeof(v) / sizeof(uint4);
+    float top;
+    if constexpr (sizeof(T) == 2) {
+      using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+      T2* w = reinterpret_cast<T2*>(v);
+      T2 most[4] = {w[0], w[1], w[2], w[3]};
 #pragma unroll
-    for (int i = 1; i < N; ++i) top = fmaxf(top, f[i]);
-    s.raise(top);
-    if (!(s.m > -INFINITY)) {                           // nothing but excluded entries so far, or NaN
+      for (int i = 4; i < 4 * n; ++i) most[i & 3] = __hmax2(most[i & 3], w[i]);
+      const T2 all = __hmax2(__hmax2(most[0], most[1]), __hmax2(most[2], most[3]));
+      top = fmaxf(to_float(T(all.x)), to_float(T(all.y)));
+      s.raise(top);
+      if (s.m > kFar) {
+        const T lowest = T(kFloor);
+        const T2 lowest2 = T2(lowest, lowest);
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (f[i] != f[i]) s.l = f[i];
+        for (int i = 0; i < 4 * n; ++i) w[i] = __hmax2_nan(w[i], lowest2);
+      }
+    } else {
+      float* w = reinterpret_cast<float*>(v);
+      float most[4] = {w[0], w[1], w[2], w[3]};
+#pragma unroll
+      for (int i = 4; i < 4 * n; ++i) most[i & 3] = fmaxf(most[i & 3], w[i]);
+      top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+      s.raise(top);
+      if (s.m > kFar) {
+#pragma unroll
+        for (int i = 0; i < 4 * n; ++i) w[i] = w[i] < kFloor ? kFloor : w[i];   // (a NaN stays)
+      }
+    }
+    if (s.m > kFar) {
+#pragma unroll
+      for (int q = 0; q < n; ++q) {
+        float f[N], l0 = 0.f, l1 = 0.f, e0 = 0.f, e1 = 0.f;       // (sums of a few, so that a thread's thousands do not lose bits)
+        unpack<T>(v[q], f);
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+          float a = f[i], b = f[i + 1];
+          ptx::add2(a, b, -s.m, -s.m);
+          ptx::mul2(a, b, kLog2e, kLog2e);
+          const float wa = exp2_approx(a), wb = exp2_approx(b);
+          ptx::add2(l0, l1, wa, wb);
+          ptx::fma2(e0, e1, wa, wb, a, b, e0, e1);
+        }
+        s.l += l0 + l1;
+        s.e += e0 + e1;
+      }
       return;
     }
-    Stats part = {s.m, 0.f, 0.f};                       // (sums of a few, so that a thread's thousands do not lose bits)
+#pragma unroll 1
+    for (int q = 0; q < n; ++q) {
+      float f[N];
+      unpack<T>(v[q], f);
+      if (s.m > -INFINITY) {
+        Stats part = {s.m, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < N; ++i) part.add(f[i]);
-    s.l += part.l;
-    s.e += part.e;
+        for (int i = 0; i < N; ++i) part.add(f[i]);
+        s.l += part.l;
+        s.e += part.e;
+      } else {                                          // nothing but excluded entries so far, or NaN
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (f[i] != f[i]) s.l = f[i];
+      }
+    }
   };
   for (int i = begin + tid; i < body; i += kThreads) one(to_float(x[i]));
   int i = tid;
@@ -162,10 +216,12 @@ token_logprobs_kernel(const LogprobParams p) {
     uint4 v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) v[u] = __ldg(xv + i + u * kThreads);
-#pragma unroll
-    for (int u = 0; u < U; ++u) many(v[u]);
+    many(v);
   }
-  for (; i < vecs; i += kThreads) many(__ldg(xv + i));
+  for (; i < vecs; i += kThreads) {
+    uint4 v[1] = {__ldg(xv + i)};
+    many(v);
+  }
   for (int j = tail + tid; j < end; j += kThreads) one(to_float(x[j]));
 
   // ---- statistics of the CTA ------------------------------------------------------------------------------------------
@@ -319,27 +375,33 @@ token_logprobs_kernel(const LogprobParams p) {
       asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(sm_stats[0].m) : "memory");
       asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(sm_stats[0].l) : "memory");
       asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(sm_stats[0].e) : "memory");
+      int n = 0;
+      while (n < k && sm_best[n] != 0) ++n;
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(ptx::map_to_rank(ptx::smem_u32(&in_count[rank]), 0)), "r"(n) : "memory");
     }
     ptx::cluster_arrive();
     ptx::cluster_wait();
     if (rank != 0) return;
     s = in_stats[0];
     for (int r = 1; r < c; ++r) s.join(in_stats[r]);
-    const int n = tid / kMaxTop, j = tid % kMaxTop;     // (8 x 32 places)
-    if (n < c && j < k) {
-      const unsigned long long v = in_best[n * kMaxTop + j];
-      int r = j;                                        // those before it in its own list, and those above it in the others
-      for (int o = 0; o < c; ++o)
-        if (o != n)
-          for (int u = 0; u < k && in_best[o * kMaxTop + u] > v; ++u) ++r;
-      if (r < k && v != 0) sm_best[r] = v;
+    int real = 0;
+    for (int o = 0; o < c; ++o) real += in_count[o];
+    for (int n = warp; n < c; n += kWarps) {            // a warp has a CTA's list, a lane an entry
+      if (lane >= in_count[n]) continue;
+      const unsigned long long v = in_best[n * kMaxTop + lane];
+      int r = lane;                                     // those before it in its own list, and those above it in the others
+      for (int o = 0; o < c; ++o) {
+        if (o == n) continue;
+        int lo = 0, hi = in_count[o];
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (in_best[o * kMaxTop + mid] > v) lo = mid + 1; else hi = mid;
+        }
+        r += lo;
+      }
+      if (r < k) sm_best[r] = v;
     }
-    if (tid < k) {                                      // (fewer real values than k: the places behind them are empty)
-      int real = 0;
-      for (int o = 0; o < c; ++o)
-        for (int u = 0; u < k; ++u) real += in_best[o * kMaxTop + u] != 0;
-      if (tid >= real) sm_best[tid] = 0;
-    }
+    if (tid < k && tid >= real) sm_best[tid] = 0;       // (fewer real values than k)
     __syncthreads();
   } else {
     s = sm_stats[0];
@@ -397,8 +459,19 @@ extern "C" int b200_token_logprobs(const void* logits, int32_t dtype, int64_t st
   if (rc) return rc;
   LogprobParams p = {logits, static_cast<const int*>(tokens), static_cast<float*>(logprob), static_cast<float*>(entropy),
                      static_cast<float*>(top_logprob), static_cast<int*>(top_token), stride, rows, (int)V, top};
+  // CTAs of a row: the fewest rounds of CTAs, each as long as its slice of the row and what begins and ends it (about 14000 entries, and
+  // 2000 for each CTA of the cluster).  us, fp16, 20 alternatives: one row of 32000 8.9 with four CTAs, 10.1 with eight; 64 rows 9.6 with
+  // four, 14.8 with eight.  Threads, CTAs an SM and loads in flight, 2048 rows: 256, 5, 4 42.5; 256, 6, 4 42; 256, 4, 4 47; 128, 12, 4 50.
+  const int64_t slots = (int64_t)sm_count() * kCtasPerSm;
   int c = 1;
-  while (c < kMaxCluster && rows * c * 2 <= 2 * sm_count() && V / (c * 2) >= 2048) c *= 2;
+  int64_t least = 0;
+  for (int w = 1; w <= kMaxCluster && (w == 1 || V / w >= 2048); w *= 2) {
+    const int64_t cost = (rows * w + slots - 1) / slots * (V / w + 14000 + 2000 * w);
+    if (w == 1 || cost < least) {
+      least = cost;
+      c = w;
+    }
+  }
   auto launch = [&](auto kern) {
     const int64_t y = rows < 32768 ? rows : 32768;
     cudaLaunchConfig_t cfg = {};

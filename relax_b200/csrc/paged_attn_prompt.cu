@@ -311,22 +311,6 @@ __device__ __forceinline__ bool wait_relaxed(uint64_t* bar, uint32_t parity, vol
   return false;
 }
 
-__device__ __forceinline__ unsigned long long pair64(float a, float b) {
-  return (unsigned long long)__float_as_uint(b) << 32 | __float_as_uint(a);
-}
-__device__ __forceinline__ void fma2(float& x, float& y, float ax, float ay, float bx, float by, float cx, float cy) {
-  unsigned long long d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(pair64(ax, ay)), "l"(pair64(bx, by)), "l"(pair64(cx, cy)));
-  x = __uint_as_float((uint32_t)d);
-  y = __uint_as_float((uint32_t)(d >> 32));
-}
-__device__ __forceinline__ void add2(float& x, float& y, float ax, float ay) {
-  unsigned long long d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair64(x, y)), "l"(pair64(ax, ay)));
-  x = __uint_as_float((uint32_t)d);
-  y = __uint_as_float((uint32_t)(d >> 32));
-}
-
 // 2^x of two values without the special-function unit: x = n + f with n the nearest whole number (by adding 1.5 * 2^23, whose sum has n
 // in its low bits), a polynomial of degree kDegree for 2^f on [-1/2, 1/2] (least largest relative error, found by the exchange
 // algorithm: 7.5e-5 for degree 3, 2.6e-6 for degree 4; a weight is rounded to 2^-12 or worse right after), n added to the exponent.
@@ -363,12 +347,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 constexpr int kPlain = 0, kCapped = 1, kSloped = 2, kGeneral = 3;
 constexpr int kPolyOfEight = 2;                 // pairs of weights of eight that go that way
 
-__device__ __forceinline__ void mul2(float& x, float& y, float ax, float ay) {
-  unsigned long long d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair64(x, y)), "l"(pair64(ax, ay)));
-  x = __uint_as_float((uint32_t)d);
-  y = __uint_as_float((uint32_t)(d >> 32));
-}
 // cap * tanh(scale * x / cap) in the exponent of 2, of two scores.  Small: |scale * x / cap| <= 0.4, where tanh's Taylor series to the
 // ninth power is 1e-6 off; nearly all scores are, and the other form takes two special functions for each.
 struct Cap {

@@ -237,6 +237,29 @@ __device__ __forceinline__ void pin_loaded(const uint4& v) {
 }
 __device__ __forceinline__ void pin_loaded(uint32_t v) { asm volatile("" ::"r"(v) : "memory"); }
 
+// ---- two fp32 operations in one instruction -----------------------------------------------------------
+__device__ __forceinline__ unsigned long long pair64(float a, float b) {
+  return (unsigned long long)__float_as_uint(b) << 32 | __float_as_uint(a);
+}
+__device__ __forceinline__ void fma2(float& x, float& y, float ax, float ay, float bx, float by, float cx, float cy) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(pair64(ax, ay)), "l"(pair64(bx, by)), "l"(pair64(cx, cy)));
+  x = __uint_as_float((uint32_t)d);
+  y = __uint_as_float((uint32_t)(d >> 32));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float ax, float ay) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair64(x, y)), "l"(pair64(ax, ay)));
+  x = __uint_as_float((uint32_t)d);
+  y = __uint_as_float((uint32_t)(d >> 32));
+}
+__device__ __forceinline__ void mul2(float& x, float& y, float ax, float ay) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair64(x, y)), "l"(pair64(ax, ay)));
+  x = __uint_as_float((uint32_t)d);
+  y = __uint_as_float((uint32_t)(d >> 32));
+}
+
 // ---- named barriers ---------------------------------------------------------------------------
 __device__ __forceinline__ void bar_sync(int id, int nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
