@@ -1,10 +1,11 @@
 // Attention of a few rows (query heads of one key head x new tokens) over a paged key-value cache, split over the length and joined.
 //
-// Work: the rows of a sequence that share a key head are cut into tiles of R = 8 or 16.  The keys that a tile can see (a prefix and
-// a range behind it) are units of 16 tokens; a tile with more than c units is cut into chunks of about c, one CTA each, c chosen on the
-// device from all lengths so that the chunks fill the GPU once.  So sequences of any mixture of lengths are balanced, and what the
-// host knows is a bound only.  A tile that was cut leaves partial sums in scratch memory, and the CTA that arrives last adds them up in
-// the order of the chunks (the same bits whoever comes last).
+// Work: the rows of a sequence that share a key head are a tile of R = 8 or 16 (more rows than that: several tiles).  The keys that a
+// tile can see (a prefix and a range behind it) are units of 16 tokens.  All units, in the order sequence, tile, key head, unit, are
+// divided evenly among the warps that the GPU holds at once, on the device, from the lengths: any mixture of lengths is balanced, and
+// what the host knows is a bound only.  A warp's share is a part of one tile or the end of one, whole ones, and the beginning of another.
+// A whole tile goes out from registers; parts are added up in shared memory, and those of tiles that several CTAs share in scratch memory,
+// by the CTA that arrives last, in the order of the parts (the same bits whoever comes last).
 //
 // A warp takes one unit (head_dim 64: two) at a time, straight from global memory into the registers of mma.sync operands, with no
 // shared memory between: scores^T [16 tokens x 8 rows] = K q^T, out^T [head_dim x 8 rows] += V^T p.  The dims of a k-step and the rows of
@@ -15,6 +16,10 @@
 // The next unit's keys and values are requested as soon as this one's are used.  The running maximum is raised only where a score
 // is above it by more than 8 (in the exponent of 2), so the usual unit needs a vote instead of a reduction over lanes; weights
 // stay below 2^8, fp32 sums take that.  Weights are rounded to the cache's type for the product with V.
+//
+// What bounds it: HBM for long caches (131000 tokens of 8 key heads, 537 MB, 89 us: 6.0 TB/s, 0.92 of a copy; 64 sequences of 37 to 2047
+// tokens, 135 MB, 35 us: 3.9); latency for short ones (32 heads at 2011, 33 MB, 16.6 us: 2 until the shares are known, 7.6 for two or three
+// units a warp, 7 for the joins).  Before, chunks of equal length as CTAs of their own took 157, 45 and 17.5 us.
 #include "paged_common.cuh"
 
 namespace b200 {

@@ -5,12 +5,22 @@
 // tensor cores multiply for one tile, the other's scores go through the softmax.
 //     S = Q K^T   tcgen05.mma, both operands in shared memory, 128 x 128 fp32 in tensor memory
 //     P           a thread has a row: maximum, 2^(s - m), sum, rounded to the cache's type, stored over S as the next operand
-//     O += P V    tcgen05.mma, P in tensor memory, V [token][dim] in shared memory (rows along N)
+//     O += P V    tcgen05.mma, P in tensor memory, V [token][dim] in shared memory (rows along N); the first 64 keys' products run
+//                 beside the weights of the others
 // O stays in tensor memory; it is multiplied only when a row's maximum has grown by more than 2^8 since it was last set, by the softmax
 // warps themselves: S of a block complete means that O of the block before is, since the MMAs of a CTA complete in order.
 //
 // Warps: 0 TMA (the pages of a block: one load per page and 64 dims; a page behind the last token lies outside the tensor map, which
-// gives zeros), 1 MMA, 2 zeroes the values of a block that nobody sees, 3 hands out the work, 4..7 and 8..11 the rows of the two tiles.
+// gives zeros), 1 MMA, 2 zeroes the values of a block that nobody sees, 3 hands out the work (Plan), 4..7 and 8..11 the rows of the two tiles.
+//
+// What bounds it: a prompt of 8192 tokens of 32 heads over 8 key heads takes 476 us alone (1155 TFLOP/s, 0.71 of cuBLAS' burst), 556 in a
+// row of calls, where the power cap lowers the clock.  The same launches without the softmax take 342 us: S reads 8 KB of shared memory for
+// every 64 clocks of the tensor core and V and the ring's filling the rest of its 128 bytes a clock.  A block takes 3500 clocks: the
+// softmax of a tile 2100 (of which the special-function unit has 770) and its products 1300 behind it; the other tile's fill the gaps of
+// both.  Short prompts (2048 x 32 heads 53 us, 0.40): 12000 clocks until the first scores, 9000 between two items of a CTA.
+// Measured and not kept, us for 8192 tokens where the present form took 485: all 128 scores of a row in registers 494 (and 70 instead of 50
+// for 2048: the longer code waits for its instructions), 64 at a time 551, 32 at a time 529, two threads a row 535..596, scores in two
+// halves of N = 64 with a buffer each 523 (412 instead of 342 without the softmax).
 #include <atomic>
 #include <type_traits>
 
@@ -345,7 +355,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 // What happens to a score before the softmax: a scale > 0; that and a cap; that and a bias by distance; anything.
 constexpr int kPlain = 0, kCapped = 1, kSloped = 2, kGeneral = 3;
-constexpr int kPolyOfEight = 2;                 // pairs of weights of eight that go that way
+// Pairs of weights of eight that go that way: 8192 tokens 0 487, 2 479, 3 495, 4 596 us.
+constexpr int kPolyOfEight = 2;
 
 // cap * tanh(scale * x / cap) in the exponent of 2, of two scores.  Small: |scale * x / cap| <= 0.4, where tanh's Taylor series to the
 // ninth power is 1e-6 off; nearly all scores are, and the other form takes two special functions for each.
@@ -631,9 +642,9 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         if (!wait(&sm.s_full[t], n_s & 1, abort_flag, 12)) { ok = false; break; }
         ++n_s;
         tc_fence_after_sync();
-        // First pass: the maximum, 32 columns at a time, the next ones on their way; scores that a cap, a bias or a mask changes go
-        // back to tensor memory.  Second pass: the weights.  (All 128 scores in registers spilled, and with this much shared memory a
-        // spilled value comes from L2.)
+        // First pass: the maximum, 32 columns at a time, the next ones on their way; scores that a mask changes, or a cap or a bias where
+        // its short form does not hold, go back to tensor memory.  Second pass: the weights.  (What does not fit in registers comes from
+        // L2 with this much shared memory, and so do the instructions of long code.)
         const int from = range.unit(u) * kBlock;
         const bool whole = from + kBlock <= range.pre || (from + kBlock - 1 <= tile_first && tile_last - from < window && tile_first >= 0);
         uint32_t raw[2][32];

@@ -156,6 +156,59 @@ def run_again(c):
     return out
 
 
+def test_many_sequences(cuda_lib):
+    """More sequences than the scheduling warp keeps in shared memory, some without rows, one much longer than the others."""
+    new = [(i * 37) % 50 for i in range(90)]
+    past = [(i * 53) % 200 for i in range(90)]
+    new[40], past[40] = 300, 3000
+    run(Case(new, past, 4, 2, 64, 32))
+    run(Case([1] * 150, [(i * 97) % 700 for i in range(150)], 4, 1, 128, 16, ragged=False))
+
+
+@pytest.mark.parametrize("new,past", [(40, 20000), (513, 5000), (17, 9000)])
+def test_a_part_of_a_long_text(cuda_lib, new, past):
+    """Few rows behind a long context: the context is cut into chunks that several CTAs share."""
+    c = Case([new], [past], 8, 2, 128, 128)
+    first = run(c)
+    assert torch.equal(run_again(c), first)
+    run(c, window=2000, prefix=[700])
+    run(c, cap=7.0)
+    run(c, slopes=[2.0 ** -(i + 4) for i in range(8)])
+
+
+def test_rows_by_a_bound_only(cuda_lib):
+    """max_query is a bound: a larger one, or none, gives the same values by another kernel."""
+    c = Case([3, 1, 4], [100, 30, 0], 4, 2)
+    want = run(c)
+    for most in (4, 5, 100, None):
+        out = ops.paged_attention(c.q, *c.args(), starts=c.starts, max_query=most)
+        torch.cuda.synchronize()
+        assert_within(out, c.reference())
+        assert (out - want).abs().max() < 2e-3
+
+
+def test_the_way_without_the_extension(cuda_lib, monkeypatch):
+    c = Case([5, 60], [100, 3], 8, 2)
+    want = run(c, window=50)
+    monkeypatch.setattr(ops, "_native", False)
+    monkeypatch.setattr(ops, "_torch_call", lambda: False)
+    assert torch.equal(run(c, window=50), want)
+
+
+def test_a_prompt_in_a_graph(cuda_lib):
+    c = Case([200, 40], [0, 900], 8, 2)
+    want = run(c)
+    graph, out = torch.cuda.CUDAGraph(), torch.empty_like(want)
+    with torch.cuda.graph(graph):
+        ops.paged_attention(c.q, *c.args(), starts=c.starts, max_query=200, out=out)
+    for _ in range(3):
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    assert cuda_lib.b200_device_error_flags() == 0
+
+
 def test_refusals(cuda_lib):
     c = Case([1, 1], [3, 4], 8, 2, ragged=False)
 
