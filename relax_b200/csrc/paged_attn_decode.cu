@@ -402,54 +402,65 @@ paged_decode_kernel(const PagedAttnParams p) {
   };
   const int64_t cta_begin = share(blockIdx.x * kWarps), cta_end = share(blockIdx.x * kWarps + kWarps);
   int left[2] = {-1, -1};                       // slots of tiles that other CTAs share: begun before this one's part, ended behind it
+  {
+    // lane x < 2 kWarps has piece x; the pieces of a tile are a group, whose first one stands for it
+    const Piece mine = sm_piece[min(lane, 2 * kWarps - 1)];
+    const bool there = lane < 2 * kWarps && mine.rows > 0;
+    unsigned rest = __ballot_sync(0xffffffffu, there);
+    int task = 0;
 #pragma unroll 1
-  for (int s0 = 0; s0 < 2 * kWarps;) {
-    if (sm_piece[s0].rows == 0) { ++s0; continue; }
-    const Piece w = sm_piece[s0];
-    int s1 = s0 + 1;                            // slots [s0, s1) are of this tile, or empty
-    while (s1 < 2 * kWarps && (sm_piece[s1].rows == 0 || sm_piece[s1].first == w.first)) ++s1;
-    const bool begun = w.first >= cta_begin, whole = begun && w.first + w.units <= cta_end;
-    const int part = (2 * blockIdx.x + begun) * R;
-    if (!whole) left[begun] = s0;
+    while (rest) {
+      const int s0 = __ffs(rest) - 1;
+      const Piece w = sm_piece[s0];
+      const unsigned group = __ballot_sync(0xffffffffu, there && mine.first == w.first);
+      rest &= ~group;
+      const bool begun = w.first >= cta_begin, whole = begun && w.first + w.units <= cta_end;
+      const int part = (2 * blockIdx.x + begun) * R;
+      if (!whole) left[begun] = s0;
 #pragma unroll 1
-    for (int r = warp; r < w.rows; r += kWarps) {
-      const int x = s0 + lane;
-      const bool there = x < s1 && sm_piece[x < 2 * kWarps ? x : 0].rows > 0;
-      const float m = there ? sm_m[x][r] : -INFINITY, M = warp_max(m);
-      const float f = m == -INFINITY ? 0.f : exp2_approx(m - M);
-      const float L = warp_add(there ? sm_l[x][r] * f : 0.f);
+      for (int r = 0; r < w.rows; ++r) {
+        if (task++ % kWarps != warp) continue;  // (the rows of all groups in turn)
+        const bool in = group >> lane & 1;
+        const float m = in ? sm_m[in ? lane : 0][r] : -INFINITY, M = warp_max(m);
+        const float f = m == -INFINITY ? 0.f : exp2_approx(m - M);
+        const float L = warp_add(in ? sm_l[in ? lane : 0][r] * f : 0.f);
 #pragma unroll
-      for (int i = 0; i < kDims; ++i) v[i] = 0.f;
-#pragma unroll 1
-      for (int y = s0; y < s1; ++y) {
-        const float fy = __shfl_sync(0xffffffffu, f, y - s0);
-        if (fy != 0.f) add(fy, sm_o + (y * R + r) * kPitch);
-      }
-      if (whole) {
-        put(w, r, L);
-      } else {
-        store(p.partial + (int64_t)(part + r) * D);
-        if (lane == 0) *reinterpret_cast<float2*>(p.partial_ml + 2 * (part + r)) = make_float2(M, L);
+        for (int i = 0; i < kDims; ++i) v[i] = 0.f;
+#pragma unroll
+        for (int y = 0; y < 2 * kWarps; ++y) {
+          const float fy = __shfl_sync(0xffffffffu, f, y);
+          if (fy != 0.f) add(fy, sm_o + (y * R + r) * kPitch);
+        }
+        if (whole) {
+          put(w, r, L);
+        } else {
+          store(p.partial + (int64_t)(part + r) * D);
+          if (lane == 0) *reinterpret_cast<float2*>(p.partial_ml + 2 * (part + r)) = make_float2(M, L);
+        }
       }
     }
-    s0 = s1;
   }
   if (left[0] < 0 && left[1] < 0) return;
   // the CTAs from that of a tile's first unit to that of its last; its counter is the first one's
-  __syncthreads();
-  if (threadIdx.x < 2 && left[threadIdx.x] >= 0) {
-    const Piece w = sm_piece[left[threadIdx.x]];
-    __threadfence();                            // (of everybody's stores: the barrier has put them before it)
+  int first_cta = 0, last_cta = 0;
+  const int shared = threadIdx.x < 2 ? left[threadIdx.x] : -1;
+  if (shared >= 0) {
+    const Piece w = sm_piece[shared];
     auto owner = [&](int64_t unit) {
       const int64_t n = (unit + 1) * warps - 1;
       return (int)(small ? (unsigned)n / (unsigned)total : n / total) / kWarps;
     };
-    const int first = owner(w.first), last = owner(w.first + w.units - 1);
-    const int n = atomicAdd(p.arrived + first, 1);
-    if (n == last - first) p.arrived[first] = 0;          // (as the next launch expects it)
-    __threadfence();
-    sm_first[threadIdx.x] = first;
-    sm_parts[threadIdx.x] = n == last - first ? n + 1 : 0;
+    first_cta = owner(w.first);
+    last_cta = owner(w.first + w.units - 1);
+  }
+  __syncthreads();
+  if (shared >= 0) {
+    int n;                                      // (everybody's stores: the barrier has put them before this thread's release)
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(n) : "l"(p.arrived + first_cta) : "memory");
+    const bool last = n == last_cta - first_cta;
+    if (last) p.arrived[first_cta] = 0;         // (as the next launch expects it)
+    sm_first[threadIdx.x] = first_cta;
+    sm_parts[threadIdx.x] = last ? n + 1 : 0;
   }
   __syncthreads();
 #pragma unroll 1

@@ -49,6 +49,7 @@ struct PromptParams {
   CUtensorMap tm_k, tm_v;                      // {D, page, kv_heads, pages}, box {64, page, 1, 1}, SWIZZLE_128B
   PagedAttnParams a;
   int tile_tokens;
+  int wide_out;                                // out is 32-byte aligned
   unsigned long long per_pair;                 // 2^40 / (tokens of a pair), rounded up: n of them divided exactly up to 2^32
   int* next;                                   // the next item, CTAs that are through
 };
@@ -141,68 +142,79 @@ struct Plan {
   __device__ __forceinline__ void find(const PromptParams& p, int index, int lane, Work& w) {
     const PagedAttnParams& a = p.a;
     const int h = index % a.c.kv_heads, rank = index / a.c.kv_heads;
-    // the largest x such that more than `rank` chunks belong to pairs with x blocks or more; ranks only grow, so it only falls: from the last
-    // one downwards in growing steps, then between
-    auto count = [&](int at) {
-      int n = 0;
+    int tile, n, in, cut = 0, parts = 0;
+    if (a.c.batch == 1) {                      // the order is the pairs' own, the last one first
+      n = chunks(kept[0]);
+      if (rank >= pairs(p, kept[0]) * n) return;
+      w.b = 0;
+      tile = pairs(p, kept[0]) - 1 - (n > 1 ? rank / n : rank);
+      in = n > 1 ? rank % n : 0;
+    } else {
+      // the largest x such that more than `rank` chunks belong to pairs with x blocks or more; ranks only grow, so it only falls: from the last
+      // one downwards in growing steps, then between
+      auto count = [&](int at) {
+        int n = 0;
 #pragma unroll 1
-      for (int b = lane; b < a.c.batch; b += 32) {
-        const Seq q = sequence(p, b);
-        n += at_least(p, q, at) * chunks(q);
-      }
-      return (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
-    };
-    int x = 0, above = level + 1, step = 1;
+        for (int b = lane; b < a.c.batch; b += 32) {
+          const Seq q = sequence(p, b);
+          n += at_least(p, q, at) * chunks(q);
+        }
+        return (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
+      };
+      int x = 0, above = level + 1, step = 1;
 #pragma unroll 1
-    while (above - x > 1) {
-      const int mid = x > 0 || step > above ? (x + above) >> 1 : max(above - step, 1);
-      const int n = count(mid);
-      step *= 2;
-      if (n > rank) {
-        x = mid;
-      } else {
-        above = mid;
-        behind = n;
+      while (above - x > 1) {
+        const int mid = x > 0 || step > above ? (x + above) >> 1 : max(above - step, 1);
+        const int n = count(mid);
+        step *= 2;
+        if (n > rank) {
+          x = mid;
+        } else {
+          above = mid;
+          behind = n;
+        }
       }
-    }
-    if (x == 0) return;
-    level = x;
-    int in = rank - behind;
+      if (x == 0) return;
+      level = x;
+      in = rank - behind;
 #pragma unroll 1
-    for (int b0 = 0;; b0 += 32) {              // (ends: there are more than `in` of them)
-      Seq q = {};
-      int here = 0;
-      if (b0 + lane < a.c.batch) {
-        q = sequence(p, b0 + lane);
-        here = (at_least(p, q, x) - at_least(p, q, x + 1)) * chunks(q);
+      for (int b0 = 0;; b0 += 32) {              // (ends: there are more than `in` of them)
+        Seq q = {};
+        int here = 0;
+        if (b0 + lane < a.c.batch) {
+          q = sequence(p, b0 + lane);
+          here = (at_least(p, q, x) - at_least(p, q, x + 1)) * chunks(q);
+        }
+        const int upto = warp_scan(here, lane);
+        const unsigned hit = __ballot_sync(0xffffffffu, upto > in);
+        if (hit) {
+          const int l = __ffs(hit) - 1;
+          in -= __shfl_sync(0xffffffffu, upto - here, l);
+          w.b = b0 + l;
+          break;
+        }
+        in -= __shfl_sync(0xffffffffu, upto, 31);
+        if (b0 + 32 >= a.c.batch) return;
       }
-      const int upto = warp_scan(here, lane);
-      const unsigned hit = __ballot_sync(0xffffffffu, upto > in);
-      if (hit) {
-        const int l = __ffs(hit) - 1;
-        in -= __shfl_sync(0xffffffffu, upto - here, l);
-        w.b = b0 + l;
-        break;
-      }
-      in -= __shfl_sync(0xffffffffu, upto, 31);
-      if (b0 + 32 >= a.c.batch) return;
+      const Seq q = sequence(p, w.b);
+      n = chunks(q);
+      tile = pairs(p, q) - at_least(p, q, x + 1) - 1 - (n > 1 ? in / n : in);
+      in = n > 1 ? in % n : 0;
+      // place in scratch memory: behind the cut pairs of the sequences in front
+      if (n > 1)
+#pragma unroll 1
+        for (int b = lane; b < w.b; b += 32) {
+          const Seq o = sequence(p, b);
+          if (chunks(o) > 1) {
+            cut += pairs(p, o);
+            parts += pairs(p, o) * chunks(o);
+          }
+        }
+      cut = (int)__reduce_add_sync(0xffffffffu, (unsigned)cut);
+      parts = (int)__reduce_add_sync(0xffffffffu, (unsigned)parts);
     }
     const Seq q = sequence(p, w.b);
     const Sequence s = {q.first, q.rows, q.base + q.rows};
-    const int n = chunks(q), tile = pairs(p, q) - at_least(p, q, x + 1) - 1 - in / n;
-    // place in scratch memory: behind the cut pairs of the sequences in front
-    int cut = 0, parts = 0;
-    if (n > 1)
-#pragma unroll 1
-      for (int b = lane; b < w.b; b += 32) {
-        const Seq o = sequence(p, b);
-        if (chunks(o) > 1) {
-          cut += pairs(p, o);
-          parts += pairs(p, o) * chunks(o);
-        }
-      }
-    cut = (int)__reduce_add_sync(0xffffffffu, (unsigned)cut);
-    parts = (int)__reduce_add_sync(0xffffffffu, (unsigned)parts);
     w.h = h;
     w.first = s.first;
     w.rows = s.rows;
@@ -210,13 +222,17 @@ struct Plan {
     w.length = s.length;
     w.token = tile * 2 * p.tile_tokens;
     w.chunks = n;
-    w.chunk = in % n;
+    w.chunk = in;
     w.cut_tile = ((cut + tile) * a.c.kv_heads + h) * 2;
     w.part = (parts + tile * n + w.chunk) * a.c.kv_heads + h;
     w.part_step = a.c.kv_heads;
     w.range.set(a, s, w.b, w.token, min(w.token + 2 * p.tile_tokens, s.rows) - 1);
-    w.u0 = (int)((int64_t)w.range.units * w.chunk / w.chunks);
-    w.u1 = (int)((int64_t)w.range.units * (w.chunk + 1) / w.chunks);
+    w.u0 = 0;
+    w.u1 = w.range.units;
+    if (n > 1) {
+      w.u0 = (int)((int64_t)w.range.units * w.chunk / n);
+      w.u1 = (int)((int64_t)w.range.units * (w.chunk + 1) / n);
+    }
 #pragma unroll 1
     for (int t = 0; t < 2; ++t) {
       const int from = w.token + t * p.tile_tokens;
@@ -435,179 +451,179 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kAuxRegs));
-  if (warp == 0) {
-    // ---------------------------------------------------------------------- TMA
-    const int per_page = 7 - a.c.page_log2, pages = 1 << per_page;       // of a block
-    uint32_t pos = 0, items = 0;
-    auto issued = [&]() {
-      if (lane == 0) mbar_arrive(&sm.issued);
-      work_done();
-    };
-    for (const Work* wp; (wp = next_work()) != nullptr; issued()) {
-      const Work& w = *wp;
-      if (w.u1 == w.u0) continue;
-      if (items > 0 && !wait_relaxed(&sm.q_empty, (items - 1) & 1, abort_flag, 2)) break;
-      ++items;
-      const int tiles = w.token + p.tile_tokens < w.rows ? 2 : 1;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&sm.q_full, (uint32_t)(tiles * kHalves * p.tile_tokens * a.group * 128));
-        for (int t = 0; t < tiles; ++t)
-          for (int i = 0; i < kHalves; ++i)
-            tma_load_3d(sm.q[t] + i * kHalfBytes, &p.tm_q, i * 64, w.h * a.group, w.first + w.token + t * p.tile_tokens, &sm.q_full);
-      }
-      // lane: page lane % pages of the block, dims 64 * (lane / pages); the page numbers a block ahead
-      const int in_block = lane & (pages - 1), half = lane >> per_page;
-      const int used = (w.length + (1 << a.c.page_log2) - 1) >> a.c.page_log2;
-      const Range<kBlock> range = w.range;
-      const int b = w.b, h = w.h, u1 = w.u1;
-      auto page_at = [&](int u) {
-        const int i = range.unit(u) * pages + in_block;
-        return i < used ? page_of(a.c, b, i) : a.c.pages;                 // (behind the last page: outside the map)
+    if (warp == 0) {
+      // ---------------------------------------------------------------------- TMA
+      const int per_page = 7 - a.c.page_log2, pages = 1 << per_page;       // of a block
+      uint32_t pos = 0, items = 0;
+      auto issued = [&]() {
+        if (lane == 0) mbar_arrive(&sm.issued);
+        work_done();
       };
-      int id = page_at(w.u0);
-      bool ok = true;
-      for (int u = w.u0; ok && u < u1; ++u) {
-        const int id_next = u + 1 < u1 ? page_at(u + 1) : 0;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          const uint32_t slot = pos % kStages, round = pos / kStages;
-          if (round > 0 && !wait_relaxed(&sm.empty[slot], (round - 1) & 1, abort_flag, 3)) { ok = false; break; }
-          if (lane == 0) mbar_arrive_expect_tx(&sm.full[slot], kBlockBytes);
-          __syncwarp();
-          if (half < kHalves)
-            tma_load_4d(sm.ring[slot] + half * kHalfBytes + (in_block << (a.c.page_log2 + 7)), kv ? &p.tm_v : &p.tm_k, half * 64, 0, h, id,
-                        &sm.full[slot]);
-          ++pos;
+      for (const Work* wp; (wp = next_work()) != nullptr; issued()) {
+        const Work& w = *wp;
+        if (w.u1 == w.u0) continue;
+        if (items > 0 && !wait_relaxed(&sm.q_empty, (items - 1) & 1, abort_flag, 2)) break;
+        ++items;
+        const int tiles = w.token + p.tile_tokens < w.rows ? 2 : 1;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&sm.q_full, (uint32_t)(tiles * kHalves * p.tile_tokens * a.group * 128));
+          for (int t = 0; t < tiles; ++t)
+            for (int i = 0; i < kHalves; ++i)
+              tma_load_3d(sm.q[t] + i * kHalfBytes, &p.tm_q, i * 64, w.h * a.group, w.first + w.token + t * p.tile_tokens, &sm.q_full);
         }
-        id = id_next;
-      }
-      if (!ok) break;
-    }
-  } else if (warp == 1) {
-    // ---------------------------------------------------------------------- MMA
-    const uint64_t dq = umma_desc_k128(smem_u32(sm.q[0]));
-    const uint64_t dk = umma_desc_k128(smem_u32(sm.ring[0]));
-    const uint64_t dv = umma_desc_mn128(smem_u32(sm.ring[0]), kHalfBytes);
-    constexpr uint32_t kStep = kBlockBytes >> 4, kHalfStep = kHalfBytes >> 4;
-    uint32_t pos = 0, vblocks = 0, items = 0, n_p[2] = {0, 0}, n_o[2] = {0, 0};
-    auto scores = [&](int t, uint32_t slot) {
+        // lane: page lane % pages of the block, dims 64 * (lane / pages); the page numbers a block ahead
+        const int in_block = lane & (pages - 1), half = lane >> per_page;
+        const int used = (w.length + (1 << a.c.page_log2) - 1) >> a.c.page_log2;
+        const Range<kBlock> range = w.range;
+        const int b = w.b, h = w.h, u1 = w.u1;
+        auto page_at = [&](int u) {
+          const int i = range.unit(u) * pages + in_block;
+          return i < used ? page_of(a.c, b, i) : a.c.pages;                 // (behind the last page: outside the map)
+        };
+        int id = page_at(w.u0);
+        bool ok = true;
+        for (int u = w.u0; ok && u < u1; ++u) {
+          const int id_next = u + 1 < u1 ? page_at(u + 1) : 0;
 #pragma unroll
-      for (int i = 0; i < kHalves; ++i)
-        mma4_ss(tmem + t * 128, dq + t * kStep + i * kHalfStep, dk + (uint64_t)(slot * kStep) + i * kHalfStep, kIdescS, i > 0);
-      umma_commit(&sm.s_full[t]);
-    };
-    bool ok = true;
-    for (const Work* wp; ok && (wp = next_work()) != nullptr; work_done()) {
-      const int u0 = wp->u0, u1 = wp->u1, last[2] = {wp->last[0], wp->last[1]};
-      const Sight sees[2] = {Sight(*wp, 0), Sight(*wp, 1)};
-      if (u1 == u0) continue;
-      if (!wait(&sm.q_full, items & 1, abort_flag, 4)) break;
-      ++items;
-      bool begun[2] = {false, false};
-      uint32_t slot = pos % kStages;
-      if (!wait(&sm.full[slot], (pos / kStages) & 1, abort_flag, 5)) break;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-        if (sees[t](u0)) scores(t, slot);
-      umma_commit(&sm.empty[slot]);
-      if (u1 - u0 == 1) umma_commit(&sm.q_empty);
-      ++pos;
-      for (int u = u0; ok && u < u1; ++u) {
-        const uint32_t vslot = pos % kStages;
-        ++pos;
-        const bool more = u + 1 < u1;
-        const uint32_t kslot = pos % kStages, kround = pos / kStages;
-        bool keys = false;
-        ok = wait(&sm.ready[vblocks % kReady], (vblocks / kReady) & 1, abort_flag, 6);
-        ++vblocks;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (ok && sees[t](u)) {
-            if (!begun[t] && n_o[t] > 0) ok = wait(&sm.o_empty[t], (n_o[t] - 1) & 1, abort_flag, 7);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {         // (the first half's products run beside the second half's weights)
-              ok = ok && wait(&sm.p_ready[t][h], n_p[t] & 1, abort_flag, 8);
-              if (!ok) break;
-              tc_fence_after_sync();
-              mma4_ts(tmem + 256 + t * D, tmem + t * 128 + 32 * h, dv + (uint64_t)(vslot * kStep) + h * 512, kIdescO, begun[t] || h > 0);
-            }
-            begun[t] = true;
-            ++n_p[t];
-            if (ok && u == last[t]) {
-              umma_commit(&sm.o_full[t]);
-              ++n_o[t];
-            }
+          for (int kv = 0; kv < 2; ++kv) {
+            const uint32_t slot = pos % kStages, round = pos / kStages;
+            if (round > 0 && !wait_relaxed(&sm.empty[slot], (round - 1) & 1, abort_flag, 3)) { ok = false; break; }
+            if (lane == 0) mbar_arrive_expect_tx(&sm.full[slot], kBlockBytes);
+            __syncwarp();
+            if (half < kHalves)
+              tma_load_4d(sm.ring[slot] + half * kHalfBytes + (in_block << (a.c.page_log2 + 7)), kv ? &p.tm_v : &p.tm_k, half * 64, 0, h, id,
+                          &sm.full[slot]);
+            ++pos;
           }
-          if (ok && more && sees[t](u + 1)) {
-            if (!keys) ok = wait(&sm.full[kslot], kround & 1, abort_flag, 9);
-            keys = true;
-            if (ok) scores(t, kslot);
-          }
+          id = id_next;
         }
-        if (ok && more && !keys) ok = wait(&sm.full[kslot], kround & 1, abort_flag, 9);
         if (!ok) break;
-        umma_commit(&sm.empty[vslot]);
-        if (more) {
-          umma_commit(&sm.empty[kslot]);
-          if (u + 2 == u1) umma_commit(&sm.q_empty);
+      }
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------------- MMA
+      const uint64_t dq = umma_desc_k128(smem_u32(sm.q[0]));
+      const uint64_t dk = umma_desc_k128(smem_u32(sm.ring[0]));
+      const uint64_t dv = umma_desc_mn128(smem_u32(sm.ring[0]), kHalfBytes);
+      constexpr uint32_t kStep = kBlockBytes >> 4, kHalfStep = kHalfBytes >> 4;
+      uint32_t pos = 0, vblocks = 0, items = 0, n_p[2] = {0, 0}, n_o[2] = {0, 0};
+      auto scores = [&](int t, uint32_t slot) {
+#pragma unroll
+        for (int i = 0; i < kHalves; ++i)
+          mma4_ss(tmem + t * 128, dq + t * kStep + i * kHalfStep, dk + (uint64_t)(slot * kStep) + i * kHalfStep, kIdescS, i > 0);
+        umma_commit(&sm.s_full[t]);
+      };
+      bool ok = true;
+      for (const Work* wp; ok && (wp = next_work()) != nullptr; work_done()) {
+        const int u0 = wp->u0, u1 = wp->u1, last[2] = {wp->last[0], wp->last[1]};
+        const Sight sees[2] = {Sight(*wp, 0), Sight(*wp, 1)};
+        if (u1 == u0) continue;
+        if (!wait(&sm.q_full, items & 1, abort_flag, 4)) break;
+        ++items;
+        bool begun[2] = {false, false};
+        uint32_t slot = pos % kStages;
+        if (!wait(&sm.full[slot], (pos / kStages) & 1, abort_flag, 5)) break;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (sees[t](u0)) scores(t, slot);
+        umma_commit(&sm.empty[slot]);
+        if (u1 - u0 == 1) umma_commit(&sm.q_empty);
+        ++pos;
+        for (int u = u0; ok && u < u1; ++u) {
+          const uint32_t vslot = pos % kStages;
           ++pos;
-        }
-      }
-    }
-  } else if (warp == 2) {
-    // ---------------------------------------------------------------------- values that nobody sees: 0 * NaN is NaN
-    uint32_t pos = 0, vblocks = 0;
-    bool ok = true;
-    for (const Work* wp; ok && (wp = next_work()) != nullptr; work_done()) {
-      const Range<kBlock> range = wp->range;
-      const int u1 = wp->u1;
-      for (int u = wp->u0; u < u1; ++u, pos += 2) {
-        const uint32_t slot = (pos + 1) % kStages, round = (pos + 1) / kStages;
-        if (!wait_relaxed(&sm.full[slot], round & 1, abort_flag, 10)) { ok = false; break; }
-        const int from = range.unit(u) * kBlock;
-        const bool whole = from + kBlock <= range.pre || (from >= range.low && from + kBlock <= range.high);
-        if (!whole) {
-          for (int i = lane; i < kBlock * 8 * kHalves; i += 32) {
-            const int token = from + ((i >> 3) & (kBlock - 1));
-            if (!(token < range.pre || (token >= range.low && token < range.high)))
-              reinterpret_cast<uint4*>(sm.ring[slot])[i] = make_uint4(0, 0, 0, 0);
+          const bool more = u + 1 < u1;
+          const uint32_t kslot = pos % kStages, kround = pos / kStages;
+          bool keys = false;
+          ok = wait(&sm.ready[vblocks % kReady], (vblocks / kReady) & 1, abort_flag, 6);
+          ++vblocks;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (ok && sees[t](u)) {
+              if (!begun[t] && n_o[t] > 0) ok = wait(&sm.o_empty[t], (n_o[t] - 1) & 1, abort_flag, 7);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {         // (the first half's products run beside the second half's weights)
+                ok = ok && wait(&sm.p_ready[t][h], n_p[t] & 1, abort_flag, 8);
+                if (!ok) break;
+                tc_fence_after_sync();
+                mma4_ts(tmem + 256 + t * D, tmem + t * 128 + 32 * h, dv + (uint64_t)(vslot * kStep) + h * 512, kIdescO, begun[t] || h > 0);
+              }
+              begun[t] = true;
+              ++n_p[t];
+              if (ok && u == last[t]) {
+                umma_commit(&sm.o_full[t]);
+                ++n_o[t];
+              }
+            }
+            if (ok && more && sees[t](u + 1)) {
+              if (!keys) ok = wait(&sm.full[kslot], kround & 1, abort_flag, 9);
+              keys = true;
+              if (ok) scores(t, kslot);
+            }
           }
-          fence_proxy_async_smem();
-          __syncwarp();
+          if (ok && more && !keys) ok = wait(&sm.full[kslot], kround & 1, abort_flag, 9);
+          if (!ok) break;
+          umma_commit(&sm.empty[vslot]);
+          if (more) {
+            umma_commit(&sm.empty[kslot]);
+            if (u + 2 == u1) umma_commit(&sm.q_empty);
+            ++pos;
+          }
         }
-        if (lane == 0) mbar_arrive(&sm.ready[vblocks % kReady]);
-        ++vblocks;
+      }
+    } else if (warp == 2) {
+      // ---------------------------------------------------------------------- values that nobody sees: 0 * NaN is NaN
+      uint32_t pos = 0, vblocks = 0;
+      bool ok = true;
+      for (const Work* wp; ok && (wp = next_work()) != nullptr; work_done()) {
+        const Range<kBlock> range = wp->range;
+        const int u1 = wp->u1;
+        for (int u = wp->u0; u < u1; ++u, pos += 2) {
+          const uint32_t slot = (pos + 1) % kStages, round = (pos + 1) / kStages;
+          if (!wait_relaxed(&sm.full[slot], round & 1, abort_flag, 10)) { ok = false; break; }
+          const int from = range.unit(u) * kBlock;
+          const bool whole = from + kBlock <= range.pre || (from >= range.low && from + kBlock <= range.high);
+          if (!whole) {
+            for (int i = lane; i < kBlock * 8 * kHalves; i += 32) {
+              const int token = from + ((i >> 3) & (kBlock - 1));
+              if (!(token < range.pre || (token >= range.low && token < range.high)))
+                reinterpret_cast<uint4*>(sm.ring[slot])[i] = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          if (lane == 0) mbar_arrive(&sm.ready[vblocks % kReady]);
+          ++vblocks;
+        }
+      }
+    } else {
+      // ---------------------------------------------------------------------- the work, longest tiles first
+      Plan plan(p, lane, sm.kept);
+      for (uint32_t i = 0;; ++i) {
+        const uint32_t slot = i % kWorks, round = i / kWorks;
+        if (round > 0 && !wait_relaxed(&sm.work_empty[slot], (round - 1) & 1, abort_flag, 11)) break;
+        // the next item is taken when this one's loads are all on their way, two or three blocks before its end: taken earlier, the CTA with
+        // the longest item would get one of the second longest too
+        if (i > 0 && !wait_relaxed(&sm.issued, (i - 1) & 1, abort_flag, 15)) break;
+        int index = blockIdx.x;
+        if (i > 0) {
+          if (lane == 0) index = gridDim.x + atomicAdd(p.next, 1);
+          index = __shfl_sync(0xffffffffu, index, 0);
+        }
+        Work w;
+        w.b = -1;
+        plan.find(p, index, lane, w);
+        if (lane == 0) {
+          sm.work[slot] = w;
+          mbar_arrive(&sm.work_full[slot]);
+        }
+        if (w.b < 0) break;
+      }
+      // the CTA that comes last leaves the counters as the next launch expects them
+      if (lane == 0 && atomicAdd(p.next + 1, 1) == (int)gridDim.x - 1) {
+        p.next[0] = 0;
+        p.next[1] = 0;
       }
     }
-  } else {
-    // ---------------------------------------------------------------------- the work, longest tiles first
-    Plan plan(p, lane, sm.kept);
-    for (uint32_t i = 0;; ++i) {
-      const uint32_t slot = i % kWorks, round = i / kWorks;
-      if (round > 0 && !wait_relaxed(&sm.work_empty[slot], (round - 1) & 1, abort_flag, 11)) break;
-      // the next item is taken when this one's loads are all on their way, two or three blocks before its end: taken earlier, the CTA with
-      // the longest item would get one of the second longest too
-      if (i > 0 && !wait_relaxed(&sm.issued, (i - 1) & 1, abort_flag, 15)) break;
-      int index = blockIdx.x;
-      if (i > 0) {
-        if (lane == 0) index = gridDim.x + atomicAdd(p.next, 1);
-        index = __shfl_sync(0xffffffffu, index, 0);
-      }
-      Work w;
-      w.b = -1;
-      plan.find(p, index, lane, w);
-      if (lane == 0) {
-        sm.work[slot] = w;
-        mbar_arrive(&sm.work_full[slot]);
-      }
-      if (w.b < 0) break;
-    }
-    // the CTA that comes last leaves the counters as the next launch expects them
-    if (lane == 0 && atomicAdd(p.next + 1, 1) == (int)gridDim.x - 1) {
-      p.next[0] = 0;
-      p.next[1] = 0;
-    }
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegs));
     // ---------------------------------------------------------------------- the rows
@@ -823,12 +839,16 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
             }
             if (mine) {
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                uint32_t v[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  v[k] = some ? pack2(T(), __uint_as_float(o[h][8 * j + 2 * k]) * inv, __uint_as_float(o[h][8 * j + 2 * k + 1]) * inv) : 0u;
-                reinterpret_cast<uint4*>(out)[2 * (i + h) + j] = make_uint4(v[0], v[1], v[2], v[3]);
+              for (int j = 0; j < 8; ++j)
+                o[h][j] = some ? pack2(T(), __uint_as_float(o[h][2 * j]) * inv, __uint_as_float(o[h][2 * j + 1]) * inv) : 0u;
+              uint4* to = reinterpret_cast<uint4*>(out) + 2 * (i + h);
+              if (p.wide_out) {                  // (whole sectors: every lane has another row)
+                asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(o[h][0]), "r"(o[h][1]), "r"(o[h][2]), "r"(o[h][3]),
+                             "r"(o[h][4]), "r"(o[h][5]), "r"(o[h][6]), "r"(o[h][7])
+                             : "memory");
+              } else {
+                to[0] = make_uint4(o[h][0], o[h][1], o[h][2], o[h][3]);
+                to[1] = make_uint4(o[h][4], o[h][5], o[h][6], o[h][7]);
               }
             }
           }
@@ -935,6 +955,7 @@ int launch_paged_prompt(const char* who, const B200PagedCache* c, PagedAttnParam
     if ((rc = make_tmap(v ? &p.tm_v : &p.tm_k, type, 4, v ? c->v_pages : c->k_pages, d, s, b, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
   }
   a.slots = sm_count();
+  p.wide_out = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0;
   p.per_pair = ((1ull << 40) + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
   p.next = a.arrived + kCutTiles;
   p.a = a;
