@@ -370,15 +370,6 @@ paged_decode_kernel(const PagedAttnParams p) {
   __syncthreads();
   constexpr int kDims = D / 32;
   float v[kDims];
-  auto add = [&](float f, const float* from) {
-    if (kDims == 4) {
-      const float4 o = *reinterpret_cast<const float4*>(from + 4 * lane);
-      v[0] = fmaf(f, o.x, v[0]); v[1] = fmaf(f, o.y, v[1]); v[kDims - 2] = fmaf(f, o.z, v[kDims - 2]); v[kDims - 1] = fmaf(f, o.w, v[kDims - 1]);
-    } else {
-      const float2 o = *reinterpret_cast<const float2*>(from + 2 * lane);
-      v[0] = fmaf(f, o.x, v[0]); v[1] = fmaf(f, o.y, v[1]);
-    }
-  };
   auto store = [&](float* to) {
     if (kDims == 4) *reinterpret_cast<float4*>(to + 4 * lane) = make_float4(v[0], v[1], v[kDims - 2], v[kDims - 1]);
     else *reinterpret_cast<float2*>(to + 2 * lane) = make_float2(v[0], v[1]);
@@ -424,12 +415,25 @@ paged_decode_kernel(const PagedAttnParams p) {
         const float m = in ? sm_m[in ? lane : 0][r] : -INFINITY, M = warp_max(m);
         const float f = m == -INFINITY ? 0.f : exp2_approx(m - M);
         const float L = warp_add(in ? sm_l[in ? lane : 0][r] * f : 0.f);
+        float o[2 * kWarps][kDims];
+#pragma unroll
+        for (int y = 0; y < 2 * kWarps; ++y) {  // (all at once; what is in the places of no piece is not used)
+          const float* from = sm_o + (y * R + r) * kPitch + kDims * lane;
+          if (kDims == 4) {
+            const float4 q = *reinterpret_cast<const float4*>(from);
+            o[y][0] = q.x; o[y][1] = q.y; o[y][kDims - 2] = q.z; o[y][kDims - 1] = q.w;
+          } else {
+            const float2 q = *reinterpret_cast<const float2*>(from);
+            o[y][0] = q.x; o[y][1] = q.y;
+          }
+        }
 #pragma unroll
         for (int i = 0; i < kDims; ++i) v[i] = 0.f;
 #pragma unroll
         for (int y = 0; y < 2 * kWarps; ++y) {
           const float fy = __shfl_sync(0xffffffffu, f, y);
-          if (fy != 0.f) add(fy, sm_o + (y * R + r) * kPitch);
+#pragma unroll
+          for (int i = 0; i < kDims; ++i) v[i] = fy != 0.f ? fmaf(fy, o[y][i], v[i]) : v[i];
         }
         if (whole) {
           put(w, r, L);
