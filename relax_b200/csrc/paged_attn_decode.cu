@@ -1,8 +1,8 @@
 // Attention of a few rows (query heads of one key head x new tokens) over a paged key-value cache, split over the length and joined.
 //
 // Work: the rows of a sequence that share a key head are a tile of R = 8 or 16 (more rows than that: several tiles).  The keys that a
-// tile can see (a prefix and a range behind it) are units of 16 tokens.  All units, in the order sequence, tile, key head, unit, are
-// divided evenly among the warps that the GPU holds at once, on the device, from the lengths: any mixture of lengths is balanced, and
+// tile can see (a prefix and a range behind it) are units of 16 tokens, and a few more stand for its beginning.  All units, in the order
+// sequence, tile, key head, unit, are divided evenly among the warps that the GPU holds at once, on the device, from the lengths: any mixture of lengths is balanced, and
 // what the host knows is a bound only.  A warp's share is a part of one tile or the end of one, whole ones, and the beginning of another.
 // A whole tile goes out from registers; parts are added up in shared memory, and those of tiles that several CTAs share in scratch memory,
 // by the CTA that arrives last, in the order of the parts (the same bits whoever comes last).
@@ -18,8 +18,8 @@
 // stay below 2^8, fp32 sums take that.  Weights are rounded to the cache's type for the product with V.
 //
 // What bounds it: HBM for long caches (131000 tokens of 8 key heads, 537 MB, 89 us: 6.0 TB/s, 0.92 of a copy; 64 sequences of 37 to 2047
-// tokens, 135 MB, 35 us: 3.9); latency for short ones (32 heads at 2011, 33 MB, 16.6 us: 2 until the shares are known, 7.6 for two or three
-// units a warp, 7 for the joins).  Before, chunks of equal length as CTAs of their own took 157, 45 and 17.5 us.
+// tokens, 135 MB, 31 us: 4.4); latency for short ones (32 heads at 2011, 33 MB, 13.4 us: 2 until the shares are known, 7 for two or three
+// units a warp, 4 for the joins).  Before, chunks of equal length as CTAs of their own took 157, 45 and 17.5 us.
 #include "paged_common.cuh"
 
 namespace b200 {
@@ -28,6 +28,9 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kUnit = 16;
+// A tile's beginning (its queries, the first page numbers, the way to its first keys) counts as so many units of its share: 0, 1, 2, 4 units
+// 15.1, 14.1, 13.8, 13.2 us for 32 heads at 2011, 34.3, 31.4, 30.7, 31.0 for 64 ragged sequences, 23.8, 23.8, 22.5, 22.3 for 33 with a window.
+constexpr int kStart = 3;
 constexpr int kCtasPerSm1 = 3, kCtasPerSm2 = 2;       // of tiles of 8 rows, of 16
 __device__ __forceinline__ void mma(__half, float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -79,7 +82,7 @@ paged_decode_kernel(const PagedAttnParams p) {
     const int tiles = tiles_of(x);
     Range<kUnit> r;
     r.set(p, x, i, 0, x.rows - 1);
-    per_tile = tiles > 0 ? max(r.units, 1) : 0;           // (rows that see nothing have a result too)
+    per_tile = tiles > 0 ? kStart + max(r.units, 1) : 0;  // (rows that see nothing have a result too)
     return (int64_t)per_tile * tiles * kv;
   };
   int64_t mine = 0;
@@ -138,224 +141,227 @@ paged_decode_kernel(const PagedAttnParams p) {
 
   int pieces = 0;
   while (at < end) {
-    // ---- a part of one tile: units [u_begin, u_end) of per_tile ---------------------------------------------------------------
+    // ---- a part of one tile: units [u_begin, u_end) of all of its ---------------------------------------------------------------
     const Sequence s = sequence_of(p.c, b);
-    const int in_seq = (int)(at - before), index = in_seq / per_tile, u_begin = in_seq - index * per_tile;
-    const int u_end = (int)min((int64_t)per_tile, u_begin + (end - at));
-    const int tile = index / kv, h = index - tile * kv;
-    const int rows = s.rows * p.group, row0 = tile * R, nrows = min(rows - row0, R);
-    const int base = s.length - s.rows;
-    const int position0 = base + row0 / p.group, position1 = base + (row0 + nrows - 1) / p.group;
-    Range<kUnit> range;
-    range.set(p, s, b, 0, s.rows - 1);
+    const int in_seq = (int)(at - before), index = in_seq / per_tile, v_begin = in_seq - index * per_tile;
+    const int v_end = (int)min((int64_t)per_tile, v_begin + (end - at));
+    const int u_begin = max(v_begin - kStart, 0), u_end = v_end - kStart, units = per_tile - kStart;
+    if (u_end > 0) {
+      const int tile = index / kv, h = index - tile * kv;
+      const int rows = s.rows * p.group, row0 = tile * R, nrows = min(rows - row0, R);
+      const int base = s.length - s.rows;
+      const int position0 = base + row0 / p.group, position1 = base + (row0 + nrows - 1) / p.group;
+      Range<kUnit> range;
+      range.set(p, s, b, 0, s.rows - 1);
 
-    const T* kbase = static_cast<const T*>(p.c.k) + (int64_t)h * page * D + 8 * t;
-    const T* vbase = static_cast<const T*>(p.c.v) + (int64_t)h * page * D + 8 * g;
-    // units of step i; past the end the last one stands in and is masked
-    auto unit_at = [&](int i, int sub) { return range.unit(min(u_begin + i * SUB + sub, u_end - 1)); };
-    auto page_at = [&](int i, int sub) { return page_of(p.c, b, unit_at(i, sub) >> (p.c.page_log2 - 4)); };
-    uint4 kr[SUB][2][KC], vr[SUB][4][VC];
-    auto load_k = [&](int i, const int (&id)[SUB]) {
+      const T* kbase = static_cast<const T*>(p.c.k) + (int64_t)h * page * D + 8 * t;
+      const T* vbase = static_cast<const T*>(p.c.v) + (int64_t)h * page * D + 8 * g;
+      // units of step i; past the end the last one stands in and is masked
+      auto unit_at = [&](int i, int sub) { return range.unit(min(u_begin + i * SUB + sub, u_end - 1)); };
+      auto page_at = [&](int i, int sub) { return page_of(p.c, b, unit_at(i, sub) >> (p.c.page_log2 - 4)); };
+      uint4 kr[SUB][2][KC], vr[SUB][4][VC];
+      auto load_k = [&](int i, const int (&id)[SUB]) {
 #pragma unroll
-      for (int x = 0; x < SUB; ++x) {
-        const T* src = kbase + id[x] * p.c.k_stride + (int64_t)((unit_at(i, x) * kUnit) & (page - 1)) * D;
+        for (int x = 0; x < SUB; ++x) {
+          const T* src = kbase + id[x] * p.c.k_stride + (int64_t)((unit_at(i, x) * kUnit) & (page - 1)) * D;
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+          for (int r = 0; r < 2; ++r)
 #pragma unroll
-          for (int j = 0; j < KC; ++j) kr[x][r][j] = load16(src + (g + 8 * r) * D + 32 * j);
+            for (int j = 0; j < KC; ++j) kr[x][r][j] = load16(src + (g + 8 * r) * D + 32 * j);
+        }
+      };
+      auto load_v = [&](int i, const int (&id)[SUB]) {
+#pragma unroll
+        for (int x = 0; x < SUB; ++x) {
+          const T* src = vbase + id[x] * p.c.v_stride + (int64_t)((unit_at(i, x) * kUnit) & (page - 1)) * D;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < VC; ++j) vr[x][r][j] = load16(src + (2 * t + (r & 1) + 8 * (r >> 1)) * D + 64 * j);
+        }
+      };
+      const int steps = (u_end - u_begin + SUB - 1) / SUB;
+      int id[SUB];
+#pragma unroll
+      for (int x = 0; x < SUB; ++x) id[x] = page_at(0, x);
+      // queries: the B operand's row g of a tile of eight
+      uint4 qf[NT][KC];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int r = row0 + 8 * n + g;
+        const T* src = static_cast<const T*>(p.q) + (int64_t)(s.first + r / p.group) * p.q_stride + (int64_t)(h * p.group + r % p.group) * D;
+#pragma unroll
+        for (int j = 0; j < KC; ++j) qf[n][j] = 8 * n + g < nrows ? load16(src + 32 * j + 8 * t) : make_uint4(0, 0, 0, 0);
       }
-    };
-    auto load_v = [&](int i, const int (&id)[SUB]) {
+      load_k(0, id);
+      load_v(0, id);
 #pragma unroll
-      for (int x = 0; x < SUB; ++x) {
-        const T* src = vbase + id[x] * p.c.v_stride + (int64_t)((unit_at(i, x) * kUnit) & (page - 1)) * D;
+      for (int x = 0; x < SUB; ++x) id[x] = 1 < steps ? page_at(1, x) : 0;
+      // this lane's rows in the accumulators: 8 n + 2 t + e
+      int position[NT][2];
+      float slope[NT][2];
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int j = 0; j < VC; ++j) vr[x][r][j] = load16(src + (2 * t + (r & 1) + 8 * (r >> 1)) * D + 64 * j);
+        for (int e = 0; e < 2; ++e) {
+          const int r = row0 + 8 * n + 2 * t + e;
+          position[n][e] = r < rows ? base + r / p.group : -1;
+          slope[n][e] = kExtra && p.slopes && r < rows ? p.slopes[h * p.group + r % p.group] * kLog2e : 0.f;
+        }
+      float m[NT][2], l[NT][2], acc[NT][MT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) { m[n][e] = -INFINITY; l[n][e] = 0.f; }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[n][i][j] = 0.f;
       }
-    };
-    const int steps = (u_end - u_begin + SUB - 1) / SUB;
-    int id[SUB];
-#pragma unroll
-    for (int x = 0; x < SUB; ++x) id[x] = page_at(0, x);
-    // queries: the B operand's row g of a tile of eight
-    uint4 qf[NT][KC];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int r = row0 + 8 * n + g;
-      const T* src = static_cast<const T*>(p.q) + (int64_t)(s.first + r / p.group) * p.q_stride + (int64_t)(h * p.group + r % p.group) * D;
-#pragma unroll
-      for (int j = 0; j < KC; ++j) qf[n][j] = 8 * n + g < nrows ? load16(src + 32 * j + 8 * t) : make_uint4(0, 0, 0, 0);
-    }
-    load_k(0, id);
-    load_v(0, id);
-#pragma unroll
-    for (int x = 0; x < SUB; ++x) id[x] = 1 < steps ? page_at(1, x) : 0;
-    // this lane's rows in the accumulators: 8 n + 2 t + e
-    int position[NT][2];
-    float slope[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = row0 + 8 * n + 2 * t + e;
-        position[n][e] = r < rows ? base + r / p.group : -1;
-        slope[n][e] = kExtra && p.slopes && r < rows ? p.slopes[h * p.group + r % p.group] * kLog2e : 0.f;
-      }
-    float m[NT][2], l[NT][2], acc[NT][MT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) { m[n][e] = -INFINITY; l[n][e] = 0.f; }
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[n][i][j] = 0.f;
-    }
 #pragma unroll 1
-    for (int i = 0; i < steps; ++i) {
-      const bool more = i + 1 < steps;
-      int id_next[SUB];
+      for (int i = 0; i < steps; ++i) {
+        const bool more = i + 1 < steps;
+        int id_next[SUB];
 #pragma unroll
-      for (int x = 0; x < SUB; ++x) id_next[x] = i + 2 < steps ? page_at(i + 2, x) : 0;
-      // scores of tokens g (0, 1) and g + 8 (2, 3), rows 2 t (0, 2) and 2 t + 1 (1, 3)
-      float sc[SUB][NT][4];
+        for (int x = 0; x < SUB; ++x) id_next[x] = i + 2 < steps ? page_at(i + 2, x) : 0;
+        // scores of tokens g (0, 1) and g + 8 (2, 3), rows 2 t (0, 2) and 2 t + 1 (1, 3)
+        float sc[SUB][NT][4];
 #pragma unroll
-      for (int x = 0; x < SUB; ++x)
+        for (int x = 0; x < SUB; ++x)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+          for (int n = 0; n < NT; ++n) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) sc[x][n][j] = 0.f;
+            for (int j = 0; j < 4; ++j) sc[x][n][j] = 0.f;
 #pragma unroll
-          for (int j = 0; j < KC; ++j) {
-            mma(T(), sc[x][n], kr[x][0][j].x, kr[x][1][j].x, kr[x][0][j].y, kr[x][1][j].y, qf[n][j].x, qf[n][j].y);
-            mma(T(), sc[x][n], kr[x][0][j].z, kr[x][1][j].z, kr[x][0][j].w, kr[x][1][j].w, qf[n][j].z, qf[n][j].w);
-          }
-        }
-      if (more) load_k(i + 1, id);
-      bool above = false;
-#pragma unroll
-      for (int x = 0; x < SUB; ++x) {
-        const int first = unit_at(i, x) * kUnit;
-        const bool there = u_begin + i * SUB + x < u_end;
-        // every row sees the whole unit (rows past the tile's end come out as something finite that nobody stores)
-        const bool whole = there && position0 >= 0 &&
-                           (first + kUnit <= range.pre || (first + kUnit - 1 <= position0 && position1 - first < window));
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int token = first + g + 8 * (j >> 1), at = position[n][j & 1];
-            float v = sc[x][n][j];
-            if (kExtra && p.cap > 0.f) v = cap_log2 * (1.f - __fdividef(2.f, exp2_approx(v * cap_in) + 1.f));
-            else v *= to_log2;
-            if (kExtra) v -= slope[n][j & 1] * fabsf((float)(at - token));
-            if (!whole) {
-              const bool seen = there && at >= 0 && (token < range.pre || (token <= at && at - token < window));
-              if (!seen) v = -INFINITY;
+            for (int j = 0; j < KC; ++j) {
+              mma(T(), sc[x][n], kr[x][0][j].x, kr[x][1][j].x, kr[x][0][j].y, kr[x][1][j].y, qf[n][j].x, qf[n][j].y);
+              mma(T(), sc[x][n], kr[x][0][j].z, kr[x][1][j].z, kr[x][0][j].w, kr[x][1][j].w, qf[n][j].z, qf[n][j].w);
             }
-            sc[x][n][j] = v;
-            above |= v > m[n][j & 1] + kSlack;
           }
-        if (!whole) {                             // what nobody sees may be anything, and 0 * NaN is NaN
+        if (more) load_k(i + 1, id);
+        bool above = false;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int token = first + 2 * t + (r & 1) + 8 * (r >> 1);
-            if (!(there && (token < range.pre || (token >= range.low && token < range.high))))
+        for (int x = 0; x < SUB; ++x) {
+          const int first = unit_at(i, x) * kUnit;
+          const bool there = u_begin + i * SUB + x < u_end;
+          // every row sees the whole unit (rows past the tile's end come out as something finite that nobody stores)
+          const bool whole = there && position0 >= 0 &&
+                             (first + kUnit <= range.pre || (first + kUnit - 1 <= position0 && position1 - first < window));
 #pragma unroll
-              for (int j = 0; j < VC; ++j) vr[x][r][j] = make_uint4(0, 0, 0, 0);
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int token = first + g + 8 * (j >> 1), at = position[n][j & 1];
+              float v = sc[x][n][j];
+              if (kExtra && p.cap > 0.f) v = cap_log2 * (1.f - __fdividef(2.f, exp2_approx(v * cap_in) + 1.f));
+              else v *= to_log2;
+              if (kExtra) v -= slope[n][j & 1] * fabsf((float)(at - token));
+              if (!whole) {
+                const bool seen = there && at >= 0 && (token < range.pre || (token <= at && at - token < window));
+                if (!seen) v = -INFINITY;
+              }
+              sc[x][n][j] = v;
+              above |= v > m[n][j & 1] + kSlack;
+            }
+          if (!whole) {                             // what nobody sees may be anything, and 0 * NaN is NaN
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int token = first + 2 * t + (r & 1) + 8 * (r >> 1);
+              if (!(there && (token < range.pre || (token >= range.low && token < range.high))))
+#pragma unroll
+                for (int j = 0; j < VC; ++j) vr[x][r][j] = make_uint4(0, 0, 0, 0);
+            }
           }
         }
-      }
-      if (__any_sync(0xffffffffu, above)) {
+        if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float v = m[n][e];
+            for (int e = 0; e < 2; ++e) {
+              float v = m[n][e];
 #pragma unroll
-            for (int x = 0; x < SUB; ++x) v = fmaxf(v, fmaxf(sc[x][n][e], sc[x][n][e + 2]));
+              for (int x = 0; x < SUB; ++x) v = fmaxf(v, fmaxf(sc[x][n][e], sc[x][n][e + 2]));
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-            const float f = v == -INFINITY ? 1.f : exp2_approx(m[n][e] - v);
-            m[n][e] = v;
-            l[n][e] *= f;
+              for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+              const float f = v == -INFINITY ? 1.f : exp2_approx(m[n][e] - v);
+              m[n][e] = v;
+              l[n][e] *= f;
 #pragma unroll
-            for (int k = 0; k < MT; ++k) { acc[n][k][e] *= f; acc[n][k][e + 2] *= f; }
-          }
-      }
-#pragma unroll
-      for (int x = 0; x < SUB; ++x) {
-        uint32_t pb[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float w[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            w[j] = sc[x][n][j] == -INFINITY ? 0.f : exp2_approx(sc[x][n][j] - m[n][j & 1]);
-            l[n][j & 1] += w[j];
-          }
-          pb[n][0] = transpose8x8(pack2(T(), w[0], w[1]));
-          pb[n][1] = transpose8x8(pack2(T(), w[2], w[3]));
+              for (int k = 0; k < MT; ++k) { acc[n][k][e] *= f; acc[n][k][e + 2] *= f; }
+            }
         }
 #pragma unroll
-        for (int k = 0; k < MT; ++k) {
-          // row g of the tile: dim 8 g + k, row g + 8: dim 64 + 8 g + k (head_dim 64: 8 g + 4 + k)
-          const int k1 = D == 128 ? k : k + 4, j1 = VC - 1;
-          const unsigned s0 = k & 1 ? 0x7632 : 0x5410, s1 = k1 & 1 ? 0x7632 : 0x5410;
-          const uint32_t a0 = __byte_perm(word(vr[x][0][0], k / 2), word(vr[x][1][0], k / 2), s0);
-          const uint32_t a1 = __byte_perm(word(vr[x][0][j1], k1 / 2), word(vr[x][1][j1], k1 / 2), s1);
-          const uint32_t a2 = __byte_perm(word(vr[x][2][0], k / 2), word(vr[x][3][0], k / 2), s0);
-          const uint32_t a3 = __byte_perm(word(vr[x][2][j1], k1 / 2), word(vr[x][3][j1], k1 / 2), s1);
+        for (int x = 0; x < SUB; ++x) {
+          uint32_t pb[NT][2];
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma(T(), acc[n][k], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+          for (int n = 0; n < NT; ++n) {
+            float w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              w[j] = sc[x][n][j] == -INFINITY ? 0.f : exp2_approx(sc[x][n][j] - m[n][j & 1]);
+              l[n][j & 1] += w[j];
+            }
+            pb[n][0] = transpose8x8(pack2(T(), w[0], w[1]));
+            pb[n][1] = transpose8x8(pack2(T(), w[2], w[3]));
+          }
+#pragma unroll
+          for (int k = 0; k < MT; ++k) {
+            // row g of the tile: dim 8 g + k, row g + 8: dim 64 + 8 g + k (head_dim 64: 8 g + 4 + k)
+            const int k1 = D == 128 ? k : k + 4, j1 = VC - 1;
+            const unsigned s0 = k & 1 ? 0x7632 : 0x5410, s1 = k1 & 1 ? 0x7632 : 0x5410;
+            const uint32_t a0 = __byte_perm(word(vr[x][0][0], k / 2), word(vr[x][1][0], k / 2), s0);
+            const uint32_t a1 = __byte_perm(word(vr[x][0][j1], k1 / 2), word(vr[x][1][j1], k1 / 2), s1);
+            const uint32_t a2 = __byte_perm(word(vr[x][2][0], k / 2), word(vr[x][3][0], k / 2), s0);
+            const uint32_t a3 = __byte_perm(word(vr[x][2][j1], k1 / 2), word(vr[x][3][j1], k1 / 2), s1);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma(T(), acc[n][k], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+          }
         }
-      }
-      if (more) load_v(i + 1, id);
+        if (more) load_v(i + 1, id);
 #pragma unroll
-      for (int x = 0; x < SUB; ++x) id[x] = id_next[x];
+        for (int x = 0; x < SUB; ++x) id[x] = id_next[x];
+      }
+      // ---- the warp's rows: a whole tile goes out, a part of one to shared memory -------------------------------------------------
+      const bool all = u_begin == 0 && u_end == units;
+      const int slot = 2 * warp + (pieces > 0);
+      if (!all && lane == 0) sm_piece[slot] = {at - v_begin + kStart, s.first, tile, h, units, nrows};
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o);
+          const int r = 8 * n + 2 * t + e;
+          // dims 8 g .. + 7 and 64 + 8 g .. + 7 (head_dim 64: 8 g .. + 7)
+          if (all) {
+            const float sum = l[n][e], inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;       // (NaN stays)
+            if (r < nrows) {
+              const int x = row0 + r;
+              T* out = static_cast<T*>(p.out) + ((int64_t)(s.first + x / p.group) * p.heads + h * p.group + x % p.group) * D + 8 * g;
+              uint32_t v[2][4];
+#pragma unroll
+              for (int k = 0; k < MT; k += 2) {
+                v[0][(k / 2) & 3] = pack2(T(), acc[n][k][e] * inv, acc[n][k + 1][e] * inv);
+                if (D == 128) v[1][k / 2] = pack2(T(), acc[n][k][e + 2] * inv, acc[n][k + 1][e + 2] * inv);
+                else v[0][2 + k / 2] = pack2(T(), acc[n][k][e + 2] * inv, acc[n][k + 1][e + 2] * inv);
+              }
+              *reinterpret_cast<uint4*>(out) = make_uint4(v[0][0], v[0][1], v[0][2], v[0][3]);
+              if (D == 128) *reinterpret_cast<uint4*>(out + 64) = make_uint4(v[1][0], v[1][1], v[1][2], v[1][3]);
+            }
+          } else {
+            if (g == 0) { sm_m[slot][r] = m[n][e]; sm_l[slot][r] = l[n][e]; }
+            float* to = sm_o + (slot * R + r) * kPitch;
+#pragma unroll
+            for (int k = 0; k < MT; k += 4) {
+              *reinterpret_cast<float4*>(to + 8 * g + k) = make_float4(acc[n][k][e], acc[n][k + 1][e], acc[n][k + 2][e], acc[n][k + 3][e]);
+              *reinterpret_cast<float4*>(to + (D == 128 ? 64 + 8 * g + k : 8 * g + 4 + k)) =
+                  make_float4(acc[n][k][e + 2], acc[n][k + 1][e + 2], acc[n][k + 2][e + 2], acc[n][k + 3][e + 2]);
+            }
+          }
+        }
+      pieces += !all;
     }
-    // ---- the warp's rows: a whole tile goes out, a part of one to shared memory -------------------------------------------------
-    const bool all = u_begin == 0 && u_end == per_tile;
-    const int slot = 2 * warp + (pieces > 0);
-    if (!all && lane == 0) sm_piece[slot] = {at - u_begin, s.first, tile, h, per_tile, nrows};
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o);
-        const int r = 8 * n + 2 * t + e;
-        // dims 8 g .. + 7 and 64 + 8 g .. + 7 (head_dim 64: 8 g .. + 7)
-        if (all) {
-          const float sum = l[n][e], inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;       // (NaN stays)
-          if (r < nrows) {
-            const int x = row0 + r;
-            T* out = static_cast<T*>(p.out) + ((int64_t)(s.first + x / p.group) * p.heads + h * p.group + x % p.group) * D + 8 * g;
-            uint32_t v[2][4];
-#pragma unroll
-            for (int k = 0; k < MT; k += 2) {
-              v[0][(k / 2) & 3] = pack2(T(), acc[n][k][e] * inv, acc[n][k + 1][e] * inv);
-              if (D == 128) v[1][k / 2] = pack2(T(), acc[n][k][e + 2] * inv, acc[n][k + 1][e + 2] * inv);
-              else v[0][2 + k / 2] = pack2(T(), acc[n][k][e + 2] * inv, acc[n][k + 1][e + 2] * inv);
-            }
-            *reinterpret_cast<uint4*>(out) = make_uint4(v[0][0], v[0][1], v[0][2], v[0][3]);
-            if (D == 128) *reinterpret_cast<uint4*>(out + 64) = make_uint4(v[1][0], v[1][1], v[1][2], v[1][3]);
-          }
-        } else {
-          if (g == 0) { sm_m[slot][r] = m[n][e]; sm_l[slot][r] = l[n][e]; }
-          float* to = sm_o + (slot * R + r) * kPitch;
-#pragma unroll
-          for (int k = 0; k < MT; k += 4) {
-            *reinterpret_cast<float4*>(to + 8 * g + k) = make_float4(acc[n][k][e], acc[n][k + 1][e], acc[n][k + 2][e], acc[n][k + 3][e]);
-            *reinterpret_cast<float4*>(to + (D == 128 ? 64 + 8 * g + k : 8 * g + 4 + k)) =
-                make_float4(acc[n][k][e + 2], acc[n][k + 1][e + 2], acc[n][k + 2][e + 2], acc[n][k + 3][e + 2]);
-          }
-        }
-      }
-    pieces += !all;
-    at += u_end - u_begin;
+    at += v_end - v_begin;
     if (at < end && at - before == seq_units) {           // the next sequence that has rows
       before += seq_units;
       do {
