@@ -94,8 +94,9 @@ struct Plan {
     if (x <= 1 || !p.a.causal || need <= 0) return all;
     return max(all - (pairs_of(p, need) - 1), 0);
   }
-  // Several ways to cut, one a lane: the longest pairs into 1, 2, ... chunks, all others into chunks no longer.  What a way costs: its rounds of items over the
-  // CTAs times an item's average length, 3 blocks of time for its beginning and end and 6 more for partial results; or the longest item.
+  // Several ways to cut, one a lane: the longest pairs into 1, 2, ... chunks, all others into chunks no longer.  What a way costs: its
+  // rounds of items over the CTAs times an item's average length, 3 blocks of time for its beginning and end and 6 more for partial
+  // results; or the longest item.
   __device__ __forceinline__ Plan(const PromptParams& p, int lane, Seq* memory) : c(0x3fffffff), kept(memory) {
     const PagedAttnParams& a = p.a;
     int64_t total = 0;
@@ -702,7 +703,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
           }
           top = all_tops();
           if (kForm == kCapped) {
-            direct = __all_sync(0xffffffffu, fmaxf(fabsf(top), fabsf(fminf(lows[0], lows[1]))) * cap.per_cap <= 0.4f);
+            direct = __all_sync(0xffffffffu, !mine || fmaxf(fabsf(top), fabsf(fminf(lows[0], lows[1]))) * cap.per_cap <= 0.4f);
             top = cap.any(top, a.cap);
           } else if (kForm == kPlain) {
             top *= to_log2;
@@ -747,7 +748,8 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
           top = all_tops() * (kForm == kPlain ? to_log2 : 1.f);
         }
         tmem_ld_32x32b_x32(s_at, raw[0]);
-        const bool above = top > m + kSlack;
+        // (A row of the tile that is nobody's holds whatever the shared memory held: it must not send the others through the longer ways.)
+        const bool above = mine && top > m + kSlack;
         if (__any_sync(0xffffffffu, above)) {
           const float to = fmaxf(m, top), f = to == -INFINITY ? 1.f : exp2_approx(m - to);
           m = to;

@@ -107,60 +107,6 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {
   return v;
 }
 
-// The split of all sequences into tiles of rows (tiles_of: how many a sequence has) and of a tile's units into chunks, as every warp works
-// it out for itself.  A sequence of more than c units is cut, all its tiles into the same number of chunks.
-struct Item {
-  int b, tile, chunk, chunks;
-  int cut_tile, cut_chunk;     // of those that are cut, for their place in scratch memory
-};
-template <int kUnit, class Tiles>
-__device__ __forceinline__ int units_of(const PagedAttnParams& p, int b, Tiles tiles_of, int& tiles) {
-  const Sequence s = sequence_of(p.c, b);
-  tiles = tiles_of(s);
-  Range<kUnit> r;
-  r.set(p, s, b, 0, s.rows - 1);
-  return tiles > 0 ? r.units : 0;               // (of one tile; a bound where several differ)
-}
-template <int kUnit, class Tiles>
-__device__ __forceinline__ int64_t total_units(const PagedAttnParams& p, int lane, Tiles tiles_of) {
-  int64_t total = 0;
-  for (int i = lane; i < p.c.batch; i += 32) {
-    int tiles;
-    const int u = units_of<kUnit>(p, i, tiles_of, tiles);
-    total += (int64_t)u * tiles;
-  }
-  return warp_sum64(total) * p.c.kv_heads;
-}
-template <int kUnit, class Tiles>
-__device__ __forceinline__ bool find_item(const PagedAttnParams& p, int index, int c, int lane, Tiles tiles_of, Item& item) {
-  int before = 0, cut_tiles = 0, cut_chunks = 0;
-  for (int base = 0; base < p.c.batch; base += 32) {
-    int tiles = 0, n = 1;
-    if (base + lane < p.c.batch) {
-      const int u = units_of<kUnit>(p, base + lane, tiles_of, tiles);
-      n = max((u + c - 1) / c, 1);
-    }
-    const int mine = tiles * n, cut = n > 1 ? tiles : 0, cutc = n > 1 ? mine : 0;
-    const int upto = warp_scan(mine, lane), cut_upto = warp_scan(cut, lane), cutc_upto = warp_scan(cutc, lane);
-    const unsigned hit = __ballot_sync(0xffffffffu, before + upto > index);
-    if (hit) {
-      const int l = __ffs(hit) - 1;
-      const int in = index - before - __shfl_sync(0xffffffffu, upto - mine, l);
-      item.chunks = __shfl_sync(0xffffffffu, n, l);
-      item.b = base + l;
-      item.tile = in / item.chunks;
-      item.chunk = in - item.tile * item.chunks;
-      item.cut_tile = cut_tiles + __shfl_sync(0xffffffffu, cut_upto - cut, l) + item.tile;
-      item.cut_chunk = cut_chunks + __shfl_sync(0xffffffffu, cutc_upto - cutc, l) + in;
-      return true;
-    }
-    before += __shfl_sync(0xffffffffu, upto, 31);
-    cut_tiles += __shfl_sync(0xffffffffu, cut_upto, 31);
-    cut_chunks += __shfl_sync(0xffffffffu, cutc_upto, 31);
-  }
-  return false;
-}
-
 // Scratch memory: counters of cut tiles, two more of the many-rows kernel's, and partial results.  Partial results of the many-rows kernel are 256
 // rows; of its items at most so many times as there are slots are cut.
 constexpr int kCutTiles = 2048, kPartsOfSlots = 4;
