@@ -13,11 +13,13 @@
 // Warps: 0 TMA (the pages of a block: one load per page and 64 dims; a page behind the last token lies outside the tensor map, which
 // gives zeros), 1 MMA, 2 zeroes the values of a block that nobody sees, 3 hands out the work (Plan), 4..7 and 8..11 the rows of the two tiles.
 //
-// What bounds it: a prompt of 8192 tokens of 32 heads over 8 key heads takes 476 us alone (1155 TFLOP/s, 0.71 of cuBLAS' burst), 556 in a
+// What bounds it: a prompt of 8192 tokens of 32 heads over 8 key heads takes 466 us (1180 TFLOP/s, 0.72 of cuBLAS' burst), 536 in a long
 // row of calls, where the power cap lowers the clock.  The same launches without the softmax take 342 us: S reads 8 KB of shared memory for
 // every 64 clocks of the tensor core and V and the ring's filling the rest of its 128 bytes a clock.  A block takes 3500 clocks: the
 // softmax of a tile 2100 (of which the special-function unit has 770) and its products 1300 behind it; the other tile's fill the gaps of
-// both.  Short prompts (2048 x 32 heads 53 us, 0.40): 12000 clocks until the first scores, 9000 between two items of a CTA.
+// both.  Short prompts (2048 x 32 heads 45 us, 0.47): 12000 clocks until the first scores, 9000 between two items of a CTA.  A cap adds
+// six packed operations for two scores: 512 tokens of 28 heads on 30000 take 371 us (600 TFLOP/s), with the cap by Taylor's series 408.
+// 120 CTAs have half of a pair's keys each there; 28 have nothing, since thirds or sevenths would cost more in beginnings and joins.
 // Measured and not kept, us for 8192 tokens where the present form took 485: all 128 scores of a row in registers 494 (and 70 instead of 50
 // for 2048: the longer code waits for its instructions), 64 at a time 551, 32 at a time 529, two threads a row 535..596, scores in two
 // halves of N = 64 with a buffer each 523 (412 instead of 342 without the softmax).
@@ -375,22 +377,25 @@ constexpr int kPlain = 0, kCapped = 1, kSloped = 2, kGeneral = 3;
 // Pairs of weights of eight that go that way: 8192 tokens 0 487, 2 479, 3 495, 4 596 us.
 constexpr int kPolyOfEight = 2;
 
-// cap * tanh(scale * x / cap) in the exponent of 2, of two scores.  Small: |scale * x / cap| <= 0.4, where tanh's Taylor series to the
-// ninth power is 1e-6 off; nearly all scores are, and the other form takes two special functions for each.
+// cap * tanh(scale * x / cap) in the exponent of 2, of two scores, less a row's maximum.  Small: u = scale * x / cap, |u| <= 0.4, where a
+// cubic in u^2 through the Chebyshev points of [0, 0.16] is tanh(u) / u to 1.6e-7 (Taylor's series needs two terms more); nearly all
+// scores are, and the other form takes two special functions for each.
 struct Cap {
-  float per_cap, to_log2;
-  __device__ __forceinline__ Cap(float scale, float cap) : per_cap(cap > 0.f ? scale / cap : 0.f), to_log2(scale * kLog2e) {}
-  __device__ __forceinline__ void small(float& x, float& y) const {
-    float u = x, v = y;
-    mul2(u, v, per_cap, per_cap);
-    mul2(u, v, u, v);
-    float pu = 62.f / 2835.f, pv = pu;
-    fma2(pu, pv, pu, pv, u, v, -17.f / 315.f, -17.f / 315.f);
-    fma2(pu, pv, pu, pv, u, v, 2.f / 15.f, 2.f / 15.f);
-    fma2(pu, pv, pu, pv, u, v, -1.f / 3.f, -1.f / 3.f);
-    fma2(pu, pv, pu, pv, u, v, 1.f, 1.f);
-    mul2(x, y, to_log2, to_log2);
-    mul2(x, y, pu, pv);
+  float per_cap, c[4];
+  __device__ __forceinline__ Cap(float scale, float cap) : per_cap(cap > 0.f ? scale / cap : 0.f) {
+    c[0] = 0.999999901f * kLog2e * cap;
+    c[1] = -0.333313563f * kLog2e * cap;
+    c[2] = 0.132708743f * kLog2e * cap;
+    c[3] = -0.0475493467f * kLog2e * cap;
+  }
+  __device__ __forceinline__ void small(float& x, float& y, float minus) const {
+    mul2(x, y, per_cap, per_cap);
+    float u = x, v = y, pu, pv;
+    mul2(u, v, x, y);
+    fma2(pu, pv, u, v, c[3], c[3], c[2], c[2]);
+    fma2(pu, pv, pu, pv, u, v, c[1], c[1]);
+    fma2(pu, pv, pu, pv, u, v, c[0], c[0]);
+    fma2(x, y, x, y, pu, pv, minus, minus);
   }
   __device__ __forceinline__ float any(float x, float cap) const {
     return cap * kLog2e * (1.f - __fdividef(2.f, exp2_approx(x * (2.f * kLog2e * per_cap)) + 1.f));
@@ -789,8 +794,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
                   fma2(bv, bw, (float)(2 * j), (float)(2 * j + 1), slope, slope, at_i, at_i);
                   fma2(v, w, v, w, scale_log2, scale_log2, bv, bw);
                 } else if (kForm == kCapped && !changed) {
-                  cap.small(v, w);
-                  add2(v, w, minus, minus);
+                  cap.small(v, w, minus);
                 } else if (kForm == kPlain) {
                   fma2(v, w, v, w, scale_log2, scale_log2, minus, minus);
                 } else {
