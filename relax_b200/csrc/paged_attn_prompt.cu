@@ -18,8 +18,11 @@
 // every 64 clocks of the tensor core and V and the ring's filling the rest of its 128 bytes a clock.  A block takes 3500 clocks: the
 // softmax of a tile 2100 (of which the special-function unit has 770) and its products 1300 behind it; the other tile's fill the gaps of
 // both.  Short prompts (2048 x 32 heads 45 us, 0.47): 12000 clocks until the first scores, 9000 between two items of a CTA.  A cap adds
-// six packed operations for two scores: 512 tokens of 28 heads on 30000 take 371 us (600 TFLOP/s), with the cap by Taylor's series 408.
-// 120 CTAs have half of a pair's keys each there; 28 have nothing, since thirds or sevenths would cost more in beginnings and joins.
+// six packed operations for two scores: 512 tokens of 28 heads on 30000 take 325 us (685 TFLOP/s), without a cap 230.  120 CTAs have half of
+// a pair's keys each there; sevenths on all of them take 313 with the cap and 240 without.
+// Partial results lie with the rows side by side, so that a row's thread adds up its own and reads 8 x 16 bytes of two parts at a time; with
+// the dims side by side and a part after the other that took 41 us for two parts, and 100 tokens on 5000 (32 heads, ten parts) 174 instead
+// of 40.
 // Measured and not kept, us for 8192 tokens where the present form took 485: all 128 scores of a row in registers 494 (and 70 instead of 50
 // for 2048: the longer code waits for its instructions), 64 at a time 551, 32 at a time 529, two threads a row 535..596, scores in two
 // halves of N = 64 with a buffer each 523 (412 instead of 342 without the softmax).
@@ -860,10 +863,10 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
           }
         }
       } else {
-        const int64_t row = ((int64_t)w.part * 2 + t) * kRows + r;
-        a.partial_ml[row * 2] = m;
-        a.partial_ml[row * 2 + 1] = sum;
-        float* to = a.partial + row * D;
+        // 16 bytes of all rows lie together, so a warp's store and load is one piece
+        const int64_t tile = ((int64_t)w.part * 2 + t) * kRows;
+        reinterpret_cast<float2*>(a.partial_ml)[tile + r] = make_float2(m, sum);
+        uint4* to = reinterpret_cast<uint4*>(a.partial + tile * D) + r;
 #pragma unroll 1
         for (int i = 0; i < D / 16; ++i) {
           uint32_t o[16];
@@ -873,8 +876,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            reinterpret_cast<uint4*>(to)[4 * i + j] =
-                any && sum != 0.f ? make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]) : make_uint4(0, 0, 0, 0);
+            to[(4 * i + j) * kRows] = any && sum != 0.f ? make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]) : make_uint4(0, 0, 0, 0);
         }
       }
       if (any) {
@@ -897,30 +899,44 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       tile_barrier();
       if (!last) continue;
       __threadfence();
-      const int64_t part0 = (int64_t)w.part - (int64_t)w.chunk * w.part_step;
-      constexpr int kQuads = D / 4;
-      int i0 = r;
-      asm volatile("" : "+r"(i0));               // (else what follows from it is worked out once and held in registers all along)
+      if (!mine) continue;
+      const int64_t tile = (((int64_t)w.part - (int64_t)w.chunk * w.part_step) * 2 + t) * kRows, step = (int64_t)w.part_step * 2 * kRows;
+      float2* ml = reinterpret_cast<float2*>(a.partial_ml) + tile + r;
+      float M = -INFINITY, L = 0.f;
+#pragma unroll 4
+      for (int k = 0; k < w.chunks; ++k) M = fmaxf(M, __ldcg(&ml[k * step].x));
+#pragma unroll 4
+      for (int k = 0; k < w.chunks; ++k) {         // the maximum's place takes the part's weight
+        const float2 of = __ldcg(&ml[k * step]);
+        const float f = of.x == -INFINITY ? 0.f : exp2_approx(of.x - M);
+        L += of.y * f;
+        __stcg(&ml[k * step].x, f);
+      }
+      const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
+      T* out = static_cast<T*>(a.out) + ((int64_t)(w.first + token) * a.heads + head) * D;
+      const float4* from = reinterpret_cast<const float4*>(a.partial + tile * D) + r;
+      constexpr int kAtOnce = 8;
 #pragma unroll 1
-      for (int i = i0; i < kRows * kQuads; i += 128) {
-        const int row = i / kQuads, d = (i % kQuads) * 4;
-        const int tok_in = row / a.group, tok = w.token + t * p.tile_tokens + tok_in;
-        if (tok_in >= p.tile_tokens || tok >= w.rows) break;
-        float M = -INFINITY, L = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int k = 0; k < w.chunks; ++k) M = fmaxf(M, __ldcg(a.partial_ml + (((part0 + (int64_t)k * w.part_step) * 2 + t) * kRows + row) * 2));
-#pragma unroll 1
+      for (int q = 0; q < D / 4; q += kAtOnce) {
+        float v[4 * kAtOnce];
+#pragma unroll
+        for (int j = 0; j < 4 * kAtOnce; ++j) v[j] = 0.f;
+#pragma unroll 2
         for (int k = 0; k < w.chunks; ++k) {
-          const int64_t x = ((part0 + (int64_t)k * w.part_step) * 2 + t) * kRows + row;
-          const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.partial_ml + x * 2));
-          const float4 o = __ldcg(reinterpret_cast<const float4*>(a.partial + x * D + d));
-          if (ml.x == -INFINITY && ml.y == 0.f) continue;
-          const float f = exp2_approx(ml.x - M);
-          L += ml.y * f;
-          v[0] += o.x * f; v[1] += o.y * f; v[2] += o.z * f; v[3] += o.w * f;
+          const float f = __ldcg(&ml[k * step].x);
+#pragma unroll
+          for (int j = 0; j < kAtOnce; ++j) {
+            const float4 o = __ldcg(from + k * step * (D / 4) + (q + j) * kRows);
+            v[4 * j] += o.x * f; v[4 * j + 1] += o.y * f; v[4 * j + 2] += o.z * f; v[4 * j + 3] += o.w * f;
+          }
         }
-        const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
-        T* out = static_cast<T*>(a.out) + ((int64_t)(w.first + tok) * a.heads + w.h * a.group + row - tok_in * a.group) * D + d;
-        *reinterpret_cast<uint2*>(out) = make_uint2(pack2(T(), v[0] * inv, v[1] * inv), pack2(T(), v[2] * inv, v[3] * inv));
+#pragma unroll
+        for (int j = 0; j < kAtOnce; j += 2) {
+          uint32_t x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = pack2(T(), v[4 * j + 2 * i] * inv, v[4 * j + 2 * i + 1] * inv);
+          reinterpret_cast<uint4*>(out)[(q + j) / 2] = make_uint4(x[0], x[1], x[2], x[3]);
+        }
       }
     }
   }

@@ -61,8 +61,8 @@ struct PagedAttnParams {
   float scale, cap;
   const float* slopes;
   const int* prefix;
-  float* partial;              // [chunk of a cut tile][rows][D], and the maxima and sums of all of them
-  float* partial_ml;           // [chunk of a cut tile][2][rows]
+  float* partial;              // few rows: [part][row][D]; many rows: [part][tile of two][D / 4][row][4]
+  float* partial_ml;           // their rows' maxima and sums, in pairs
   int* arrived;                // [cut tile]
   int slots;                   // CTAs that run at once
 };
@@ -107,8 +107,8 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {
   return v;
 }
 
-// Scratch memory: counters of cut tiles, two more of the many-rows kernel's, and partial results.  Partial results of the many-rows kernel are 256
-// rows; of its items at most so many times as there are slots are cut.
+// Scratch memory: counters of cut tiles, two more of the many-rows kernel's, and partial results.  Partial results of the many-rows
+// kernel are 256 rows; of its items at most so many times as there are slots are cut.
 constexpr int kCutTiles = 2048, kPartsOfSlots = 4;
 static_assert((kCutTiles + 2) * 4 <= B200_PAGED_ZEROED_BYTES, "the counters");
 
