@@ -899,7 +899,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       tile_barrier();
       if (!last) continue;
       __threadfence();
-      if (!mine) continue;
+      if (!mine) continue;                       // (work_done brings the warp together again)
       const int64_t tile = (((int64_t)w.part - (int64_t)w.chunk * w.part_step) * 2 + t) * kRows, step = (int64_t)w.part_step * 2 * kRows;
       float2* ml = reinterpret_cast<float2*>(a.partial_ml) + tile + r;
       float M = -INFINITY, L = 0.f;
