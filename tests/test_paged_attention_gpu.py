@@ -176,6 +176,17 @@ def test_a_part_of_a_long_text(cuda_lib, new, past):
     run(c, slopes=[2.0 ** -(i + 4) for i in range(8)])
 
 
+@pytest.mark.parametrize("heads,kv,dim,dtype", [(14, 2, 128, "bf16"), (8, 2, 64, "fp16"), (4, 4, 128, "fp16")])
+@pytest.mark.parametrize("new,past", [([100], [3000]), ([70, 1, 40], [2500, 5, 4000]), ([300], [900])])
+def test_parts_that_are_joined(cuda_lib, new, past, heads, kv, dim, dtype):
+    """Many rows of a long text on few key heads: cut into parts, some of which a mask leaves empty, with tiles that are not full."""
+    c = Case(new, past, heads, kv, dim, 64, dtype)
+    run(c)
+    run(c, cap=5.0)
+    run(c, cap=200.0, window=500, prefix=[300] * len(new))
+    run(c, slopes=[2.0 ** -i for i in range(heads)], causal=False)
+
+
 def test_rows_by_a_bound_only(cuda_lib):
     """max_query is a bound: a larger one, or none, gives the same values by another kernel."""
     c = Case([3, 1, 4], [100, 30, 0], 4, 2)
