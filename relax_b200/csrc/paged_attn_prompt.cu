@@ -671,7 +671,8 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         // its short form does not hold, go back to tensor memory.  Second pass: the weights.  (What does not fit in registers comes from
         // L2 with this much shared memory, and so do the instructions of long code.)
         const int from = range.unit(u) * kBlock;
-        const bool whole = from + kBlock <= range.pre || (from + kBlock - 1 <= tile_first && tile_last - from < window && tile_first >= 0);
+        // (a row without a position sees nothing, the prefix neither)
+        const bool whole = tile_first >= 0 && (from + kBlock <= range.pre || (from + kBlock - 1 <= tile_first && tile_last - from < window));
         uint32_t raw[2][32];
         float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};      // (four chains: one would be 64 dependent steps)
         float top;

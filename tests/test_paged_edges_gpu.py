@@ -1,0 +1,33 @@
+"""Attention over the paged cache and log probabilities at the ends of their ranges: rows without a place among many rows."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from paged_util import Case, assert_within
+from relax_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def attention(c, **kw):
+    out = torch.full((c.tokens, c.heads, c.dim), float("nan"), dtype=c.q.dtype, device="cuda")
+    kw = {n: torch.tensor(v, dtype=torch.int32 if n == "prefix" else torch.float32).cuda() if n in ("prefix", "slopes") and v is not None else v
+          for n, v in kw.items()}
+    ops.paged_attention(c.q, *c.args(), starts=c.starts, max_query=max(c.new), out=out, **kw)
+    torch.cuda.synchronize()
+    return out
+
+
+FORMS = [dict(), dict(cap=9.0), dict(slopes=[2.0 ** -(i + 2) for i in range(8)]), dict(cap=9.0, slopes=[2.0 ** -(i + 2) for i in range(8)])]
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("new,length,kv", [([300], [200], 2), ([150], [20], 2), ([200, 40, 33], [150, 43, 0], 2), ([70], [66], 8), ([9, 150], [4, 149], 1)])
+def test_many_rows_without_a_place_are_zero(cuda_lib, new, length, kv, form):
+    """More rows than the sequence has tokens, in the kernel for many rows: those before its beginning see nothing, whatever the mask."""
+    c = Case(new, [n - m for n, m in zip(length, new)], 8, kv)
+    nowhere = torch.cat([torch.arange(m) < m - n for n, m in zip(length, new)])
+    for mask in (dict(), dict(causal=False), dict(prefix=[130] * len(new)), dict(prefix=[1000] * len(new)), dict(window=50, prefix=[129] * len(new))):
+        out = attention(c, **form, **mask)
+        assert (out[nowhere.cuda()] == 0).all(), (mask, "rows without a place")
+        assert_within(out, c.reference(**form, **mask), str(mask))
