@@ -607,7 +607,8 @@ int b200_paged_attention(const B200PagedCache* cache, const B200PagedAttention* 
   p.heads = a->heads;
   p.group = a->heads / cache->kv_heads;
   p.causal = a->causal != 0;
-  p.window = a->window;
+  // A window as long as a row of the table hides nothing.  (Up to 2^30, so that sums with it stay below 2^31.)
+  p.window = a->window >= (int64_t)cache->table_width * cache->page_size ? 0 : a->window;
   p.scale = a->scale;
   p.cap = a->cap;
   p.slopes = static_cast<const float*>(a->slopes);

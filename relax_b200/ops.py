@@ -391,12 +391,14 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         out = torch.empty((q.shape[0], heads, dim), dtype=q.dtype, device=q.device)
     elif out.dtype is not q.dtype or out.shape != q.shape or not out.is_contiguous():
         raise ValueError("out is a contiguous tensor of q's shape and type")
+    if window < 0:
+        raise ValueError(f"window is the number of tokens that a row sees, or 0: got {window}")
     _same_device(q.device, k_pages=k_pages, v_pages=v_pages, page_table=page_table, lengths=lengths, starts=starts, slopes=slopes,
                  prefix=prefix, out=out, scratch=scratch)
     with _on(q.device):
         if scratch is None:
             scratch = _stream_scratch(q.device)
-        args = _lib.PagedAttention(q.data_ptr(), q.stride(0) if q.shape[0] > 1 else heads * dim, out.data_ptr(), heads, int(causal), int(window),
+        args = _lib.PagedAttention(q.data_ptr(), q.stride(0) if q.shape[0] > 1 else heads * dim, out.data_ptr(), heads, int(causal), min(int(window), 2 ** 31 - 1),
                                    dim ** -0.5 if scale is None else scale, cap, None if slopes is None else slopes.data_ptr(),
                                    _index("prefix", prefix, (cache.batch,)))
         _lib.check(_lib.lib().b200_paged_attention(ctypes.byref(cache), ctypes.byref(args), scratch.data_ptr(),

@@ -1,4 +1,5 @@
-"""Attention over the paged cache and log probabilities at the ends of their ranges: rows without a place among many rows."""
+"""Attention over the paged cache and log probabilities at the ends of their ranges: rows without a place among many rows,
+windows without an end."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -31,3 +32,22 @@ def test_many_rows_without_a_place_are_zero(cuda_lib, new, length, kv, form):
         out = attention(c, **form, **mask)
         assert (out[nowhere.cuda()] == 0).all(), (mask, "rows without a place")
         assert_within(out, c.reference(**form, **mask), str(mask))
+
+
+@pytest.mark.parametrize("new,past", [([1, 1, 1], [300, 0, 40]), ([60, 1, 200], [300, 2, 0]), ([5, 2], [-3, 20]), ([200, 70], [-50, 600])])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 200, 2 ** 33, 2 ** 32 + 5])
+def test_a_window_without_an_end(cuda_lib, new, past, window):
+    """Windows near the largest whole number, and beyond it, hide nothing: the same bits as without one."""
+    c = Case(new, past, 8, 2)
+    want = attention(c)
+    assert_within(want, c.reference())
+    assert torch.equal(attention(c, window=window), want)
+    want = attention(c, prefix=[9] * len(new))
+    assert torch.equal(attention(c, window=window, prefix=[9] * len(new)), want)
+
+
+def test_a_window_that_is_no_number_of_tokens(cuda_lib):
+    c = Case([1], [30], 4, 2)
+    for window in (-1, -2 ** 31, -2 ** 32 + 5):
+        with pytest.raises(ValueError, match="window"):
+            attention(c, window=window)
