@@ -86,7 +86,7 @@ class PagedCache:
         shape = (pages, kv_heads, page_size, head_dim)
         self.k = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(layers)]
         self.v = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(layers)]
-        self.width = -(-max_tokens // page_size)
+        self.max_tokens, self.width = max_tokens, -(-max_tokens // page_size)
         self.table_host = np.full((batch, self.width), -1, np.int32)
         self.lengths_host = np.zeros(batch, np.int32)
         self.free = list(range(pages - 1, -1, -1))
@@ -94,8 +94,8 @@ class PagedCache:
     def extend(self, seq: int, tokens: int) -> None:
         """Room for `tokens` more of sequence `seq`; raises, and changes nothing, where the table or the pool has none."""
         have, want = -(-int(self.lengths_host[seq]) // self.page_size), -(-(int(self.lengths_host[seq]) + tokens) // self.page_size)
-        if tokens < 0 or want > self.width:
-            raise ValueError(f"sequence {seq} cannot grow by {tokens} tokens: at most {self.width} pages of {self.page_size}")
+        if tokens < 0 or int(self.lengths_host[seq]) + tokens > self.max_tokens:
+            raise ValueError(f"sequence {seq} of {int(self.lengths_host[seq])} tokens cannot grow by {tokens}: at most {self.max_tokens}")
         if want - have > len(self.free):
             raise MemoryError(f"{want - have} pages wanted, {len(self.free)} free")
         for i in range(have, want):
