@@ -148,7 +148,6 @@ class PagedDecoder:
         pages = batch * -(-max_tokens // cfg.page_size) if pages is None else pages
         self.cache = PagedCache(len(layers), cfg.kv_heads, cfg.head_dim, cfg.page_size, pages, batch, max_tokens, device=device)
         self.cos, self.sin = rope_tables(max_tokens, cfg.rotary, cfg.theta, cfg.scaling, device)
-        self.scratch = ops.paged_attention_scratch(self.device)
 
     def _stream(self):
         return torch.cuda.current_stream(self.device).cuda_stream
@@ -187,7 +186,7 @@ class PagedDecoder:
                 q = ops.paged_rope_append(qkv, self.cos, self.sin, self.cache.k[i], self.cache.v[i], table, lengths, starts=starts,
                                           interleaved=cfg.interleaved)
                 a = ops.paged_attention(q, self.cache.k[i], self.cache.v[i], table, lengths, starts=starts, max_query=longest, window=cfg.window,
-                                        cap=cfg.cap, scratch=self.scratch)
+                                        cap=cfg.cap)
                 delta = ops.q4f16_matmul(a.view(T, -1), *w["o"])
                 gu = ops.q4f16_matmul(self._norm(x, delta, w["norm2"], h), *w["gu"])
                 _lib.check(self.L.b200_silu_mul(gu.data_ptr(), act.data_ptr(), T, cfg.inter, self._stream()))
