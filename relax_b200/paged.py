@@ -12,6 +12,7 @@ from __future__ import annotations
 import argparse
 import dataclasses
 import math
+import operator
 
 import numpy as np
 import torch
@@ -159,22 +160,29 @@ class PagedDecoder:
 
     def forward(self, seqs, tokens, every: bool = False) -> torch.Tensor:
         """Takes `tokens[i]` (a list) as the next tokens of sequence `seqs[i]`: their keys and values go to the cache; the logits of the last
-        of each, or with `every` of all of them, come back, fp16 [rows, vocab]."""
-        cfg, counts = self.cfg, [len(t) for t in tokens]
+        of each, or with `every` of all of them, come back, fp16 [rows, vocab].  A call that raises leaves the sequences as they were."""
+        counts = [len(t) for t in tokens]
         if len(seqs) != len(tokens) or len(set(seqs)) != len(seqs) or min(counts, default=0) < 1:
             raise ValueError("every sequence once, with one token at least")
+        ids = [operator.index(t) for ts in tokens for t in ts]
+        if not 0 <= min(ids) <= max(ids) < self.embed.shape[0]:
+            raise ValueError(f"tokens are 0 to {self.embed.shape[0] - 1}, got {min(ids)} to {max(ids)}")
         done = []
         try:
             for s, n in zip(seqs, counts):
                 self.cache.extend(s, n)
                 done.append((s, n))
-        except Exception:
+            return self._forward(list(seqs), ids, counts, every)
+        except BaseException:                       # (nothing may count that has no keys in every layer)
             for s, n in done:
                 self.cache.shrink(s, n)
             raise
+
+    def _forward(self, seqs, ids, counts, every: bool) -> torch.Tensor:
+        cfg = self.cfg
         with torch.cuda.device(self.device):
-            table, lengths = self.cache.tables(list(seqs))
-            ids = torch.tensor([t for ts in tokens for t in ts], dtype=torch.int32, device=self.device)
+            table, lengths = self.cache.tables(seqs)
+            ids = torch.tensor(ids, dtype=torch.int32, device=self.device)
             T, H, f16 = ids.shape[0], cfg.hidden, dict(dtype=torch.float16, device=self.device)
             longest = max(counts)
             starts = None if longest == 1 else torch.tensor(np.concatenate([[0], np.cumsum(counts)]), dtype=torch.int32, device=self.device)

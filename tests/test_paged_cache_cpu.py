@@ -22,3 +22,38 @@ def test_a_sequence_holds_max_tokens_and_no_more(page_size):
     with pytest.raises(ValueError, match="100"):
         c.extend(1, 1)
     assert c.lengths_host.tolist() == [100, 100] and len(c.free) == 20 - 2 * -(-100 // page_size)
+
+
+def decoder(**kw):
+    """A decoder whose first operator fails: there is no GPU here."""
+    cfg = paged.PagedConfig(hidden=128, heads=2, kv_heads=1, inter=128, layers=1, vocab=50, head_dim=64, rotary=64, **kw)
+    embed = torch.zeros((50, 128), dtype=torch.float16)
+    return paged.PagedDecoder(cfg, [], embed, torch.ones(128, dtype=torch.float16), embed, batch=3, max_tokens=40, device="cpu")
+
+
+def test_a_call_that_fails_leaves_the_sequences_as_they_were():
+    m = decoder()
+    m.cache.extend(1, 17)
+    table, free = m.cache.table_host.copy(), list(m.cache.free)
+
+    def as_it_was():
+        return m.cache.lengths_host.tolist() == [0, 17, 0] and (m.cache.table_host == table).all() and sorted(m.cache.free) == sorted(free)
+
+    for tokens in ([[1, 2], ["a", 3]], [[1, 2], [None]], [[1, 2], [3.5]]):
+        with pytest.raises(TypeError):
+            m.forward([0, 1], tokens)
+        assert as_it_was(), tokens
+    for tokens in ([[1, 2], [50]], [[-1], [3]], [[1], [2 ** 40]]):
+        with pytest.raises(ValueError, match="0 to 49"):
+            m.forward([0, 1], tokens)
+        assert as_it_was(), tokens
+    with pytest.raises(Exception):                  # behind the tables: the first operator finds no GPU
+        m.forward([0, 1], [[1, 2], [3]])
+    assert as_it_was()
+    for error in (MemoryError, KeyboardInterrupt):
+        def fails(*args, error=error):
+            raise error
+        m._forward = fails
+        with pytest.raises(error):
+            m.forward([2, 1], [[1, 2] * 17, [3]])
+        assert as_it_was()
