@@ -92,11 +92,18 @@ class PagedCache:
         self.lengths_host = np.zeros(batch, np.int32)
         self.free = list(range(pages - 1, -1, -1))
 
+    def length(self, seq: int) -> int:
+        """Tokens of a sequence.  (A negative number names no place: it would be another name for one of the last.)"""
+        if not 0 <= seq < len(self.lengths_host):
+            raise IndexError(f"place {seq} of the cache: there are {len(self.lengths_host)}")
+        return int(self.lengths_host[seq])
+
     def extend(self, seq: int, tokens: int) -> None:
         """Room for `tokens` more of sequence `seq`; raises, and changes nothing, where the table or the pool has none."""
-        have, want = -(-int(self.lengths_host[seq]) // self.page_size), -(-(int(self.lengths_host[seq]) + tokens) // self.page_size)
-        if tokens < 0 or int(self.lengths_host[seq]) + tokens > self.max_tokens:
-            raise ValueError(f"sequence {seq} of {int(self.lengths_host[seq])} tokens cannot grow by {tokens}: at most {self.max_tokens}")
+        length = self.length(seq)
+        have, want = -(-length // self.page_size), -(-(length + tokens) // self.page_size)
+        if tokens < 0 or length + tokens > self.max_tokens:
+            raise ValueError(f"sequence {seq} of {length} tokens cannot grow by {tokens}: at most {self.max_tokens}")
         if want - have > len(self.free):
             raise MemoryError(f"{want - have} pages wanted, {len(self.free)} free")
         for i in range(have, want):
@@ -105,7 +112,8 @@ class PagedCache:
 
     def shrink(self, seq: int, tokens: int) -> None:
         """Forgets the last `tokens` of a sequence and gives back the pages that only they were in."""
-        have, keep = int(self.lengths_host[seq]), int(self.lengths_host[seq]) - tokens
+        have = self.length(seq)
+        keep = have - tokens
         if not 0 <= keep <= have:
             raise ValueError(f"sequence {seq} has {have} tokens: {tokens} of them cannot be forgotten")
         for i in range(-(-keep // self.page_size), -(-have // self.page_size)):
@@ -115,7 +123,7 @@ class PagedCache:
 
     def release(self, seq: int) -> None:
         """Gives the pages of a sequence back."""
-        self.shrink(seq, int(self.lengths_host[seq]))
+        self.shrink(seq, self.length(seq))
 
     def tables(self, seqs):
         """Page table and lengths of these sequences on the device, as the operators take them; the table as wide as the longest needs."""
@@ -216,7 +224,7 @@ class PagedDecoder:
         """Greedy tokens behind the prompts: (tokens, their log probabilities, entropies), each [sequences][new_tokens]; `top` alternatives are
         looked at.  Uses places 0 .. of the cache, which have to be empty, and gives their pages back."""
         seqs = list(range(len(prompts)))
-        if any(self.cache.lengths_host[s] for s in seqs):
+        if any(self.cache.length(s) for s in seqs):
             raise ValueError("the first places of the cache are in use")
         chosen, logprobs, entropies = [], [], []
         try:
@@ -236,7 +244,7 @@ class PagedDecoder:
 
     def score(self, seq: int, tokens):
         """Log probability of every token of a text but its first, given those before it (sequence place `seq`, which has to be empty)."""
-        if self.cache.lengths_host[seq]:
+        if self.cache.length(seq):
             raise ValueError(f"place {seq} of the cache is in use")
         try:
             logits = self.forward([seq], [list(tokens)], every=True)

@@ -57,3 +57,14 @@ def test_a_call_that_fails_leaves_the_sequences_as_they_were():
         with pytest.raises(error):
             m.forward([2, 1], [[1, 2] * 17, [3]])
         assert as_it_was()
+
+
+def test_a_negative_number_names_no_place():
+    """-1 would be another name of the last place: the same sequence twice in a call, and a text scored in a place that is in use."""
+    m = decoder()
+    m.cache.extend(2, 5)
+    for call in (lambda: m.forward([-1, 2], [[1], [2]]), lambda: m.forward([3], [[1]]), lambda: m.score(-1, [1, 2]),
+                 lambda: m.cache.extend(-1, 1), lambda: m.cache.shrink(-1, 1), lambda: m.cache.release(-1), lambda: m.cache.release(3)):
+        with pytest.raises(IndexError, match="place"):
+            call()
+        assert m.cache.lengths_host.tolist() == [0, 0, 5] and len(m.cache.free) == m.cache.pages - 1
