@@ -270,7 +270,7 @@ struct Smem {
   uint64_t q_full, q_empty;
   uint64_t full[kStages], empty[kStages], ready[kReady];
   uint64_t s_full[2], p_ready[2][2], o_full[2], o_empty[2];       // [tile][half of a block]
-  uint64_t work_full[kWorks], work_empty[kWorks], issued;
+  uint64_t work_full[kWorks], work_empty[kWorks], issued, joined[2];
   Work work[kWorks];
   uint32_t tmem_base;
   int abort_flag;
@@ -326,21 +326,30 @@ __device__ __forceinline__ void mma4_ts(uint32_t d, uint32_t a, uint64_t b, uint
       : "memory");
 }
 
-// Bounded wait; false: it ran out, here or in another warp, and the kernel ends.
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int code) {
-  if (mbar_try_wait(bar, parity)) return true;
-  if (*abort_flag) return false;
-  if (mbar_wait_ns(bar, parity, kWaitNs)) return true;
+// Bounded wait of a whole warp; false: it ran out, here or in another warp, and the kernel ends.  The lanes vote on every outcome: tensor
+// memory is read and written by whole warps, so one lane must not go on where another has given up.  (A barrier that is complete stays so
+// until this warp has gone on: lanes can only see it late.)
+template <bool kRelaxed>
+__device__ __forceinline__ bool wait_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int code) {
+  const uint64_t t0 = globaltimer_ns();
+  for (uint32_t i = 1; i < 0x7fffffffu; ++i) {
+    if (kRelaxed) __nanosleep(100);
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, *abort_flag != 0)) return false;
+    if ((i & 127u) == 0 && __any_sync(0xffffffffu, globaltimer_ns() - t0 > kWaitNs)) break;
+  }
   *abort_flag = 1;
   atomicExch(&g_prompt_error, code);
   return false;
 }
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return wait_long<false>(bar, parity, abort_flag, code);
+}
+// The same with a pause between two looks, for warps that have time.
 __device__ __forceinline__ bool wait_relaxed(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int code) {
-  if (*abort_flag) return false;
-  if (mbar_wait_ns_relaxed(bar, parity, kWaitNs)) return true;
-  *abort_flag = 1;
-  atomicExch(&g_prompt_error, code);
-  return false;
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return wait_long<true>(bar, parity, abort_flag, code);
 }
 
 // 2^x of two values without the special-function unit: x = n + f with n the nearest whole number (by adding 1.5 * 2^23, whose sum has n
@@ -429,6 +438,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       mbar_init(&sm.p_ready[t][1], 4);
       mbar_init(&sm.o_full[t], 1);
       mbar_init(&sm.o_empty[t], 4);
+      mbar_init(&sm.joined[t], 4);
     }
     mbar_init(&sm.issued, 1);
     for (int i = 0; i < kWorks; ++i) { mbar_init(&sm.work_full[i], 1); mbar_init(&sm.work_empty[i], 11); }
@@ -638,11 +648,14 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
     // ---------------------------------------------------------------------- the rows
     const int t = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t s_at = tmem + t * 128 + ((uint32_t)((warp & 3) * 32) << 16), o_at = s_at - t * 128 + 256 + t * D;
-    uint32_t n_s = 0, n_o = 0;
+    uint32_t phases = 0;                         // parities: bit 0 of s_full, 1 of o_full, 2 of joined
     bool ok = true;
+    // The four warps of the tile meet; false: one of them has given up (a barrier without a limit would wait for it for ever).
     auto tile_barrier = [&]() {
-      if (t == 0) bar_sync(1, 128);
-      else bar_sync(2, 128);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.joined[t]);
+      phases ^= 4;
+      return wait(&sm.joined[t], phases >> 2 & 1 ^ 1, abort_flag, 14);
     };
     const int token_in_tile = r / a.group, head_in_group = r - token_in_tile * a.group;
     const float to_log2 = a.scale * kLog2e;
@@ -664,8 +677,8 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       bool begun = false;
       for (int u = u0; u < u1; ++u) {
         if (!sees(u)) continue;
-        if (!wait(&sm.s_full[t], n_s & 1, abort_flag, 12)) { ok = false; break; }
-        ++n_s;
+        if (!wait(&sm.s_full[t], phases & 1, abort_flag, 12)) { ok = false; break; }
+        phases ^= 1;
         tc_fence_after_sync();
         // First pass: the maximum, 32 columns at a time, the next ones on their way; scores that a mask changes, or a cap or a bias where
         // its short form does not hold, go back to tensor memory.  Second pass: the weights.  (What does not fit in registers comes from
@@ -829,8 +842,8 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       const float sum = m == -INFINITY ? 0.f : (l[0] + l[1]) + (l[2] + l[3]);   // (a row that saw nothing: 2^-126 of every key)
       const bool any = w.last[t] >= 0;
       if (any) {
-        if (!wait(&sm.o_full[t], n_o & 1, abort_flag, 13)) break;
-        ++n_o;
+        if (!wait(&sm.o_full[t], phases >> 1 & 1, abort_flag, 13)) break;
+        phases ^= 2;
         tc_fence_after_sync();
       }
       if (w.chunks == 1) {
@@ -888,16 +901,16 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       if (w.chunks == 1) continue;
       // ---- a tile that was cut: the CTA that comes last adds up, in the order of the chunks -------------------------------------
       __threadfence();
-      tile_barrier();
+      if (!tile_barrier()) break;
       if (r == 0) {
         int* counter = a.arrived + w.cut_tile + t;
         const int n = atomicAdd(counter, 1);
         sm.last_here[t] = n == w.chunks - 1;
         if (n == w.chunks - 1) *counter = 0;
       }
-      tile_barrier();
+      if (!tile_barrier()) break;
       const bool last = sm.last_here[t] != 0;
-      tile_barrier();
+      if (!tile_barrier()) break;
       if (!last) continue;
       __threadfence();
       if (!mine) continue;                       // (work_done brings the warp together again)
