@@ -499,8 +499,9 @@ B200_API int b200_paged_rope_append(const B200PagedCache* cache, const void* qkv
  *   visible: j < lengths[b], and (causal = 0; or j < prefix[b]; or j <= position and (window = 0 or position - j < window))
  * A row without a visible key gets zeros.  A key that no row of a sequence sees may hold anything; every value that some row sees has to be finite.
  * The weights of the sum are rounded to the cache's type, as the operands of the tensor cores are.
- * scratch: b200_paged_attention_scratch_bytes() bytes of device memory, of which the caller zeroes the first B200_PAGED_ZEROED_BYTES once and
- * every call leaves them zeroed; calls that share it must be ordered (one stream).  Allocates nothing.  heads <= 128 * kv_heads. */
+ * scratch: b200_paged_attention_scratch_bytes() bytes of device memory, of which the caller zeroes the first B200_PAGED_ZEROED_BYTES once,
+ * before the first call: counters, which every call (one that ran into the limit of a wait too) leaves fit for the next.  Calls that share it must
+ * be ordered (one stream).  Allocates nothing.  heads <= 128 * kv_heads. */
 #define B200_PAGED_ZEROED_BYTES 16384
 typedef struct {
   const void* q;       /* [tokens, heads, head_dim], rows q_stride apart, 16-byte aligned, q_stride a multiple of 8 */

@@ -599,7 +599,7 @@ int b200_paged_attention(const B200PagedCache* cache, const B200PagedAttention* 
   if (!a->q || !a->out || !aligned16(a->q) || !aligned16(a->out)) return fail(B200_EINVAL, "%s: q and out must be non-null and 16-byte aligned", who);
   if (!scratch || !aligned16(scratch)) return fail(B200_EINVAL, "%s: scratch must be non-null and 16-byte aligned", who);
   if ((rc = ensure_device())) return rc;
-  if (scratch_bytes < b200_paged_attention_scratch_bytes() || sm_count() * kCtasPerSm1 > kCutTiles)
+  if (scratch_bytes < b200_paged_attention_scratch_bytes() || sm_count() * kCtasPerSm1 > kFewCounters)
     return fail(B200_EINVAL, "%s: scratch of %lld bytes is less than b200_paged_attention_scratch_bytes()", who, (long long)scratch_bytes);
   p.q = a->q;
   p.out = a->out;

@@ -56,7 +56,8 @@ struct PromptParams {
   int tile_tokens;
   int wide_out;                                // out is 32-byte aligned
   unsigned long long per_pair;                 // 2^40 / (tokens of a pair), rounded up: n of them divided exactly up to 2^32
-  int* next;                                   // the next item, CTAs that are through
+  unsigned long long* counters;                // [cut tile]
+  PromptWords* words;
 };
 
 struct Work {
@@ -275,6 +276,7 @@ struct Smem {
   uint32_t tmem_base;
   int abort_flag;
   int last_here[2];
+  unsigned epoch;
   Plan::Seq kept[kKept];
 };
 
@@ -616,6 +618,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       }
     } else {
       // ---------------------------------------------------------------------- the work, longest tiles first
+      if (lane == 0) sm.epoch = __ldcg(&p.words->epoch);   // (handed over with the first descriptor)
       Plan plan(p, lane, sm.kept);
       for (uint32_t i = 0;; ++i) {
         const uint32_t slot = i % kWorks, round = i / kWorks;
@@ -625,7 +628,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         if (i > 0 && !wait_relaxed(&sm.issued, (i - 1) & 1, abort_flag, 15)) break;
         int index = blockIdx.x;
         if (i > 0) {
-          if (lane == 0) index = gridDim.x + atomicAdd(p.next, 1);
+          if (lane == 0) index = gridDim.x + atomicAdd(&p.words->next, 1);
           index = __shfl_sync(0xffffffffu, index, 0);
         }
         Work w;
@@ -637,10 +640,11 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         }
         if (w.b < 0) break;
       }
-      // the CTA that comes last leaves the counters as the next launch expects them
-      if (lane == 0 && atomicAdd(p.next + 1, 1) == (int)gridDim.x - 1) {
-        p.next[0] = 0;
-        p.next[1] = 0;
+      // the CTA that comes last leaves the words as the next launch expects them (a CTA that has given up comes here too)
+      if (lane == 0 && atomicAdd(&p.words->through, 1) == (int)gridDim.x - 1) {
+        p.words->next = 0;
+        p.words->through = 0;
+        p.words->epoch = sm.epoch + 1;
       }
     }
   } else {
@@ -903,10 +907,12 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       __threadfence();
       if (!tile_barrier()) break;
       if (r == 0) {
-        int* counter = a.arrived + w.cut_tile + t;
-        const int n = atomicAdd(counter, 1);
-        sm.last_here[t] = n == w.chunks - 1;
-        if (n == w.chunks - 1) *counter = 0;
+        // A counter holds a launch's number above its parts that have arrived: what an earlier launch left, whole or half counted because a
+        // wait ran out, gives way.  (The first one's result is not waited for.)
+        unsigned long long* counter = p.counters + w.cut_tile + t;
+        const unsigned long long none = (unsigned long long)sm.epoch << 32;
+        atomicMax(counter, none);
+        sm.last_here[t] = atomicAdd(counter, 1ull) - none == (unsigned long long)(w.chunks - 1);
       }
       if (!tile_barrier()) break;
       const bool last = sm.last_here[t] != 0;
@@ -993,11 +999,13 @@ int launch_paged_prompt(const char* who, const B200PagedCache* c, PagedAttnParam
   a.slots = sm_count();
   p.wide_out = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0;
   p.per_pair = ((1ull << 40) + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
-  p.next = a.arrived + kCutTiles;
+  p.counters = reinterpret_cast<unsigned long long*>(a.arrived + kFewCounters);
+  p.words = reinterpret_cast<PromptWords*>(p.counters + kCutTiles);
   p.a = a;
   // pairs of tiles of all sequences, at most, and their chunks
   const int64_t pairs = (c->tokens + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens) + c->batch;
   const int64_t most = pairs * c->kv_heads + (int64_t)kPartsOfSlots * a.slots;
+  if (kPartsOfSlots * a.slots > kCutTiles) return fail(B200_EINVAL, "%s: more than %d multiprocessors", who, kCutTiles / kPartsOfSlots);
   if (most > 0x3fffffffLL) return fail(B200_EINVAL, "%s: too many rows", who);
   auto launch = [&](auto kern, size_t bytes, SmemLimit& limit, std::atomic<int>& regs) {
     const size_t smem = bytes + 1024;

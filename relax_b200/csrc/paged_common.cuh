@@ -63,7 +63,7 @@ struct PagedAttnParams {
   const int* prefix;
   float* partial;              // few rows: [part][row][D]; many rows: [part][tile of two][D / 4][row][4]
   float* partial_ml;           // their rows' maxima and sums, in pairs
-  int* arrived;                // [cut tile]
+  int* arrived;                // few rows: [CTA]
   int slots;                   // CTAs that run at once
 };
 constexpr float kLog2e = 1.4426950408889634f;
@@ -107,10 +107,14 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {
   return v;
 }
 
-// Scratch memory: counters of cut tiles, two more of the many-rows kernel's, and partial results.  Partial results of the many-rows
-// kernel are 256 rows; of its items at most so many times as there are slots are cut.
-constexpr int kCutTiles = 2048, kPartsOfSlots = 4;
-static_assert((kCutTiles + 2) * 4 <= B200_PAGED_ZEROED_BYTES, "the counters");
+// Scratch memory: counters of the few-rows kernel (32 bits), counters of the many-rows kernel's cut tiles (64 bits) and its words, and partial
+// results.  Partial results of the many-rows kernel are 256 rows; of its items at most so many times as there are slots are cut.
+constexpr int kFewCounters = 2048, kCutTiles = 1016, kPartsOfSlots = 4;
+struct PromptWords {
+  int next, through;           // the next item; CTAs that are through: zero between launches
+  unsigned epoch;              // launches so far
+};
+static_assert(kFewCounters * 4 + kCutTiles * 8 + sizeof(PromptWords) <= B200_PAGED_ZEROED_BYTES, "the counters");
 
 // The kernel for many rows (paged_attn_prompt.cu).
 int launch_paged_prompt(const char* who, const B200PagedCache* c, PagedAttnParams p, cudaStream_t stream);

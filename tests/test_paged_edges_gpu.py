@@ -51,3 +51,20 @@ def test_a_window_that_is_no_number_of_tokens(cuda_lib):
     for window in (-1, -2 ** 31, -2 ** 32 + 5):
         with pytest.raises(ValueError, match="window"):
             attention(c, window=window)
+
+
+def test_what_a_call_that_gave_up_leaves_behind(cuda_lib):
+    """Counters of tiles that were cut, left half counted as by a call in which a wait ran out, do not reach the next call."""
+    c = Case([140], [6000], 8, 2)
+    scratch = ops.paged_attention_scratch("cuda")
+    want = attention(c, scratch=scratch)
+    assert_within(want, c.reference())
+    for left in range(1, 24):                              # (one less than its parts: the first part that arrives would be taken for the last)
+        counters = scratch[8192:8192 + 8 * 1016].view(torch.int64)
+        assert (counters != 0).any()
+        counters.fill_((int(counters.max()) >> 32 << 32) + left)
+        scratch[16384:].view(torch.float32).fill_(float("nan"))     # (what a tile that is joined too early reads)
+        assert torch.equal(attention(c, scratch=scratch), want), left
+    few = Case([1, 1], [3000, 50], 8, 2)                   # the other kernel, in the same memory
+    assert_within(attention(few, scratch=scratch), few.reference())
+    assert torch.equal(attention(c, scratch=scratch), want)
