@@ -495,7 +495,7 @@ B200_API int b200_paged_rope_append(const B200PagedCache* cache, const void* qkv
                                     void* q_out, void* cuda_stream);
 
 /* out[row, h] = sum_j softmax_j(s_j) v_j over the visible keys j of the row's sequence, of key head h / (heads / kv_heads):
- *   s = scale * q . k;  cap > 0: s = cap * tanh(s / cap);  slopes: s -= slopes[h] * |position - j|
+ *   s = scale * q . k;  cap > 0 (at most 1e30): s = cap * tanh(s / cap);  slopes: s -= slopes[h] * |position - j|
  *   visible: j < lengths[b], and (causal = 0; or j < prefix[b]; or j <= position and (window = 0 or position - j < window))
  * A row without a visible key gets zeros.  A key that no row of a sequence sees may hold anything; every value that some row sees has to be finite.
  * The weights of the sum are rounded to the cache's type, as the operands of the tensor cores are.

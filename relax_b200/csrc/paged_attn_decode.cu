@@ -59,7 +59,8 @@ struct Piece {
   int row, tile, h, units, rows;                // the sequence's first row; rows of the tile, 0: no piece
 };
 
-template <typename T, int D, int NT, bool kExtra>
+// kExtra: 1 with a cap or a bias, 2 with a cap for which Cap::any will not do.
+template <typename T, int D, int NT, int kExtra>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kCtasPerSm1 : kCtasPerSm2)
 paged_decode_kernel(const PagedAttnParams p) {
   constexpr int R = 8 * NT;                     // rows of a tile
@@ -137,7 +138,6 @@ paged_decode_kernel(const PagedAttnParams p) {
   const int page = 1 << p.c.page_log2;
   const int window = p.window ? p.window : 0x7fffffff;
   const float to_log2 = p.scale * kLog2e;
-  const float cap_in = kExtra && p.cap > 0.f ? 2.f * p.scale / p.cap * kLog2e : 0.f, cap_log2 = p.cap * kLog2e;
 
   int pieces = 0;
   while (at < end) {
@@ -239,6 +239,21 @@ paged_decode_kernel(const PagedAttnParams p) {
             }
           }
         if (more) load_k(i + 1, id);
+        if (kExtra == 2) {
+#pragma unroll
+          for (int x = 0; x < SUB; ++x)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) sc[x][n][j] = p.capped.of(sc[x][n][j]);
+        } else if (kExtra && p.cap > 0.f) {
+#pragma unroll
+          for (int x = 0; x < SUB; ++x)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) sc[x][n][j] = p.capped.any(sc[x][n][j]);
+        }
         bool above = false;
 #pragma unroll
         for (int x = 0; x < SUB; ++x) {
@@ -253,8 +268,7 @@ paged_decode_kernel(const PagedAttnParams p) {
             for (int j = 0; j < 4; ++j) {
               const int token = first + g + 8 * (j >> 1), at = position[n][j & 1];
               float v = sc[x][n][j];
-              if (kExtra && p.cap > 0.f) v = cap_log2 * (1.f - __fdividef(2.f, exp2_approx(v * cap_in) + 1.f));
-              else v *= to_log2;
+              if (!(kExtra && p.cap > 0.f)) v *= to_log2;
               if (kExtra) v -= slope[n][j & 1] * fabsf((float)(at - token));
               if (!whole) {
                 const bool seen = there && at >= 0 && (token < range.pre || (token <= at && at - token < window));
@@ -552,13 +566,17 @@ int launch_decode(const char* who, const B200PagedCache* c, PagedAttnParams p, c
     count_launch();
     return B200_OK;
   };
-  const bool extra = p.cap > 0.f || p.slopes;
+  const int extra = p.cap > 0.f && p.capped.wide() ? 2 : p.cap > 0.f || p.slopes ? 1 : 0;
   auto by_form = [&](auto type, auto dim) {
     using T = decltype(type);
     constexpr int D = decltype(dim)::value;
-    static SmemLimit limit[4];
-    if (narrow) return extra ? launch(paged_decode_kernel<T, D, 1, true>, limit[3]) : launch(paged_decode_kernel<T, D, 1, false>, limit[2]);
-    return extra ? launch(paged_decode_kernel<T, D, 2, true>, limit[1]) : launch(paged_decode_kernel<T, D, 2, false>, limit[0]);
+    static SmemLimit limit[2][3];
+    auto by_rows = [&](auto tiles, SmemLimit* of) {
+      constexpr int NT = decltype(tiles)::value;
+      return extra == 0 ? launch(paged_decode_kernel<T, D, NT, 0>, of[0])
+           : extra == 1 ? launch(paged_decode_kernel<T, D, NT, 1>, of[1]) : launch(paged_decode_kernel<T, D, NT, 2>, of[2]);
+    };
+    return narrow ? by_rows(std::integral_constant<int, 1>(), limit[0]) : by_rows(std::integral_constant<int, 2>(), limit[1]);
   };
   auto by_dim = [&](auto type) {
     return c->head_dim == 128 ? by_form(type, std::integral_constant<int, 128>()) : by_form(type, std::integral_constant<int, 64>());
@@ -591,7 +609,7 @@ int b200_paged_attention(const B200PagedCache* cache, const B200PagedAttention* 
   if (a->heads <= 0 || a->heads % cache->kv_heads || a->heads / cache->kv_heads > 128)
     return fail(B200_EINVAL, "%s: heads is a multiple of kv_heads, up to 128 times as many; got %d and %d", who, a->heads, cache->kv_heads);
   if (a->window < 0 || (a->window && !a->causal)) return fail(B200_EINVAL, "%s: a window is positive and needs causal", who);
-  if (!(a->scale == a->scale) || !(a->cap >= 0.f)) return fail(B200_EINVAL, "%s: scale is a number, cap a number >= 0", who);
+  if (!(a->scale == a->scale) || !(a->cap >= 0.f && a->cap <= 1e30f)) return fail(B200_EINVAL, "%s: scale is a number, cap a number from 0 to 1e30", who);
   if (cache->tokens == 0) return B200_OK;
   if (cache->batch == 0 || cache->max_query == 0) return fail(B200_EINVAL, "%s: rows without sequences", who);
   if (a->q_stride < (int64_t)a->heads * cache->head_dim || a->q_stride % 8)
@@ -611,6 +629,7 @@ int b200_paged_attention(const B200PagedCache* cache, const B200PagedAttention* 
   p.window = a->window >= (int64_t)cache->table_width * cache->page_size ? 0 : a->window;
   p.scale = a->scale;
   p.cap = a->cap;
+  p.capped = Cap(a->scale, a->cap);
   p.slopes = static_cast<const float*>(a->slopes);
   p.prefix = static_cast<const int*>(a->prefix);
   char* at = static_cast<char*>(scratch);

@@ -387,36 +387,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 // What happens to a score before the softmax: a scale > 0; that and a cap; that and a bias by distance; anything.
-constexpr int kPlain = 0, kCapped = 1, kSloped = 2, kGeneral = 3;
+constexpr int kPlain = 0, kCapped = 1, kSloped = 2, kGeneral = 3;     // (and kWide: with a cap for which Cap::any will not do)
 // Pairs of weights of eight that go that way: 8192 tokens 0 487, 2 479, 3 495, 4 596 us.
 constexpr int kPolyOfEight = 2;
 
-// cap * tanh(scale * x / cap) in the exponent of 2, of two scores, less a row's maximum.  Small: u = scale * x / cap, |u| <= 0.4, where a
-// cubic in u^2 through the Chebyshev points of [0, 0.16] is tanh(u) / u to 1.6e-7 (Taylor's series needs two terms more); nearly all
-// scores are, and the other form takes two special functions for each.
-struct Cap {
-  float per_cap, c[4];
-  __device__ __forceinline__ Cap(float scale, float cap) : per_cap(cap > 0.f ? scale / cap : 0.f) {
-    c[0] = 0.999999901f * kLog2e * cap;
-    c[1] = -0.333313563f * kLog2e * cap;
-    c[2] = 0.132708743f * kLog2e * cap;
-    c[3] = -0.0475493467f * kLog2e * cap;
-  }
-  __device__ __forceinline__ void small(float& x, float& y, float minus) const {
-    mul2(x, y, per_cap, per_cap);
-    float u = x, v = y, pu, pv;
-    mul2(u, v, x, y);
-    fma2(pu, pv, u, v, c[3], c[3], c[2], c[2]);
-    fma2(pu, pv, pu, pv, u, v, c[1], c[1]);
-    fma2(pu, pv, pu, pv, u, v, c[0], c[0]);
-    fma2(x, y, x, y, pu, pv, minus, minus);
-  }
-  __device__ __forceinline__ float any(float x, float cap) const {
-    return cap * kLog2e * (1.f - __fdividef(2.f, exp2_approx(x * (2.f * kLog2e * per_cap)) + 1.f));
-  }
-};
-
-template <typename T, int D, int kForm>
+template <typename T, int D, int kForm, bool kWide>
 __global__ void __launch_bounds__(kThreads, 1)
 paged_prompt_kernel(const __grid_constant__ PromptParams p) {
   using Shared = Smem<D>;
@@ -730,7 +705,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
           top = all_tops();
           if (kForm == kCapped) {
             direct = __all_sync(0xffffffffu, !mine || fmaxf(fabsf(top), fabsf(fminf(lows[0], lows[1]))) * cap.per_cap <= 0.4f);
-            top = cap.any(top, a.cap);
+            top = cap.small(top);
           } else if (kForm == kPlain) {
             top *= to_log2;
           }
@@ -748,8 +723,13 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
             tmem_ld_32x32b_x32(s_at + 32 * i, x);
             tmem_ld_wait();
             if (kForm == kCapped || (kForm == kGeneral && a.cap > 0.f)) {
+              if (!kWide) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(cap.any(__uint_as_float(x[j]), a.cap));
+                for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(cap.any(__uint_as_float(x[j])));
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(a.capped.of(__uint_as_float(x[j])));
+              }
             } else if (kForm != kPlain) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * to_log2);
@@ -1035,14 +1015,18 @@ int launch_paged_prompt(const char* who, const B200PagedCache* c, PagedAttnParam
     return B200_OK;
   };
   const int form = !(a.scale > 0.f) || (a.cap > 0.f && a.slopes) ? kGeneral : a.cap > 0.f ? kCapped : a.slopes ? kSloped : kPlain;
+  const bool wide = a.cap > 0.f && a.capped.wide();
   auto by_form = [&](auto type_, auto dim) {
     using T = decltype(type_);
     constexpr int N = decltype(dim)::value;
-    static SmemLimit limit[4];
-    static std::atomic<int> regs[4];
-    auto kern = form == kPlain ? paged_prompt_kernel<T, N, kPlain> : form == kCapped ? paged_prompt_kernel<T, N, kCapped>
-              : form == kSloped ? paged_prompt_kernel<T, N, kSloped> : paged_prompt_kernel<T, N, kGeneral>;
-    return launch(kern, sizeof(Smem<N>), limit[form], regs[form]);
+    static SmemLimit limit[6];
+    static std::atomic<int> regs[6];
+    const int at = form + (wide ? form == kCapped ? 3 : 2 : 0);
+    auto kern = form == kPlain ? paged_prompt_kernel<T, N, kPlain, false>
+              : form == kSloped ? paged_prompt_kernel<T, N, kSloped, false>
+              : form == kCapped ? wide ? paged_prompt_kernel<T, N, kCapped, true> : paged_prompt_kernel<T, N, kCapped, false>
+                                : wide ? paged_prompt_kernel<T, N, kGeneral, true> : paged_prompt_kernel<T, N, kGeneral, false>;
+    return launch(kern, sizeof(Smem<N>), limit[at], regs[at]);
   };
   auto by_dim = [&](auto type_) {
     return c->head_dim == 128 ? by_form(type_, std::integral_constant<int, 128>()) : by_form(type_, std::integral_constant<int, 64>());

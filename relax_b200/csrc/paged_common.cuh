@@ -51,6 +51,54 @@ __device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// cap * tanh(scale * x / cap) in the exponent of 2, u = scale * x / cap.
+//   small  |u| <= 0.4, where nearly all scores are: a cubic in u^2 through the Chebyshev points of [0, 0.16] is tanh(u) / u to 1.0e-7
+//          (Taylor's series needs two terms more)
+//   any    two special functions; exact to a few 2^-23 of the cap, not of the score
+//   of     each where it holds.  Up to a cap of 128 `any` alone changes a weight by 5e-5 at most, a tenth of its rounding to 16 bits; with
+//          a cap of 10^4 it changes weights by 0.004, and far above that it leaves nothing of a score
+struct Cap {
+  float per_cap, log2_cap, c[4];
+  Cap() = default;
+  __host__ __device__ Cap(float scale, float cap) : per_cap(cap > 0.f ? scale / cap : 0.f), log2_cap(cap * kLog2e) {
+    c[0] = 0.999999901f * log2_cap;
+    c[1] = -0.333313563f * log2_cap;
+    c[2] = 0.132708743f * log2_cap;
+    c[3] = -0.0475493467f * log2_cap;
+  }
+  bool wide() const { return log2_cap > 128.f * kLog2e; }                       // `any` will not do
+  // two of them, less a row's maximum
+  __device__ __forceinline__ void small(float& x, float& y, float minus) const {
+    ptx::mul2(x, y, per_cap, per_cap);
+    float u = x, v = y, pu, pv;
+    ptx::mul2(u, v, x, y);
+    ptx::fma2(pu, pv, u, v, c[3], c[3], c[2], c[2]);
+    ptx::fma2(pu, pv, pu, pv, u, v, c[1], c[1]);
+    ptx::fma2(pu, pv, pu, pv, u, v, c[0], c[0]);
+    ptx::fma2(x, y, x, y, pu, pv, minus, minus);
+  }
+  __device__ __forceinline__ float small(float x) const {
+    const float u = x * per_cap, v = u * u;
+    return u * fmaf(fmaf(fmaf(v, c[3], c[2]), v, c[1]), v, c[0]);
+  }
+  __device__ __forceinline__ float any(float x) const {
+    return log2_cap * (1.f - __fdividef(2.f, exp2_approx(x * (2.f * kLog2e * per_cap)) + 1.f));
+  }
+  __device__ __forceinline__ float of(float x) const {
+    float y;                                    // (both, and one of them: a branch for each score takes more than twice as long)
+    asm("{\n.reg .pred p;\nsetp.le.f32 p, %1, 0f3ECCCCCD;\nselp.f32 %0, %2, %3, p;\n}" : "=f"(y) : "f"(fabsf(x * per_cap)), "f"(small(x)), "f"(any(x)));
+    return y;
+  }
+};
+
 // What both attention kernels get.
 struct PagedAttnParams {
   PagedParams c;
@@ -59,6 +107,7 @@ struct PagedAttnParams {
   int64_t q_stride;
   int heads, group, causal, window;
   float scale, cap;
+  Cap capped;
   const float* slopes;
   const int* prefix;
   float* partial;              // few rows: [part][row][D]; many rows: [part][tile of two][D / 4][row][4]
@@ -66,14 +115,7 @@ struct PagedAttnParams {
   int* arrived;                // few rows: [CTA]
   int slots;                   // CTAs that run at once
 };
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.f;  // how far above the running maximum a score may lie, log2
-
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // Units of kUnit tokens that some row of a tile sees: those below `pre`, then those of [low, high).
 template <int kUnit>

@@ -1,11 +1,11 @@
 """Attention over the paged cache and log probabilities at the ends of their ranges: rows without a place among many rows,
-windows without an end."""
+windows without an end, caps far above the scores."""
 import pytest
 
 torch = pytest.importorskip("torch")
 
 from paged_util import Case, assert_within
-from relax_b200 import ops
+from relax_b200 import B200Error, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +68,34 @@ def test_what_a_call_that_gave_up_leaves_behind(cuda_lib):
     few = Case([1, 1], [3000, 50], 8, 2)                   # the other kernel, in the same memory
     assert_within(attention(few, scratch=scratch), few.reference())
     assert torch.equal(attention(c, scratch=scratch), want)
+
+
+@pytest.mark.parametrize("cap", [1e3, 1e4, 1e6, 1e9, 1e30])
+@pytest.mark.parametrize("new,past,dim,dtype", [([1, 1], [300, 40], 128, "fp16"), ([3], [90], 64, "bf16"), ([60, 5], [300, 0], 128, "fp16"), ([300], [0], 64, "bf16")])
+@pytest.mark.parametrize("more", [dict(), dict(window=33, prefix=[2, 2]), dict(slopes=[2.0 ** -(i + 2) for i in range(8)])])
+def test_a_cap_far_above_the_scores_changes_little(cuda_lib, cap, new, past, dim, dtype, more):
+    """The value is the definition's, with the cap; the bound that of scores without one: tanh of a small number is exact to fp32."""
+    c = Case(new, past, 8, 2, dim, 16, dtype)
+    c.q.mul_(8.0)
+    if "prefix" in more:
+        more = {**more, "prefix": more["prefix"][:len(new)]}
+    out = attention(c, cap=cap, **more)
+    assert_within(out, (c.reference(cap=cap, **more)[0], c.reference(**more)[1]))
+
+
+@pytest.mark.parametrize("scale", [None, -0.2])
+@pytest.mark.parametrize("new,past", [([1, 1, 4], [300, 40, 20]), ([60, 5], [300, 0])])
+def test_scores_below_and_above_a_cap(cuda_lib, new, past, scale):
+    """Both forms of tanh in one block of keys, and blocks of one of them."""
+    c = Case(new, past, 8, 2)
+    for factor in (0.5, 4.0, 16.0):
+        c.q.mul_(factor)
+        for more in (dict(), dict(window=40, prefix=[3] * len(new)), dict(slopes=[2.0 ** -(i + 2) for i in range(8)])):
+            assert_within(attention(c, cap=20.0, scale=scale, **more), c.reference(cap=20.0, scale=scale, **more), f"{factor} {more}")
+
+
+def test_caps_that_are_refused(cuda_lib):
+    c = Case([1], [30], 4, 2)
+    for cap in (-1.0, float("nan"), float("inf"), 1e31):
+        with pytest.raises(B200Error, match="cap"):
+            attention(c, cap=cap)
