@@ -522,7 +522,7 @@ B200_API int b200_paged_attention(const B200PagedCache* cache, const B200PagedAt
  *   top_token[row, i], top_logprob[row, i], i < top: the likeliest entries, equal ones by index; int32, fp32 (top = 0: both may be NULL)
  * A logit of -inf is an excluded entry: probability 0.  A row of nothing else has logprob -inf and entropy 0; one with a NaN or +inf
  * has NaN everywhere and tokens 0 .. top - 1.  dtype B200_F16, B200_BF16 or B200_F32; rows `stride` elements apart (any alignment of the type's
- * size; 16 bytes are faster); logprob and entropy may be NULL (tokens too, without logprob).  0 <= top <= 32, top <= V < 2^31.  One launch, no scratch. */
+ * size; 16 bytes are faster); logprob and entropy may be NULL (tokens too, without logprob).  0 <= top <= 32, top <= V < 2^31 - 4096.  One launch, no scratch. */
 B200_API int b200_token_logprobs(const void* logits, int32_t dtype, int64_t stride, const void* tokens, void* logprob, void* entropy,
                                  void* top_logprob, void* top_token, int64_t rows, int64_t V, int32_t top, void* cuda_stream);
 

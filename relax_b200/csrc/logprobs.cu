@@ -446,7 +446,8 @@ extern "C" int b200_token_logprobs(const void* logits, int32_t dtype, int64_t st
                                    void* top_logprob, void* top_token, int64_t rows, int64_t V, int32_t top, void* stream) {
   const char* who = "token_logprobs";
   if (dtype != B200_F16 && dtype != B200_BF16 && dtype != B200_F32) return fail(B200_EINVAL, "%s: dtype %d is not fp16, bf16 or fp32", who, dtype);
-  if (rows < 0 || V <= 0 || V >= 0x7fffffffLL - 64) return fail(B200_EINVAL, "%s: bad sizes %lld x %lld", who, (long long)rows, (long long)V);
+  // (an index runs past the row's end by up to a step of all threads before it is looked at: that has to fit in 31 bits)
+  if (rows < 0 || V <= 0 || V >= (1LL << 31) - 4096) return fail(B200_EINVAL, "%s: bad sizes %lld x %lld", who, (long long)rows, (long long)V);
   if (top < 0 || top > kMaxTop || top > V) return fail(B200_EINVAL, "%s: top is at most %d and V, got %d", who, kMaxTop, top);
   if (rows == 0) return B200_OK;
   const unsigned size = dtype == B200_F32 ? 4 : 2;
