@@ -144,6 +144,8 @@ token_logprobs_kernel(const LogprobParams p) {
   // count as kFloor: weight 0, and 0 times a number instead of 0 times infinity.  Then four operations an entry beside the special
   // function, two entries an instruction.
   constexpr float kFloor = std::is_same<T, __half>::value ? -65504.f : -1e30f, kFar = std::is_same<T, __half>::value ? -65000.f : -1e29f;
+  // (Where it is near the type's largest value, the distance to others in the exponent of 2 leaves fp32: that goes entry by entry too.)
+  auto amid = [](float m) { return m > kFar && (std::is_same<T, __half>::value || m < 2e38f); };
   auto many = [&](auto& v) {                            // uint4 [n]
     constexpr int n = sizeof(v) / sizeof(uint4);
     float top;
@@ -156,7 +158,7 @@ token_logprobs_kernel(const LogprobParams p) {
       const T2 all = __hmax2(__hmax2(most[0], most[1]), __hmax2(most[2], most[3]));
       top = fmaxf(to_float(T(all.x)), to_float(T(all.y)));
       s.raise(top);
-      if (s.m > kFar) {
+      if (amid(s.m)) {
         const T lowest = T(kFloor);
         const T2 lowest2 = T2(lowest, lowest);
 #pragma unroll
@@ -169,12 +171,12 @@ token_logprobs_kernel(const LogprobParams p) {
       for (int i = 4; i < 4 * n; ++i) most[i & 3] = fmaxf(most[i & 3], w[i]);
       top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
       s.raise(top);
-      if (s.m > kFar) {
+      if (amid(s.m)) {
 #pragma unroll
         for (int i = 0; i < 4 * n; ++i) w[i] = w[i] < kFloor ? kFloor : w[i];   // (a NaN stays)
       }
     }
-    if (s.m > kFar) {
+    if (amid(s.m)) {
 #pragma unroll
       for (int q = 0; q < n; ++q) {
         float f[N], l0 = 0.f, l1 = 0.f, e0 = 0.f, e1 = 0.f;       // (sums of a few, so that a thread's thousands do not lose bits)

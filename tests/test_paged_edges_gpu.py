@@ -1,5 +1,7 @@
 """Attention over the paged cache and log probabilities at the ends of their ranges: rows without a place among many rows,
-windows without an end, caps far above the scores."""
+windows without an end, caps far above the scores, logits near the largest value."""
+import math
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -99,3 +101,27 @@ def test_caps_that_are_refused(cuda_lib):
     for cap in (-1.0, float("nan"), float("inf"), 1e31):
         with pytest.raises(B200Error, match="cap"):
             attention(c, cap=cap)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [40, 5000, 70001])
+def test_entropy_of_logits_near_the_largest_value(cuda_lib, dtype, V):
+    """A distance beyond fp32's range (in the exponent of 2) is a weight of zero, not zero times infinity."""
+    big = 3e38
+    x = torch.zeros((6, V), dtype=dtype, device="cuda")
+    x[0, 7] = big
+    x[1, 7], x[1, 9], x[1, 11] = big, -big, float("-inf")
+    x[2] = big
+    x[3, ::2] = big
+    x[4] = -big
+    x[4, 5] = big
+    x[5] = float(torch.finfo(dtype).min)
+    x[5, 5:9] = float(torch.finfo(dtype).max)
+    said = ops.token_logprobs(x, torch.full((6,), 7, dtype=torch.int32).cuda(), top=2)
+    even = (V + 1) // 2
+    want = torch.tensor([0.0, 0.0, math.log(V), math.log(even), 0.0, math.log(4)], dtype=torch.float64)
+    assert ((said.entropy.double().cpu() - want).abs() <= 2.0 ** -19 * (1 + want)).all(), said.entropy
+    sure = torch.tensor([0.0, 0.0, -math.log(V), 0.0, 0.0, -math.log(4)], dtype=torch.float64)
+    for r in (0, 1, 2, 5):
+        assert abs(float(said.logprob[r]) - sure[r]) <= 2.0 ** -20 * (1 + abs(sure[r]))
+    assert said.top_token[:, 0].tolist() == [7, 7, 0, 0, 5, 5]
