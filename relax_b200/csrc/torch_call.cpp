@@ -157,7 +157,7 @@ bool paged_cache(PyObject* const* args, int64_t tokens, at::ScalarType type, B20
   if (k->scalar_type() != type || v->scalar_type() != type || k->dim() != 4 || v->sizes() != k->sizes()) return false;
   const int64_t page = k->size(2), dim = k->size(3);
   for (const at::Tensor* t : {k, v})
-    if (t->stride(3) != 1 || t->stride(2) != dim || t->stride(1) != page * dim) return false;
+    if (t->stride(3) != 1 || t->stride(2) != dim || (t->size(1) > 1 && t->stride(1) != page * dim)) return false;
   if (table->scalar_type() != at::kInt || table->dim() != 2 || (table->size(1) > 1 && table->stride(1) != 1)) return false;
   const int64_t batch = table->size(0), width = table->size(1);
   if (args[3] == Py_None || !optional_vector(args[3], at::kInt, batch, &lengths) || !optional_vector(args[4], at::kInt, batch + 1, &starts)) return false;
@@ -170,8 +170,9 @@ bool paged_cache(PyObject* const* args, int64_t tokens, at::ScalarType type, B20
   c->page_size = (int32_t)page;
   c->head_dim = (int32_t)dim;
   c->pages = k->size(0);
-  c->k_page_stride = k->stride(0);
-  c->v_page_stride = v->stride(0);
+  // (the stride of a dimension of one entry says nothing)
+  c->k_page_stride = k->size(0) > 1 ? k->stride(0) : k->size(1) * page * dim;
+  c->v_page_stride = v->size(0) > 1 ? v->stride(0) : k->size(1) * page * dim;
   c->k_pages = const_cast<void*>(k->const_data_ptr());
   c->v_pages = const_cast<void*>(v->const_data_ptr());
   c->batch = (int32_t)batch;
@@ -241,7 +242,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t tokens = q->size(0), heads = q->size(1);
     B200PagedCache c = {};
     if (dev < 0 || tokens == 0 || heads > INT32_MAX || !paged_cache(args + 1, tokens, q->scalar_type(), &c, dev)) Py_RETURN_NONE;
-    if (q->size(2) != c.head_dim || q->stride(2) != 1 || q->stride(1) != c.head_dim) Py_RETURN_NONE;
+    if (q->size(2) != c.head_dim || q->stride(2) != 1 || (heads > 1 && q->stride(1) != c.head_dim)) Py_RETURN_NONE;
     if (!optional_vector(args[11], at::kFloat, heads, &slopes) || !optional_vector(args[12], at::kInt, c.batch, &prefix)) Py_RETURN_NONE;
     if ((slopes && slopes->get_device() != dev) || (prefix && prefix->get_device() != dev)) Py_RETURN_NONE;
     B200PagedAttention a = {};

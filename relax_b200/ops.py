@@ -278,9 +278,9 @@ def _paged_cache(rows, k_pages, v_pages, page_table, lengths, starts, max_query)
     if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
         raise ValueError(f"pages are [pages, kv_heads, page_size, head_dim], both alike: got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
     pages, kv_heads, page_size, head_dim = k_pages.shape
-    inner = (page_size * head_dim, head_dim, 1)
+    whole = kv_heads * page_size * head_dim             # (the stride of a dimension of one entry says nothing)
     for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if t.stride()[1:] != inner:
+        if t.stride()[2:] != (head_dim, 1) or (kv_heads > 1 and t.stride(1) != page_size * head_dim):
             raise ValueError(f"the heads of a page of {name} must be contiguous: strides {t.stride()}")
     if page_table.dtype is not torch.int32 or page_table.dim() != 2 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
         raise ValueError("page_table is an int32 tensor [batch, pages of the longest sequence] with contiguous rows")
@@ -293,8 +293,8 @@ def _paged_cache(rows, k_pages, v_pages, page_table, lengths, starts, max_query)
     elif max_query is None:
         max_query = tokens
     stride = page_table.stride(0) if batch > 1 else width
-    return _lib.PagedCache(_CACHE_TYPES[k_pages.dtype], kv_heads, head_dim, page_size, pages, k_pages.stride(0), v_pages.stride(0),
-                           k_pages.data_ptr(), v_pages.data_ptr(), batch, width, int(max_query), stride, tokens, page_table.data_ptr(),
+    return _lib.PagedCache(_CACHE_TYPES[k_pages.dtype], kv_heads, head_dim, page_size, pages,
+                           *(t.stride(0) if pages > 1 else whole for t in (k_pages, v_pages)), k_pages.data_ptr(), v_pages.data_ptr(), batch, width, int(max_query), stride, tokens, page_table.data_ptr(),
                            _index("lengths", lengths, (batch,)), _index("starts", starts, (batch + 1,)))
 
 
@@ -382,7 +382,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             return result
     cache = _paged_cache(q, k_pages, v_pages, page_table, lengths, starts, max_query)
     kv, dim = cache.kv_heads, cache.head_dim
-    if q.dtype is not k_pages.dtype or q.dim() != 3 or q.shape[2] != dim or (q.shape[0] and q.stride()[1:] != (dim, 1)):
+    if q.dtype is not k_pages.dtype or q.dim() != 3 or q.shape[2] != dim or (q.shape[0] and (q.stride(2) != 1 or (q.shape[1] > 1 and q.stride(1) != dim))):
         raise ValueError(f"q is [tokens, heads, {dim}] of the pages' type, a token's heads contiguous")
     heads = q.shape[1]
     if slopes is not None and (slopes.dtype is not torch.float32 or slopes.shape != (heads,) or not slopes.is_contiguous()):

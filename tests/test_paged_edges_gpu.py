@@ -125,3 +125,24 @@ def test_entropy_of_logits_near_the_largest_value(cuda_lib, dtype, V):
     for r in (0, 1, 2, 5):
         assert abs(float(said.logprob[r]) - sure[r]) <= 2.0 ** -20 * (1 + abs(sure[r]))
     assert said.top_token[:, 0].tolist() == [7, 7, 0, 0, 5, 5]
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("new,past", [([1, 1], [300, 40]), ([40], [100])])
+def test_the_stride_of_a_single_entry_says_nothing(cuda_lib, monkeypatch, native, new, past):
+    """One key head, one query head, one page: views whose strides of these dimensions are any numbers."""
+    if not native:
+        monkeypatch.setattr(ops, "_native", False)
+        monkeypatch.setattr(ops, "_torch_call", lambda: False)
+    c = Case(new, past, 1, 1)
+    want = attention(c)
+    c.k, c.v = (t.transpose(1, 2).contiguous().transpose(1, 2) for t in (c.k, c.v))     # pages by token, then head
+    c.q = c.q.as_strided(c.q.shape, (128, 7, 1))
+    assert c.k.stride(1) != 16 * 128 and c.q.stride(1) != 128
+    assert torch.equal(attention(c), want)
+    short = Case([1], [9], 2, 2, ragged=False)
+    want = attention(short)
+    page = short.table[0, :1].long()
+    short.k, short.v = (t[page][0].as_strided((1, 2, 16, 128), (3, 2048, 128, 1)) for t in (short.k, short.v))
+    short.table = torch.zeros((1, 1), dtype=torch.int32, device="cuda")
+    assert torch.equal(attention(short), want)
