@@ -220,9 +220,9 @@ class PagedDecoder:
                                        self._stream()))
         return logits
 
-    def generate(self, prompts, new_tokens: int, top: int = 1):
-        """Greedy tokens behind the prompts: (tokens, their log probabilities, entropies), each [sequences][new_tokens]; `top` alternatives are
-        looked at.  Uses places 0 .. of the cache, which have to be empty, and gives their pages back."""
+    def generate(self, prompts, new_tokens: int):
+        """Greedy tokens behind the prompts: (tokens, their log probabilities, entropies), each [sequences][new_tokens].  Uses places 0 .. of the
+        cache, which have to be empty, and gives their pages back."""
         seqs = list(range(len(prompts)))
         if any(self.cache.length(s) for s in seqs):
             raise ValueError("the first places of the cache are in use")
@@ -231,7 +231,7 @@ class PagedDecoder:
             logits = self.forward(seqs, prompts)
             for step in range(new_tokens):
                 none = torch.zeros(len(seqs), dtype=torch.int32, device=self.device)
-                said = ops.token_logprobs(logits, none, top=max(top, 1))
+                said = ops.token_logprobs(logits, none, top=1)
                 chosen.append(said.top_token[:, 0].tolist())
                 logprobs.append(said.top_logprob[:, 0].tolist())
                 entropies.append(said.entropy.tolist())

@@ -68,3 +68,10 @@ def test_a_negative_number_names_no_place():
         with pytest.raises(IndexError, match="place"):
             call()
         assert m.cache.lengths_host.tolist() == [0, 0, 5] and len(m.cache.free) == m.cache.pages - 1
+
+
+def test_generation_takes_what_it_uses():
+    """It had an argument that said how many alternatives to look at, which changed nothing."""
+    import inspect
+
+    assert list(inspect.signature(paged.PagedDecoder.generate).parameters) == ["self", "prompts", "new_tokens"]
