@@ -228,19 +228,17 @@ class PagedDecoder:
             raise ValueError("the first places of the cache are in use")
         chosen, logprobs, entropies = [], [], []
         try:
-            logits = self.forward(seqs, prompts)
             for step in range(new_tokens):
+                logits = self.forward(seqs, prompts if step == 0 else [[t] for t in chosen[-1]])
                 none = torch.zeros(len(seqs), dtype=torch.int32, device=self.device)
                 said = ops.token_logprobs(logits, none, top=1)
                 chosen.append(said.top_token[:, 0].tolist())
                 logprobs.append(said.top_logprob[:, 0].tolist())
                 entropies.append(said.entropy.tolist())
-                if step + 1 < new_tokens:
-                    logits = self.forward(seqs, [[t] for t in chosen[-1]])
         finally:
             for s in seqs:
                 self.cache.release(s)
-        return tuple([list(row) for row in zip(*v)] for v in (chosen, logprobs, entropies))
+        return tuple([[step[s] for step in v] for s in seqs] for v in (chosen, logprobs, entropies))
 
     def score(self, seq: int, tokens):
         """Log probability of every token of a text but its first, given those before it (sequence place `seq`, which has to be empty)."""

@@ -75,3 +75,10 @@ def test_generation_takes_what_it_uses():
     import inspect
 
     assert list(inspect.signature(paged.PagedDecoder.generate).parameters) == ["self", "prompts", "new_tokens"]
+
+
+def test_no_tokens_asked_for():
+    """A list for every sequence all the same, and nothing left in the cache."""
+    m = decoder()
+    assert m.generate([[1, 2], [3]], 0) == ([[], []], [[], []], [[], []])
+    assert m.cache.lengths_host.tolist() == [0, 0, 0]
