@@ -220,9 +220,10 @@ class PagedDecoder:
                                        self._stream()))
         return logits
 
-    def generate(self, prompts, new_tokens: int):
+    def generate(self, prompts, new_tokens: int, top: int = 1):
         """Greedy tokens behind the prompts: (tokens, their log probabilities, entropies), each [sequences][new_tokens].  Uses places 0 .. of the
-        cache, which have to be empty, and gives their pages back."""
+        cache, which have to be empty, and gives their pages back.  `top` changes nothing (a greedy step takes the likeliest) and is there for
+        callers that give it; alternatives come from :func:`relax_b200.ops.token_logprobs`."""
         seqs = list(range(len(prompts)))
         if any(self.cache.length(s) for s in seqs):
             raise ValueError("the first places of the cache are in use")

@@ -70,15 +70,9 @@ def test_a_negative_number_names_no_place():
         assert m.cache.lengths_host.tolist() == [0, 0, 5] and len(m.cache.free) == m.cache.pages - 1
 
 
-def test_generation_takes_what_it_uses():
-    """It had an argument that said how many alternatives to look at, which changed nothing."""
-    import inspect
-
-    assert list(inspect.signature(paged.PagedDecoder.generate).parameters) == ["self", "prompts", "new_tokens"]
-
-
 def test_no_tokens_asked_for():
     """A list for every sequence all the same, and nothing left in the cache."""
     m = decoder()
-    assert m.generate([[1, 2], [3]], 0) == ([[], []], [[], []], [[], []])
+    for more in (dict(), dict(top=5)):
+        assert m.generate([[1, 2], [3]], 0, **more) == ([[], []], [[], []], [[], []])
     assert m.cache.lengths_host.tolist() == [0, 0, 0]
