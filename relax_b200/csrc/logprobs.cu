@@ -27,7 +27,9 @@ constexpr int kThreads = 256, kWarps = kThreads / 32, kCtasPerSm = 5;
 constexpr int kMaxTop = 32, kMaxCluster = 8;
 constexpr int kGroups = 64;                     // of four neighbouring threads
 constexpr int kList = 512;                      // elements above the bound, elements equal to it
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLn2 = 0.6931471805599453f;
+using ptx::exp2_approx;
+using ptx::kLog2e;
 
 struct LogprobParams {
   const void* logits;
@@ -40,11 +42,6 @@ struct LogprobParams {
   int V, top;
 };
 
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }

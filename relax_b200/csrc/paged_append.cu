@@ -132,8 +132,6 @@ paged_append_kernel(const AppendParams p) {
     for (int i = threadIdx.x; i < p.heads * D / 8; i += kThreads) reinterpret_cast<uint4*>(q)[i] = make_uint4(0, 0, 0, 0);
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 }  // namespace
 
 int paged_params(const char* who, const B200PagedCache* c, PagedParams* out) {

@@ -540,8 +540,6 @@ paged_decode_kernel(const PagedAttnParams p) {
   }
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 int launch_decode(const char* who, const B200PagedCache* c, PagedAttnParams p, cudaStream_t stream) {
   const int64_t most = (int64_t)c->max_query * p.group;          // rows of a sequence that share a key head
   const bool narrow = most <= 8;
@@ -591,8 +589,9 @@ using namespace b200;
 
 extern "C" {
 
-// The counters, the maxima and sums of chunks, their partial results.  Here a cut tile has more than a slot's share of the units and its
-// chunks at least half of that: fewer cut tiles than slots, twice as many chunks at most, of 16 rows.  The many-rows kernel needs more.
+// The counters, the maxima and sums of parts, their partial results.  The few-rows kernel has two parts a CTA at most (a tile that began before
+// its share, one that ends behind it) of 8 rows (three CTAs an SM) or 16 (two): 64 rows an SM.  The many-rows kernel has kPartsOfSlots of 256.
+static_assert(2 * kCtasPerSm1 * 8 <= kPartsOfSlots * 256 && 2 * kCtasPerSm2 * 16 <= kPartsOfSlots * 256, "partial results of the few-rows kernel");
 static int64_t scratch_rows() { return (int64_t)kPartsOfSlots * sm_count() * 256; }
 
 int64_t b200_paged_attention_scratch_bytes(void) {

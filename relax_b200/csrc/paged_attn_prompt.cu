@@ -55,7 +55,7 @@ struct PromptParams {
   PagedAttnParams a;
   int tile_tokens;
   int wide_out;                                // out is 32-byte aligned
-  unsigned long long per_pair;                 // 2^40 / (tokens of a pair), rounded up: n of them divided exactly up to 2^32
+  unsigned long long per_pair;                 // 2^40 / (tokens of a pair), rounded up: exact below 2^24 pairs
   unsigned long long* counters;                // [cut tile]
   PromptWords* words;
 };
@@ -355,24 +355,21 @@ __device__ __forceinline__ bool wait_relaxed(uint64_t* bar, uint32_t parity, vol
 }
 
 // 2^x of two values without the special-function unit: x = n + f with n the nearest whole number (by adding 1.5 * 2^23, whose sum has n
-// in its low bits), a polynomial of degree kDegree for 2^f on [-1/2, 1/2] (least largest relative error, found by the exchange
-// algorithm: 7.5e-5 for degree 3, 2.6e-6 for degree 4; a weight is rounded to 2^-12 or worse right after), n added to the exponent.
+// in its low bits), a polynomial of degree 4 for 2^f on [-1/2, 1/2] (least largest relative error, found by the exchange
+// algorithm: 2.7e-6; a weight is rounded to 2^-12 or worse right after), n added to the exponent.
 // x from -126 on, below that 2^-126.
-constexpr int kDegree = 4;
 __device__ __forceinline__ void exp2_poly(float& x, float& y) {
-  constexpr float c3[4] = {0.99992806f, 0.69326097f, 0.24261113f, 0.05517167f};
-  constexpr float c4[5] = {0.9999993f, 0.6931218f, 0.24024744f, 0.05591786f, 0.009570102f};
-  auto c = [&](int i) { return kDegree == 3 ? c3[i & 3] : c4[i]; };
+  constexpr float c[5] = {0.9999993f, 0.6931218f, 0.24024744f, 0.05591786f, 0.009570102f};
   constexpr float kMagic = 12582912.f;
   const float u = fmaxf(x, -126.f), v = fmaxf(y, -126.f);
-  float tu = u, tv = v, nu, nv, fu, fv, pu = c(kDegree), pv = pu;
+  float tu = u, tv = v, nu, nv, fu, fv, pu = c[4], pv = pu;
   add2(tu, tv, kMagic, kMagic);
   nu = tu;
   nv = tv;
   add2(nu, nv, -kMagic, -kMagic);
   fma2(fu, fv, nu, nv, -1.f, -1.f, u, v);
 #pragma unroll
-  for (int i = kDegree - 1; i >= 0; --i) fma2(pu, pv, pu, pv, fu, fv, c(i), c(i));
+  for (int i = 3; i >= 0; --i) fma2(pu, pv, pu, pv, fu, fv, c[i], c[i]);
   x = __uint_as_float(__float_as_uint(pu) + (__float_as_uint(tu) << 23));
   y = __uint_as_float(__float_as_uint(pv) + (__float_as_uint(tv) << 23));
 }
@@ -986,7 +983,7 @@ int launch_paged_prompt(const char* who, const B200PagedCache* c, PagedAttnParam
   const int64_t pairs = (c->tokens + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens) + c->batch;
   const int64_t most = pairs * c->kv_heads + (int64_t)kPartsOfSlots * a.slots;
   if (kPartsOfSlots * a.slots > kCutTiles) return fail(B200_EINVAL, "%s: more than %d multiprocessors", who, kCutTiles / kPartsOfSlots);
-  if (most > 0x3fffffffLL) return fail(B200_EINVAL, "%s: too many rows", who);
+  if (most > 0x3fffffffLL || pairs >= 1 << 24) return fail(B200_EINVAL, "%s: too many rows", who);
   auto launch = [&](auto kern, size_t bytes, SmemLimit& limit, std::atomic<int>& regs) {
     const size_t smem = bytes + 1024;
     int e = raise_smem_limit(limit, reinterpret_cast<const void*>(kern), smem, who);

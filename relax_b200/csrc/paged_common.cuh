@@ -51,13 +51,8 @@ __device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-constexpr float kLog2e = 1.4426950408889634f;
-
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
+using ptx::exp2_approx;
+using ptx::kLog2e;
 
 // cap * tanh(scale * x / cap) in the exponent of 2, u = scale * x / cap.
 //   small  |u| <= 0.4, where nearly all scores are: a cubic in u^2 through the Chebyshev points of [0, 0.16] is tanh(u) / u to 1.0e-7
@@ -160,6 +155,8 @@ static_assert(kFewCounters * 4 + kCutTiles * 8 + sizeof(PromptWords) <= B200_PAG
 
 // The kernel for many rows (paged_attn_prompt.cu).
 int launch_paged_prompt(const char* who, const B200PagedCache* c, PagedAttnParams p, cudaStream_t stream);
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Launch parameters of a checked descriptor; `who` names the entry point in messages.
 int paged_params(const char* who, const B200PagedCache* c, PagedParams* out);

@@ -237,6 +237,14 @@ __device__ __forceinline__ void pin_loaded(const uint4& v) {
 }
 __device__ __forceinline__ void pin_loaded(uint32_t v) { asm volatile("" ::"r"(v) : "memory"); }
 
+// ---- 2^x on the special-function unit ----------------------------------------------------------------
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // ---- two fp32 operations in one instruction -----------------------------------------------------------
 __device__ __forceinline__ unsigned long long pair64(float a, float b) {
   return (unsigned long long)__float_as_uint(b) << 32 | __float_as_uint(a);

@@ -25,7 +25,7 @@ def test_warps_of_a_tile_meet_within_a_limit():
 def test_the_lanes_of_a_warp_give_up_together():
     """Tensor memory is read by whole warps: a lane that saw a barrier complete must not go on where another one gave up."""
     text = code()
-    waits = text[text.index("bool wait_long("):text.index("constexpr int kDegree")] if "bool wait_long(" in text else ""
+    waits = text[text.index("bool wait_long("):text.index("void exp2_poly(")] if "bool wait_long(" in text else ""
     assert waits and text.count("mbar_try_wait(") == waits.count("__all_sync(0xffffffffu, mbar_try_wait(bar, parity))") == 3
     assert not re.search(r"\bmbar_wait", text)
     assert "__any_sync(0xffffffffu, *abort_flag" in waits and "kWaitNs" in waits
