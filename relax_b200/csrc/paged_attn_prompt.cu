@@ -378,9 +378,9 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
   asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
+__device__ __forceinline__ float max3(float a, float b, float c) {        // (NaN where one of them is)
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 // What happens to a score before the softmax: a scale > 0; that and a cap; that and a bias by distance; anything.
@@ -669,7 +669,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
 #pragma unroll
           for (int j = 0; j < 16; ++j) tops[j & 3] = max3(tops[j & 3], __uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]));
         };
-        auto all_tops = [&]() { return fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])); };
+        auto all_tops = [&]() { return max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]); };
         const float bias = kForm == kSloped ? -slope * (float)(at - from) : 0.f;       // of the block's first key, which lies before the row
         bool direct = whole && kForm != kGeneral && (kForm != kSloped || from + kBlock - 1 <= tile_first);
         if (direct) {
@@ -751,6 +751,11 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
           top = all_tops() * (kForm == kPlain ? to_log2 : 1.f);
         }
         tmem_ld_32x32b_x32(s_at, raw[0]);
+        // A score that is no number, or infinite, makes the row NaN.  (Not by itself: the polynomial takes it for a small one.)
+        if (!(top < INFINITY)) {
+          m = INFINITY;
+          l[0] = NAN;
+        }
         // (A row of the tile that is nobody's holds whatever the shared memory held: it must not send the others through the longer ways.)
         const bool above = mine && top > m + kSlack;
         if (__any_sync(0xffffffffu, above)) {

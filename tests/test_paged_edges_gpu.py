@@ -1,5 +1,5 @@
 """Attention over the paged cache and log probabilities at the ends of their ranges: rows without a place among many rows,
-windows without an end, caps far above the scores, logits near the largest value."""
+windows without an end, caps far above the scores, logits near the largest value, keys that are no numbers."""
 import math
 
 import pytest
@@ -146,3 +146,26 @@ def test_the_stride_of_a_single_entry_says_nothing(cuda_lib, monkeypatch, native
     short.k, short.v = (t[page][0].as_strided((1, 2, 16, 128), (3, 2048, 128, 1)) for t in (short.k, short.v))
     short.table = torch.zeros((1, 1), dtype=torch.int32, device="cuda")
     assert torch.equal(attention(short), want)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("new,past,dim,dtype", [([1, 1], [300, 40], 128, "fp16"), ([3], [90], 64, "bf16"), ([200], [0], 128, "fp16"), ([40], [2000], 64, "bf16"), ([140], [6000], 128, "fp16")])
+def test_a_broken_key_is_not_passed_over(cuda_lib, new, past, dim, dtype, bad):
+    """Rows that see a key with a NaN or an infinity in it come out as NaN, wherever in a block it lies; rows that do not see it are as they were."""
+    c = Case(new, past, 8, 2, dim, 16, dtype)
+    position = torch.cat([torch.arange(n, n + m) for n, m in zip(past, new)])
+    first = c.starts_list[:-1]
+    for at in list(range(min(c.length[0], 34))) + [c.length[0] // 2]:
+        where = (int(c.table[0, at // 16]), slice(None), at % 16)
+        kept = c.k[where].clone()
+        c.k[where] = bad
+        for more in (dict(), dict(slopes=[2.0 ** -(i + 2) for i in range(8)]), dict(window=max(new) + 3), dict(cap=20.0)):
+            if more.get("cap") and bad == float("inf"):
+                continue                                        # (the cap makes it a number)
+            sees = position[:new[0]] >= at
+            if "window" in more:
+                sees &= position[:new[0]] - at < more["window"]
+            out = attention(c, **more)[:new[0]].cpu()
+            assert torch.isnan(out[sees]).all(), (at, more)
+            assert torch.isfinite(out[~sees]).all(), (at, more)
+        c.k[where] = kept
