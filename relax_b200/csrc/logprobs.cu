@@ -461,7 +461,8 @@ extern "C" int b200_token_logprobs(const void* logits, int32_t dtype, int64_t st
                      static_cast<float*>(top_logprob), static_cast<int*>(top_token), stride, rows, (int)V, top};
   // CTAs of a row: the fewest rounds of CTAs, each as long as its slice of the row and what begins and ends it (about 14000 entries, and
   // 2000 for each CTA of the cluster).  us, fp16, 20 alternatives: one row of 32000 8.9 with four CTAs, 10.1 with eight; 64 rows 9.6 with
-  // four, 14.8 with eight.  Threads, CTAs an SM and loads in flight, 2048 rows: 256, 5, 4 42.5; 256, 6, 4 42; 256, 4, 4 47; 128, 12, 4 50.
+  // four, 14.8 with eight.  Threads, CTAs an SM and loads in flight, 2048 rows: 256, 5, 4 42.5 (31.2 without
+  // alternatives); 256, 6, 4 42; 256, 4, 4 47; 128, 12, 4 50.
   const int64_t slots = (int64_t)sm_count() * kCtasPerSm;
   int c = 1;
   int64_t least = 0;

@@ -17,9 +17,9 @@
 // is above it by more than 8 (in the exponent of 2), so the usual unit needs a vote instead of a reduction over lanes; weights
 // stay below 2^8, fp32 sums take that.  Weights are rounded to the cache's type for the product with V.
 //
-// What bounds it: HBM for long caches (131000 tokens of 8 key heads, 537 MB, 89 us: 6.0 TB/s, 0.92 of a copy; 64 sequences of 37 to 2047
-// tokens, 135 MB, 31 us: 4.4); latency for short ones (32 heads at 2011, 33 MB, 13.4 us: 2 until the shares are known, 7 for two or three
-// units a warp, 4 for the joins).  Before, chunks of equal length as CTAs of their own took 157, 45 and 17.5 us.
+// What bounds it: HBM for long caches (131000 tokens of 8 key heads, 537 MB, 90 us: 6.0 TB/s, 0.91 of a copy; 512 sequences of 37 to 2047
+// tokens 182 us: 5.9; 64 of them, 135 MB, 31 us: 4.4); latency for short ones (32 heads at 2011, 33 MB, 13.6 us: 2 until the shares are
+// known, 7 for two or three units a warp, 4 for the joins).  Before, chunks of equal length as CTAs of their own took 157, 45 and 17.5 us.
 #include "paged_common.cuh"
 
 namespace b200 {
@@ -28,8 +28,9 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kUnit = 16;
-// A tile's beginning (its queries, the first page numbers, the way to its first keys) counts as so many units of its share: 0, 1, 2, 4 units
-// 15.1, 14.1, 13.8, 13.2 us for 32 heads at 2011, 34.3, 31.4, 30.7, 31.0 for 64 ragged sequences, 23.8, 23.8, 22.5, 22.3 for 33 with a window.
+// A tile's beginning (its queries, the first page numbers, the way to its first keys) counts as so many units of its share: 0, 1, 2, 3, 4 units
+// 15.2, 14.4, 14.1, 13.6, 13.4 us for 32 heads at 2011, 34.4, 31.2, 30.9, 31.1, 31.1 for 64 ragged sequences, 23.9, 23.8, 22.5, 22.4, 22.3 for
+// 33 with a window.
 constexpr int kStart = 3;
 constexpr int kCtasPerSm1 = 3, kCtasPerSm2 = 2;       // of tiles of 8 rows, of 16
 __device__ __forceinline__ void mma(__half, float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {

@@ -13,16 +13,19 @@
 // Warps: 0 TMA (the pages of a block: one load per page and 64 dims; a page behind the last token lies outside the tensor map, which
 // gives zeros), 1 MMA, 2 zeroes the values of a block that nobody sees, 3 hands out the work (Plan), 4..7 and 8..11 the rows of the two tiles.
 //
-// What bounds it: a prompt of 8192 tokens of 32 heads over 8 key heads takes 466 us (1180 TFLOP/s, 0.72 of cuBLAS' burst), 536 in a long
-// row of calls, where the power cap lowers the clock.  The same launches without the softmax take 342 us: S reads 8 KB of shared memory for
-// every 64 clocks of the tensor core and V and the ring's filling the rest of its 128 bytes a clock.  A block takes 3500 clocks: the
+// What bounds it: a prompt of 8192 tokens of 32 heads over 8 key heads takes 460 us (1200 TFLOP/s, 0.73 of cuBLAS' burst), 537 in a long
+// row of calls, where the power cap lowers the clock (1030, 0.74 of cuBLAS' rate there).  The same
+// launches without the softmax take 342 us: S reads 8 KB of shared memory for every 64 clocks of the tensor core and V and the ring's
+// filling the rest of its 128 bytes a clock.  A block takes 3500 clocks: the
 // softmax of a tile 2100 (of which the special-function unit has 770) and its products 1300 behind it; the other tile's fill the gaps of
-// both.  Short prompts (2048 x 32 heads 45 us, 0.47): 12000 clocks until the first scores, 9000 between two items of a CTA.  A cap adds
-// six packed operations for two scores: 512 tokens of 28 heads on 30000 take 325 us (685 TFLOP/s), without a cap 230.  120 CTAs have half of
-// a pair's keys each there; sevenths on all of them take 313 with the cap and 240 without.
+// both.  Short prompts (2048 x 32 heads 50.5 us, 0.42): 12000 clocks until the first scores, 9000 between two items of a CTA.  A cap adds
+// six packed operations for two scores as long as all of a block are below 0.4 of it: 512 tokens of 28 heads on 30000 take 331 us (670
+// TFLOP/s), without a cap 254.  Larger ones go through tensor memory with two special functions each: 570 with queries eight times as
+// large, and 85 instead of 64 for a prompt of 2048 with a cap of 30.  120 CTAs have half of a pair's keys each in that chunk; sevenths on
+// all of them took 4 % less with the cap and 4 % more without.
 // Partial results lie with the rows side by side, so that a row's thread adds up its own and reads 8 x 16 bytes of two parts at a time; with
 // the dims side by side and a part after the other that took 41 us for two parts, and 100 tokens on 5000 (32 heads, ten parts) 174 instead
-// of 40.
+// of 38.
 // Measured and not kept, us for 8192 tokens where the present form took 485: all 128 scores of a row in registers 494 (and 70 instead of 50
 // for 2048: the longer code waits for its instructions), 64 at a time 551, 32 at a time 529, two threads a row 535..596, scores in two
 // halves of N = 64 with a buffer each 523 (412 instead of 342 without the softmax).

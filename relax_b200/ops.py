@@ -340,8 +340,9 @@ _scratch: dict = {}     # (device, stream) -> memory of paged_attention calls on
 
 
 def paged_attention_scratch(device) -> torch.Tensor:
-    """Memory that paged_attention calls of one stream may share (``scratch=``): where several streams or captured graphs make such
-    calls at the same time, each needs its own."""
+    """Memory (79 MB) that paged_attention calls of one stream may share (``scratch=``): where several streams or captured graphs make
+    such calls at the same time, each needs its own.  A call without it takes the stream's, which is kept; in a captured graph each takes
+    and zeroes its own: one for the graph saves that."""
     with _on(device):
         size = int(_lib.lib().b200_paged_attention_scratch_bytes())
         if size < 0:
