@@ -141,7 +141,8 @@ paged_decode_kernel(const PagedAttnParams p) {
   const float to_log2 = p.scale * kLog2e;
 
   int pieces = 0;
-  while (at < end) {
+  // (Lengths that somebody changes under the launch give no result; they must not lead behind the last sequence, or round and round.)
+  while (at < end && per_tile > 0) {
     // ---- a part of one tile: units [u_begin, u_end) of all of its ---------------------------------------------------------------
     const Sequence s = sequence_of(p.c, b);
     const int in_seq = (int)(at - before), index = in_seq / per_tile, v_begin = in_seq - index * per_tile;
@@ -381,8 +382,9 @@ paged_decode_kernel(const PagedAttnParams p) {
       before += seq_units;
       do {
         ++b;
-        seq_units = units_of(b, per_tile);
-      } while (seq_units == 0);
+        per_tile = 0;
+        seq_units = b < p.c.batch ? units_of(b, per_tile) : 0;
+      } while (seq_units == 0 && b < p.c.batch);
     }
   }
 

@@ -29,3 +29,14 @@ def test_the_lanes_of_a_warp_give_up_together():
     assert waits and text.count("mbar_try_wait(") == waits.count("__all_sync(0xffffffffu, mbar_try_wait(bar, parity))") == 3
     assert not re.search(r"\bmbar_wait", text)
     assert "__any_sync(0xffffffffu, *abort_flag" in waits and "kWaitNs" in waits
+
+
+def test_the_few_rows_kernel_ends_whatever_the_lengths_do():
+    """A warp reads the lengths more than once.  Where they change in between (a caller that writes them on another stream, which gives no
+    result), its walk over the sequences stays inside the batch, and a sequence without work does not keep it where it is."""
+    with open(SOURCE.replace("paged_attn_prompt", "paged_attn_decode")) as f:
+        text = re.sub(r"//[^\n]*", "", f.read())
+    walk = text[text.index("int pieces = 0;"):text.index("__syncthreads();", text.index("int pieces = 0;"))]
+    assert "while (at < end && per_tile > 0) {" in walk
+    assert re.findall(r"units_of\([^)]*\)", walk) == ["units_of(b, per_tile)"] and "b < p.c.batch ? units_of(b, per_tile) : 0" in walk
+    assert "while (seq_units == 0 && b < p.c.batch);" in walk
