@@ -516,6 +516,76 @@ B200_API int64_t b200_paged_attention_scratch_bytes(void);
 B200_API int b200_paged_attention(const B200PagedCache* cache, const B200PagedAttention* args, void* scratch, int64_t scratch_bytes,
                                   void* cuda_stream);
 
+/* ---- the same over pages of 8 bits ---------------------------------------------------------------
+ * Pages hold e4m3 codes (strides in codes, multiples of 16), scales fp16 [pages, kv_heads, page_size / 16], one for 16 tokens of a head, all of it contiguous:
+ * a value is code * scale.  The descriptor's dtype is that of the rows (q, qkv, results).  A scale is positive, of any block that a
+ * row sees; what no token has reached, codes and scales, may be anything.
+ *
+ * b200_paged8_rope_append: as b200_paged_rope_append, k and v rounded to the rows' type as there, then stored by their block's scale:
+ *   need = the smallest power of two by which the block's new tokens are at most 448 in size, from 2^-24 to 2^7
+ *   scale = need where no earlier token is in the block, else the larger one of need and what it was; then the earlier tokens' codes are
+ *   scaled anew.  Codes are rounded to nearest even; what is more than 448 * 2^7 in size becomes that, what is no finite number NaN.
+ * b200_paged8_attention: as b200_paged_attention; q is taken in fp16 (of bf16 rows: up to 65504 in size), weights are rounded to fp16.
+ * Scratch memory as there; calls of both may share it where they are ordered. */
+typedef struct {
+  void* k_scales;
+  void* v_scales;
+} B200PagedScales;
+B200_API int b200_paged8_rope_append(const B200PagedCache* cache, const B200PagedScales* scales, const void* qkv, int64_t qkv_stride,
+                                     int32_t heads, const void* cos_t, const void* sin_t, int64_t table_rows, int32_t rotary,
+                                     int32_t interleaved, const void* positions, void* q_out, void* cuda_stream);
+B200_API int b200_paged8_attention(const B200PagedCache* cache, const B200PagedScales* scales, const B200PagedAttention* args, void* scratch,
+                                   int64_t scratch_bytes, void* cuda_stream);
+
+/* ---- pages and rows of a call, from the lengths of its sequences -----------------------------------
+ * counts[b] > 0: sequence b gets so many new tokens; < 0: it forgets its last ones; lengths are those before.  With P = page_size,
+ * have = ceil(length / P), want = ceil((length + count) / P):
+ *   pages given back: table[b][want .. have - 1] of every sequence, in order, onto the free list (free_pages[0 .. free_count - 1], the
+ *   last one on top); then pages taken from its top, in order of sequence and place: table[b][have .. want - 1]
+ *   starts [batch + 1]: rows before each sequence; positions and slots (int64: page * P + offset) of every row, -1 behind the last one
+ *   lengths_out = length + count, free_count_out.  What it forgets stays in the table's row, behind its length.
+ * status 0: done.  n > 0: n pages are lacking; -1: a length, before or after, is not in 0 .. max_tokens (0: what the table holds); -2: more than `rows` new tokens;
+ * -3: the free list is shorter than nothing or longer than its room (`pages` entries).  Where it is not 0 table and free list stay as they were, lengths_out =
+ * lengths, free_count_out = free_count, starts are 0 and positions and slots -1.
+ * lengths_out may be lengths, free_count_out free_count.  All int32 but slots; batch <= 8192; one launch. */
+typedef struct {
+  int32_t batch, table_width, page_size, max_tokens;
+  int64_t table_stride, pages, rows;
+  void* page_table;        /* [batch, table_width], rows table_stride apart */
+  const void* lengths;     /* [batch] */
+  const void* counts;      /* [batch] */
+  void* free_pages;        /* [pages] */
+  const void* free_count;  /* [1] */
+  void* lengths_out;       /* [batch] */
+  void* starts;            /* [batch + 1] */
+  void* positions;         /* [rows] */
+  void* slots;             /* int64 [rows] */
+  void* free_count_out;    /* [1] */
+  void* status;            /* [1] */
+} B200PagedPlan;
+B200_API int b200_paged_plan(const B200PagedPlan* plan, void* cuda_stream);
+
+/* ---- a token of every row, drawn with a given random number ----------------------------------------
+ * w_i = exp((x_i - max) / temperature); in the order (logit downwards, index upwards) what stays is the first n entries, n the least of
+ *   top_k (<= 0, or V and more: all);  how many it takes until their weights reach top_p of those of the top_k (>= 1: all; <= 0: one);
+ *   how many have w >= min_p (<= 0: all; more than 1 counts as 1)
+ * token = the first entry, by index, for which the weights of what stays up to it are more than uniform[row] times all of what stays
+ * (0 <= uniform < 1; from 1 on the last one, below 0 or NaN the first); logprob = the logarithm of its share, fp32 (may be NULL).
+ * temperature <= 0 or NaN: the first of the largest logits, logprob 0.  A logit of -inf is an excluded entry: a row of nothing else has token -1 and
+ * logprob -inf; one with a NaN or +inf token -1 and logprob NaN.  Weights and sums are fp64, their error below 2^-42.
+ * A pointer that is not NULL gives every row its own setting (fp32 [rows], top_ks int32 [rows]) and wins over the number.
+ * logits as for b200_token_logprobs; uniform fp32 [rows], token int32 [rows].  One launch, no scratch. */
+typedef struct {
+  float temperature, top_p, min_p;
+  int32_t top_k;
+  const void* temperatures;
+  const void* top_ks;
+  const void* top_ps;
+  const void* min_ps;
+} B200Sampling;
+B200_API int b200_sample_tokens(const void* logits, int32_t dtype, int64_t stride, const void* uniform, const B200Sampling* how, void* token,
+                                void* logprob, int64_t rows, int64_t V, void* cuda_stream);
+
 /* ---- what the logits of a row say ----------------------------------------------------------------
  * p = softmax(logits[row, 0..V)), statistics in fp32:
  *   logprob[row] = log p[tokens[row]], fp32 (a token outside 0..V-1: -inf);  entropy[row] = -sum p log p, fp32 (0 log 0 = 0)

@@ -110,6 +110,33 @@ class PagedAttention(ctypes.Structure):
     ]
 
 
+class PagedScales(ctypes.Structure):
+    """B200PagedScales of include/b200_q4f16.h."""
+
+    _fields_ = [("k_scales", ctypes.c_void_p), ("v_scales", ctypes.c_void_p)]
+
+
+class PagedPlan(ctypes.Structure):
+    """B200PagedPlan of include/b200_q4f16.h."""
+
+    _fields_ = [
+        ("batch", ctypes.c_int32), ("table_width", ctypes.c_int32), ("page_size", ctypes.c_int32), ("max_tokens", ctypes.c_int32),
+        ("table_stride", ctypes.c_int64), ("pages", ctypes.c_int64), ("rows", ctypes.c_int64),
+        ("page_table", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("counts", ctypes.c_void_p), ("free_pages", ctypes.c_void_p),
+        ("free_count", ctypes.c_void_p), ("lengths_out", ctypes.c_void_p), ("starts", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p), ("free_count_out", ctypes.c_void_p), ("status", ctypes.c_void_p),
+    ]
+
+
+class Sampling(ctypes.Structure):
+    """B200Sampling of include/b200_q4f16.h."""
+
+    _fields_ = [
+        ("temperature", ctypes.c_float), ("top_p", ctypes.c_float), ("min_p", ctypes.c_float), ("top_k", ctypes.c_int32),
+        ("temperatures", ctypes.c_void_p), ("top_ks", ctypes.c_void_p), ("top_ps", ctypes.c_void_p), ("min_ps", ctypes.c_void_p),
+    ]
+
+
 # name -> (restype, argtypes); one entry per prototype in include/b200_q4f16.h
 _vp, _i64, _ci = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
 _dlp = ctypes.POINTER(DLTensor)
@@ -175,6 +202,11 @@ PROTOTYPES = {
                                      _vp, _vp]),
     "b200_paged_attention_scratch_bytes": (_i64, []),
     "b200_paged_attention": (_ci, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedAttention), _vp, _i64, _vp]),
+    "b200_paged8_rope_append": (_ci, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedScales), _vp, _i64, ctypes.c_int32, _vp, _vp, _i64,
+                                      ctypes.c_int32, ctypes.c_int32, _vp, _vp, _vp]),
+    "b200_paged8_attention": (_ci, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedScales), ctypes.POINTER(PagedAttention), _vp, _i64, _vp]),
+    "b200_paged_plan": (_ci, [ctypes.POINTER(PagedPlan), _vp]),
+    "b200_sample_tokens": (_ci, [_vp, ctypes.c_int32, _i64, _vp, ctypes.POINTER(Sampling), _vp, _vp, _i64, _i64, _vp]),
     "b200_token_logprobs": (_ci, [_vp, ctypes.c_int32, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, ctypes.c_int32, _vp]),
     "b200_launch_count": (_i64, []),
     "b200_reset_launch_count": (None, []),

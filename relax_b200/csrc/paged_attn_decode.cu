@@ -20,6 +20,8 @@
 // What bounds it: HBM for long caches (131000 tokens of 8 key heads, 537 MB, 90 us: 6.0 TB/s, 0.91 of a copy; 512 sequences of 37 to 2047
 // tokens 182 us: 5.9; 64 of them, 135 MB, 31 us: 4.4); latency for short ones (32 heads at 2011, 33 MB, 13.6 us: 2 until the shares are
 // known, 7 for two or three units a warp, 4 for the joins).  Before, chunks of equal length as CTAs of their own took 157, 45 and 17.5 us.
+#include <type_traits>
+
 #include "paged_common.cuh"
 
 namespace b200 {
@@ -53,6 +55,16 @@ __device__ __forceinline__ uint4 load16(const void* p) {
   asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
+__device__ __forceinline__ uint2 load8(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float log2_approx(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 // A tile's part of a warp that is not the whole tile.
 struct Piece {
@@ -61,12 +73,19 @@ struct Piece {
 };
 
 // kExtra: 1 with a cap or a bias, 2 with a cap for which Cap::any will not do.
-template <typename T, int D, int NT, int kExtra>
+// kBytes: pages of 8 bits with a scale for each unit.  Codes become fp16 in registers, exactly; the scale of a key goes into the factor of
+// its scores, that of a value into the exponent of its weight: m is the maximum of s + log2 v, a weight 2^(s + log2 v - m), so that it has
+// its bits whatever the blocks' sizes are, and the sum takes it by 1 / v.
+template <typename T, int D, int NT, int kExtra, bool kBytes>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kCtasPerSm1 : kCtasPerSm2)
 paged_decode_kernel(const PagedAttnParams p) {
   constexpr int R = 8 * NT;                     // rows of a tile
-  constexpr int SUB = 128 / D;                  // units a warp takes at a time
+  using M = typename std::conditional<kBytes, __half, T>::type;          // what is multiplied
+  constexpr int SUB = (kBytes ? 256 : 128) / D; // units a warp takes at a time
   constexpr int KC = D / 32, VC = D / 64, MT = D / 16;
+  constexpr int KB = D / 64, VW = D / 32;       // 8 bits: loads of a key's dims, words of a value's
+  // the dims of a lane in the result: kDim g .. and kDim g + kDim1 ..
+  constexpr int kDim = kBytes && D == 128 ? 16 : 8, kDim1 = kBytes && D == 128 ? 8 : D == 128 ? 64 : 4;
   constexpr int kPitch = D + 4;
   extern __shared__ __align__(16) float sm_o[];           // [2 kWarps][R][kPitch]: a warp's first piece and its last
   __shared__ float sm_m[2 * kWarps][R], sm_l[2 * kWarps][R];
@@ -162,7 +181,28 @@ paged_decode_kernel(const PagedAttnParams p) {
       auto unit_at = [&](int i, int sub) { return range.unit(min(u_begin + i * SUB + sub, u_end - 1)); };
       auto page_at = [&](int i, int sub) { return page_of(p.c, b, unit_at(i, sub) >> (p.c.page_log2 - 4)); };
       uint4 kr[SUB][2][KC], vr[SUB][4][VC];
+      // (pages of 8 bits: tokens as above; K dims 64 j + 16 t .. + 15, V dims 16 g .. + 15, with head_dim 64 8 g .. + 7)
+      uint4 kb[SUB][2][KB];
+      uint32_t vb[SUB][4][VW];
+      float k_scale[SUB], v_scale[SUB], k_next[SUB], v_next[SUB];
+      auto scale_at = [&](const __half* scales, int i, int x, int id) {
+        const int in_page = ((unit_at(i, x) * kUnit) & (page - 1)) / kUnit;
+        return __half2float(__ldg(scales + (((int64_t)id * kv + h) << (p.c.page_log2 - 4)) + in_page));
+      };
       auto load_k = [&](int i, const int (&id)[SUB]) {
+        if constexpr (kBytes) {
+#pragma unroll
+          for (int x = 0; x < SUB; ++x) {
+            const unsigned char* src = static_cast<const unsigned char*>(p.c.k) + id[x] * p.c.k_stride +
+                                       ((int64_t)h * page + ((unit_at(i, x) * kUnit) & (page - 1))) * D + 16 * t;
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int j = 0; j < KB; ++j) kb[x][r][j] = load16(src + (g + 8 * r) * D + 64 * j);
+            k_next[x] = scale_at(p.k_scales, i, x, id[x]);
+          }
+          return;
+        }
 #pragma unroll
         for (int x = 0; x < SUB; ++x) {
           const T* src = kbase + id[x] * p.c.k_stride + (int64_t)((unit_at(i, x) * kUnit) & (page - 1)) * D;
@@ -173,6 +213,26 @@ paged_decode_kernel(const PagedAttnParams p) {
         }
       };
       auto load_v = [&](int i, const int (&id)[SUB]) {
+        if constexpr (kBytes) {
+#pragma unroll
+          for (int x = 0; x < SUB; ++x) {
+            const unsigned char* src = static_cast<const unsigned char*>(p.c.v) + id[x] * p.c.v_stride +
+                                       ((int64_t)h * page + ((unit_at(i, x) * kUnit) & (page - 1))) * D + kDim * g;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const unsigned char* from = src + (2 * t + (r & 1) + 8 * (r >> 1)) * D;
+              if constexpr (D == 128) {
+                const uint4 v = load16(from);
+                vb[x][r][0] = v.x; vb[x][r][1] = v.y; vb[x][r][VW - 2] = v.z; vb[x][r][VW - 1] = v.w;
+              } else {
+                const uint2 v = load8(from);
+                vb[x][r][0] = v.x; vb[x][r][1] = v.y;
+              }
+            }
+            v_next[x] = scale_at(p.v_scales, i, x, id[x]);
+          }
+          return;
+        }
 #pragma unroll
         for (int x = 0; x < SUB; ++x) {
           const T* src = vbase + id[x] * p.c.v_stride + (int64_t)((unit_at(i, x) * kUnit) & (page - 1)) * D;
@@ -193,7 +253,14 @@ paged_decode_kernel(const PagedAttnParams p) {
         const int r = row0 + 8 * n + g;
         const T* src = static_cast<const T*>(p.q) + (int64_t)(s.first + r / p.group) * p.q_stride + (int64_t)(h * p.group + r % p.group) * D;
 #pragma unroll
-        for (int j = 0; j < KC; ++j) qf[n][j] = 8 * n + g < nrows ? load16(src + 32 * j + 8 * t) : make_uint4(0, 0, 0, 0);
+        for (int j = 0; j < KC; ++j) {
+          const int d = kBytes ? 64 * (j / 2) + 16 * t + 8 * (j & 1) : 32 * j + 8 * t;
+          qf[n][j] = 8 * n + g < nrows ? load16(src + d) : make_uint4(0, 0, 0, 0);
+          if constexpr (!std::is_same<T, M>::value) {
+            auto half = [](uint32_t w) { const float2 v = unpack2(T(), w); return pack2(M(), v.x, v.y); };
+            qf[n][j] = make_uint4(half(qf[n][j].x), half(qf[n][j].y), half(qf[n][j].z), half(qf[n][j].w));
+          }
+        }
       }
       load_k(0, id);
       load_v(0, id);
@@ -226,6 +293,10 @@ paged_decode_kernel(const PagedAttnParams p) {
         int id_next[SUB];
 #pragma unroll
         for (int x = 0; x < SUB; ++x) id_next[x] = i + 2 < steps ? page_at(i + 2, x) : 0;
+        if constexpr (kBytes) {
+#pragma unroll
+          for (int x = 0; x < SUB; ++x) { k_scale[x] = k_next[x]; v_scale[x] = v_next[x]; }
+        }
         // scores of tokens g (0, 1) and g + 8 (2, 3), rows 2 t (0, 2) and 2 t + 1 (1, 3)
         float sc[SUB][NT][4];
 #pragma unroll
@@ -234,13 +305,43 @@ paged_decode_kernel(const PagedAttnParams p) {
           for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) sc[x][n][j] = 0.f;
-#pragma unroll
-            for (int j = 0; j < KC; ++j) {
-              mma(T(), sc[x][n], kr[x][0][j].x, kr[x][1][j].x, kr[x][0][j].y, kr[x][1][j].y, qf[n][j].x, qf[n][j].y);
-              mma(T(), sc[x][n], kr[x][0][j].z, kr[x][1][j].z, kr[x][0][j].w, kr[x][1][j].w, qf[n][j].z, qf[n][j].w);
-            }
           }
+        if constexpr (kBytes) {
+#pragma unroll
+          for (int x = 0; x < SUB; ++x)
+#pragma unroll
+            for (int j = 0; j < KB; ++j)
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                const uint32_t c0 = word(kb[x][0][j], w), c1 = word(kb[x][1][j], w);
+                const uint32_t a0 = e4m3_to_half2(c0 & 0xffffu), a1 = e4m3_to_half2(c1 & 0xffffu);
+                const uint32_t a2 = e4m3_to_half2(c0 >> 16), a3 = e4m3_to_half2(c1 >> 16);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                  const uint4 f = qf[n][2 * j + w / 2];
+                  mma(M(), sc[x][n], a0, a1, a2, a3, w & 1 ? f.z : f.x, w & 1 ? f.w : f.y);
+                }
+              }
+        } else {
+#pragma unroll
+          for (int x = 0; x < SUB; ++x)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int j = 0; j < KC; ++j) {
+                mma(T(), sc[x][n], kr[x][0][j].x, kr[x][1][j].x, kr[x][0][j].y, kr[x][1][j].y, qf[n][j].x, qf[n][j].y);
+                mma(T(), sc[x][n], kr[x][0][j].z, kr[x][1][j].z, kr[x][0][j].w, kr[x][1][j].w, qf[n][j].z, qf[n][j].w);
+              }
+        }
         if (more) load_k(i + 1, id);
+        if (kBytes && kExtra && p.cap > 0.f) {
+#pragma unroll
+          for (int x = 0; x < SUB; ++x)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) sc[x][n][j] *= k_scale[x];
+        }
         if (kExtra == 2) {
 #pragma unroll
           for (int x = 0; x < SUB; ++x)
@@ -264,13 +365,15 @@ paged_decode_kernel(const PagedAttnParams p) {
           // every row sees the whole unit (rows past the tile's end come out as something finite that nobody stores)
           const bool whole = there && position0 >= 0 &&
                              (first + kUnit <= range.pre || (first + kUnit - 1 <= position0 && position1 - first < window));
+          const float factor = kBytes ? to_log2 * k_scale[x] : to_log2, log2_v = kBytes ? log2_approx(v_scale[x]) : 0.f;
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const int token = first + g + 8 * (j >> 1), at = position[n][j & 1];
               float v = sc[x][n][j];
-              if (!(kExtra && p.cap > 0.f)) v *= to_log2;
+              if (!(kExtra && p.cap > 0.f)) v = kBytes ? fmaf(v, factor, log2_v) : v * to_log2;
+              else if (kBytes) v += log2_v;
               if (kExtra) v -= slope[n][j & 1] * fabsf((float)(at - token));
               if (!whole) {
                 const bool seen = there && at >= 0 && (token < range.pre || (token <= at && at - token < window));
@@ -285,7 +388,10 @@ paged_decode_kernel(const PagedAttnParams p) {
               const int token = first + 2 * t + (r & 1) + 8 * (r >> 1);
               if (!(there && (token < range.pre || (token >= range.low && token < range.high))))
 #pragma unroll
-                for (int j = 0; j < VC; ++j) vr[x][r][j] = make_uint4(0, 0, 0, 0);
+                for (int j = 0; j < (kBytes ? VW : VC); ++j) {
+                  if constexpr (kBytes) vb[x][r][j] = 0;
+                  else vr[x][r][j] = make_uint4(0, 0, 0, 0);
+                }
             }
           }
         }
@@ -309,16 +415,36 @@ paged_decode_kernel(const PagedAttnParams p) {
 #pragma unroll
         for (int x = 0; x < SUB; ++x) {
           uint32_t pb[NT][2];
+          const float per_v = kBytes ? __fdividef(1.f, v_scale[x]) : 1.f;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             float w[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               w[j] = sc[x][n][j] == -INFINITY ? 0.f : exp2_approx(sc[x][n][j] - m[n][j & 1]);
-              l[n][j & 1] += w[j];
+              if (!kBytes) l[n][j & 1] += w[j];
+              else if (w[j] != 0.f) l[n][j & 1] = fmaf(w[j], per_v, l[n][j & 1]);      // (what nobody sees may have any scale)
             }
-            pb[n][0] = transpose8x8(pack2(T(), w[0], w[1]));
-            pb[n][1] = transpose8x8(pack2(T(), w[2], w[3]));
+            pb[n][0] = transpose8x8(pack2(M(), w[0], w[1]));
+            pb[n][1] = transpose8x8(pack2(M(), w[2], w[3]));
+          }
+          if constexpr (kBytes) {
+            // row g of the tile: dim kDim g + k, row g + 8: dim kDim g + kDim / 2 + k; a permutation pairs two dims of two tokens
+#pragma unroll
+            for (int k = 0; k < MT; k += 2) {
+              const int w0 = k / 4, w1 = (k + kDim / 2) / 4;
+              const unsigned s = k & 2 ? 0x7362 : 0x5140;
+              const uint32_t c0 = __byte_perm(vb[x][0][w0], vb[x][1][w0], s), c1 = __byte_perm(vb[x][0][w1], vb[x][1][w1], s);
+              const uint32_t c2 = __byte_perm(vb[x][2][w0], vb[x][3][w0], s), c3 = __byte_perm(vb[x][2][w1], vb[x][3][w1], s);
+#pragma unroll
+              for (int o = 0; o < 2; ++o) {
+                const uint32_t a0 = e4m3_to_half2(o ? c0 >> 16 : c0 & 0xffffu), a1 = e4m3_to_half2(o ? c1 >> 16 : c1 & 0xffffu);
+                const uint32_t a2 = e4m3_to_half2(o ? c2 >> 16 : c2 & 0xffffu), a3 = e4m3_to_half2(o ? c3 >> 16 : c3 & 0xffffu);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma(M(), acc[n][k + o], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+              }
+            }
+            continue;
           }
 #pragma unroll
           for (int k = 0; k < MT; ++k) {
@@ -348,12 +474,12 @@ paged_decode_kernel(const PagedAttnParams p) {
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o);
           const int r = 8 * n + 2 * t + e;
-          // dims 8 g .. + 7 and 64 + 8 g .. + 7 (head_dim 64: 8 g .. + 7)
+          // dims 8 g .. + 7 and 64 + 8 g .. + 7 (head_dim 64: 8 g .. + 7; 8 bits: 16 g .. + 15)
           if (all) {
             const float sum = l[n][e], inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;       // (NaN stays)
             if (r < nrows) {
               const int x = row0 + r;
-              T* out = static_cast<T*>(p.out) + ((int64_t)(s.first + x / p.group) * p.heads + h * p.group + x % p.group) * D + 8 * g;
+              T* out = static_cast<T*>(p.out) + ((int64_t)(s.first + x / p.group) * p.heads + h * p.group + x % p.group) * D + kDim * g;
               uint32_t v[2][4];
 #pragma unroll
               for (int k = 0; k < MT; k += 2) {
@@ -362,15 +488,15 @@ paged_decode_kernel(const PagedAttnParams p) {
                 else v[0][2 + k / 2] = pack2(T(), acc[n][k][e + 2] * inv, acc[n][k + 1][e + 2] * inv);
               }
               *reinterpret_cast<uint4*>(out) = make_uint4(v[0][0], v[0][1], v[0][2], v[0][3]);
-              if (D == 128) *reinterpret_cast<uint4*>(out + 64) = make_uint4(v[1][0], v[1][1], v[1][2], v[1][3]);
+              if (D == 128) *reinterpret_cast<uint4*>(out + kDim1) = make_uint4(v[1][0], v[1][1], v[1][2], v[1][3]);
             }
           } else {
             if (g == 0) { sm_m[slot][r] = m[n][e]; sm_l[slot][r] = l[n][e]; }
             float* to = sm_o + (slot * R + r) * kPitch;
 #pragma unroll
             for (int k = 0; k < MT; k += 4) {
-              *reinterpret_cast<float4*>(to + 8 * g + k) = make_float4(acc[n][k][e], acc[n][k + 1][e], acc[n][k + 2][e], acc[n][k + 3][e]);
-              *reinterpret_cast<float4*>(to + (D == 128 ? 64 + 8 * g + k : 8 * g + 4 + k)) =
+              *reinterpret_cast<float4*>(to + kDim * g + k) = make_float4(acc[n][k][e], acc[n][k + 1][e], acc[n][k + 2][e], acc[n][k + 3][e]);
+              *reinterpret_cast<float4*>(to + kDim * g + kDim1 + k) =
                   make_float4(acc[n][k][e + 2], acc[n][k + 1][e + 2], acc[n][k + 2][e + 2], acc[n][k + 3][e + 2]);
             }
           }
@@ -543,6 +669,7 @@ paged_decode_kernel(const PagedAttnParams p) {
   }
 }
 
+template <bool kBytes>
 int launch_decode(const char* who, const B200PagedCache* c, PagedAttnParams p, cudaStream_t stream) {
   const int64_t most = (int64_t)c->max_query * p.group;          // rows of a sequence that share a key head
   const bool narrow = most <= 8;
@@ -574,8 +701,8 @@ int launch_decode(const char* who, const B200PagedCache* c, PagedAttnParams p, c
     static SmemLimit limit[2][3];
     auto by_rows = [&](auto tiles, SmemLimit* of) {
       constexpr int NT = decltype(tiles)::value;
-      return extra == 0 ? launch(paged_decode_kernel<T, D, NT, 0>, of[0])
-           : extra == 1 ? launch(paged_decode_kernel<T, D, NT, 1>, of[1]) : launch(paged_decode_kernel<T, D, NT, 2>, of[2]);
+      return extra == 0 ? launch(paged_decode_kernel<T, D, NT, 0, kBytes>, of[0])
+           : extra == 1 ? launch(paged_decode_kernel<T, D, NT, 1, kBytes>, of[1]) : launch(paged_decode_kernel<T, D, NT, 2, kBytes>, of[2]);
     };
     return narrow ? by_rows(std::integral_constant<int, 1>(), limit[0]) : by_rows(std::integral_constant<int, 2>(), limit[1]);
   };
@@ -602,11 +729,16 @@ int64_t b200_paged_attention_scratch_bytes(void) {
   return B200_PAGED_ZEROED_BYTES + scratch_rows() * (2 + 128) * (int64_t)sizeof(float);
 }
 
-int b200_paged_attention(const B200PagedCache* cache, const B200PagedAttention* a, void* scratch, int64_t scratch_bytes, void* stream) {
-  const char* who = "paged_attention";
+static int paged_attention(const char* who, const B200PagedCache* cache, const B200PagedScales* scales, const B200PagedAttention* a, void* scratch,
+                           int64_t scratch_bytes, void* stream, bool bytes) {
   PagedAttnParams p = {};
   int rc = paged_params(who, cache, &p.c);
   if (rc) return rc;
+  if (bytes) {
+    if ((rc = paged8_scales(who, cache, scales))) return rc;
+    p.k_scales = static_cast<const __half*>(scales->k_scales);
+    p.v_scales = static_cast<const __half*>(scales->v_scales);
+  }
   if (!a) return fail(B200_EINVAL, "%s: null argument descriptor", who);
   if (a->heads <= 0 || a->heads % cache->kv_heads || a->heads / cache->kv_heads > 128)
     return fail(B200_EINVAL, "%s: heads is a multiple of kv_heads, up to 128 times as many; got %d and %d", who, a->heads, cache->kv_heads);
@@ -640,8 +772,18 @@ int b200_paged_attention(const B200PagedCache* cache, const B200PagedAttention* 
   p.partial = p.partial_ml + 2 * scratch_rows();
   // Rows of a sequence that share a key head: up to 16 are two operand tiles of the few-rows kernel; more are cut into tiles that
   // each read the keys again, where the kernel for many rows reads them once for 256.
-  if ((int64_t)cache->max_query * p.group <= 16) return launch_decode(who, cache, p, static_cast<cudaStream_t>(stream));
+  if (bytes) return launch_decode<true>(who, cache, p, static_cast<cudaStream_t>(stream));
+  if ((int64_t)cache->max_query * p.group <= 16) return launch_decode<false>(who, cache, p, static_cast<cudaStream_t>(stream));
   return launch_paged_prompt(who, cache, p, static_cast<cudaStream_t>(stream));
+}
+
+int b200_paged_attention(const B200PagedCache* cache, const B200PagedAttention* a, void* scratch, int64_t scratch_bytes, void* stream) {
+  return paged_attention("paged_attention", cache, nullptr, a, scratch, scratch_bytes, stream, false);
+}
+
+int b200_paged8_attention(const B200PagedCache* cache, const B200PagedScales* scales, const B200PagedAttention* a, void* scratch,
+                          int64_t scratch_bytes, void* stream) {
+  return paged_attention("paged8_attention", cache, scales, a, scratch, scratch_bytes, stream, true);
 }
 
 }  // extern "C"

@@ -107,6 +107,8 @@ struct PagedAttnParams {
   const int* prefix;
   float* partial;              // few rows: [part][row][D]; many rows: [part][tile of two][D / 4][row][4]
   float* partial_ml;           // their rows' maxima and sums, in pairs
+  const __half* k_scales;      // pages of 8 bits: [pages, kv_heads, page / 16]
+  const __half* v_scales;
   int* arrived;                // few rows: [CTA]
   int slots;                   // CTAs that run at once
 };
@@ -153,6 +155,13 @@ struct PromptWords {
 };
 static_assert(kFewCounters * 4 + kCutTiles * 8 + sizeof(PromptWords) <= B200_PAGED_ZEROED_BYTES, "the counters");
 
+// Two e4m3 codes (the low one first) as fp16 values, which hold them exactly.
+__device__ __forceinline__ uint32_t e4m3_to_half2(uint32_t codes) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)codes));
+  return r;
+}
+
 // The kernel for many rows (paged_attn_prompt.cu).
 int launch_paged_prompt(const char* who, const B200PagedCache* c, PagedAttnParams p, cudaStream_t stream);
 
@@ -160,5 +169,7 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 // Launch parameters of a checked descriptor; `who` names the entry point in messages.
 int paged_params(const char* who, const B200PagedCache* c, PagedParams* out);
+// The scales of pages of 8 bits, beside a checked descriptor.
+int paged8_scales(const char* who, const B200PagedCache* c, const B200PagedScales* s);
 
 }  // namespace b200

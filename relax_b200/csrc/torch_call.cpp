@@ -32,6 +32,10 @@ struct Entry {
   decltype(&b200_paged_rope_append) paged_rope_append = nullptr;
   decltype(&b200_paged_attention) paged_attention = nullptr;
   decltype(&b200_token_logprobs) token_logprobs = nullptr;
+  decltype(&b200_paged8_rope_append) paged8_rope_append = nullptr;
+  decltype(&b200_paged8_attention) paged8_attention = nullptr;
+  decltype(&b200_paged_plan) paged_plan = nullptr;
+  decltype(&b200_sample_tokens) sample_tokens = nullptr;
 } g_entry;
 
 const at::Tensor* plain(PyObject* o) {
@@ -150,11 +154,20 @@ bool number(PyObject* o, double* out) {
   return true;
 }
 
-// The pages, the table and the lengths of a call with `tokens` rows of `type` on `dev`.
-bool paged_cache(PyObject* const* args, int64_t tokens, at::ScalarType type, B200PagedCache* c, int dev) {
+// The pages, the table and the lengths of a call with `tokens` rows of `type` on `dev`; `scales`: two arguments, None where the pages are
+// of the rows' type, the scales where they are of 8 bits.
+bool paged_cache(PyObject* const* args, int64_t tokens, at::ScalarType type, B200PagedCache* c, int dev, PyObject* const* scales, B200PagedScales* s) {
   const at::Tensor *k = plain(args[0]), *v = plain(args[1]), *table = plain(args[2]), *lengths, *starts;
   if (!k || !v || !table || (type != at::kHalf && type != at::kBFloat16)) return false;
-  if (k->scalar_type() != type || v->scalar_type() != type || k->dim() != 4 || v->sizes() != k->sizes()) return false;
+  const at::ScalarType stored = scales[0] == Py_None && scales[1] == Py_None ? type : at::kFloat8_e4m3fn;
+  if (k->scalar_type() != stored || v->scalar_type() != stored || k->dim() != 4 || v->sizes() != k->sizes()) return false;
+  for (int i = 0; stored != type && i < 2; ++i) {
+    const at::Tensor* t = plain(scales[i]);
+    if (!t || t->scalar_type() != at::kHalf || t->dim() != 3 || !t->is_contiguous() || t->get_device() != dev || t->size(0) != k->size(0) ||
+        t->size(1) != k->size(1) || t->size(2) != k->size(2) / 16)
+      return false;
+    (i ? s->v_scales : s->k_scales) = const_cast<void*>(t->const_data_ptr());
+  }
   const int64_t page = k->size(2), dim = k->size(3);
   for (const at::Tensor* t : {k, v})
     if (t->stride(3) != 1 || t->stride(2) != dim || (t->size(1) > 1 && t->stride(1) != page * dim)) return false;
@@ -194,10 +207,10 @@ at::Tensor result_of(PyObject* given, at::IntArrayRef sizes, const at::Tensor& l
   return *t;
 }
 
-// paged_rope_append(qkv, cos, sin, k, v, table, lengths, starts, interleaved, positions, out)
+// paged_rope_append(qkv, cos, sin, k, v, table, lengths, starts, interleaved, positions, out, k_scales, v_scales)
 PyObject* paged_rope_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 11) {
-    PyErr_SetString(PyExc_TypeError, "paged_rope_append() takes 11 arguments");
+  if (n != 13) {
+    PyErr_SetString(PyExc_TypeError, "paged_rope_append() takes 13 arguments");
     return nullptr;
   }
   try {
@@ -207,7 +220,8 @@ PyObject* paged_rope_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int dev = common_device({qkv, cos, sin});
     const int64_t tokens = qkv->size(0);
     B200PagedCache c = {};
-    if (dev < 0 || !PyBool_Check(args[8]) || !paged_cache(args + 3, tokens, qkv->scalar_type(), &c, dev)) Py_RETURN_NONE;
+    B200PagedScales scales = {};
+    if (dev < 0 || !PyBool_Check(args[8]) || !paged_cache(args + 3, tokens, qkv->scalar_type(), &c, dev, args + 11, &scales)) Py_RETURN_NONE;
     if (!optional_vector(args[9], at::kInt, tokens, &positions) || (positions && positions->get_device() != dev)) Py_RETURN_NONE;
     if (c.head_dim == 0 || qkv->size(1) % c.head_dim || cos->size(1) > c.head_dim) Py_RETURN_NONE;
     const int64_t heads = qkv->size(1) / c.head_dim - 2 * (int64_t)c.kv_heads;
@@ -218,8 +232,12 @@ PyObject* paged_rope_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t stride = tokens > 1 ? qkv->stride(0) : qkv->size(1);
     int rc;
     Py_BEGIN_ALLOW_THREADS
-    rc = g_entry.paged_rope_append(&c, qkv->const_data_ptr(), stride, (int32_t)heads, cos->const_data_ptr(), sin->const_data_ptr(), cos->size(0),
-                                   (int32_t)(2 * cos->size(1)), args[8] == Py_True, pointer(positions), out.mutable_data_ptr(), stream);
+    if (scales.k_scales)
+      rc = g_entry.paged8_rope_append(&c, &scales, qkv->const_data_ptr(), stride, (int32_t)heads, cos->const_data_ptr(), sin->const_data_ptr(),
+                                      cos->size(0), (int32_t)(2 * cos->size(1)), args[8] == Py_True, pointer(positions), out.mutable_data_ptr(), stream);
+    else
+      rc = g_entry.paged_rope_append(&c, qkv->const_data_ptr(), stride, (int32_t)heads, cos->const_data_ptr(), sin->const_data_ptr(), cos->size(0),
+                                     (int32_t)(2 * cos->size(1)), args[8] == Py_True, pointer(positions), out.mutable_data_ptr(), stream);
     Py_END_ALLOW_THREADS
     if (rc != 0) Py_RETURN_NONE;
     return THPVariable_Wrap(out);
@@ -228,10 +246,10 @@ PyObject* paged_rope_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
 }
 
-// paged_attention(q, k, v, table, lengths, starts, max_query, scale, causal, window, cap, slopes, prefix, out, scratch)
+// paged_attention(q, k, v, table, lengths, starts, max_query, scale, causal, window, cap, slopes, prefix, out, scratch, k_scales, v_scales)
 PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 15) {
-    PyErr_SetString(PyExc_TypeError, "paged_attention() takes 15 arguments");
+  if (n != 17) {
+    PyErr_SetString(PyExc_TypeError, "paged_attention() takes 17 arguments");
     return nullptr;
   }
   try {
@@ -241,7 +259,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int dev = common_device({q, scratch});
     const int64_t tokens = q->size(0), heads = q->size(1);
     B200PagedCache c = {};
-    if (dev < 0 || tokens == 0 || heads > INT32_MAX || !paged_cache(args + 1, tokens, q->scalar_type(), &c, dev)) Py_RETURN_NONE;
+    B200PagedScales scales = {};
+    if (dev < 0 || tokens == 0 || heads > INT32_MAX || !paged_cache(args + 1, tokens, q->scalar_type(), &c, dev, args + 15, &scales)) Py_RETURN_NONE;
     if (q->size(2) != c.head_dim || q->stride(2) != 1 || (heads > 1 && q->stride(1) != c.head_dim)) Py_RETURN_NONE;
     if (!optional_vector(args[11], at::kFloat, heads, &slopes) || !optional_vector(args[12], at::kInt, c.batch, &prefix)) Py_RETURN_NONE;
     if ((slopes && slopes->get_device() != dev) || (prefix && prefix->get_device() != dev)) Py_RETURN_NONE;
@@ -270,7 +289,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     void* stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
     int rc;
     Py_BEGIN_ALLOW_THREADS
-    rc = g_entry.paged_attention(&c, &a, scratch->mutable_data_ptr(), (int64_t)scratch->nbytes(), stream);
+    rc = scales.k_scales ? g_entry.paged8_attention(&c, &scales, &a, scratch->mutable_data_ptr(), (int64_t)scratch->nbytes(), stream)
+                         : g_entry.paged_attention(&c, &a, scratch->mutable_data_ptr(), (int64_t)scratch->nbytes(), stream);
     Py_END_ALLOW_THREADS
     if (rc != 0) Py_RETURN_NONE;
     return THPVariable_Wrap(out);
@@ -318,22 +338,144 @@ PyObject* token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
 }
 
-// bind(set_stream, matmul, matmul_layout, dequantize, paged_rope_append, paged_attention, token_logprobs): addresses of the loaded
-// library's entry points.
+// paged_plan(table, lengths, counts, free_pages, free_count, page_size, rows, max_tokens, out): (lengths, starts, positions, slots, free_count,
+// status), `out` a tuple of them or None
+PyObject* paged_plan(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 9) {
+    PyErr_SetString(PyExc_TypeError, "paged_plan() takes 9 arguments");
+    return nullptr;
+  }
+  try {
+    if (!g_entry.paged_plan || at::impl::torch_function_mode_enabled()) Py_RETURN_NONE;
+    const at::Tensor *table = plain(args[0]), *lengths, *counts, *free_pages = plain(args[3]), *free_count;
+    if (!table || table->scalar_type() != at::kInt || table->dim() != 2 || (table->size(1) > 1 && table->stride(1) != 1)) Py_RETURN_NONE;
+    const int64_t batch = table->size(0), width = table->size(1);
+    if (args[1] == Py_None || args[2] == Py_None || args[4] == Py_None || !free_pages || free_pages->dim() != 1) Py_RETURN_NONE;
+    if (!optional_vector(args[1], at::kInt, batch, &lengths) || !optional_vector(args[2], at::kInt, batch, &counts) ||
+        free_pages->scalar_type() != at::kInt || !free_pages->is_contiguous() || !optional_vector(args[4], at::kInt, 1, &free_count))
+      Py_RETURN_NONE;
+    const int dev = common_device({table, lengths, counts, free_pages, free_count});
+    int64_t page, rows, most;
+    if (dev < 0 || !whole(args[5], 0, INT32_MAX, &page) || !whole(args[6], 0, INT32_MAX, &rows) || !whole(args[7], 0, INT32_MAX, &most)) Py_RETURN_NONE;
+    if (batch > INT32_MAX || width > INT32_MAX) Py_RETURN_NONE;
+    at::Tensor out[6];
+    const int64_t sizes[6] = {batch, batch + 1, rows, rows, 1, 1};
+    const auto i32 = table->options().requires_grad(false);
+    if (args[8] != Py_None && (!PyTuple_Check(args[8]) || PyTuple_GET_SIZE(args[8]) != 6)) Py_RETURN_NONE;
+    for (int i = 0; i < 6; ++i) {
+      const at::ScalarType type = i == 3 ? at::kLong : at::kInt;
+      if (args[8] == Py_None) {
+        out[i] = at::empty({sizes[i]}, i32.dtype(type));
+        continue;
+      }
+      const at::Tensor* t = plain(PyTuple_GET_ITEM(args[8], i));
+      if (!t || t->scalar_type() != type || t->dim() != 1 || t->size(0) != sizes[i] || !t->is_contiguous() || t->get_device() != dev) Py_RETURN_NONE;
+      out[i] = *t;
+    }
+    B200PagedPlan p = {};
+    p.batch = (int32_t)batch;
+    p.table_width = (int32_t)width;
+    p.page_size = (int32_t)page;
+    p.max_tokens = (int32_t)most;
+    p.table_stride = batch > 1 ? table->stride(0) : width;
+    p.pages = free_pages->size(0);
+    p.rows = rows;
+    p.page_table = table->mutable_data_ptr();
+    p.lengths = lengths->const_data_ptr();
+    p.counts = counts->const_data_ptr();
+    p.free_pages = free_pages->mutable_data_ptr();
+    p.free_count = free_count->const_data_ptr();
+    void** results[6] = {&p.lengths_out, &p.starts, &p.positions, &p.slots, &p.free_count_out, &p.status};
+    for (int i = 0; i < 6; ++i) *results[i] = out[i].mutable_data_ptr();
+    void* stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_entry.paged_plan(&p, stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) Py_RETURN_NONE;
+    return Py_BuildValue("(NNNNNN)", THPVariable_Wrap(out[0]), THPVariable_Wrap(out[1]), THPVariable_Wrap(out[2]), THPVariable_Wrap(out[3]),
+                         THPVariable_Wrap(out[4]), THPVariable_Wrap(out[5]));
+  } catch (const std::exception&) {
+    Py_RETURN_NONE;
+  }
+}
+
+// A setting: a number, or a tensor of one for each row.
+bool setting(PyObject* o, at::ScalarType type, int64_t rows, int dev, double* value, const void** of_rows) {
+  *value = 0;
+  *of_rows = nullptr;
+  const at::Tensor* t = plain(o);
+  if (t) {
+    *of_rows = t->const_data_ptr();
+    return t->scalar_type() == type && t->dim() == 1 && t->size(0) == rows && t->is_contiguous() && t->get_device() == dev;
+  }
+  int64_t i;
+  if (type != at::kInt) return number(o, value);
+  if (!whole(o, 0, INT32_MAX, &i)) return false;
+  *value = (double)i;
+  return true;
+}
+
+// sample_tokens(logits, uniform, temperature, top_k, top_p, min_p): (token, logprob)
+PyObject* sample_tokens(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 6) {
+    PyErr_SetString(PyExc_TypeError, "sample_tokens() takes 6 arguments");
+    return nullptr;
+  }
+  try {
+    if (!g_entry.sample_tokens || at::impl::torch_function_mode_enabled()) Py_RETURN_NONE;
+    const at::Tensor *x = plain(args[0]), *uniform;
+    if (!x || x->dim() != 2 || (x->size(1) > 1 && x->stride(1) != 1)) Py_RETURN_NONE;
+    const int64_t rows = x->size(0), V = x->size(1);
+    if (args[1] == Py_None || !optional_vector(args[1], at::kFloat, rows, &uniform) || rows == 0) Py_RETURN_NONE;
+    const int dev = common_device({x, uniform});
+    const at::ScalarType t = x->scalar_type();
+    if (dev < 0 || (t != at::kHalf && t != at::kBFloat16 && t != at::kFloat)) Py_RETURN_NONE;
+    B200Sampling how = {};
+    double temperature, k, top_p, min_p;
+    if (!setting(args[2], at::kFloat, rows, dev, &temperature, &how.temperatures) || !setting(args[3], at::kInt, rows, dev, &k, &how.top_ks) ||
+        !setting(args[4], at::kFloat, rows, dev, &top_p, &how.top_ps) || !setting(args[5], at::kFloat, rows, dev, &min_p, &how.min_ps))
+      Py_RETURN_NONE;
+    how.temperature = (float)temperature;
+    how.top_k = (int32_t)k;
+    how.top_p = (float)top_p;
+    how.min_p = (float)min_p;
+    const auto fp32 = x->options().dtype(at::kFloat).requires_grad(false);
+    const at::Tensor token = at::empty({rows}, fp32.dtype(at::kInt)), logprob = at::empty({rows}, fp32);
+    void *p0 = token.mutable_data_ptr(), *p1 = logprob.mutable_data_ptr();
+    void* stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_entry.sample_tokens(x->const_data_ptr(), t == at::kHalf ? B200_F16 : t == at::kBFloat16 ? B200_BF16 : B200_F32,
+                               rows > 1 ? x->stride(0) : V, uniform->const_data_ptr(), &how, p0, p1, rows, V, stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) Py_RETURN_NONE;
+    return Py_BuildValue("(NN)", THPVariable_Wrap(token), THPVariable_Wrap(logprob));
+  } catch (const std::exception&) {
+    Py_RETURN_NONE;
+  }
+}
+
+// bind(set_stream, matmul, matmul_layout, dequantize, paged_rope_append, paged_attention, token_logprobs, paged8_rope_append, paged8_attention,
+// paged_plan, sample_tokens): addresses of the loaded library's entry points.
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  constexpr Py_ssize_t kEntries = 7;
+  constexpr Py_ssize_t kEntries = 11;
   void* p[kEntries] = {};
   for (Py_ssize_t i = 0; n == kEntries && i < n; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
   if (PyErr_Occurred()) return nullptr;
   bool all = n == kEntries;
   for (void* q : p) all = all && q;
   if (!all) {
-    PyErr_SetString(PyExc_TypeError, "bind() takes the addresses of seven entry points");
+    PyErr_SetString(PyExc_TypeError, "bind() takes the addresses of eleven entry points");
     return nullptr;
   }
   g_entry.paged_rope_append = reinterpret_cast<decltype(g_entry.paged_rope_append)>(p[4]);
   g_entry.paged_attention = reinterpret_cast<decltype(g_entry.paged_attention)>(p[5]);
   g_entry.token_logprobs = reinterpret_cast<decltype(g_entry.token_logprobs)>(p[6]);
+  g_entry.paged8_rope_append = reinterpret_cast<decltype(g_entry.paged8_rope_append)>(p[7]);
+  g_entry.paged8_attention = reinterpret_cast<decltype(g_entry.paged8_attention)>(p[8]);
+  g_entry.paged_plan = reinterpret_cast<decltype(g_entry.paged_plan)>(p[9]);
+  g_entry.sample_tokens = reinterpret_cast<decltype(g_entry.sample_tokens)>(p[10]);
   g_entry.set_stream = reinterpret_cast<decltype(g_entry.set_stream)>(p[0]);
   g_entry.matmul = reinterpret_cast<decltype(g_entry.matmul)>(p[1]);
   g_entry.matmul_layout = reinterpret_cast<decltype(g_entry.matmul_layout)>(p[2]);
@@ -347,6 +489,8 @@ PyMethodDef kMethods[] = {
     {"paged_rope_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_rope_append)), METH_FASTCALL, nullptr},
     {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_attention)), METH_FASTCALL, nullptr},
     {"token_logprobs", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(token_logprobs)), METH_FASTCALL, nullptr},
+    {"paged_plan", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_plan)), METH_FASTCALL, nullptr},
+    {"sample_tokens", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(sample_tokens)), METH_FASTCALL, nullptr},
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

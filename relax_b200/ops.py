@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import importlib.util
+import operator
 import typing
 
 import torch
@@ -157,7 +158,8 @@ def _torch_call():
             L = _lib.lib()
             module.bind(*(ctypes.cast(fn, ctypes.c_void_p).value
                           for fn in (L.b200_set_stream, L.b200_q4f16_matmul, L.b200_q4f16_matmul_layout, L.b200_q4f16_dequantize,
-                                     L.b200_paged_rope_append, L.b200_paged_attention, L.b200_token_logprobs)))
+                                     L.b200_paged_rope_append, L.b200_paged_attention, L.b200_token_logprobs, L.b200_paged8_rope_append,
+                                     L.b200_paged8_attention, L.b200_paged_plan, L.b200_sample_tokens)))
             _native = module
     return _native
 
@@ -271,13 +273,21 @@ def _index(name, t, shape):
     return t.data_ptr()
 
 
-def _paged_cache(rows, k_pages, v_pages, page_table, lengths, starts, max_query) -> _lib.PagedCache:
+def _paged_cache(rows, k_pages, v_pages, page_table, lengths, starts, max_query, k_scales=None, v_scales=None) -> _lib.PagedCache:
     """The descriptor of a call over `rows` (whose first dimension is the tokens of the call), its tensors checked."""
-    if k_pages.dtype not in _CACHE_TYPES or v_pages.dtype is not k_pages.dtype:
-        raise ValueError(f"pages are fp16 or bf16, both alike: got {k_pages.dtype} and {v_pages.dtype}")
+    eight = k_pages.dtype is torch.float8_e4m3fn
+    if (k_pages.dtype not in _CACHE_TYPES and not eight) or v_pages.dtype is not k_pages.dtype:
+        raise ValueError(f"pages are fp16, bf16 or float8_e4m3fn, both alike: got {k_pages.dtype} and {v_pages.dtype}")
+    if (k_scales is not None) != eight or (v_scales is not None) != eight:
+        raise ValueError("pages of float8_e4m3fn need k_scales and v_scales, others take none")
+    if eight and rows.dtype not in _CACHE_TYPES:
+        raise ValueError(f"rows are fp16 or bf16, got {rows.dtype}")
     if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
         raise ValueError(f"pages are [pages, kv_heads, page_size, head_dim], both alike: got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
     pages, kv_heads, page_size, head_dim = k_pages.shape
+    for name, t in (("k_scales", k_scales), ("v_scales", v_scales)) if eight else ():
+        if t.dtype is not torch.float16 or tuple(t.shape) != (pages, kv_heads, page_size // 16) or not t.is_contiguous():
+            raise ValueError(f"{name} is a contiguous fp16 tensor of shape {(pages, kv_heads, page_size // 16)}, got {t.dtype} {tuple(t.shape)}")
     whole = kv_heads * page_size * head_dim             # (the stride of a dimension of one entry says nothing)
     for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
         if t.stride()[2:] != (head_dim, 1) or (kv_heads > 1 and t.stride(1) != page_size * head_dim):
@@ -293,28 +303,33 @@ def _paged_cache(rows, k_pages, v_pages, page_table, lengths, starts, max_query)
     elif max_query is None:
         max_query = tokens
     stride = page_table.stride(0) if batch > 1 else width
-    return _lib.PagedCache(_CACHE_TYPES[k_pages.dtype], kv_heads, head_dim, page_size, pages,
+    return _lib.PagedCache(_CACHE_TYPES[rows.dtype if eight else k_pages.dtype], kv_heads, head_dim, page_size, pages,
                            *(t.stride(0) if pages > 1 else whole for t in (k_pages, v_pages)), k_pages.data_ptr(), v_pages.data_ptr(), batch, width, int(max_query), stride, tokens, page_table.data_ptr(),
                            _index("lengths", lengths, (batch,)), _index("starts", starts, (batch + 1,)))
 
 
 def paged_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                       page_table: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor | None = None, interleaved: bool = False,
-                      positions: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                      positions: torch.Tensor | None = None, out: torch.Tensor | None = None, k_scales: torch.Tensor | None = None,
+                      v_scales: torch.Tensor | None = None) -> torch.Tensor:
     """Turns q and k of qkv [tokens, (heads + 2 kv_heads) * head_dim] by their positions, stores k and v in the pages and returns
     q [tokens, heads, head_dim].
 
     ``lengths`` [batch] counts the tokens of every sequence with the new ones; rows ``starts[b] .. starts[b + 1] - 1`` are the newest of
     sequence b (None: one row each).  cos and sin, fp32 [positions, r / 2], turn the first r values of a head: pairs (i, i + r / 2), or
-    (2 i, 2 i + 1) with ``interleaved``; ``positions`` (int32 [tokens]) names other rows of the tables than the tokens' places."""
+    (2 i, 2 i + 1) with ``interleaved``; ``positions`` (int32 [tokens]) names other rows of the tables than the tokens' places.
+
+    Pages of float8_e4m3fn hold values divided by the scale of their block of 16 tokens: ``k_scales`` and ``v_scales``, fp16
+    [pages, kv_heads, page_size / 16].  The scale is the smallest power of two (2^-24 to 2^7) by which the new tokens fit, and not smaller than that
+    of earlier tokens of the block, which are scaled anew where it grows.  Larger values are stored as 448 * 2^7, what is not finite as NaN."""
     native = _native or _torch_call()
     if native:
-        q = native.paged_rope_append(qkv, cos, sin, k_pages, v_pages, page_table, lengths, starts, interleaved, positions, out)
+        q = native.paged_rope_append(qkv, cos, sin, k_pages, v_pages, page_table, lengths, starts, interleaved, positions, out, k_scales, v_scales)
         if q is not None:
             return q
-    cache = _paged_cache(qkv, k_pages, v_pages, page_table, lengths, starts, 1)
+    cache = _paged_cache(qkv, k_pages, v_pages, page_table, lengths, starts, 1, k_scales, v_scales)
     kv, dim = cache.kv_heads, cache.head_dim
-    if qkv.dtype is not k_pages.dtype or qkv.dim() != 2 or (qkv.shape[1] > 1 and qkv.stride(1) != 1) or qkv.shape[1] % dim:
+    if (k_scales is None and qkv.dtype is not k_pages.dtype) or qkv.dim() != 2 or (qkv.shape[1] > 1 and qkv.stride(1) != 1) or qkv.shape[1] % dim:
         raise ValueError(f"qkv is [tokens, (heads + 2 kv_heads) * {dim}] of the pages' type with contiguous rows")
     heads = qkv.shape[1] // dim - 2 * kv
     if heads <= 0:
@@ -327,11 +342,12 @@ def paged_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k
     elif out.dtype is not qkv.dtype or out.shape != (qkv.shape[0], heads, dim) or not out.is_contiguous():
         raise ValueError(f"out is a contiguous [tokens, {heads}, {dim}] of qkv's type")
     _same_device(qkv.device, k_pages=k_pages, v_pages=v_pages, page_table=page_table, lengths=lengths, starts=starts, cos=cos, sin=sin,
-                 positions=positions, out=out)
+                 positions=positions, out=out, k_scales=k_scales, v_scales=v_scales)
     stride = qkv.stride(0) if qkv.shape[0] > 1 else qkv.shape[1]
+    scales = () if k_scales is None else (ctypes.byref(_lib.PagedScales(k_scales.data_ptr(), v_scales.data_ptr())),)
     with _on(qkv.device):
-        _lib.check(_lib.lib().b200_paged_rope_append(
-            ctypes.byref(cache), qkv.data_ptr(), stride, heads, cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1],
+        _lib.check((_lib.lib().b200_paged8_rope_append if scales else _lib.lib().b200_paged_rope_append)(
+            ctypes.byref(cache), *scales, qkv.data_ptr(), stride, heads, cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1],
             int(interleaved), _index("positions", positions, (qkv.shape[0],)), out.data_ptr(), _stream_ptr(qkv.device)))
     return out
 
@@ -365,25 +381,27 @@ def _stream_scratch(device) -> torch.Tensor:
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
                     starts: torch.Tensor | None = None, max_query: int | None = None, scale: float | None = None, causal: bool = True,
                     window: int = 0, cap: float = 0.0, slopes: torch.Tensor | None = None, prefix: torch.Tensor | None = None,
-                    out: torch.Tensor | None = None, scratch: torch.Tensor | None = None) -> torch.Tensor:
+                    out: torch.Tensor | None = None, scratch: torch.Tensor | None = None, k_scales: torch.Tensor | None = None,
+                    v_scales: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of the rows q [tokens, heads, head_dim] over the keys and values of their sequences in the pages.
 
     ``lengths``, ``starts`` and the rows of a sequence as in :func:`paged_rope_append`, which has stored their keys before;
     ``max_query``: no sequence has more rows (None: the number of tokens).  A row at position t sees key j where j < prefix[b], or j <= t and
     (``window`` = 0 or t - j < window); ``causal`` = False: every key of its sequence.  Scores are scale * q.k (scale: 1 / sqrt(head_dim)),
     with ``cap`` > 0 cap * tanh(score / cap), with ``slopes`` (fp32 [heads]) less slopes[h] * |t - j|.  A row that sees nothing gets zeros.
-    ``scratch``: see :func:`paged_attention_scratch`; None takes memory that belongs to the current stream."""
+    ``scratch``: see :func:`paged_attention_scratch`; None takes memory that belongs to the current stream.
+    ``k_scales``, ``v_scales``: of pages of float8_e4m3fn, as in :func:`paged_rope_append`; q, fp16 or bf16, is taken in fp16."""
     native = _native or _torch_call()
     if native and q.is_cuda and torch._C._cuda_getDevice() == q.device.index:
         if scratch is None:
             scratch = _stream_scratch(q.device)
         result = native.paged_attention(q, k_pages, v_pages, page_table, lengths, starts, max_query, scale, causal, window, cap, slopes,
-                                        prefix, out, scratch)
+                                        prefix, out, scratch, k_scales, v_scales)
         if result is not None:
             return result
-    cache = _paged_cache(q, k_pages, v_pages, page_table, lengths, starts, max_query)
+    cache = _paged_cache(q, k_pages, v_pages, page_table, lengths, starts, max_query, k_scales, v_scales)
     kv, dim = cache.kv_heads, cache.head_dim
-    if q.dtype is not k_pages.dtype or q.dim() != 3 or q.shape[2] != dim or (q.shape[0] and (q.stride(2) != 1 or (q.shape[1] > 1 and q.stride(1) != dim))):
+    if (k_scales is None and q.dtype is not k_pages.dtype) or q.dim() != 3 or q.shape[2] != dim or (q.shape[0] and (q.stride(2) != 1 or (q.shape[1] > 1 and q.stride(1) != dim))):
         raise ValueError(f"q is [tokens, heads, {dim}] of the pages' type, a token's heads contiguous")
     heads = q.shape[1]
     if slopes is not None and (slopes.dtype is not torch.float32 or slopes.shape != (heads,) or not slopes.is_contiguous()):
@@ -395,16 +413,115 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if window < 0:
         raise ValueError(f"window is the number of tokens that a row sees, or 0: got {window}")
     _same_device(q.device, k_pages=k_pages, v_pages=v_pages, page_table=page_table, lengths=lengths, starts=starts, slopes=slopes,
-                 prefix=prefix, out=out, scratch=scratch)
+                 prefix=prefix, out=out, scratch=scratch, k_scales=k_scales, v_scales=v_scales)
+    scales = () if k_scales is None else (ctypes.byref(_lib.PagedScales(k_scales.data_ptr(), v_scales.data_ptr())),)
     with _on(q.device):
         if scratch is None:
             scratch = _stream_scratch(q.device)
         args = _lib.PagedAttention(q.data_ptr(), q.stride(0) if q.shape[0] > 1 else heads * dim, out.data_ptr(), heads, int(causal), min(int(window), 2 ** 31 - 1),
                                    dim ** -0.5 if scale is None else scale, cap, None if slopes is None else slopes.data_ptr(),
                                    _index("prefix", prefix, (cache.batch,)))
-        _lib.check(_lib.lib().b200_paged_attention(ctypes.byref(cache), ctypes.byref(args), scratch.data_ptr(),
-                                                   scratch.numel() * scratch.element_size(), _stream_ptr(q.device)))
+        _lib.check((_lib.lib().b200_paged8_attention if scales else _lib.lib().b200_paged_attention)(
+            ctypes.byref(cache), *scales, ctypes.byref(args), scratch.data_ptr(), scratch.numel() * scratch.element_size(), _stream_ptr(q.device)))
     return out
+
+
+class PagedPlan(typing.NamedTuple):
+    lengths: torch.Tensor
+    starts: torch.Tensor
+    positions: torch.Tensor
+    slots: torch.Tensor
+    free_count: torch.Tensor
+    status: torch.Tensor
+
+
+def paged_plan_buffers(batch: int, rows: int, device) -> PagedPlan:
+    """Memory for the results of :func:`paged_plan` (``out=``)."""
+    i32 = dict(dtype=torch.int32, device=device)
+    return PagedPlan(torch.empty(batch, **i32), torch.empty(batch + 1, **i32), torch.empty(rows, **i32),
+                     torch.empty(rows, dtype=torch.int64, device=device), torch.empty(1, **i32), torch.empty(1, **i32))
+
+
+def paged_plan(page_table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
+               page_size: int, rows: int, max_tokens: int = 0, out: PagedPlan | None = None) -> PagedPlan:
+    """Pages and rows of a call, on the device: sequence b of ``lengths[b]`` tokens gets ``counts[b]`` new ones, or forgets ``-counts[b]``.
+
+    All int32.  Pages that a sequence no longer needs go onto the list ``free_pages`` (its first ``free_count[0]`` entries are free, the last on
+    top), then those it needs are taken from its top into ``page_table`` [batch, width]; both are changed in place.  The results: ``lengths`` after
+    the call, ``starts`` [batch + 1] of its rows, ``positions`` and ``slots`` (int64: page * page_size + offset) of ``rows`` rows, -1 behind the last
+    one, ``free_count``, and ``status``: 0; or so many pages are lacking; -1: a length is not in 0 .. ``max_tokens`` (0: what a row of the table
+    holds); -2: more than ``rows`` new tokens; -3: the free list is not one.  Where it is not 0 nothing has changed and starts are 0.
+    ``out``: memory for the results; its ``lengths`` and ``free_count`` may be the arguments' own."""
+    native = _native or _torch_call()
+    if native:
+        found = native.paged_plan(page_table, lengths, counts, free_pages, free_count, page_size, rows, max_tokens, out)
+        if found is not None:
+            return out if out is not None else PagedPlan(*found)
+    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError("page_table is an int32 tensor [batch, pages of the longest sequence] with contiguous rows")
+    batch, width = page_table.shape
+    if free_pages.dim() != 1:
+        raise ValueError("free_pages is a list of page numbers")
+    if rows < 0:
+        raise ValueError(f"rows is how many new tokens a call has room for, got {rows}")
+    i32 = [_index(name, t, shape) for name, t, shape in (("lengths", lengths, (batch,)), ("counts", counts, (batch,)),
+                                                         ("free_pages", free_pages, tuple(free_pages.shape)), ("free_count", free_count, (1,)))]
+    _same_device(page_table.device, lengths=lengths, counts=counts, free_pages=free_pages, free_count=free_count)
+    if out is None:
+        out = paged_plan_buffers(batch, rows, page_table.device)
+    results = [_index(f"out.{name}", t, shape) for name, t, shape in (("lengths", out.lengths, (batch,)), ("starts", out.starts, (batch + 1,)),
+                                                                      ("positions", out.positions, (rows,)))]
+    if out.slots.dtype is not torch.int64 or out.slots.shape != (rows,) or not out.slots.is_contiguous():
+        raise ValueError(f"out.slots is a contiguous int64 tensor of {rows}")
+    results += [out.slots.data_ptr(), _index("out.free_count", out.free_count, (1,)), _index("out.status", out.status, (1,))]
+    _same_device(page_table.device, **{f"out.{n}": t for n, t in out._asdict().items()})
+    plan = _lib.PagedPlan(batch, width, page_size, max_tokens, page_table.stride(0) if batch > 1 else width, free_pages.shape[0], rows,
+                          page_table.data_ptr(), *i32, *results)
+    with _on(page_table.device):
+        _lib.check(_lib.lib().b200_paged_plan(ctypes.byref(plan), _stream_ptr(page_table.device)))
+    return out
+
+
+class SampledTokens(typing.NamedTuple):
+    token: torch.Tensor
+    logprob: torch.Tensor
+
+
+def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> SampledTokens:
+    """A token of every row of logits [rows, V] (fp16, bf16 or fp32), drawn with the random numbers ``uniform`` (fp32 [rows], in [0, 1)), and the
+    logarithm of its share among what could have come: (int32 [rows], fp32 [rows]).
+
+    Weights are exp((logit - largest) / temperature).  Of the entries in the order (logit downwards, index upwards) stay the ``top_k`` first
+    (<= 0: all), of those the fewest whose weights reach ``top_p`` of theirs (>= 1: all), and what has ``min_p`` of the largest weight; the token is the
+    first one by index with the weights up to it above ``uniform`` times all.  temperature <= 0: the first of the largest logits.  Each setting is a number or
+    a tensor [rows] (fp32; top_k int32).  A logit of -inf is an excluded entry; a row without others, or with a NaN or +inf, has token -1."""
+    native = _native or _torch_call()
+    if native:
+        found = native.sample_tokens(logits, uniform, temperature, top_k, top_p, min_p)
+        if found is not None:
+            return SampledTokens(*found)
+    if logits.dtype not in _LOGIT_TYPES or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits are an fp16, bf16 or fp32 tensor [rows, V] with contiguous rows")
+    rows, V = logits.shape
+    numbers, pointers, tensors = [], [], {"uniform": uniform}
+    if uniform.dtype is not torch.float32 or uniform.shape != (rows,) or not uniform.is_contiguous():
+        raise ValueError(f"uniform is a contiguous fp32 tensor of {rows}")
+    for name, value, kind in (("temperature", temperature, torch.float32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32),
+                              ("top_k", top_k, torch.int32)):
+        if isinstance(value, torch.Tensor):
+            if value.dtype is not kind or value.shape != (rows,) or not value.is_contiguous():
+                raise ValueError(f"{name} is a number or a contiguous {kind} tensor of {rows}, got {value.dtype} {tuple(value.shape)}")
+            tensors[name] = value
+        numbers.append(0 if isinstance(value, torch.Tensor) else max(min(operator.index(value), 2 ** 31 - 1), 0) if kind is torch.int32 else float(value))
+        pointers.append(value.data_ptr() if isinstance(value, torch.Tensor) else None)
+    _same_device(logits.device, **tensors)
+    token = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    logprob = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    how = _lib.Sampling(*numbers, pointers[0], pointers[3], pointers[1], pointers[2])
+    with _on(logits.device):
+        _lib.check(_lib.lib().b200_sample_tokens(logits.data_ptr(), _LOGIT_TYPES[logits.dtype], logits.stride(0) if rows > 1 else V, uniform.data_ptr(),
+                                                 ctypes.byref(how), token.data_ptr(), logprob.data_ptr(), rows, V, _stream_ptr(logits.device)))
+    return SampledTokens(token, logprob)
 
 
 class TokenLogprobs(typing.NamedTuple):
