@@ -104,6 +104,7 @@ int gemm_error_read_and_clear();
 int gemm_ws_error_read_and_clear();
 int layer_error_read_and_clear();
 int paged_prompt_error_read_and_clear();
+int paged8_prompt_error_read_and_clear();
 
 // Lets `kern` be launched with `bytes` of dynamic shared memory on the current device (`limit`: that kernel's own).
 int raise_smem_limit(SmemLimit& limit, const void* kern, size_t bytes, const char* who);

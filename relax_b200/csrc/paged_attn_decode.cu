@@ -772,9 +772,10 @@ static int paged_attention(const char* who, const B200PagedCache* cache, const B
   p.partial = p.partial_ml + 2 * scratch_rows();
   // Rows of a sequence that share a key head: up to 16 are two operand tiles of the few-rows kernel; more are cut into tiles that
   // each read the keys again, where the kernel for many rows reads them once for 256.
-  if (bytes) return launch_decode<true>(who, cache, p, static_cast<cudaStream_t>(stream));
-  if ((int64_t)cache->max_query * p.group <= 16) return launch_decode<false>(who, cache, p, static_cast<cudaStream_t>(stream));
-  return launch_paged_prompt(who, cache, p, static_cast<cudaStream_t>(stream));
+  const bool few = (int64_t)cache->max_query * p.group <= 16;
+  const cudaStream_t on = static_cast<cudaStream_t>(stream);
+  if (bytes) return few ? launch_decode<true>(who, cache, p, on) : launch_paged8_prompt(who, cache, p, on);
+  return few ? launch_decode<false>(who, cache, p, on) : launch_paged_prompt(who, cache, p, on);
 }
 
 int b200_paged_attention(const B200PagedCache* cache, const B200PagedAttention* a, void* scratch, int64_t scratch_bytes, void* stream) {

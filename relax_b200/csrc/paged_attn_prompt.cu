@@ -29,6 +29,8 @@
 // Measured and not kept, us for 8192 tokens where the present form took 485: all 128 scores of a row in registers 494 (and 70 instead of 50
 // for 2048: the longer code waits for its instructions), 64 at a time 551, 32 at a time 529, two threads a row 535..596, scores in two
 // halves of N = 64 with a buffer each 523 (412 instead of 342 without the softmax).
+// Pages of 8 bits (kBytes; a translation unit of its own, paged_attn_prompt8.cu): TMA brings the codes of a block into a ring of their own, and
+// four more warps (12..15) make fp16 tiles of them, code times the scale of its 16 tokens, in the ring from which the products are made as always.
 #include <atomic>
 #include <type_traits>
 
@@ -41,20 +43,28 @@ namespace {
 
 using namespace ptx;
 
+#ifdef B200_PAGED_BYTES
+constexpr bool kBytes = true;                  // pages of 8 bits
+#else
+constexpr bool kBytes = false;
+#endif
 constexpr int kRows = 128;                     // of a tile
 constexpr int kBlock = 128;                    // tokens of a block of keys
-constexpr int kThreads = 384;
+constexpr int kThreads = kBytes ? 512 : 384;
+constexpr int kTurners = 4;                    // 8 bits: warps that make fp16 tiles of codes
 constexpr int kHalfBytes = kBlock * 128;       // 64 dims of a block
 constexpr int kReady = 4;                      // value blocks between the zeroing warp and the MMA warp
 constexpr int kWorks = 2;                      // work descriptors in flight
 constexpr int kKept = 64;                      // sequences whose sizes the scheduling warp keeps
 constexpr uint64_t kWaitNs = 4000000000ull;
-constexpr int kAuxRegs = 72, kRowRegs = 216, kLaunchRegs = 168;      // 128 x 72 + 256 x 216 = 384 x 168
+constexpr int kRaw = 2;                        // blocks of codes in flight
+// 128 x 72 + 256 x 216 = 384 x 168; 256 x 48 + 256 x 208 = 512 x 128
+constexpr int kAuxRegs = kBytes ? 48 : 72, kRowRegs = kBytes ? 208 : 216, kLaunchRegs = kBytes ? 128 : 168;
 __device__ int g_prompt_error = 0;
 
 struct PromptParams {
   CUtensorMap tm_q;                            // {D, heads, tokens}, box {64, group, tokens of a tile}, SWIZZLE_128B
-  CUtensorMap tm_k, tm_v;                      // {D, page, kv_heads, pages}, box {64, page, 1, 1}, SWIZZLE_128B
+  CUtensorMap tm_k, tm_v;                      // {D, page, kv_heads, pages}, box {64, page, 1, 1}, SWIZZLE_128B; 8 bits: box {D, page, 1, 1}
   PagedAttnParams a;
   int tile_tokens;
   int wide_out;                                // out is 32-byte aligned
@@ -267,10 +277,12 @@ struct Sight {
 
 template <int D>
 struct Smem {
-  static constexpr int kStages = D == 128 ? 5 : 8;
+  static constexpr int kStages = D == 64 ? 8 : kBytes ? 4 : 5;
   static constexpr int kBlockBytes = kHalfBytes * (D / 64);
   unsigned char q[2][kBlockBytes];
   unsigned char ring[kStages][kBlockBytes];
+  unsigned char raw[kBytes ? kRaw : 1][kBytes ? kBlock * D : 16];
+  uint64_t raw_full[kRaw], raw_empty[kRaw], q_ready;
   uint64_t q_full, q_empty;
   uint64_t full[kStages], empty[kStages], ready[kReady];
   uint64_t s_full[2], p_ready[2][2], o_full[2], o_empty[2];       // [tile][half of a block]
@@ -391,13 +403,22 @@ constexpr int kPlain = 0, kCapped = 1, kSloped = 2, kGeneral = 3;     // (and kW
 // Pairs of weights of eight that go that way: 8192 tokens 0 487, 2 479, 3 495, 4 596 us.
 constexpr int kPolyOfEight = 2;
 
+// Pairs of 16-bit values to fp16; a bf16 value beyond fp16's range becomes an infinity.
+__device__ __forceinline__ uint32_t to_half2(__half, uint32_t v) { return v; }
+__device__ __forceinline__ uint32_t to_half2(__nv_bfloat16, uint32_t v) {
+  const float2 f = unpack2(__nv_bfloat16(), v);
+  return pack2(__half(), f.x, f.y);
+}
+
 template <typename T, int D, int kForm, bool kWide>
 __global__ void __launch_bounds__(kThreads, 1)
 paged_prompt_kernel(const __grid_constant__ PromptParams p) {
   using Shared = Smem<D>;
   constexpr int kStages = Shared::kStages, kBlockBytes = Shared::kBlockBytes, kHalves = D / 64;
-  constexpr uint32_t kIdescS = umma_idesc_16bit_f32(kRows, kBlock, std::is_same<T, __nv_bfloat16>::value, false);
-  constexpr uint32_t kIdescO = umma_idesc_16bit_f32(kRows, D, std::is_same<T, __nv_bfloat16>::value, true);
+  using M = typename std::conditional<kBytes, __half, T>::type;          // what is multiplied
+  constexpr bool kTurnQ = !std::is_same<T, M>::value;
+  constexpr uint32_t kIdescS = umma_idesc_16bit_f32(kRows, kBlock, std::is_same<M, __nv_bfloat16>::value, false);
+  constexpr uint32_t kIdescO = umma_idesc_16bit_f32(kRows, D, std::is_same<M, __nv_bfloat16>::value, true);
   extern __shared__ unsigned char smem_unaligned[];
   Shared& sm = *reinterpret_cast<Shared*>(smem_unaligned + ((1024u - (smem_u32(smem_unaligned) & 1023u)) & 1023u));
   volatile int* abort_flag = &sm.abort_flag;
@@ -407,8 +428,10 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
     sm.abort_flag = 0;
     mbar_init(&sm.q_full, 1);
     mbar_init(&sm.q_empty, 1);
-    for (int i = 0; i < kStages; ++i) { mbar_init(&sm.full[i], 1); mbar_init(&sm.empty[i], 1); }
-    for (int i = 0; i < kReady; ++i) mbar_init(&sm.ready[i], 1);
+    for (int i = 0; i < kStages; ++i) { mbar_init(&sm.full[i], kBytes ? kTurners : 1); mbar_init(&sm.empty[i], 1); }
+    for (int i = 0; i < kReady; ++i) mbar_init(&sm.ready[i], kBytes ? kTurners : 1);
+    for (int i = 0; i < kRaw; ++i) { mbar_init(&sm.raw_full[i], 1); mbar_init(&sm.raw_empty[i], kTurners); }
+    mbar_init(&sm.q_ready, kTurners);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sm.s_full[t], 1);
       mbar_init(&sm.p_ready[t][0], 4);
@@ -418,7 +441,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       mbar_init(&sm.joined[t], 4);
     }
     mbar_init(&sm.issued, 1);
-    for (int i = 0; i < kWorks; ++i) { mbar_init(&sm.work_full[i], 1); mbar_init(&sm.work_empty[i], 11); }
+    for (int i = 0; i < kWorks; ++i) { mbar_init(&sm.work_full[i], 1); mbar_init(&sm.work_empty[i], kBytes ? 10 + kTurners : 11); }
     mbar_fence_init();
   }
   if (warp == 1) {
@@ -482,6 +505,16 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
           const int id_next = u + 1 < u1 ? page_at(u + 1) : 0;
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
+            if constexpr (kBytes) {
+              const uint32_t slot = pos % kRaw, round = pos / kRaw;
+              if (round > 0 && !wait_relaxed(&sm.raw_empty[slot], (round - 1) & 1, abort_flag, 3)) { ok = false; break; }
+              if (lane == 0) mbar_arrive_expect_tx(&sm.raw_full[slot], kBlock * D);
+              __syncwarp();
+              if (half == 0)
+                tma_load_4d(sm.raw[slot] + (in_block << a.c.page_log2) * D, kv ? &p.tm_v : &p.tm_k, 0, 0, h, id, &sm.raw_full[slot]);
+              ++pos;
+              continue;
+            }
             const uint32_t slot = pos % kStages, round = pos / kStages;
             if (round > 0 && !wait_relaxed(&sm.empty[slot], (round - 1) & 1, abort_flag, 3)) { ok = false; break; }
             if (lane == 0) mbar_arrive_expect_tx(&sm.full[slot], kBlockBytes);
@@ -513,7 +546,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         const int u0 = wp->u0, u1 = wp->u1, last[2] = {wp->last[0], wp->last[1]};
         const Sight sees[2] = {Sight(*wp, 0), Sight(*wp, 1)};
         if (u1 == u0) continue;
-        if (!wait(&sm.q_full, items & 1, abort_flag, 4)) break;
+        if (!wait(kTurnQ ? &sm.q_ready : &sm.q_full, items & 1, abort_flag, 4)) break;
         ++items;
         bool begun[2] = {false, false};
         uint32_t slot = pos % kStages;
@@ -570,7 +603,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       // ---------------------------------------------------------------------- values that nobody sees: 0 * NaN is NaN
       uint32_t pos = 0, vblocks = 0;
       bool ok = true;
-      for (const Work* wp; ok && (wp = next_work()) != nullptr; work_done()) {
+      for (const Work* wp; !kBytes && ok && (wp = next_work()) != nullptr; work_done()) {
         const Range<kBlock> range = wp->range;
         const int u1 = wp->u1;
         for (int u = wp->u0; u < u1; ++u, pos += 2) {
@@ -620,6 +653,103 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         p.words->next = 0;
         p.words->through = 0;
         p.words->epoch = sm.epoch + 1;
+      }
+    }
+  } else if (kBytes && warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kAuxRegs));
+    // ---------------------------------------------------------------------- 8 bits: tiles of fp16, in the layout in which TMA would put them
+    if constexpr (kBytes) {
+      const int turner = warp - 12;
+      uint32_t pos = 0, vblocks = 0, items = 0;
+      bool ok = true;
+      for (const Work* wp; ok && (wp = next_work()) != nullptr; work_done()) {
+        const Work& w = *wp;
+        const Range<kBlock> range = w.range;
+        const int u1 = w.u1;
+        if (w.u1 == w.u0) continue;
+        if (kTurnQ) {                                          // the queries, where they lie
+          if (!wait(&sm.q_full, items & 1, abort_flag, 16)) break;
+          const int tiles = w.token + p.tile_tokens < w.rows ? 2 : 1;
+          uint4* at = reinterpret_cast<uint4*>(sm.q[0]);
+#pragma unroll 4
+          for (int i = turner * 32 + lane; i < tiles * (kBlockBytes / 16); i += kTurners * 32) {
+            const uint4 v = at[i];
+            at[i] = make_uint4(to_half2(T(), v.x), to_half2(T(), v.y), to_half2(T(), v.z), to_half2(T(), v.w));
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.q_ready);
+        }
+        ++items;
+        const int used = (w.length + (1 << a.c.page_log2) - 1) >> a.c.page_log2;
+        // lane 0..7: the scale of 16 keys, 8..15: of 16 values; a block ahead
+        auto scale_at = [&](int u) {
+          const int token = range.unit(u) * kBlock + 16 * (lane & 7), page = token >> a.c.page_log2;
+          if (lane >= 16 || page >= used) return __float2half(0.f);
+          const int64_t id = page_of(a.c, w.b, page);
+          const int in_page = (token & ((1 << a.c.page_log2) - 1)) >> 4;
+          return __ldg((lane < 8 ? a.k_scales : a.v_scales) + ((id * a.c.kv_heads + w.h) << (a.c.page_log2 - 4)) + in_page);
+        };
+        __half scale = scale_at(w.u0);
+        for (int u = w.u0; ok && u < u1; ++u) {
+          const __half next = u + 1 < u1 ? scale_at(u + 1) : scale;
+          const int from = range.unit(u) * kBlock;
+          const bool whole = from + kBlock <= range.pre || (from >= range.low && from + kBlock <= range.high);
+#pragma unroll 1
+          for (int kv = 0; kv < 2; ++kv, ++pos) {
+            const uint32_t raw = pos % kRaw, slot = pos % kStages, round = pos / kStages;
+            if (!wait(&sm.raw_full[raw], (pos / kRaw) & 1, abort_flag, 10) ||
+                (round > 0 && !wait(&sm.empty[slot], (round - 1) & 1, abort_flag, 17))) {
+              ok = false;
+              break;
+            }
+            // 16 codes a lane and step: a token is D / 16 lanes, 16 tokens D / 32 steps
+            constexpr int kLanes = D / 16;
+            const uint4* codes = reinterpret_cast<const uint4*>(sm.raw[raw]) + lane;
+            const int piece = lane % kLanes;                   // dims 16 piece .. + 15: chunks 2 (piece & 3), + 1 of half piece / 4
+            unsigned char* to = sm.ring[slot] + (piece >> 2) * kHalfBytes;
+            const int flip = piece >> 2 & 1;                   // (which of its two chunks first: the halves' banks are the same)
+#pragma unroll
+            for (int g = turner * (kBlock / 16 / kTurners); g < (turner + 1) * (kBlock / 16 / kTurners); ++g) {
+              const __half2 by = __half2half2(__shfl_sync(0xffffffffu, scale, 8 * kv + g));
+              uint4 c[D / 32];
+#pragma unroll
+              for (int i = 0; i < D / 32; ++i) c[i] = codes[(g * (D / 32) + i) * 32];
+#pragma unroll
+              for (int i = 0; i < D / 32; ++i) {
+                const int token = (g * (D / 32) + i) * (32 / kLanes) + lane / kLanes;
+                const uint32_t words[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+                uint32_t v[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                  const uint32_t two = e4m3_to_half2(k & 1 ? words[k / 2] >> 16 : words[k / 2] & 0xffffu);
+                  const __half2 value = __hmul2(*reinterpret_cast<const __half2*>(&two), by);
+                  v[k] = *reinterpret_cast<const uint32_t*>(&value);
+                }
+                if (kv && !whole) {
+                  const int at = from + token;
+                  if (!(at < range.pre || (at >= range.low && at < range.high)))
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] = 0;
+                }
+                unsigned char* row = to + token * 128;
+                const int chunk = 2 * (piece & 3);
+                const uint4 lo = make_uint4(v[0], v[1], v[2], v[3]), hi = make_uint4(v[4], v[5], v[6], v[7]);
+                *reinterpret_cast<uint4*>(row + (((chunk + flip) ^ (token & 7)) << 4)) = flip ? hi : lo;
+                *reinterpret_cast<uint4*>(row + (((chunk + 1 - flip) ^ (token & 7)) << 4)) = flip ? lo : hi;
+              }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(&sm.raw_empty[raw]);
+              mbar_arrive(&sm.full[slot]);
+              if (kv) mbar_arrive(&sm.ready[vblocks % kReady]);
+            }
+          }
+          ++vblocks;
+          scale = next;
+        }
       }
     }
   } else {
@@ -813,7 +943,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
                   w = exp2_approx(w);
                 }
                 add2(l[2 * (j & 1)], l[2 * (j & 1) + 1], v, w);
-                packed[j] = pack2(T(), v, w);
+                packed[j] = pack2(M(), v, w);
               }
               tmem_st_32x32b_x16(s_at + 16 * (i + h), packed);
             }
@@ -962,7 +1092,11 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
 
 }  // namespace
 
+#ifdef B200_PAGED_BYTES
+int launch_paged8_prompt(const char* who, const B200PagedCache* c, PagedAttnParams a, cudaStream_t stream) {
+#else
 int launch_paged_prompt(const char* who, const B200PagedCache* c, PagedAttnParams a, cudaStream_t stream) {
+#endif
   PromptParams p;
   p.tile_tokens = kRows / a.group;
   const uint32_t page = (uint32_t)c->page_size, group = (uint32_t)a.group;
@@ -977,9 +1111,12 @@ int launch_paged_prompt(const char* who, const B200PagedCache* c, PagedAttnParam
   }
   for (int v = 0; v < 2; ++v) {
     const uint64_t d[4] = {D, page, (uint64_t)c->kv_heads, (uint64_t)c->pages};
-    const uint64_t s[3] = {D * 2, (uint64_t)page * D * 2, (uint64_t)(v ? c->v_page_stride : c->k_page_stride) * 2};
-    const uint32_t b[4] = {64, page, 1, 1};
-    if ((rc = make_tmap(v ? &p.tm_v : &p.tm_k, type, 4, v ? c->v_pages : c->k_pages, d, s, b, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
+    constexpr uint64_t kSize = kBytes ? 1 : 2;
+    const uint64_t s[3] = {D * kSize, (uint64_t)page * D * kSize, (uint64_t)(v ? c->v_page_stride : c->k_page_stride) * kSize};
+    const uint32_t b[4] = {kBytes ? (uint32_t)D : 64u, page, 1, 1};
+    if ((rc = make_tmap(v ? &p.tm_v : &p.tm_k, kBytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type, 4, v ? c->v_pages : c->k_pages, d, s, b,
+                        kBytes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B)))
+      return rc;
   }
   a.slots = sm_count();
   p.wide_out = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0;
@@ -1039,7 +1176,11 @@ int launch_paged_prompt(const char* who, const B200PagedCache* c, PagedAttnParam
   return c->dtype == B200_F16 ? by_dim(__half()) : by_dim(__nv_bfloat16());
 }
 
+#ifdef B200_PAGED_BYTES
+int paged8_prompt_error_read_and_clear() {
+#else
 int paged_prompt_error_read_and_clear() {
+#endif
   int v = 0, zero = 0;
   if (cudaMemcpyFromSymbol(&v, g_prompt_error, sizeof(int)) != cudaSuccess) return 0xff;
   if (v) cudaMemcpyToSymbol(g_prompt_error, &zero, sizeof(int));

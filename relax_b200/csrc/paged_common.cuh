@@ -164,6 +164,7 @@ __device__ __forceinline__ uint32_t e4m3_to_half2(uint32_t codes) {
 
 // The kernel for many rows (paged_attn_prompt.cu).
 int launch_paged_prompt(const char* who, const B200PagedCache* c, PagedAttnParams p, cudaStream_t stream);
+int launch_paged8_prompt(const char* who, const B200PagedCache* c, PagedAttnParams p, cudaStream_t stream);    // over pages of 8 bits
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
