@@ -572,7 +572,8 @@ B200_API int b200_paged_plan(const B200PagedPlan* plan, void* cuda_stream);
  * token = the first entry, by index, for which the weights of what stays up to it are more than uniform[row] times all of what stays
  * (0 <= uniform < 1; from 1 on the last one, below 0 or NaN the first); logprob = the logarithm of its share, fp32 (may be NULL).
  * temperature <= 0 or NaN: the first of the largest logits, logprob 0.  A logit of -inf is an excluded entry: a row of nothing else has token -1 and
- * logprob -inf; one with a NaN or +inf token -1 and logprob NaN.  Weights and sums are fp64, their error below 2^-42.
+ * logprob -inf; one with a NaN or +inf token -1 and logprob NaN.  Weights have 37 bits, sums are fp64; an entry whose weight is below e^-690,
+ * or whose logit is more than 3.4e38 below the largest, counts as excluded.
  * A pointer that is not NULL gives every row its own setting (fp32 [rows], top_ks int32 [rows]) and wins over the number.
  * logits as for b200_token_logprobs; uniform fp32 [rows], token int32 [rows].  One launch, no scratch. */
 typedef struct {

@@ -6,13 +6,14 @@
 // is above the random number times the whole.
 //
 // Which token it is hangs on comparisons of sums: with weights in 32 bits one row in eight of 32000 entries would have a border within the rounding
-// of its sum.  Weights and sums are fp64: w = exp2(t), t = (x - max) log2(e) / T, by Tang's method: t = n / 64 + r, a table of 2^(j / 64)
-// and Taylor's polynomial of degree 4 of e^(r ln 2) (|r| <= 1 / 128, so its rest is 3.9e-14 of the weight).  The GPU has half as many fp64 units as
-// fp32 ones; ten operations an entry are a third of what its special functions would take for as many fp32 weights with a correction.
+// of its sum.  Sums are fp64 and weights 2^-37 exact, by Tang's method: (x - max) log2(e) / T = (n + r) / 64, 2^n/64 from a table of 2^(j / 64),
+// 2^r/64 = 1 + r (c1 + r (c2 + r c3)) with the least largest relative error on |r| <= 0.51 (found by linear programming: 6.7e-12; 1 stays
+// exact, so that sums of equal largest logits are whole numbers).  Nine fp64 operations an entry and one a sum: the GPU has half as many fp64
+// units as fp32 ones, and a pass that took n and the exponents through whole numbers waited for the issue of 49 instructions an entry.
 //
 // Passes over the row (a CTA of 512 threads, few rows over a cluster; all passes but the first out of L2):
 //   1  the maximum
-//   2  with top_k or top_p: how many entries lie in each of 4096 bins of width T / 128 below the maximum
+//   2  with top_k or top_p: how many entries lie in each of 2048 bins of T / 92 below the maximum (n, but from fp32)
 //   3  top_k: the bin with the border is known; its entries are put in order.  top_p: the counts times the bins' weights tell the bin but
 //      for an error in the fourth digit; the exact sum above that bin and its neighbours, and their entries in order, find the border or say
 //      on which side it lies.  Where a bin holds more entries than the list (nearly equal logits) the border is found by bisection of the keys.
@@ -29,14 +30,18 @@ namespace b200 {
 
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kFew = 512, kMany = 256;          // threads of a CTA where there are few rows, or many
 constexpr int kMaxCluster = 8;
-constexpr int kBins = 4096;
-constexpr float kBinsPerNat = 128.f;
-constexpr int kList = 1536;                     // entries of the bins around a border
-constexpr int kTable = 64;                      // 2^(j / 64)
-constexpr double kLn2 = 0.6931471805599453094, kLog2e = 1.4426950408889634074;
+constexpr int kBins = 2048;                     // 22 nats; counted again where that is not enough:
+constexpr int kWide = 32;                       // bins so many times as wide, 710 nats
+constexpr int kAhead = 2;                       // vectors under way while one is worked on
+constexpr int kList = 1024;                     // entries of the bins around a border
+constexpr int kTableLog2 = 6, kTable = 1 << kTableLog2;                  // 2^(j / 64)
+constexpr int kCopies = 8;                      // of the table: fewer lanes ask the same bank for different entries
+constexpr double kLog2e = 1.4426950408889634074;
+constexpr double kDepth = 690.;                 // weights from e^-690 on are normal numbers
 
+using ptx::exp2_approx;
 typedef unsigned long long u64;
 
 struct SampleParams {
@@ -69,8 +74,9 @@ __device__ __forceinline__ uint32_t key_of(float v) {
 }
 __device__ __forceinline__ u64 entry_of(float v, int index) { return (u64)key_of(v) << 32 | (uint32_t)~index; }
 
-// A row as vectors of 16 bytes on their own grid: its first element is element `lead` of vector 0.  What lies outside the row is -inf,
-// an excluded entry.
+// A row as vectors of 16 bytes on their own grid: its first element is element `lead` of vector 0.  The first and the last vector may reach
+// beyond the row (not beyond the 16 bytes that hold its ends, so not beyond the memory that it lies in); what they hold there becomes -inf, an
+// excluded entry.
 template <typename T>
 struct Row {
   static constexpr int N = Vec<T>::N;
@@ -85,52 +91,138 @@ struct Row {
     count = (int)(((int64_t)lead + size + N - 1) / N);
   }
   __device__ __forceinline__ int first(int j) const { return j * N - lead; }          // index of a vector's first element
-  __device__ __forceinline__ void load(int j, float (&f)[N]) const {
+  __device__ __forceinline__ uint4 load(int j) const {
+    uint4 v = __ldg(vectors + j);
     const int at = first(j);
-    if (at >= 0 && at + N <= V) {
-      const uint4 v = __ldg(vectors + j);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    if (at < 0 || at > V - N) {
+      constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00u : 0xff80u;
+      uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(T) == 4) {
-          f[i] = __uint_as_float(w[i]);
-        } else if constexpr (std::is_same<T, __half>::value) {
-          const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-          f[2 * i] = u.x;
-          f[2 * i + 1] = u.y;
-        } else {
-          f[2 * i] = __uint_as_float(w[i] << 16);
-          f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
+      for (int i = 0; i < N; ++i) {
+        if (at + i >= 0 && at + i < V) continue;
+        if (sizeof(T) == 4) w[i & 3] = kNone;
+        else w[i / 2] = i & 1 ? (w[i / 2] & 0xffffu) | kNone << 16 : (w[i / 2] & 0xffff0000u) | kNone;
       }
-    } else {
+      v = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    return v;
+  }
+  __device__ __forceinline__ static void unpack(const uint4& v, float (&f)[N]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = at + i >= 0 && at + i < V ? to_float(x[at + i]) : -INFINITY;
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        f[i] = __uint_as_float(w[i]);
+      } else if constexpr (std::is_same<T, __half>::value) {
+        const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        f[2 * i] = u.x;
+        f[2 * i + 1] = u.y;
+      } else {
+        f[2 * i] = __uint_as_float(w[i] << 16);
+        f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
     }
   }
+  // the largest (the least) value of a vector, NaN where there is one
+  template <bool kLeast>
+  __device__ __forceinline__ static float extreme(const uint4& v) {
+    if constexpr (sizeof(T) == 4) {
+      float a = __uint_as_float(v.x);
+      for (const uint32_t u : {v.y, v.z, v.w}) {
+        if (kLeast) asm("min.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(__uint_as_float(u)));
+        else asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(__uint_as_float(u)));
+      }
+      return a;
+    } else {
+      using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+      const T2* w = reinterpret_cast<const T2*>(&v);
+      const T2 a = kLeast ? __hmin2_nan(__hmin2_nan(w[0], w[1]), __hmin2_nan(w[2], w[3])) : __hmax2_nan(__hmax2_nan(w[0], w[1]), __hmax2_nan(w[2], w[3]));
+      return to_float(kLeast ? __hmin_nan(T(a.x), T(a.y)) : __hmax_nan(T(a.x), T(a.y)));
+    }
+  }
+  // The type's least number that is not below an fp32 one; the elements of a vector (bits) that reach `from` and do not reach `to`.
+  __device__ __forceinline__ static T up(float v) {
+    if constexpr (sizeof(T) == 4) return v;
+    else if constexpr (std::is_same<T, __half>::value) return __float2half_ru(v);
+    else return __float2bfloat16_ru(v);
+  }
+  __device__ __forceinline__ static unsigned between(const uint4& v, T from, T to) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t in[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        in[i] = __uint_as_float(w[i]) >= from && __uint_as_float(w[i]) < to ? 1u << i : 0u;
+      } else {
+        using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        const T2 x = *reinterpret_cast<const T2*>(&w[i]);
+        in[i] = __hge2_mask(x, T2(from, from)) & __hlt2_mask(x, T2(to, to));
+      }
+    }
+    if ((in[0] | in[1] | in[2] | in[3]) == 0) return 0;
+    unsigned bits = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bits |= sizeof(T) == 4 ? in[i] : (in[i] & 1u) << (2 * i) | (in[i] >> 31) << (2 * i + 1);
+    return bits;
+  }
+  __device__ __forceinline__ static float highest(const uint4& v) { return extreme<false>(v); }
+  __device__ __forceinline__ static float lowest(const uint4& v) { return extreme<true>(v); }
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
+// An entry's value.
+__device__ __forceinline__ float value_of(u64 e) {
+  const uint32_t k = (uint32_t)(e >> 32);
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+// The last entry that stays, as a pass compares with it: values from `value` on up to the index, from `next` on behind it.
+struct Border {
+  float value, next;
+  int index;
+  __device__ __forceinline__ explicit Border(u64 e) : value(value_of(e)), next(value_of(e + (1ull << 32))), index((int)min(~(uint32_t)e, 0x7fffffffu)) {}
+};
+// sum += w where v >= from
+__device__ __forceinline__ void add_from(double& sum, double w, float v, float from) {
+  asm("{\n.reg .pred p;\nsetp.ge.f32 p, %1, %2;\n@p add.f64 %0, %0, %3;\n}" : "+d"(sum) : "f"(v), "f"(from), "d"(w));
+}
+
+__device__ __forceinline__ int mul(int a, int b) {
+  int r;
+  asm("mul.lo.s32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// What the CTAs of a row tell each other.
+struct Note {
+  double a, b;
+  int n, m;
+};
+
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads)
 sample_tokens_kernel(const SampleParams p) {
+  constexpr int kWarps = kThreads / 32, kBuckets = 2 * kThreads, kEach = kList / kThreads;
+  static_assert(2 * kBuckets <= kBins, "buckets");
   constexpr int N = Vec<T>::N;
-  __shared__ double sm_table[kTable];
-  __shared__ int sm_bins[kBins];
-  __shared__ __align__(16) u64 sm_list[kList];
-  __shared__ __align__(16) u64 sm_own[kList];   // this CTA's part of the list; then the list's weights in order
-  double* sm_order = reinterpret_cast<double*>(sm_own);
-  __shared__ double sm_warp[kWarps], sm_sum;    // of warps, of the CTA
-  __shared__ int sm_warp_n[kWarps], sm_count;
-  __shared__ float sm_max;
-  __shared__ int sm_index;
-  __shared__ u64 sm_found;
+  __shared__ double sm_table[kTable * kCopies];
+  __shared__ __align__(16) int sm_bins[kBins];
+  __shared__ __align__(16) u64 sm_own[2][kList], sm_list[kList];          // this CTA's part of the list; all of it
+  __shared__ __align__(16) u64 sm_sorted[kList];
+  int* sm_bucket = sm_bins;                     // [2][kBuckets], when the bins are no longer wanted
+  __shared__ Note sm_notes[2][kMaxCluster];
+  __shared__ double sm_warp[kWarps], sm_segment[kWarps];
+  __shared__ float2 sm_extreme[kWarps];
+  __shared__ int sm_warp_n[kWarps], sm_count, sm_index, sm_border[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int ranks = gridDim.x, rank = blockIdx.x;
   const int64_t row = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
-  if (tid < kTable) sm_table[tid] = exp2((double)tid / kTable);
+  for (int i = tid; i < kTable * kCopies; i += kThreads) {
+    const double w = exp2((double)(i / kCopies) / kTable);
+    sm_table[i] = __hiloint2double(__double2hiint(w) - ((i / kCopies) << (20 - kTableLog2)), __double2loint(w));
+  }
   ptx::pdl_wait();
   ptx::pdl_launch_dependents();
   if (row >= p.rows) return;                    // (whole clusters)
+  if (ranks > 1) ptx::cluster_arrive_relaxed(); // (every CTA of the cluster runs before anything is stored in it)
   auto meet = [&]() {                           // all threads of the row
     if (ranks > 1) {
       ptx::cluster_arrive();
@@ -145,72 +237,83 @@ sample_tokens_kernel(const SampleParams p) {
     asm("mapa.u64 %0, %1, %2;" : "=l"(a) : "l"(at), "r"(r));
     return reinterpret_cast<decltype(at)>(a);
   };
-  // sums over all threads of the row, in an order of their own: the same bits everywhere
-  auto row_sum = [&](double v) {
+  // Everybody's notes, in the order of the CTAs.  One meeting: the next notes go to the other place, and those after them are written behind
+  // the next meeting, when these have been read.
+  int turn = 0;
+  auto exchange = [&](Note mine) {
+    if (tid < ranks) *remote(&sm_notes[turn][rank], tid) = mine;
+    meet();
+    const Note* all = sm_notes[turn];
+    turn ^= 1;
+    return all;
+  };
+  // the sum of all threads of the CTA
+  auto block_sum = [&](double v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
     if (lane == 0) sm_warp[warp] = v;
     __syncthreads();
     double s = 0.;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) s += sm_warp[w];
-    if (ranks > 1) {
-      if (tid == 0) sm_sum = s;
-      meet();
-      s = 0.;
-      for (int r = 0; r < ranks; ++r) s += *remote(&sm_sum, r);
-      meet();
-    } else {
-      __syncthreads();
-    }
+    return s;
+  };
+  auto row_sum = [&](double v) {
+    const Note* notes = exchange({block_sum(v), 0., 0, 0});
+    double s = 0.;
+    for (int r = 0; r < ranks; ++r) s += notes[r].a;
     return s;
   };
 
+  // Every CTA has a slice of the row's vectors, every warp a segment of it.
   const Row<T> x(static_cast<const T*>(p.logits) + row * p.stride, p.V);
   const int per = (x.count + ranks - 1) / ranks, begin = min(rank * per, x.count), end = min(begin + per, x.count);
+  const int share = (per + kWarps - 1) / kWarps;
+  const int from = min(begin + warp * share, end), to = min(from + share, end);
 
   // ---- 1: the maximum, NaN where there is one --------------------------------------------------------------------------------------
-  float m = -INFINITY;
-#pragma unroll 4
-  for (int j = begin + tid; j < end; j += kThreads) {
-    float f[N];
-    x.load(j, f);
-#pragma unroll
-    for (int i = 0; i < N; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(f[i]));
-  }
   auto join = [](float a, float b) {
     asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(b));
     return a;
   };
+  float m = -INFINITY;
+  for (int j = from + lane; j < to; j += 128) {
+    uint4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = x.load(min(j + 32 * i, to - 1));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = join(m, x.highest(v[i]));
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = join(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (lane == 0) sm_warp[warp] = m;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) m = join(m, (float)sm_warp[w]);
-  if (ranks > 1) {
-    if (tid == 0) sm_max = m;
-    meet();
-    for (int r = 0; r < ranks; ++r) m = join(m, *remote(&sm_max, r));
+  {
+    if (ranks > 1) ptx::cluster_wait();         // (the one at the start)
+    const Note* notes = exchange({(double)m, 0., 0, 0});
+    for (int r = 0; r < ranks; ++r) m = join(m, (float)notes[r].a);
   }
-  __syncthreads();
   const bool writes = rank == 0 && tid == 0;
-  float temperature = p.temperatures ? p.temperatures[row] : p.temperature;
+  const float temperature = p.temperatures ? p.temperatures[row] : p.temperature;
+  const int want_k = p.top_ks ? p.top_ks[row] : p.top_k;
+  const float want_p = p.top_ps ? p.top_ps[row] : p.top_p, want_min = p.min_ps ? p.min_ps[row] : p.min_p;
   if (!(m < INFINITY) || m == -INFINITY) {      // a NaN, an infinity, nothing that is allowed
     if (writes) {
       p.token[row] = -1;
       if (p.logprob) p.logprob[row] = m == -INFINITY ? -INFINITY : NAN;
     }
-    meet();                                     // (nobody reads sm_max of a CTA that is gone)
     return;
   }
-  const int want_k = p.top_ks ? p.top_ks[row] : p.top_k;
-  const float want_p = p.top_ps ? p.top_ps[row] : p.top_p, want_min = p.min_ps ? p.min_ps[row] : p.min_p;
   if (!(temperature > 0.f) || want_p <= 0.f || want_k == 1) {             // the first of the largest
     int at = 0x7fffffff;
-    for (int j = begin + tid; j < end; j += kThreads) {
+    for (int j = from + lane; j < to; j += 32) {
+      const uint4 v = x.load(j);
+      if (x.highest(v) != m) continue;
       float f[N];
-      x.load(j, f);
+      x.unpack(v, f);
 #pragma unroll
       for (int i = N - 1; i >= 0; --i)
         if (f[i] == m) at = min(at, x.first(j) + i);
@@ -220,65 +323,55 @@ sample_tokens_kernel(const SampleParams p) {
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) at = min(at, sm_warp_n[w]);
-    if (tid == 0) sm_index = at;
-    meet();
+    const Note* notes = exchange({0., 0., at, 0});
     if (writes) {
-      for (int r = 1; r < ranks; ++r) at = min(at, *remote(&sm_index, r));
+      for (int r = 1; r < ranks; ++r) at = min(at, notes[r].n);
       p.token[row] = at;
       if (p.logprob) p.logprob[row] = 0.f;
     }
-    meet();
     return;
   }
 
-  const double top = m, per_t = 1. / (double)temperature, scale = kLog2e * per_t;
-  // 2^((x - max) scale); 0 below 2^-1000
+  // (a temperature so low that the next fp32 number below the maximum is out of sight counts as one that just hides it: `offset` keeps its bits)
+  const double top = m, t_eff = fmax((double)temperature, fabs(top) * 1e-11), scale = kLog2e * kTable / t_eff, offset = -top * scale;
+  const char* table = reinterpret_cast<const char*>(sm_table + (lane & (kCopies - 1)));
+  // The bin of a value, which only grows as the value falls, as a number above 1.5 * 2^23; its low bits count.
+  constexpr float kBase = 12582912.f;
+  float bins_per = fminf((float)scale, 1e30f);
+  int unit = 1;                                 // n of a bin
+  auto bin_of = [&](float v) { return fmaf(m - v, bins_per, kBase); };
+  // 2^((x - max) log2(e) / T) = 2^n/64 2^r/64, for values from `low` on.  (A rounding of `offset` is a factor that all weights share.)
   auto weight = [&](float v) {
-    const double t = ((double)v - top) * (scale * kTable);
+    constexpr double c1 = 0.0108304246963882758, c2 = 0.000058649173078506538, c3 = 2.1173088255274404e-7;
     constexpr double kMagic = 6755399441055744.;         // 1.5 * 2^52: its sum with a number has the nearest whole one in its low bits
-    const double shifted = t + kMagic;
+    const double t = fma((double)v, scale, offset), shifted = t + kMagic, r = t - (shifted - kMagic);
     const int n = __double2loint(shifted);
-    const double r = (t - (shifted - kMagic)) * (kLn2 / kTable);
-    double w = fma(r, 1. / 24., 1. / 6.);
-    w = fma(w, r, 0.5);
-    w = fma(w, r, 1.);
-    w = fma(w, r, 1.) * sm_table[n & (kTable - 1)];
-    w = __hiloint2double(__double2hiint(w) + (n >> 6) * (1 << 20), __double2loint(w));
-    return t >= -1000. * kTable ? w : 0.;
+    // (multiplications take the other pipe; the table's entries come without their own part of the exponent that n << 14 adds)
+    const double of = *reinterpret_cast<const double*>(table + mul(n & (kTable - 1), kCopies * 8));
+    return fma(fma(fma(r, c3, c2), r, c1), r, 1.) * __hiloint2double(mul(n, 1 << (20 - kTableLog2)) + __double2hiint(of), __double2loint(of));
   };
+  // (less weight is as good as excluded, and so is what lies further below the maximum than fp32 can say)
+  const float low = fmaxf(__double2float_ru(top - kDepth * t_eff), fmaxf(m - 3.402823466e38f, -3.402823466e38f));
   const bool has_k = want_k > 0 && want_k < p.V, has_p = want_p < 1.f;
-  u64 border = 0;                               // the smallest entry that stays
+  u64 border = (u64)key_of(low) << 32;          // the smallest entry that stays
+  const u64 all_of_weight = border;
   if (want_min > 0.f) {                         // w >= min_p: a value, rounded up to the next fp32 number
-    const double low = want_min < 1.f ? top + (double)temperature * log((double)want_min) : top;
-    border = (u64)key_of(__double2float_ru(low)) << 32;
+    const double least = want_min < 1.f ? top + t_eff * log((double)want_min) : top;
+    border = max(border, (u64)key_of(__double2float_ru(least)) << 32);
   }
-
-  if (has_k || has_p) {
-    // ---- 2: how many entries lie how far below the maximum -----------------------------------------------------------------------
-    const float bins_per = fminf(kBinsPerNat / temperature, 1e30f);
-    // (grows as a value falls, and so does every rounding of it)
-    auto bin_of = [&](float v) { return min((int)fminf((m - v) * bins_per, (float)kBins), kBins - 1); };
-    for (int i = tid; i < kBins; i += kThreads) sm_bins[i] = 0;
+  int listed = 0, own_turn = 0;
+  double sum_all, sum_above;
+  // The first n entries of the list, those with the largest key(entry) first: by buckets that fall with the key, and within a bucket an entry's
+  // place is the number of larger ones.
+  auto order = [&](int n, auto key, auto bucket) {
+    int* start = sm_bucket;
+    int* end = sm_bucket + kBuckets;
+    for (int i = tid; i < kBuckets; i += kThreads) end[i] = 0;
     __syncthreads();
-#pragma unroll 2
-    for (int j = begin + tid; j < end; j += kThreads) {
-      float f[N];
-      x.load(j, f);
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (f[i] > -INFINITY) atomicAdd(&sm_bins[bin_of(f[i])], 1);
-    }
-    meet();
-    // a thread has kBins / kThreads neighbouring bins of the whole row
-    constexpr int kMine = kBins / kThreads;
-    int mine[kMine], sum = 0;
-#pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      mine[i] = 0;
-      for (int r = 0; r < ranks; ++r) mine[i] += *remote(&sm_bins[tid * kMine + i], r);
-      sum += mine[i];
-    }
-    int upto = sum;
+    for (int i = tid; i < n; i += kThreads) atomicAdd(&end[bucket(sm_list[i])], 1);
+    __syncthreads();
+    const int2 mine = reinterpret_cast<const int2*>(end)[tid];
+    int upto = mine.x + mine.y;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, upto, o);
@@ -286,307 +379,575 @@ sample_tokens_kernel(const SampleParams p) {
     }
     if (lane == 31) sm_warp_n[warp] = upto;
     __syncthreads();
-    int before = upto - sum, all = 0;
+    int before = upto - mine.x - mine.y;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < kWarps; ++w)
       if (w < warp) before += sm_warp_n[w];
-      all += sm_warp_n[w];
+    reinterpret_cast<int2*>(start)[tid] = make_int2(before, before + mine.x);
+    reinterpret_cast<int2*>(end)[tid] = make_int2(before, before + mine.x);
+    __syncthreads();
+    for (int i = tid; i < n; i += kThreads) {
+      const u64 e = sm_list[i];
+      sm_sorted[atomicAdd(&end[bucket(e)], 1)] = e;
     }
     __syncthreads();
-
-    // The entries of bins [from, to] that are not below `least`, of the whole row, in sm_list; false: more than it holds.
-    int listed = 0;
-    auto collect = [&](int from, int to, u64 least, int expected) {
-      if (expected > kList) return false;
-      if (tid == 0) sm_count = 0;
-      __syncthreads();
-      u64* own = ranks > 1 ? sm_own : sm_list;
-      for (int j = begin + tid; j < end; j += kThreads) {
-        float f[N];
-        x.load(j, f);
+    for (int i = tid; i < n; i += kThreads) {
+      const u64 e = sm_sorted[i], k = key(e);
+      const int b = bucket(e), from = start[b], to = end[b];
+      int place = from;
+      for (int q = from; q < to; ++q) place += key(sm_sorted[q]) > k;
+      sm_list[place] = e;
+    }
+    __syncthreads();
+  };
+  auto order_by_value = [&](int n) {
+    // buckets between the list's largest and its least value
+    float hi = -INFINITY, lo = INFINITY;
+    for (int i = tid; i < n; i += kThreads) {
+      const float v = value_of(sm_list[i]);
+      hi = fmaxf(hi, v);
+      lo = fminf(lo, v);
+    }
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int bin = f[i] > -INFINITY ? bin_of(f[i]) : kBins;
-          if (bin >= from && bin <= to) {
-            const u64 e = entry_of(f[i], x.first(j) + i);
-            if (e >= least) own[atomicAdd(&sm_count, 1)] = e;
+    for (int o = 16; o > 0; o >>= 1) {
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    }
+    if (lane == 0) sm_extreme[warp] = make_float2(hi, lo);
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      hi = fmaxf(hi, sm_extreme[w].x);
+      lo = fminf(lo, sm_extreme[w].y);
+    }
+    const float per = hi > lo ? fminf((kBuckets - 1) / (hi - lo), 1e30f) : 0.f;
+    order(n, [](u64 e) { return e; }, [&](u64 e) { return (int)fminf((hi - value_of(e)) * per, kBuckets - 1.f); });
+  };
+  // The parts of the list that the CTAs have (sm_own, their lengths the notes' n) in order.
+  auto put_in_order = [&](const Note* notes) {
+    listed = 0;
+    for (int r = 0; r < ranks; ++r) {
+      const int n = min(notes[r].n, kList + 1);
+      if (listed + n <= kList) {
+        const u64* other = remote(sm_own[own_turn], r);
+        for (int i = tid; i < n; i += kThreads) sm_list[listed + i] = other[i];
+      }
+      listed = min(listed + n, kList + 1);
+    }
+    own_turn ^= 1;                              // (others may still read this one)
+    __syncthreads();
+    if (listed > kList) return false;
+    order_by_value(listed);
+    return true;
+  };
+  // The values from which a bin is reached, in the row's type: all values from edge(b) on, and no others, lie in bins in front of b.  (But for
+  // fp32's last bits, in which the counts may see it differently.)
+  auto edge = [&](int b) { return b <= 0 ? T(INFINITY) : x.up(b >= kBins ? low : fmaxf(m - ((float)b - 0.5f) / bins_per, low)); };
+  // The entries of a vector whose bits are set, to this CTA's part of the list.
+  auto push = [&](unsigned hits, int first, auto also) {
+    while (hits) {
+      const int at = first + __ffs(hits) - 1;
+      hits &= hits - 1;
+      const float v = to_float(x.x[at]);
+      if (!also(v, at)) continue;
+      const int n = atomicAdd(&sm_count, 1);
+      if (n < kList) sm_own[own_turn][n] = entry_of(v, at);
+    }
+  };
+  // Without sums: the entries of bins [first, last], those of the counts.
+  auto gather = [&](int first, int last) {
+    const float from_bin = kBase + (float)first, to_bin = last == kBins - 1 ? INFINITY : kBase + (float)last;
+    const T reach = edge(last + 2), none = T(INFINITY);         // (a bin to spare)
+    if (tid == 0) sm_count = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int j = from + lane; j < to; j += 128) {
+      uint4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = x.load(min(j + 32 * i, to - 1));
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (j + 32 * i < to)
+          push(x.between(v[i], reach, none), x.first(j + 32 * i), [&](float v, int) {
+            const float bin = bin_of(v);
+            return bin >= from_bin && bin <= to_bin && v >= low;
+          });
+    }
+    __syncthreads();
+    return put_in_order(exchange({0., 0., sm_count, 0}));
+  };
+  // Sums up to every thread's two entries, in order; the sum of all.
+  auto scan = [&](const double (&w)[kList / kThreads], double& before) {
+    double own = 0., all = 0.;
+#pragma unroll
+    for (int i = 0; i < kList / kThreads; ++i) own += w[i];
+    double upto = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    __syncthreads();
+    if (lane == 31) sm_warp[warp] = upto;
+    if (tid == 0) sm_index = 0x7fffffff;
+    __syncthreads();
+    before = upto - own;
+#pragma unroll
+    for (int q = 0; q < kWarps; ++q) {
+      if (q < warp) before += sm_warp[q];
+      all += sm_warp[q];
+    }
+    return all;
+  };
+  // What a pass finds: sums over the row of all that the border `lowest` keeps and of that in the bins in front of `first`; the second
+  // of each warp's segment in sm_segment; the entries of bins [first, last] that it keeps, of the whole row and in order, in sm_own, if they fit
+  // the list.
+  auto pass = [&](int first, int last, u64 lowest) {
+    const Border kept(lowest);
+    const T above = edge(first), near = edge(last + 1);          // values from `above` on lie in front of the list, from `near` on in it
+    const float above_f = to_float(above);
+    if (tid == 0) sm_count = 0;
+    __syncthreads();
+    double s = 0., a = 0.;
+    uint4 ahead[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (from + lane + 32 * i < to) ahead[i] = x.load(from + lane + 32 * i);
+#pragma unroll 1
+    for (int j = from + lane; j < to; j += 32) {
+      const uint4 v = ahead[0];
+#pragma unroll
+      for (int i = 0; i + 1 < kAhead; ++i) ahead[i] = ahead[i + 1];
+      if (j + 32 * kAhead < to) ahead[kAhead - 1] = x.load(j + 32 * kAhead);
+      if (x.highest(v) < kept.value) continue;
+      float f[N];
+      x.unpack(v, f);
+      const int at = x.first(j);
+      if (at <= kept.index && at + N - 1 > kept.index) {           // the border's own index is among these
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (at + i > kept.index && f[i] == kept.value) f[i] = -INFINITY;
+      }
+      const float least = at > kept.index ? kept.next : kept.value;
+      // (no branch an entry: the chains of fp64 operations of several run side by side)
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        asm("{\n.reg .pred p, q;\nsetp.ge.f32 p, %2, %3;\n@p add.f64 %0, %0, %5;\nsetp.ge.and.f32 q, %2, %4, p;\n@q add.f64 %1, %1, %5;\n}"
+            : "+d"(s), "+d"(a) : "f"(f[i]), "f"(least), "f"(above_f), "d"(weight(f[i])));
+      push(x.between(v, near, above), at, [&](float v, int i) { return v >= (i > kept.index ? kept.next : kept.value); });
+    }
+    // the segments' sums, the CTA's and the row's
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      a += __shfl_xor_sync(0xffffffffu, a, o);
+    }
+    if (lane == 0) {
+      sm_warp[warp] = s;
+      sm_segment[warp] = a;
+    }
+    __syncthreads();
+    Note mine = {0., 0., sm_count, 0};
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      mine.a += sm_warp[w];
+      mine.b += sm_segment[w];
+    }
+    const Note* notes = exchange(mine);
+    sum_all = sum_above = 0.;
+    for (int r = 0; r < ranks; ++r) {
+      sum_all += notes[r].a;
+      sum_above += notes[r].b;
+    }
+    return put_in_order(notes);
+  };
+  // The largest entry e for which what(entries >= e), a sum over the row, reaches `goal`: by bisection, for rows that fit no list.
+  auto bisect = [&](u64 lowest, double goal, auto what) {
+    u64 lo = lowest, hi = ~0ull;                // what(>= lo) reaches it, what(>= hi) does not
+    while (hi - lo > 1) {
+      const u64 mid = lo + (hi - lo) / 2;
+      double s = 0.;
+      for (int j = from + lane; j < to; j += 32) {
+        float f[N];
+        x.unpack(x.load(j), f);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (f[i] >= low && entry_of(f[i], x.first(j) + i) >= mid) s += what(f[i]);
+      }
+      if (row_sum(s) >= goal) lo = mid; else hi = mid;
+    }
+    return lo;
+  };
+
+  bool segments = false;                        // sm_segment has the sums above the list, and the list what lies around the border
+  if (has_k || has_p) {
+    // ---- 2: how many entries lie how far below the maximum, and the bin in which the border lies ----------------------------------------
+    constexpr int kMost = kBins / kThreads;
+    int mine = max(kMost / ranks, 1);           // of the whole row every CTA has a part of the bins, every thread a few neighbours
+    const int bin0 = rank * (kBins / ranks) + tid * mine;
+    if (tid * mine >= kBins / ranks) mine = 0;
+    int n_of[kMost], sum;
+    float mass_of[kMost], mass = 0.f;           // the bins' weights, an estimate in fp32 by their middles
+    auto masses = [&](int n, int most) {
+      mass = 0.f;
+#pragma unroll
+      for (int i = 0; i < kMost; ++i) {
+        mass_of[i] = i < mine ? (float)min(n_of[i], max(most - n, 0)) * exp2_approx((float)((bin0 + i) * unit) * (-1.f / kTable)) : 0.f;
+        mass += mass_of[i];
+        n += n_of[i];
+      }
+    };
+    int before = 0, all = 0;                    // entries in front of this thread's bins, of the row
+    float mass_before = 0.f, mass_end = 0.f, mass_all = 0.f;         // (a thread's end is the next one's beginning to the bit)
+    auto totals = [&]() {
+      int upto = sum;
+      float mass_upto = mass;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        const float f = __shfl_up_sync(0xffffffffu, mass_upto, o);
+        if (lane >= o) { upto += v; mass_upto += f; }
+      }
+      __syncthreads();
+      if (lane == 31) { sm_warp_n[warp] = upto; sm_warp[warp] = mass_upto; }
+      if (tid == 0) sm_border[0] = -1;
+      __syncthreads();
+      before = upto - sum;
+      mass_end = mass_upto;
+      mass_before = __shfl_up_sync(0xffffffffu, mass_upto, 1);
+      if (lane == 0) mass_before = 0.f;
+      float mass_base = 0.f;
+      int slice = 0;
+      float mass_slice = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float f = (float)sm_warp[w];
+        if (w < warp) { before += sm_warp_n[w]; mass_base += f; }
+        slice += sm_warp_n[w];
+        mass_slice += f;
+      }
+      const Note* notes = exchange({(double)mass_slice, 0., slice, 0});    // (and everybody has read the bins)
+      mass_before += mass_base;
+      mass_end += mass_base;
+      all = 0;
+      mass_all = 0.f;
+      for (int r = 0; r < ranks; ++r) {
+        if (r == rank) { mass_before += mass_all; mass_end += mass_all; }
+        if (r < rank) before += notes[r].n;
+        all += notes[r].n;
+        mass_all += (float)notes[r].a;
+      }
+    };
+    auto count = [&]() {
+      for (int i = tid; i < kBins / 4; i += kThreads) reinterpret_cast<int4*>(sm_bins)[i] = make_int4(0, 0, 0, 0);
+      __syncthreads();
+      auto place_of = [&](float v) { return (int)(min(__float_as_uint(bin_of(v)), 0x4b400000u + kBins - 1) - 0x4b400000u); };
+#pragma unroll 1
+      for (int j = from + lane; j < to; j += 128) {
+        uint4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = x.load(min(j + 32 * i, to - 1));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (j + 32 * i >= to) break;
+          float f[N];
+          x.unpack(v[i], f);
+          if (x.lowest(v[i]) >= low) {
+#pragma unroll
+            for (int q = 0; q < N; ++q) atomicAdd(&sm_bins[place_of(f[q])], 1);
+          } else {
+#pragma unroll
+            for (int q = 0; q < N; ++q)
+              if (f[q] >= low) atomicAdd(&sm_bins[place_of(f[q])], 1);
           }
         }
       }
       meet();
-      if (ranks > 1) {
-        listed = 0;
-        for (int r = 0; r < ranks; ++r) {
-          const int n = *remote(&sm_count, r);
-          const u64* other = remote(sm_own, r);
-          for (int i = tid; i < n; i += kThreads) sm_list[listed + i] = other[i];
-          listed += n;
-        }
-        meet();
-      } else {
-        listed = sm_count;
-        __syncthreads();
-      }
-      return true;
-    };
-    // Place of an entry of the list in its order.
-    auto place_of = [&](u64 e) {
-      int n = 0;
-      for (int i = 0; i < listed; ++i) n += sm_list[i] > e;
-      return n;
-    };
-    // The largest entry e for which what(entries >= e), a sum over the row, reaches `goal`: by bisection, for rows that fit no list.
-    auto bisect = [&](u64 least, double goal, auto what) {
-      u64 lo = least, hi = ~0ull;               // what(>= lo) reaches it, what(>= hi) does not
-      while (hi - lo > 1) {
-        const u64 mid = lo + (hi - lo) / 2;
-        double s = 0.;
-        for (int j = begin + tid; j < end; j += kThreads) {
-          float f[N];
-          x.load(j, f);
+      sum = 0;
 #pragma unroll
-          for (int i = 0; i < N; ++i)
-            if (f[i] > -INFINITY && entry_of(f[i], x.first(j) + i) >= mid) s += what(f[i]);
+      for (int i = 0; i < kMost; ++i) n_of[i] = 0;
+      if (ranks == 1) {
+#pragma unroll
+        for (int i = 0; i < kMost; i += 4) {
+          const int4 v = *reinterpret_cast<const int4*>(sm_bins + bin0 + i);
+          n_of[i] = v.x; n_of[i + 1] = v.y; n_of[i + 2] = v.z; n_of[i + 3] = v.w;
         }
-        if (row_sum(s) >= goal) lo = mid; else hi = mid;
+      } else {
+#pragma unroll
+        for (int i = 0; i < kMost / 2; ++i) {
+          int v[kMaxCluster];
+#pragma unroll
+          for (int r = 0; r < kMaxCluster; ++r) v[r] = i < mine && r < ranks ? *remote(&sm_bins[bin0 + i], r) : 0;
+#pragma unroll
+          for (int r = 0; r < kMaxCluster; ++r) n_of[i] += v[r];
+        }
       }
-      return lo;
+#pragma unroll
+      for (int i = 0; i < kMost; ++i) sum += n_of[i];
+      if (!has_k) masses(0, 0x7fffffff);
+      totals();
     };
-
-    u64 border_k = 0;
-    if (has_k && want_k < all) {
-      // ---- 3, top_k: the bin in which the k-th entry lies ---------------------------------------------------------------------------
+    // what one thread of the row has found, to everybody
+    auto everybody = [&](int& bin, int& more) {
+      __syncthreads();
+      const Note* notes = exchange({0., 0., sm_border[0], sm_border[1]});
+      bin = -1;
+      for (int r = 0; r < ranks; ++r)
+        if (notes[r].n >= 0) {
+          bin = notes[r].n;
+          more = notes[r].m;
+        }
+      if (tid == 0) sm_border[0] = -1;
+      __syncthreads();
+    };
+    // the bin in which the k-th entry lies, and how many lie above it
+    auto find_k = [&](int& bin, int& above) {
       int n = before;
 #pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        if (n < want_k && n + mine[i] >= want_k) {
-          sm_index = tid * kMine + i;
-          sm_warp_n[0] = n;
-          sm_warp_n[1] = mine[i];
+      for (int i = 0; i < kMost; ++i) {
+        if (i < mine && n < want_k && n + n_of[i] >= want_k) {
+          sm_border[0] = bin0 + i;
+          sm_border[1] = n;
         }
-        n += mine[i];
+        n += n_of[i];
       }
-      __syncthreads();
-      const int bin = sm_index, above = sm_warp_n[0], members = sm_warp_n[1];
-      __syncthreads();
-      if (collect(bin, bin, 0, members)) {
-        for (int i = tid; i < listed; i += kThreads)
-          if (place_of(sm_list[i]) == want_k - above - 1) sm_found = sm_list[i];
-        __syncthreads();
-        border_k = sm_found;
-        __syncthreads();
-      } else {
-        border_k = bisect(0, (double)want_k, [](float) { return 1.; });
+      everybody(bin, above);
+    };
+    // the bin in which the estimated weights reach top_p, and on which side a border so near its edge that the neighbour may have it
+    auto find_p = [&](int& bin, int& edge) {
+      const float goal = mass_all * want_p;
+      float at = mass_before;
+      if (at < goal && mass_end >= goal) {
+        int in = bin0 + mine - 1, side = 0;
+        bool open = true;
+#pragma unroll
+        for (int i = 0; i < kMost; ++i) {
+          if (open && i < mine && at + mass_of[i] >= goal) {
+            in = bin0 + i;
+            side = goal - at < mass_of[i] * 0.1f ? -1 : at + mass_of[i] - goal < mass_of[i] * 0.1f ? 1 : 0;
+            open = false;
+          }
+          at += mass_of[i];
+        }
+        sm_border[0] = in;
+        sm_border[1] = side;
       }
+      edge = 0;
+      everybody(bin, edge);
+      if (bin < 0) bin = kBins - 1;             // (the sums' last bits)
+    };
+
+    int bin = 0, more = 0;
+    auto find = [&]() {
+      count();
+      if (has_k && want_k < all) find_k(bin, more);
+      else if (has_p && !has_k) find_p(bin, more);
+    };
+    find();
+    if (bin == kBins - 1) {                     // further away than the bins reach
+      unit = kWide;
+      bins_per *= 1.f / kWide;
+      find();
+    }
+    u64 border_k = all_of_weight;
+    if (has_k && want_k < all) {
+      // ---- 3, top_k ----------------------------------------------------------------------------------------------------------------------
+      const int above = more;
+      if (want_k <= kList && gather(0, bin)) {
+        // All that can stay is on the list, and everybody has it.
+        int stay = min(want_k, listed);
+        double w[kEach], before_w;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) w[i] = tid * kEach + i < stay ? weight(value_of(sm_list[tid * kEach + i])) : 0.;
+        if (has_p) {
+          const double need = (double)want_p * scan(w, before_w);
+#pragma unroll
+          for (int i = 0; i < kEach; ++i) {
+            before_w += w[i];
+            if (tid * kEach + i < stay && before_w >= need) {
+              atomicMin(&sm_index, tid * kEach + i);
+              break;
+            }
+          }
+          __syncthreads();
+          stay = min(stay, sm_index == 0x7fffffff ? stay : sm_index + 1);
+        }
+        // those below min_p's border
+        if (tid == 0) sm_count = stay;
+        __syncthreads();
+        for (int i = tid; i < stay; i += kThreads)
+          if (sm_list[i] < border) atomicMin(&sm_count, i);
+        __syncthreads();
+        stay = max(sm_count, 1);
+        // in the order of the index
+        const float per = (float)kBuckets / p.V;
+        order(stay, [](u64 e) { return (uint32_t)e; }, [&](u64 e) { return min((int)((float)~(uint32_t)e * per), kBuckets - 1); });
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) w[i] = tid * kEach + i < stay ? weight(value_of(sm_list[tid * kEach + i])) : 0.;
+        const double whole = scan(w, before_w);
+        const float u = p.uniform[row];
+        const double goal = u > 0.f ? fmin((double)u, 1.) * whole : 0.;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          before_w += w[i];
+          if (tid * kEach + i < stay && before_w > goal) {
+            atomicMin(&sm_index, tid * kEach + i);
+            break;
+          }
+        }
+        __syncthreads();
+        if (writes) {
+          const u64 e = sm_list[min(sm_index, stay - 1)];
+          p.token[row] = (int)~(uint32_t)e;
+          if (p.logprob) p.logprob[row] = (float)log(weight(value_of(e)) / whole);
+        }
+        meet();                                 // (others may still read this CTA's part of the list)
+        return;
+      }
+      if (gather(bin, bin)) border_k = sm_list[want_k - above - 1];
+      else border_k = bisect(all_of_weight, (double)want_k, [](float) { return 1.; });
+      __syncthreads();
     }
     u64 border_p = 0;
     if (has_p) {
-      // ---- 3, top_p: where the counts times the bins' weights reach it -----------------------------------------------------------------
-      const int most = has_k ? min(want_k, all) : all;
-      double mass = 0.;
-      {
-        int n = before;
-#pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-          const int c = min(mine[i], max(most - n, 0));
-          mass += c * (double)exp2f(-((float)(tid * kMine + i) + 0.5f) * (1.4426950f / kBinsPerNat));
-          n += mine[i];
-        }
+      // ---- 3, top_p ----------------------------------------------------------------------------------------------------------------------
+      int edge = more;
+      if (has_k) {
+        masses(before, min(want_k, all));
+        totals();
+        find_p(bin, edge);
       }
-      double to = mass;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double v = __shfl_up_sync(0xffffffffu, to, o);
-        if (lane >= o) to += v;
-      }
-      if (lane == 31) sm_warp[warp] = to;
-      if (tid == 0) sm_index = kBins - 1;
-      __syncthreads();
-      double goal = 0., below = to - mass;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) below += sm_warp[w];
-        goal += sm_warp[w];
-      }
-      goal *= (double)want_p;
-      if (below < goal && below + mass >= goal) {
-        int n = before;
-        double s = below;
-        int at = tid * kMine + kMine - 1;
-        for (int i = kMine - 1; i >= 0; --i) {  // (the first bin whose sum reaches it)
-          s = below;
-          n = before;
-          for (int q = 0; q <= i; ++q) {
-            int c = 0;
-#pragma unroll
-            for (int z = 0; z < kMine; ++z)
-              if (z == q) c = mine[z];
-            s += min(c, max(most - n, 0)) * (double)exp2f(-((float)(tid * kMine + q) + 0.5f) * (1.4426950f / kBinsPerNat));
-            n += c;
-          }
-          if (s >= goal) at = tid * kMine + i;
-        }
-        sm_index = at;
-      }
-      __syncthreads();
-      int bin = sm_index;
-      __syncthreads();
+      int first = max(bin + min(edge, 0), 0), last = min(bin + max(edge, 0), kBins - 1);
       bool found = false;
       for (int attempt = 0; attempt < 16 && !found; ++attempt) {
-        const int from = max(bin - 1, 0), last = min(bin + 1, kBins - 1);
-        // how many entries the three bins have
-        if (tid == 0) sm_count = 0;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kMine; ++i)
-          if (tid * kMine + i >= from && tid * kMine + i <= last) atomicAdd(&sm_count, mine[i]);
-        __syncthreads();
-        const int members = sm_count;
-        __syncthreads();
-        if (!collect(from, last, border_k, members)) break;
-        // the exact sums: of everything that top_k leaves, of what lies above these bins
-        double s = 0., a = 0.;
-        for (int j = begin + tid; j < end; j += kThreads) {
-          float f[N];
-          x.load(j, f);
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            if (!(f[i] > -INFINITY) || entry_of(f[i], x.first(j) + i) < border_k) continue;
-            const double w = weight(f[i]);
-            s += w;
-            if (bin_of(f[i]) < from) a += w;
-          }
-        }
-        const double whole = row_sum(s), above = row_sum(a), need = (double)want_p * whole;
-        if (above >= need && from > 0) {        // it lies further up
-          bin = max(from - 1, 0);
+        segments = pass(first, last, border_k);
+        if (!segments) break;
+        const double need = (double)want_p * sum_all;
+        if (sum_above >= need && first > 0) {   // it lies further up
+          last = first - 1;
+          first = max(first - 2, 0);
           continue;
         }
-        // the list in order, its sums
-        for (int i = tid; i < listed; i += kThreads) {
-          const u64 e = sm_list[i];
-          const uint32_t k = (uint32_t)(e >> 32);
-          sm_order[place_of(e)] = weight(__uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k));
-        }
-        __syncthreads();
-        constexpr int kEach = kList / kThreads;
-        double w[kEach], all_w = 0.;
+        // the list's sums, in order
+        double w[kEach], here;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) w[i] = tid * kEach + i < listed ? weight(value_of(sm_list[tid * kEach + i])) : 0.;
+        scan(w, here);
+        here += sum_above;
+        // the first place whose sum reaches what is wanted
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-          w[i] = tid * kEach + i < listed ? sm_order[tid * kEach + i] : 0.;
-          all_w += w[i];
+          here += w[i];
+          if (tid * kEach + i < listed && here >= need) {
+            atomicMin(&sm_index, tid * kEach + i);
+            break;
+          }
         }
-        double run = all_w;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double v = __shfl_up_sync(0xffffffffu, run, o);
-          if (lane >= o) run += v;
-        }
-        if (lane == 31) sm_warp[warp] = run;
-        if (tid == 0) sm_index = -1;
-        __syncthreads();
-        double at = above + (run - all_w), total = above;
-#pragma unroll
-        for (int q = 0; q < kWarps; ++q) {
-          if (q < warp) at += sm_warp[q];
-          total += sm_warp[q];
-        }
-        // the first place whose sum reaches what is wanted (sums only grow, so it is one thread's)
-        int here = -1;
-        double s_at = at;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-          const double next = s_at + w[i];
-          if (here < 0 && tid * kEach + i < listed && next >= need) here = tid * kEach + i;
-          s_at = next;
-        }
-        if (here >= 0) atomicMin(reinterpret_cast<unsigned*>(&sm_index), (unsigned)here);
         __syncthreads();
         const int place = sm_index;
-        __syncthreads();
-        if (place < 0) {
+        if (place == 0x7fffffff) {
           if (last == kBins - 1) {              // the sums differ in their last bits: everything stays
             found = true;
             break;
           }
-          bin = min(last + 1, kBins - 1);
+          first = last + 1;
+          last = min(last + 2, kBins - 1);
           continue;
         }
-        for (int i = tid; i < listed; i += kThreads)
-          if (place_of(sm_list[i]) == place) sm_found = sm_list[i];
-        __syncthreads();
-        border_p = sm_found;
-        __syncthreads();
+        border_p = sm_list[place];
         found = true;
       }
       if (!found) {
+        segments = false;
         double s = 0.;
-        for (int j = begin + tid; j < end; j += kThreads) {
+        for (int j = from + lane; j < to; j += 32) {
           float f[N];
-          x.load(j, f);
+          x.unpack(x.load(j), f);
 #pragma unroll
           for (int i = 0; i < N; ++i)
-            if (f[i] > -INFINITY && entry_of(f[i], x.first(j) + i) >= border_k) s += weight(f[i]);
+            if (f[i] >= low && entry_of(f[i], x.first(j) + i) >= border_k) s += weight(f[i]);
         }
         const double need = (double)want_p * row_sum(s);
         border_p = bisect(border_k, need, weight);
       }
     }
+    // (where min_p leaves less than the bins in front of the list, their sums are of no use)
+    if (segments && listed > 0 && border > sm_list[0]) segments = false;
+    if (listed == 0) segments = false;
     border = max(border, max(border_k, border_p));
   }
 
-  // ---- 4: the sum of what stays, and where the random number falls in it -------------------------------------------------------------
-  auto stays = [&](float v, int index) { return v > -INFINITY && entry_of(v, index) >= border; };
-  const int share = (per + kWarps - 1) / kWarps;
-  const int from = min(begin + warp * share, end), to = min(from + share, end);
-  double s = 0.;
-#pragma unroll 2
-  for (int j = from + lane; j < to; j += 32) {
-    float f[N];
-    x.load(j, f);
+  // ---- 4: the sums of what stays, a segment a warp; where the random number falls in them ----------------------------------------------
+  const Border stays(border);
+  if (segments) {
+    // what stays of the list, each to its segment, in order
+    double s = 0.;
+    for (int i = lane; i < listed; i += 32) {
+      const u64 e = sm_list[i];
+      const int j = ((int)~(uint32_t)e + x.lead) / N;
+      if (e >= border && j >= from && j < to) s += weight(value_of(e));
+    }
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (stays(f[i], x.first(j) + i)) s += weight(f[i]);
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) sm_segment[warp] += s;
+  } else {
+    double s = 0.;
+#pragma unroll 1
+    for (int j = from + lane; j < to; j += 32) {
+      const uint4 v = x.load(j);
+      if (x.highest(v) < stays.value) continue;
+      float f[N];
+      x.unpack(v, f);
+      const int at = x.first(j);
+      if (at <= stays.index && at + N - 1 > stays.index) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (at + i > stays.index && f[i] == stays.value) f[i] = -INFINITY;
+      }
+      const float least = at > stays.index ? stays.next : stays.value;
+#pragma unroll
+      for (int i = 0; i < N; ++i) add_from(s, weight(f[i]), f[i], least);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) sm_segment[warp] = s;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (lane == 0) sm_warp[warp] = s;
   __syncthreads();
   double own = 0.;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) own += sm_warp[w];
-  if (tid == 0) sm_sum = own;
-  meet();
-  double whole = 0., before = 0.;
-  int holder = -1, last = 0;                    // the CTA in which it falls; the last one with anything that stays
-  for (int r = 0; r < ranks; ++r) whole += r == rank ? own : *remote(&sm_sum, r);
+  for (int w = 0; w < kWarps; ++w) own += sm_segment[w];
+  const Note* notes = exchange({own, 0., 0, 0});
+  double sums[kMaxCluster], whole = 0.;
+#pragma unroll
+  for (int r = 0; r < kMaxCluster; ++r) {
+    sums[r] = r < ranks ? notes[r].a : 0.;
+    whole += sums[r];
+  }
   const float u = p.uniform[row];
   const double goal = u > 0.f ? fmin((double)u, 1.) * whole : 0.;
-  double run = 0.;
-  for (int r = 0; r < ranks; ++r) {
-    const double v = r == rank ? own : *remote(&sm_sum, r);
-    if (v > 0.) last = r;
-    if (holder < 0 && run + v > goal) {
+  int holder = -1, last = 0;                    // the CTA in which it falls; the last one with anything that stays
+  double run = 0., before = -1.;
+#pragma unroll
+  for (int r = 0; r < kMaxCluster; ++r) {
+    if (sums[r] > 0.) last = r;
+    if (holder < 0 && run + sums[r] > goal) {
       holder = r;
       before = run;
     }
-    run += v;
+    run += sums[r];
   }
-  if (holder < 0) {                             // u = 1, or the sums' last bits
-    holder = last;
-    before = -1.;
-  }
-  meet();                                       // (nobody reads sm_sum of a CTA that is gone)
+  if (holder < 0) holder = last;                // u = 1, or the sums' last bits: the last entry that stays
   if (rank != holder) return;
   int segment = -1, last_segment = 0;
   double at = before;
+#pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    const double v = sm_warp[w];
+    const double v = sm_segment[w];
     if (v > 0.) last_segment = w;
     if (segment < 0 && before >= 0. && at + v > goal) segment = w;
     if (segment < 0) at += v;
   }
-  const bool at_end = segment < 0;              // the last entry that stays
+  const bool at_end = segment < 0;
   if (at_end) segment = last_segment;
   const int first = min(begin + segment * share, end), behind = min(first + share, end);
   if (tid == 0) {
@@ -594,18 +955,19 @@ sample_tokens_kernel(const SampleParams p) {
     sm_count = -1;
   }
   __syncthreads();
-  // 512 vectors at a time, in order
+  // as many vectors as threads at a time, in order
   for (int base = first; base < behind; base += kThreads) {
     const int j = base + tid;
-    float f[N];
     double w[N], mine = 0.;
 #pragma unroll
     for (int i = 0; i < N; ++i) w[i] = 0.;
     if (j < behind) {
-      x.load(j, f);
+      float f[N];
+      x.unpack(x.load(j), f);
+      const int at = x.first(j);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        if (stays(f[i], x.first(j) + i)) w[i] = weight(f[i]);
+        if (f[i] >= (at + i > stays.index ? stays.next : stays.value)) w[i] = weight(f[i]);
         mine += w[i];
       }
     }
@@ -638,7 +1000,7 @@ sample_tokens_kernel(const SampleParams p) {
   if (tid == 0) {
     const int token = sm_index != 0x7fffffff ? sm_index : sm_count;
     p.token[row] = token;
-    if (p.logprob) p.logprob[row] = token >= 0 ? (float)(((double)to_float(x.x[token]) - top) * per_t - log(whole)) : NAN;
+    if (p.logprob) p.logprob[row] = token >= 0 ? (float)log(weight(to_float(x.x[token])) / whole) : NAN;
   }
 }
 
@@ -665,13 +1027,15 @@ extern "C" int b200_sample_tokens(const void* logits, int32_t dtype, int64_t str
   SampleParams p = {logits, static_cast<const float*>(uniform), static_cast<int*>(token), static_cast<float*>(logprob),
                     static_cast<const float*>(how->temperatures), static_cast<const int*>(how->top_ks), static_cast<const float*>(how->top_ps),
                     static_cast<const float*>(how->min_ps), stride, rows, (int)V, how->temperature, how->top_p, how->min_p, how->top_k};
+  // CTAs of a row: a cluster's meetings take as long as 40000 entries, so a row is cut from twice as many on, into as many parts as the GPU holds.
   int c = 1;
-  while (c < kMaxCluster && rows * c * 2 <= sm_count() && V / (2 * c) >= 2048) c *= 2;
-  auto launch = [&](auto kern) {
+  while (V >= 65536 && c < kMaxCluster && rows * c * 2 <= 2 * sm_count()) c *= 2;
+  const bool many = c == 1 && rows > 2 * sm_count();
+  auto launch = [&](auto kern, int threads) {
     const int64_t y = rows < 32768 ? rows : 32768;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)c, (unsigned)y, (unsigned)((rows + y - 1) / y));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.stream = static_cast<cudaStream_t>(stream);
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -686,6 +1050,9 @@ extern "C" int b200_sample_tokens(const void* logits, int32_t dtype, int64_t str
     count_launch();
     return B200_OK;
   };
-  return dtype == B200_F16 ? launch(sample_tokens_kernel<__half>)
-       : dtype == B200_BF16 ? launch(sample_tokens_kernel<__nv_bfloat16>) : launch(sample_tokens_kernel<float>);
+  auto by_rows = [&](auto type) {
+    using T = decltype(type);
+    return many ? launch(sample_tokens_kernel<T, kMany>, kMany) : launch(sample_tokens_kernel<T, kFew>, kFew);
+  };
+  return dtype == B200_F16 ? by_rows(__half()) : dtype == B200_BF16 ? by_rows(__nv_bfloat16()) : by_rows(float());
 }

@@ -32,7 +32,7 @@ def sample(x, u, **how):
     if not (x > -math.inf).any():
         return -1, -math.inf
     keep, w = allowed(x, **how)
-    some = w > 0
+    some = w >= math.exp(-690)                                   # less is as good as excluded
     keep, w = keep[some], w[some]
     sums = np.cumsum(w)
     goal = float(np.float32(u)) * sums[-1] if u > 0 else 0.0

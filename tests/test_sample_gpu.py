@@ -1,5 +1,5 @@
 """ops.sample_tokens against its definition in 64 bits.  The token has to be the same: both sides compare sums of weights of fp64, whose
-difference (2^-42 of a weight) would have to reach from a random number to the next border."""
+difference (2^-37 of a weight) would have to reach from a random number to the next border."""
 import math
 
 import numpy as np
@@ -23,8 +23,8 @@ def check(logits, uniform, **how):
         token, logprob = sample(x[i], u[i], **{n: v[i] if isinstance(v, list) else v for n, v in how.items()})
         assert int(got.token[i]) == token, f"row {i}: {int(got.token[i])} instead of {token}, u = {u[i]}, {how}"
         value = float(got.logprob[i])
-        if math.isfinite(logprob):                # one rounding to fp32, the weight's and the sum's 2^-42
-            assert abs(value - logprob) <= 2.0 ** -24 * abs(logprob) + 2.0 ** -40, f"row {i}"
+        if math.isfinite(logprob):                # one rounding to fp32; the weight and the sum are 2^-37 exact each
+            assert abs(value - logprob) <= 2.0 ** -24 * abs(logprob) + 2.0 ** -36, f"row {i}"
         else:
             assert math.isnan(value) == math.isnan(logprob) and (math.isnan(value) or value == logprob)
     return got
