@@ -547,7 +547,7 @@ B200_API int b200_paged8_attention(const B200PagedCache* cache, const B200PagedS
  * status 0: done.  n > 0: n pages are lacking; -1: a length, before or after, is not in 0 .. max_tokens (0: what the table holds); -2: more than `rows` new tokens;
  * -3: the free list is shorter than nothing or longer than its room (`pages` entries).  Where it is not 0 table and free list stay as they were, lengths_out =
  * lengths, free_count_out = free_count, starts are 0 and positions and slots -1.
- * lengths_out may be lengths, free_count_out free_count.  All int32 but slots; batch <= 8192; one launch. */
+ * lengths_out may be lengths, free_count_out free_count; otherwise no result shares memory with an argument.  All int32 but slots; batch <= 8192; one launch. */
 typedef struct {
   int32_t batch, table_width, page_size, max_tokens;
   int64_t table_stride, pages, rows;

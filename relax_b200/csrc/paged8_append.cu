@@ -5,10 +5,15 @@
 // codes are scaled anew: powers of two change a code's exponent only, so that nothing is rounded twice but what falls below the
 // format's smallest step.
 //
-// A block of the call is one for each token: it turns the token's query heads.  The keys and values of a block of 16 tokens are tasks, one
-// for each key head and one for its values, dealt out to the thread blocks of its tokens, a warp each: so a prompt's block of 16 tokens has 16 thread
-// blocks with a task or two each, and a single token has one with all.  A task's warp holds all its tokens, a lane D / 32 dims of each:
-// the largest value is a shuffle away, and no other warp touches the block's codes or its scale.
+// A thread block takes one token: its query heads, and a share of the keys and values of the 16 tokens that it lies in.  A task is a key head's
+// keys or its values; the thread blocks of the call's n tokens there deal the tasks out among themselves, so that each has as many (token, task)
+// pairs as a token has keys and values, whatever n is.  No other thread block touches a task's codes or its scale.
+// A thread has two chunks of 8 values of a pair, those that are turned together, as it has of the queries; the largest value of a task comes
+// together in shared memory.
+//
+// What bounds it: HBM for prompts, latency for single tokens (64 of them 5.0 us a call).  us for 8.4k tokens of 32 heads and 8 key heads, 190 MB: 40.3
+// (4.8 TB/s, 0.73 of a copy) with eight blocks an SM, 42.6 with six, 51.8 with the four that fit without a limit on registers.  Before: a warp for all
+// tokens of a task 164; a warp for a (token, task) pair, 4 values a lane, 68 (5000 instructions a token instead of 3100).
 #include <type_traits>
 
 #include "paged_common.cuh"
@@ -17,7 +22,8 @@ namespace b200 {
 
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kThreads = 128;
+constexpr int kEarly = 2;                       // of the queries' chunk pairs that are asked for before it is known where the token lies
 constexpr int kTokens = 16;                     // that share a scale
 constexpr int kMinPower = -24, kMaxPower = 7;   // of a scale: fp16's smallest number; 448 * 2^7 is the last that fp16 holds
 
@@ -49,22 +55,11 @@ __device__ __forceinline__ uint32_t codes2(float lo, float hi) {
 }
 __device__ __forceinline__ float2 values2(uint32_t codes) { return unpack2(__half(), e4m3_to_half2(codes)); }
 
-// The words of a lane's share of a token: W 16-bit pairs.
-template <int W>
-struct Words {
-  uint32_t w[W];
-};
-template <int W>
-__device__ __forceinline__ Words<W> load_words(const void* p) {
-  Words<W> r;
-  if constexpr (W == 2) {
-    const uint2 v = *static_cast<const uint2*>(p);
-    r.w[0] = v.x;
-    r.w[1] = v.y;
-  } else {
-    r.w[0] = *static_cast<const uint32_t*>(p);
-  }
-  return r;
+// 8 neighbouring numbers of a table.
+__device__ __forceinline__ void load8_floats(const float* p, float (&to)[8]) {
+  const float4 u = reinterpret_cast<const float4*>(p)[0], v = reinterpret_cast<const float4*>(p)[1];
+  to[0] = u.x; to[1] = u.y; to[2] = u.z; to[3] = u.w;
+  to[4] = v.x; to[5] = v.y; to[6] = v.z; to[7] = v.w;
 }
 
 // The table row of a token at `position`, row `row` of the call.
@@ -74,15 +69,30 @@ __device__ __forceinline__ int64_t table_row(const AppendParams& p, int row, int
 }
 
 template <typename T, int D, bool kInterleaved>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 8)
 paged8_append_kernel(const AppendParams p) {
-  constexpr int E = D / 32, W = E / 2;          // dims and words of a lane
+  constexpr int kChunks = D / 16;               // chunk pairs of a row of D values
+  constexpr int kPairs = kThreads / kChunks;    // (token, task) pairs at a time
+  constexpr uint32_t kInfinite = std::is_same<T, __half>::value ? 0x7c00 : 0x7f80;
+  __shared__ int sm_most[3][kPairs];            // largest values of the tasks at hand; the next round's are cleared a barrier before
   ptx::pdl_wait();
   ptx::pdl_launch_dependents();
   const int kv = p.c.kv_heads, page = 1 << p.c.page_log2;
-  const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = blockIdx.x, c = threadIdx.x % kChunks;
   const int half = p.rotary / 2;
+  const bool turns = 16 * c < p.rotary;         // this thread's chunk pairs, of queries and keys
+  const int o0 = !kInterleaved && turns ? 8 * c : 16 * c, o1 = !kInterleaved && turns ? half + o0 : o0 + 8;
+  const T* in = static_cast<const T*>(p.qkv) + (int64_t)row * p.qkv_stride;
   T* q = static_cast<T*>(p.q_out) + (int64_t)row * p.heads * D;
+  auto chunk = [](const T* from) { return *reinterpret_cast<const uint4*>(from); };
+  uint4 qx[kEarly], qy[kEarly];
+  int head = threadIdx.x / kChunks;
+#pragma unroll
+  for (int k = 0; k < kEarly; ++k)
+    if (head + k * kPairs < p.heads) {
+      qx[k] = chunk(in + (head + k * kPairs) * D + o0);
+      qy[k] = chunk(in + (head + k * kPairs) * D + o1);
+    }
   // the sequence of this row: the last one that starts at or before it
   int b = row;
   if (p.c.starts) {
@@ -99,149 +109,126 @@ paged8_append_kernel(const AppendParams p) {
     for (int i = threadIdx.x; i < p.heads * D / 8; i += kThreads) reinterpret_cast<uint4*>(q)[i] = make_uint4(0, 0, 0, 0);
     return;
   }
+  // a chunk pair turned by the angles of table row `at`
+  auto turn = [&](uint4& x, uint4& y, int64_t at) {
+    float cs[8], sn[8];
+    load8_floats(p.cos_t + at * half + 8 * c, cs);
+    load8_floats(p.sin_t + at * half + 8 * c, sn);
+    uint32_t* xo = &x.x;
+    uint32_t* yo = &y.x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 u = unpack2(T(), xo[j]), w = unpack2(T(), yo[j]);
+      if (kInterleaved) {                       // a word is a pair: x holds pairs 0..3 of the eight, y 4..7
+        xo[j] = pack2(T(), u.x * cs[j] - u.y * sn[j], u.y * cs[j] + u.x * sn[j]);
+        yo[j] = pack2(T(), w.x * cs[4 + j] - w.y * sn[4 + j], w.y * cs[4 + j] + w.x * sn[4 + j]);
+      } else {
+        xo[j] = pack2(T(), u.x * cs[2 * j] - w.x * sn[2 * j], u.y * cs[2 * j + 1] - w.y * sn[2 * j + 1]);
+        yo[j] = pack2(T(), w.x * cs[2 * j] + u.x * sn[2 * j], w.y * cs[2 * j + 1] + u.y * sn[2 * j + 1]);
+      }
+    }
+  };
+  const int64_t mine = table_row(p, row, position);
+  auto put_query = [&](int h, uint4 x, uint4 y) {
+    if (turns) turn(x, y, mine);
+    *reinterpret_cast<uint4*>(q + h * D + o0) = x;
+    *reinterpret_cast<uint4*>(q + h * D + o1) = y;
+  };
+  auto put_queries = [&]() {
+#pragma unroll
+    for (int k = 0; k < kEarly; ++k)
+      if (head + k * kPairs < p.heads) put_query(head + k * kPairs, qx[k], qy[k]);
+#pragma unroll 1
+    for (head += kEarly * kPairs; head < p.heads; head += kPairs) put_query(head, chunk(in + head * D + o0), chunk(in + head * D + o1));
+  };
 
   // ---- keys and values of the block of 16 tokens that this one lies in: tokens [first, first + n) are the call's ------------------
   const int begin = position & ~(kTokens - 1), first = max(begin, max(base, 0)), n = min(begin + kTokens, s.length) - first;
   const int64_t id = page_of(p.c, b, position >> p.c.page_log2);
-  const int offset = begin & (page - 1), first_row = s.first + first - base;
+  const int offset = begin & (page - 1), first_row = s.first + first - base, earlier = first - begin;
+  const int inverse = (65536 + n - 1) / n;      // (of numbers below 64 by n)
+  const int per_round = kPairs * inverse >> 16; // tasks at a time
+  const int slot = (threadIdx.x / kChunks) * inverse >> 16, r = threadIdx.x / kChunks - slot * n;
+  const T* from = static_cast<const T*>(p.qkv) + (int64_t)(first_row + r) * p.qkv_stride + p.heads * D;
+  if (threadIdx.x < kPairs) sm_most[0][threadIdx.x] = 0;
+  __syncthreads();
+  int round = 0;
+  bool queries = true;
 #pragma unroll 1
-  for (int task = position - first + n * warp; task < 2 * kv; task += n * kWarps) {
-    const bool is_v = task >= kv;
+  for (int done = 0; position - first + n * done < 2 * kv; done += per_round) {
+    const int next = round == 2 ? 0 : round + 1;
+    if (threadIdx.x < kPairs) sm_most[next][threadIdx.x] = 0;
+    const int task = position - first + n * (done + slot);
+    const bool some = slot < per_round && task < 2 * kv, is_v = task >= kv;
     const int h = is_v ? task - kv : task;
-    const T* in = static_cast<const T*>(p.qkv) + (int64_t)first_row * p.qkv_stride + (p.heads + task) * D + E * lane;
-    unsigned char* codes = static_cast<unsigned char*>(is_v ? p.c.v : p.c.k) + id * (is_v ? p.c.v_stride : p.c.k_stride) +
-                           ((int64_t)h * page + offset) * D + E * lane;
     __half* scale = (is_v ? p.v_scales : p.k_scales) + ((id * kv + h) * page + offset) / kTokens;
-    const int earlier = first - begin;
-    const float was = earlier ? __half2float(*scale) : 0.f;
-    const bool turned = !is_v && E * lane < p.rotary;
-    Words<W> x[kTokens];
-    float most = 0.f;
-    // (four tokens' loads at a time)
+    uint4 x = make_uint4(0, 0, 0, 0), y = x;
+    float was = 0.f;
+    if (some) {
+      x = chunk(from + task * D + o0);
+      y = chunk(from + task * D + o1);
+      if (earlier) was = __half2float(*scale);
+    }
+    if (queries) put_queries();                 // (the loads above are on their way)
+    queries = false;
+    uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    if (some) {
+      if (turns && !is_v) {
+        turn(x, y, table_row(p, first_row + r, first + r));
+        w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w; w[4] = y.x; w[5] = y.y; w[6] = y.z; w[7] = y.w;
+      }
+      // sizes are in the order of their bits; what is no finite number does not count
+      uint32_t most = 0;
 #pragma unroll
-    for (int r0 = 0; r0 < kTokens; r0 += 4) {
-      if (r0 >= n) break;
-      Words<W> other[4];
-      float cs[4][E], sn[4][E];
+      for (int e = 0; e < 8; ++e) most = __vmaxu2(most, w[e] & 0x7fff7fffu);
+      most = max(most & 0xffffu, most >> 16);
+      if (most >= kInfinite) {
+        most = 0;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if (r0 + r >= n) continue;
-        const T* from = in + (r0 + r) * p.qkv_stride;
-        x[r0 + r] = load_words<W>(from);
-        if (turned) {
-          const int64_t at = table_row(p, first_row + r0 + r, first + r0 + r) * half;
-          const int d = E * lane;
-          if (kInterleaved) {                   // pairs (2 i, 2 i + 1): the lane's own
-#pragma unroll
-            for (int i = 0; i < W; ++i) { cs[r][i] = p.cos_t[at + d / 2 + i]; sn[r][i] = p.sin_t[at + d / 2 + i]; }
-          } else {                              // pairs (i, i + half): the other's in another lane
-            const bool low = d < half;
-            other[r] = load_words<W>(low ? from + half : from - half);
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
-              cs[r][i] = p.cos_t[at + (low ? d : d - half) + i];
-              sn[r][i] = p.sin_t[at + (low ? d : d - half) + i];
-            }
+        for (int e = 0; e < 16; ++e) {
+          const uint32_t v = (e & 1 ? w[e / 2] >> 16 : w[e / 2]) & 0x7fffu;
+          if (v < kInfinite) most = max(most, v);
+        }
+      }
+      atomicMax(&sm_most[round][slot], (int)most);
+    }
+    __syncthreads();
+    if (some) {
+      unsigned char* codes = static_cast<unsigned char*>(is_v ? p.c.v : p.c.k) + id * (is_v ? p.c.v_stride : p.c.k_stride) + ((int64_t)h * page + offset) * D;
+      const float most = unpack2(T(), (uint32_t)sm_most[round][slot]).x;
+      const float now = fmaxf(was, power_of_two(power_for(most))), per = 1.f / now;
+      if (r == 0) {                             // the task's scale, and the earlier tokens' codes by it
+        if (was < now && earlier) {
+          const float ratio = was * per;
+          auto again = [&](uint32_t codes4) {
+            const float2 u = values2(codes4 & 0xffffu), v = values2(codes4 >> 16);
+            return codes2(u.x * ratio, u.y * ratio) | codes2(v.x * ratio, v.y * ratio) << 16;
+          };
+#pragma unroll 5
+          for (int t = 0; t < earlier; ++t) {
+            uint4* old = reinterpret_cast<uint4*>(codes + t * D) + c;
+            const uint4 v = *old;
+            *old = make_uint4(again(v.x), again(v.y), again(v.z), again(v.w));
           }
         }
+        if (c == 0) *scale = __float2half_rn(now);
       }
+      uint32_t out[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if (r0 + r >= n) continue;
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-          uint32_t& w = x[r0 + r].w[i];
-          if (turned) {
-            const float2 a = unpack2(T(), w);
-            if (kInterleaved) {
-              w = pack2(T(), a.x * cs[r][i] - a.y * sn[r][i], a.y * cs[r][i] + a.x * sn[r][i]);
-            } else {
-              const float2 o = unpack2(T(), other[r].w[i]);
-              const bool low = E * lane < half;
-              const float s0 = low ? -sn[r][2 * i] : sn[r][2 * i], s1 = low ? -sn[r][2 * i + 1] : sn[r][2 * i + 1];
-              w = pack2(T(), a.x * cs[r][2 * i] + o.x * s0, a.y * cs[r][2 * i + 1] + o.y * s1);
-            }
-          }
-          const float2 v = unpack2(T(), w);
-          // (what is no finite number does not count)
-          if (fabsf(v.x) < INFINITY) most = fmaxf(most, fabsf(v.x));
-          if (fabsf(v.y) < INFINITY) most = fmaxf(most, fabsf(v.y));
-        }
+      for (int e = 0; e < 8; ++e) {
+        float2 v = unpack2(T(), w[e]);
+        if ((w[e] & 0x7fffu) == kInfinite) v.x = NAN;                     // (a NaN's code is one anyway)
+        if ((w[e] >> 16 & 0x7fffu) == kInfinite) v.y = NAN;
+        const uint32_t two = codes2(v.x * per, v.y * per);
+        out[e / 2] = e & 1 ? out[e / 2] | two << 16 : two;
       }
+      unsigned char* to = codes + (earlier + r) * D;
+      *reinterpret_cast<uint2*>(to + o0) = make_uint2(out[0], out[1]);
+      *reinterpret_cast<uint2*>(to + o1) = make_uint2(out[2], out[3]);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    const float need = power_of_two(power_for(most)), now = fmaxf(was, need);
-    const float per = 1.f / now;
-    if (was < now && earlier) {                 // the earlier tokens' codes by the new scale
-      const float ratio = was * per;
-#pragma unroll 4
-      for (int r = 0; r < earlier; ++r) {
-        unsigned char* at = codes + r * D;
-        if constexpr (E == 4) {
-          const uint32_t c = *reinterpret_cast<const uint32_t*>(at);
-          const float2 u = values2(c & 0xffffu), v = values2(c >> 16);
-          *reinterpret_cast<uint32_t*>(at) = codes2(u.x * ratio, u.y * ratio) | codes2(v.x * ratio, v.y * ratio) << 16;
-        } else {
-          const float2 u = values2(*reinterpret_cast<const uint16_t*>(at));
-          *reinterpret_cast<uint16_t*>(at) = (uint16_t)codes2(u.x * ratio, u.y * ratio);
-        }
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < kTokens; ++r) {
-      if (r >= n) break;
-      uint32_t c[W];
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        float2 v = unpack2(T(), x[r].w[i]);
-        if (!(fabsf(v.x) < INFINITY)) v.x = NAN;
-        if (!(fabsf(v.y) < INFINITY)) v.y = NAN;
-        c[i] = codes2(v.x * per, v.y * per);
-      }
-      unsigned char* at = codes + (earlier + r) * D;
-      if constexpr (E == 4) *reinterpret_cast<uint32_t*>(at) = c[0] | c[W - 1] << 16;
-      else *reinterpret_cast<uint16_t*>(at) = (uint16_t)c[0];
-    }
-    if (lane == 0) *scale = __float2half_rn(now);
+    round = next;
   }
-
-  // ---- the token's queries: pairs of chunks of 8 values, turned or as they are ------------------------------------------------------
-  const T* in = static_cast<const T*>(p.qkv) + (int64_t)row * p.qkv_stride;
-  const int64_t at = table_row(p, row, position) * half;
-  constexpr int kPairs = D / 16;
-#pragma unroll 2
-  for (int i = threadIdx.x; i < p.heads * kPairs; i += kThreads) {
-    const int h = i / kPairs, c = i - h * kPairs;
-    const bool turn = 16 * c < p.rotary;
-    const int o0 = kInterleaved || !turn ? 16 * c : 8 * c, o1 = kInterleaved || !turn ? o0 + 8 : half + 8 * c;
-    const uint4 x = *reinterpret_cast<const uint4*>(in + h * D + o0), y = *reinterpret_cast<const uint4*>(in + h * D + o1);
-    uint32_t xo[4] = {x.x, x.y, x.z, x.w}, yo[4] = {y.x, y.y, y.z, y.w};
-    if (turn) {
-      float cs[8], sn[8];
-      const float4* cp = reinterpret_cast<const float4*>(p.cos_t + at + 8 * c);
-      const float4* sp = reinterpret_cast<const float4*>(p.sin_t + at + 8 * c);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float4 u = cp[j], w = sp[j];
-        cs[4 * j] = u.x; cs[4 * j + 1] = u.y; cs[4 * j + 2] = u.z; cs[4 * j + 3] = u.w;
-        sn[4 * j] = w.x; sn[4 * j + 1] = w.y; sn[4 * j + 2] = w.z; sn[4 * j + 3] = w.w;
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 u = unpack2(T(), xo[j]), w = unpack2(T(), yo[j]);
-        if (kInterleaved) {                     // a word is a pair: x holds pairs 0..3 of the eight, y 4..7
-          xo[j] = pack2(T(), u.x * cs[j] - u.y * sn[j], u.y * cs[j] + u.x * sn[j]);
-          yo[j] = pack2(T(), w.x * cs[4 + j] - w.y * sn[4 + j], w.y * cs[4 + j] + w.x * sn[4 + j]);
-        } else {
-          xo[j] = pack2(T(), u.x * cs[2 * j] - w.x * sn[2 * j], u.y * cs[2 * j + 1] - w.y * sn[2 * j + 1]);
-          yo[j] = pack2(T(), w.x * cs[2 * j] + u.x * sn[2 * j], w.y * cs[2 * j + 1] + u.y * sn[2 * j + 1]);
-        }
-      }
-    }
-    *reinterpret_cast<uint4*>(q + h * D + o0) = make_uint4(xo[0], xo[1], xo[2], xo[3]);
-    *reinterpret_cast<uint4*>(q + h * D + o1) = make_uint4(yo[0], yo[1], yo[2], yo[3]);
-  }
+  if (queries) put_queries();                   // (more tokens than tasks: this one has none)
 }
 
 }  // namespace

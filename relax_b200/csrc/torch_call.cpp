@@ -338,6 +338,22 @@ PyObject* token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
 }
 
+// New vectors in one piece of memory: six allocations take 4 us, as long as the kernel that fills them.
+template <int N>
+void vectors(const int64_t (&sizes)[N], const at::ScalarType (&types)[N], const at::TensorOptions& options, at::Tensor (&out)[N]) {
+  int64_t at[N], bytes = 0;
+  for (int i = 0; i < N; ++i) {
+    at[i] = bytes;
+    bytes += (sizes[i] * (int64_t)c10::elementSize(types[i]) + 15) / 16 * 16;
+  }
+  const at::Tensor whole = at::empty({bytes}, options.dtype(at::kByte));
+  for (int i = 0; i < N; ++i) {
+    out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), c10::scalarTypeToTypeMeta(types[i]));
+    out[i].unsafeGetTensorImpl()->set_storage_offset(at[i] / (int64_t)c10::elementSize(types[i]));
+    out[i].unsafeGetTensorImpl()->set_sizes_contiguous({sizes[i]});
+  }
+}
+
 // paged_plan(table, lengths, counts, free_pages, free_count, page_size, rows, max_tokens, out): (lengths, starts, positions, slots, free_count,
 // status), `out` a tuple of them or None
 PyObject* paged_plan(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -362,14 +378,11 @@ PyObject* paged_plan(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t sizes[6] = {batch, batch + 1, rows, rows, 1, 1};
     const auto i32 = table->options().requires_grad(false);
     if (args[8] != Py_None && (!PyTuple_Check(args[8]) || PyTuple_GET_SIZE(args[8]) != 6)) Py_RETURN_NONE;
-    for (int i = 0; i < 6; ++i) {
-      const at::ScalarType type = i == 3 ? at::kLong : at::kInt;
-      if (args[8] == Py_None) {
-        out[i] = at::empty({sizes[i]}, i32.dtype(type));
-        continue;
-      }
+    constexpr at::ScalarType types[6] = {at::kInt, at::kInt, at::kInt, at::kLong, at::kInt, at::kInt};
+    if (args[8] == Py_None) vectors(sizes, types, i32, out);
+    for (int i = 0; args[8] != Py_None && i < 6; ++i) {
       const at::Tensor* t = plain(PyTuple_GET_ITEM(args[8], i));
-      if (!t || t->scalar_type() != type || t->dim() != 1 || t->size(0) != sizes[i] || !t->is_contiguous() || t->get_device() != dev) Py_RETURN_NONE;
+      if (!t || t->scalar_type() != types[i] || t->dim() != 1 || t->size(0) != sizes[i] || !t->is_contiguous() || t->get_device() != dev) Py_RETURN_NONE;
       out[i] = *t;
     }
     B200PagedPlan p = {};
