@@ -20,6 +20,7 @@
 // What bounds it: HBM for long caches (131000 tokens of 8 key heads, 537 MB, 90 us: 6.0 TB/s, 0.91 of a copy; 512 sequences of 37 to 2047
 // tokens 182 us: 5.9; 64 of them, 135 MB, 31 us: 4.4); latency for short ones (32 heads at 2011, 33 MB, 13.6 us: 2 until the shares are
 // known, 7 for two or three units a warp, 4 for the joins).  Before, chunks of equal length as CTAs of their own took 157, 45 and 17.5 us.
+#include <algorithm>
 #include <type_traits>
 
 #include "paged_common.cuh"
@@ -35,6 +36,7 @@ constexpr int kUnit = 16;
 // 33 with a window.
 constexpr int kStart = 3;
 constexpr int kCtasPerSm1 = 3, kCtasPerSm2 = 2;       // of tiles of 8 rows, of 16
+constexpr int kCtas8PerSm1 = 4, kCtas8PerSm2 = 2;     // over pages of 8 bits
 __device__ __forceinline__ void mma(__half, float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -77,11 +79,11 @@ struct Piece {
 // its scores, that of a value into the exponent of its weight: m is the maximum of s + log2 v, a weight 2^(s + log2 v - m), so that it has
 // its bits whatever the blocks' sizes are, and the sum takes it by 1 / v.
 template <typename T, int D, int NT, int kExtra, bool kBytes>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kCtasPerSm1 : kCtasPerSm2)
+__global__ void __launch_bounds__(kWarps * 32, kBytes ? NT == 1 ? kCtas8PerSm1 : kCtas8PerSm2 : NT == 1 ? kCtasPerSm1 : kCtasPerSm2)
 paged_decode_kernel(const PagedAttnParams p) {
   constexpr int R = 8 * NT;                     // rows of a tile
   using M = typename std::conditional<kBytes, __half, T>::type;          // what is multiplied
-  constexpr int SUB = (kBytes ? 256 : 128) / D; // units a warp takes at a time
+  constexpr int SUB = 128 / D;                  // units a warp takes at a time
   constexpr int KC = D / 32, VC = D / 64, MT = D / 16;
   constexpr int KB = D / 64, VW = D / 32;       // 8 bits: loads of a key's dims, words of a value's
   // the dims of a lane in the result: kDim g .. and kDim g + kDim1 ..
@@ -313,9 +315,9 @@ paged_decode_kernel(const PagedAttnParams p) {
             for (int j = 0; j < KB; ++j)
 #pragma unroll
               for (int w = 0; w < 4; ++w) {
-                const uint32_t c0 = word(kb[x][0][j], w), c1 = word(kb[x][1][j], w);
-                const uint32_t a0 = e4m3_to_half2(c0 & 0xffffu), a1 = e4m3_to_half2(c1 & 0xffffu);
-                const uint32_t a2 = e4m3_to_half2(c0 >> 16), a3 = e4m3_to_half2(c1 >> 16);
+                uint32_t a0, a1, a2, a3;
+                e4m3_to_half4(word(kb[x][0][j], w), a0, a2);
+                e4m3_to_half4(word(kb[x][1][j], w), a1, a3);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                   const uint4 f = qf[n][2 * j + w / 2];
@@ -436,13 +438,15 @@ paged_decode_kernel(const PagedAttnParams p) {
               const unsigned s = k & 2 ? 0x7362 : 0x5140;
               const uint32_t c0 = __byte_perm(vb[x][0][w0], vb[x][1][w0], s), c1 = __byte_perm(vb[x][0][w1], vb[x][1][w1], s);
               const uint32_t c2 = __byte_perm(vb[x][2][w0], vb[x][3][w0], s), c3 = __byte_perm(vb[x][2][w1], vb[x][3][w1], s);
+              uint32_t a0[2], a1[2], a2[2], a3[2];
+              e4m3_to_half4(c0, a0[0], a0[1]);
+              e4m3_to_half4(c1, a1[0], a1[1]);
+              e4m3_to_half4(c2, a2[0], a2[1]);
+              e4m3_to_half4(c3, a3[0], a3[1]);
 #pragma unroll
-              for (int o = 0; o < 2; ++o) {
-                const uint32_t a0 = e4m3_to_half2(o ? c0 >> 16 : c0 & 0xffffu), a1 = e4m3_to_half2(o ? c1 >> 16 : c1 & 0xffffu);
-                const uint32_t a2 = e4m3_to_half2(o ? c2 >> 16 : c2 & 0xffffu), a3 = e4m3_to_half2(o ? c3 >> 16 : c3 & 0xffffu);
+              for (int o = 0; o < 2; ++o)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma(M(), acc[n][k + o], a0, a1, a2, a3, pb[n][0], pb[n][1]);
-              }
+                for (int n = 0; n < NT; ++n) mma(M(), acc[n][k + o], a0[o], a1[o], a2[o], a3[o], pb[n][0], pb[n][1]);
             }
             continue;
           }
@@ -517,7 +521,7 @@ paged_decode_kernel(const PagedAttnParams p) {
   // ---- pieces of the same tile in this CTA, then those of different CTAs: the one that comes last adds them up --------------------
   // A warp takes a row at a time, a lane four of its dims (head_dim 64: two), and a part's maximum and sum in a lane of its own.
   __syncthreads();
-  constexpr int kDims = D / 32;
+  constexpr int kDims = D / 32, kAtOnce = 8;   // (parts of different CTAs that are on their way: with 8 a round trip for every eight of up to 300)
   float v[kDims];
   auto store = [&](float* to) {
     if (kDims == 4) *reinterpret_cast<float4*>(to + 4 * lane) = make_float4(v[0], v[1], v[kDims - 2], v[kDims - 1]);
@@ -634,10 +638,10 @@ paged_decode_kernel(const PagedAttnParams p) {
         if (lane < n) ml = __ldcg(reinterpret_cast<const float2*>(p.partial_ml + 2 * row_of(c0 + lane, r)));
         float f = 0.f;
 #pragma unroll 1
-        for (int y0 = 0; y0 < n; y0 += 8) {
-          float o[8][kDims];
+        for (int y0 = 0; y0 < n; y0 += kAtOnce) {
+          float o[kAtOnce][kDims];
 #pragma unroll
-          for (int y = 0; y < 8; ++y) {         // (behind the end the last one again, with weight 0)
+          for (int y = 0; y < kAtOnce; ++y) {         // (behind the end the last one again, with weight 0)
             const float* from = p.partial + (int64_t)row_of(c0 + min(y0 + y, n - 1), r) * D + kDims * lane;
             if (kDims == 4) {
               const float4 q = __ldcg(reinterpret_cast<const float4*>(from));
@@ -656,7 +660,7 @@ paged_decode_kernel(const PagedAttnParams p) {
             for (int i = 0; i < kDims; ++i) v[i] *= old;
           }
 #pragma unroll
-          for (int y = 0; y < 8; ++y) {
+          for (int y = 0; y < kAtOnce; ++y) {
             const float fy = __shfl_sync(0xffffffffu, f, (y0 + y) & 31);
             if (y0 + y < n)
 #pragma unroll
@@ -674,7 +678,7 @@ int launch_decode(const char* who, const B200PagedCache* c, PagedAttnParams p, c
   const int64_t most = (int64_t)c->max_query * p.group;          // rows of a sequence that share a key head
   const bool narrow = most <= 8;
   const int R = narrow ? 8 : 16;
-  p.slots = sm_count() * (narrow ? kCtasPerSm1 : kCtasPerSm2);
+  p.slots = sm_count() * (kBytes ? narrow ? kCtas8PerSm1 : kCtas8PerSm2 : narrow ? kCtasPerSm1 : kCtasPerSm2);
   auto launch = [&](auto kern, SmemLimit& limit) {
     const size_t smem = (size_t)2 * kWarps * R * (c->head_dim + 4) * sizeof(float);
     int rc = raise_smem_limit(limit, reinterpret_cast<const void*>(kern), smem, who);
@@ -721,7 +725,8 @@ extern "C" {
 
 // The counters, the maxima and sums of parts, their partial results.  The few-rows kernel has two parts a CTA at most (a tile that began before
 // its share, one that ends behind it) of 8 rows (three CTAs an SM) or 16 (two): 64 rows an SM.  The many-rows kernel has kPartsOfSlots of 256.
-static_assert(2 * kCtasPerSm1 * 8 <= kPartsOfSlots * 256 && 2 * kCtasPerSm2 * 16 <= kPartsOfSlots * 256, "partial results of the few-rows kernel");
+static_assert(2 * std::max(kCtasPerSm1, kCtas8PerSm1) * 8 <= kPartsOfSlots * 256 && 2 * std::max(kCtasPerSm2, kCtas8PerSm2) * 16 <= kPartsOfSlots * 256,
+              "partial results of the few-rows kernel");
 static int64_t scratch_rows() { return (int64_t)kPartsOfSlots * sm_count() * 256; }
 
 int64_t b200_paged_attention_scratch_bytes(void) {
@@ -751,7 +756,7 @@ static int paged_attention(const char* who, const B200PagedCache* cache, const B
   if (!a->q || !a->out || !aligned16(a->q) || !aligned16(a->out)) return fail(B200_EINVAL, "%s: q and out must be non-null and 16-byte aligned", who);
   if (!scratch || !aligned16(scratch)) return fail(B200_EINVAL, "%s: scratch must be non-null and 16-byte aligned", who);
   if ((rc = ensure_device())) return rc;
-  if (scratch_bytes < b200_paged_attention_scratch_bytes() || sm_count() * kCtasPerSm1 > kFewCounters)
+  if (scratch_bytes < b200_paged_attention_scratch_bytes() || sm_count() * std::max(kCtasPerSm1, kCtas8PerSm1) > kFewCounters)
     return fail(B200_EINVAL, "%s: scratch of %lld bytes is less than b200_paged_attention_scratch_bytes()", who, (long long)scratch_bytes);
   p.q = a->q;
   p.out = a->out;

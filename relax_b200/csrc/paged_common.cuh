@@ -155,7 +155,11 @@ struct PromptWords {
 };
 static_assert(kFewCounters * 4 + kCutTiles * 8 + sizeof(PromptWords) <= B200_PAGED_ZEROED_BYTES, "the counters");
 
-// Two e4m3 codes (the low one first) as fp16 values, which hold them exactly.
+// Four e4m3 codes (the low ones first) as fp16 values, which hold them exactly.
+__device__ __forceinline__ void e4m3_to_half4(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}" : "=r"(lo), "=r"(hi) : "r"(codes));
+}
+// Two of them.
 __device__ __forceinline__ uint32_t e4m3_to_half2(uint32_t codes) {
   uint32_t r;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)codes));
