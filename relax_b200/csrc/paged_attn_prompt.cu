@@ -58,8 +58,8 @@ constexpr int kWorks = 2;                      // work descriptors in flight
 constexpr int kKept = 64;                      // sequences whose sizes the scheduling warp keeps
 constexpr uint64_t kWaitNs = 4000000000ull;
 constexpr int kRaw = 2;                        // blocks of codes in flight
-// 128 x 72 + 256 x 216 = 384 x 168; 256 x 48 + 256 x 208 = 512 x 128
-constexpr int kAuxRegs = kBytes ? 48 : 72, kRowRegs = kBytes ? 208 : 216, kLaunchRegs = kBytes ? 128 : 168;
+// 128 x 72 + 256 x 216 = 384 x 168; 256 x 40 + 256 x 216 = 512 x 128
+constexpr int kAuxRegs = kBytes ? 40 : 72, kRowRegs = 216, kLaunchRegs = kBytes ? 128 : 168;
 __device__ int g_prompt_error = 0;
 
 struct PromptParams {
@@ -703,40 +703,45 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
               ok = false;
               break;
             }
-            // 16 codes a lane and step: a token is D / 16 lanes, 16 tokens D / 32 steps
-            constexpr int kLanes = D / 16;
-            const uint4* codes = reinterpret_cast<const uint4*>(sm.raw[raw]) + lane;
-            const int piece = lane % kLanes;                   // dims 16 piece .. + 15: chunks 2 (piece & 3), + 1 of half piece / 4
-            unsigned char* to = sm.ring[slot] + (piece >> 2) * kHalfBytes;
-            const int flip = piece >> 2 & 1;                   // (which of its two chunks first: the halves' banks are the same)
+            // 16 codes a lane and step, 16 tokens D / 32 steps.  Lanes of four have 64 codes of a token; where a token has two such halves, neighbours
+            // of eight lanes have one half of a token and the other half of the next: the banks of all eight are different as they read and as
+            // they write (chunks of 16 bytes, 2 c and 2 c + 1, swizzled by the token).
+            const int half = D == 128 ? (lane >> 2 ^ lane >> 3) & 1 : 0;
+            const int token0 = D == 128 ? (lane >> 2 & 1) + 2 * (lane >> 4) : lane >> 2, chunk = 2 * (lane & 3);
+            const unsigned char* codes = sm.raw[raw] + token0 * D + half * 64 + (lane & 3) * 16;
+            unsigned char* to = sm.ring[slot] + half * kHalfBytes + token0 * 128;
+            constexpr int kStep = 512 / D;                     // tokens of a step
 #pragma unroll
-            for (int g = turner * (kBlock / 16 / kTurners); g < (turner + 1) * (kBlock / 16 / kTurners); ++g) {
-              const __half2 by = __half2half2(__shfl_sync(0xffffffffu, scale, 8 * kv + g));
+            for (int g = 0; g < kBlock / 16 / kTurners; ++g) {
+              const int group = turner * (kBlock / 16 / kTurners) + g;
+              const __half2 by = __half2half2(__shfl_sync(0xffffffffu, scale, 8 * kv + group));
               uint4 c[D / 32];
 #pragma unroll
-              for (int i = 0; i < D / 32; ++i) c[i] = codes[(g * (D / 32) + i) * 32];
+              for (int i = 0; i < D / 32; ++i) c[i] = *reinterpret_cast<const uint4*>(codes + (group * 16 + i * kStep) * D);
 #pragma unroll
               for (int i = 0; i < D / 32; ++i) {
-                const int token = (g * (D / 32) + i) * (32 / kLanes) + lane / kLanes;
+                const int token = group * 16 + i * kStep;      // (and token0)
                 const uint32_t words[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
                 uint32_t v[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                  const uint32_t two = e4m3_to_half2(k & 1 ? words[k / 2] >> 16 : words[k / 2] & 0xffffu);
-                  const __half2 value = __hmul2(*reinterpret_cast<const __half2*>(&two), by);
-                  v[k] = *reinterpret_cast<const uint32_t*>(&value);
+                for (int k = 0; k < 4; ++k) {
+                  e4m3_to_half4(words[k], v[2 * k], v[2 * k + 1]);
+#pragma unroll
+                  for (int o = 0; o < 2; ++o) {
+                    const __half2 value = __hmul2(*reinterpret_cast<const __half2*>(&v[2 * k + o]), by);
+                    v[2 * k + o] = *reinterpret_cast<const uint32_t*>(&value);
+                  }
                 }
                 if (kv && !whole) {
-                  const int at = from + token;
+                  const int at = from + token + token0;
                   if (!(at < range.pre || (at >= range.low && at < range.high)))
 #pragma unroll
                     for (int k = 0; k < 8; ++k) v[k] = 0;
                 }
                 unsigned char* row = to + token * 128;
-                const int chunk = 2 * (piece & 3);
-                const uint4 lo = make_uint4(v[0], v[1], v[2], v[3]), hi = make_uint4(v[4], v[5], v[6], v[7]);
-                *reinterpret_cast<uint4*>(row + (((chunk + flip) ^ (token & 7)) << 4)) = flip ? hi : lo;
-                *reinterpret_cast<uint4*>(row + (((chunk + 1 - flip) ^ (token & 7)) << 4)) = flip ? lo : hi;
+                const int flip = (token + token0) & 7;
+                *reinterpret_cast<uint4*>(row + ((chunk ^ flip) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ flip) << 4)) = make_uint4(v[4], v[5], v[6], v[7]);
               }
             }
             fence_proxy_async_smem();

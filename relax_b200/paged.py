@@ -3,9 +3,12 @@ log probabilities of what was chosen.
 
 What runs between the quantised matmuls is this library's: norm, SwiGLU and embedding as in :mod:`relax_b200.decoder`; rotary positions and
 the append to the pages, attention over the pages, log probabilities (:mod:`relax_b200.ops`).  Key heads may be fewer than query heads,
-sequences have lengths of their own, and a call takes any mixture of prompts, parts of prompts and single tokens.
+sequences have lengths of their own, and a call takes any mixture of prompts, parts of prompts and single tokens.  Keys and values are held in 16
+bits or in 8 (``cache_bits``).  :meth:`PagedDecoder.sample` draws tokens without the host between them: pages and rows planned, tokens drawn on the
+device, a step one captured graph.
 
     python -m relax_b200.paged --layers 4 --tokens 16        # random weights: two prompts, greedy tokens and their log probabilities
+    python -m relax_b200.paged --cache-bits 8 --temperature 0.8 --top-k 50 --top-p 0.9
 """
 from __future__ import annotations
 
@@ -36,11 +39,14 @@ class PagedConfig:
     page_size: int = 16
     window: int = 0                    # tokens a row sees, itself among them (0: all before it)
     cap: float = 0.0                   # of the attention scores (0: none)
+    cache_bits: int = 16               # of a key's or value's number in the pages; 8: e4m3 with a scale for 16 tokens of a head
     scaling: dict | None = None        # see rope_tables
 
     def __post_init__(self):
         if self.heads % self.kv_heads or self.head_dim not in (64, 128):
             raise ValueError("heads is a multiple of kv_heads, head_dim is 64 or 128")
+        if self.cache_bits not in (8, 16):
+            raise ValueError(f"cache_bits is 8 or 16, got {self.cache_bits}")
 
 
 def rope_tables(positions: int, rotary: int, theta: float = 10000.0, scaling: dict | None = None, device="cuda"):
@@ -87,6 +93,10 @@ class PagedCache:
         shape = (pages, kv_heads, page_size, head_dim)
         self.k = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(layers)]
         self.v = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(layers)]
+        self.scales = [{}] * layers             # what the operators take beside the pages
+        if dtype is torch.float8_e4m3fn:
+            blocks = (pages, kv_heads, page_size // 16)
+            self.scales = [{n: torch.ones(blocks, dtype=torch.float16, device=device) for n in ("k_scales", "v_scales")} for _ in range(layers)]
         self.max_tokens, self.width = max_tokens, -(-max_tokens // page_size)
         self.table_host = np.full((batch, self.width), -1, np.int32)
         self.lengths_host = np.zeros(batch, np.int32)
@@ -155,7 +165,8 @@ class PagedDecoder:
         self.device = torch.device(device)
         self.L = _lib.lib()
         pages = batch * -(-max_tokens // cfg.page_size) if pages is None else pages
-        self.cache = PagedCache(len(layers), cfg.kv_heads, cfg.head_dim, cfg.page_size, pages, batch, max_tokens, device=device)
+        self.cache = PagedCache(len(layers), cfg.kv_heads, cfg.head_dim, cfg.page_size, pages, batch, max_tokens,
+                                dtype=torch.float16 if cfg.cache_bits == 16 else torch.float8_e4m3fn, device=device)
         self.cos, self.sin = rope_tables(max_tokens, cfg.rotary, cfg.theta, cfg.scaling, device)
 
     def _stream(self):
@@ -187,29 +198,33 @@ class PagedDecoder:
             raise
 
     def _forward(self, seqs, ids, counts, every: bool) -> torch.Tensor:
-        cfg = self.cfg
         with torch.cuda.device(self.device):
             table, lengths = self.cache.tables(seqs)
             ids = torch.tensor(ids, dtype=torch.int32, device=self.device)
-            T, H, f16 = ids.shape[0], cfg.hidden, dict(dtype=torch.float16, device=self.device)
             longest = max(counts)
             starts = None if longest == 1 else torch.tensor(np.concatenate([[0], np.cumsum(counts)]), dtype=torch.int32, device=self.device)
-            x, h, act = torch.empty((T, H), **f16), torch.empty((T, H), **f16), torch.empty((T, cfg.inter), **f16)
-            _lib.check(self.L.b200_embed_rows(self.embed.data_ptr(), ids.data_ptr(), x.data_ptr(), T, H, self.embed.shape[0], self._stream()))
-            delta = None
-            for i, w in enumerate(self.layers):
-                qkv = ops.q4f16_matmul(self._norm(x, delta, w["norm1"], h), *w["qkv"])
-                q = ops.paged_rope_append(qkv, self.cos, self.sin, self.cache.k[i], self.cache.v[i], table, lengths, starts=starts,
-                                          interleaved=cfg.interleaved)
-                a = ops.paged_attention(q, self.cache.k[i], self.cache.v[i], table, lengths, starts=starts, max_query=longest, window=cfg.window,
-                                        cap=cfg.cap)
-                delta = ops.q4f16_matmul(a.view(T, -1), *w["o"])
-                gu = ops.q4f16_matmul(self._norm(x, delta, w["norm2"], h), *w["gu"])
-                _lib.check(self.L.b200_silu_mul(gu.data_ptr(), act.data_ptr(), T, cfg.inter, self._stream()))
-                delta = ops.q4f16_matmul(act, *w["down"])
-            self._norm(x, delta, self.final_norm, h)
+            h = self._rows(ids, table, lengths, starts, longest)
             rows = h if every else h[torch.tensor(np.cumsum(counts) - 1, device=self.device)]
             return self._head(rows.contiguous())
+
+    def _rows(self, ids, table, lengths, starts, longest: int, scratch=None) -> torch.Tensor:
+        """The tokens `ids` (on the device) through all layers, the last norm included."""
+        cfg = self.cfg
+        T, H, f16 = ids.shape[0], cfg.hidden, dict(dtype=torch.float16, device=self.device)
+        x, h, act = torch.empty((T, H), **f16), torch.empty((T, H), **f16), torch.empty((T, cfg.inter), **f16)
+        _lib.check(self.L.b200_embed_rows(self.embed.data_ptr(), ids.data_ptr(), x.data_ptr(), T, H, self.embed.shape[0], self._stream()))
+        delta = None
+        for i, w in enumerate(self.layers):
+            pages = (self.cache.k[i], self.cache.v[i], table, lengths)
+            qkv = ops.q4f16_matmul(self._norm(x, delta, w["norm1"], h), *w["qkv"])
+            q = ops.paged_rope_append(qkv, self.cos, self.sin, *pages, starts=starts, interleaved=cfg.interleaved, **self.cache.scales[i])
+            a = ops.paged_attention(q, *pages, starts=starts, max_query=longest, window=cfg.window, cap=cfg.cap, scratch=scratch, **self.cache.scales[i])
+            delta = ops.q4f16_matmul(a.view(T, -1), *w["o"])
+            gu = ops.q4f16_matmul(self._norm(x, delta, w["norm2"], h), *w["gu"])
+            _lib.check(self.L.b200_silu_mul(gu.data_ptr(), act.data_ptr(), T, cfg.inter, self._stream()))
+            delta = ops.q4f16_matmul(act, *w["down"])
+        self._norm(x, delta, self.final_norm, h)
+        return h
 
     def _head(self, h):
         rows, vocab = h.shape[0], self.lm_head.shape[0]
@@ -241,6 +256,75 @@ class PagedDecoder:
                 self.cache.release(s)
         return tuple([[step[s] for step in v] for s in seqs] for v in (chosen, logprobs, entropies))
 
+    def sample(self, prompts, new_tokens: int, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seed: int = 0, uniform: torch.Tensor | None = None):
+        """Drawn tokens behind the prompts: (tokens, logarithms of their shares among what could have come), each [sequences][new_tokens].  The
+        settings are those of :func:`relax_b200.ops.sample_tokens`, numbers or tensors of one for each sequence; ``uniform`` (fp32 [new_tokens,
+        sequences]) gives the random numbers, else they come from `seed`.
+
+        Uses places 0 .. of the cache, which have to be empty, and leaves them so: the tables of the call are its own, on the device.  A call that
+        finds no room for all of it raises before it begins."""
+        n, cache = len(prompts), self.cache
+        counts = [len(t) for t in prompts]
+        ids = [operator.index(t) for ts in prompts for t in ts]
+        if n == 0 or min(counts) < 1 or new_tokens < 0:
+            raise ValueError("every prompt has one token at least")
+        if not 0 <= min(ids) <= max(ids) < self.embed.shape[0]:
+            raise ValueError(f"tokens are 0 to {self.embed.shape[0] - 1}, got {min(ids)} to {max(ids)}")
+        if any(cache.length(s) for s in range(n)):
+            raise ValueError("the first places of the cache are in use")
+        if new_tokens == 0:
+            return [[] for _ in prompts], [[] for _ in prompts]
+        longest = max(counts) + new_tokens - 1   # (the last token drawn has no keys)
+        pages = sum(-(-(c + new_tokens - 1) // cache.page_size) for c in counts)
+        if longest > cache.max_tokens:
+            raise ValueError(f"a sequence of {longest} tokens: at most {cache.max_tokens}")
+        if pages > len(cache.free):
+            raise MemoryError(f"{pages} pages wanted, {len(cache.free)} free")
+        with torch.cuda.device(self.device):
+            i32 = dict(dtype=torch.int32, device=self.device)
+            if uniform is None:
+                uniform = torch.rand((new_tokens, n), device=self.device, generator=torch.Generator(device=self.device).manual_seed(seed))
+            elif uniform.shape != (new_tokens, n) or uniform.dtype is not torch.float32 or uniform.device != self.embed.device or not uniform.is_contiguous():
+                raise ValueError(f"uniform is a contiguous fp32 tensor {(new_tokens, n)} on {self.embed.device}")
+            how = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+            table = torch.full((n, -(-longest // cache.page_size)), -1, **i32)
+            free, free_count = torch.tensor(cache.free, **i32), torch.tensor([len(cache.free)], **i32)
+            lengths, ones = torch.zeros(n, **i32), torch.ones(n, **i32)
+            tokens, logprobs = torch.empty((new_tokens, n), **i32), torch.empty((new_tokens, n), dtype=torch.float32, device=self.device)
+
+            def plan(counts, rows):
+                out = ops.paged_plan_buffers(n, rows, self.device)._replace(lengths=lengths, free_count=free_count)
+                return ops.paged_plan(table, lengths, counts, free, free_count, cache.page_size, rows, cache.max_tokens, out=out)
+
+            # the prompts
+            p = plan(torch.tensor(counts, **i32), sum(counts))
+            h = self._rows(torch.tensor(ids, **i32), table, lengths, p.starts if max(counts) > 1 else None, max(counts))
+            drawn = ops.sample_tokens(self._head(h[p.starts[1:].long() - 1]), uniform[0], **how)
+            tokens[0], logprobs[0] = drawn.token, drawn.logprob
+            # the tokens behind them: what a step reads and writes lies where the graph expects it
+            token, u, scratch = drawn.token, torch.empty(n, dtype=torch.float32, device=self.device), ops.paged_attention_scratch(self.device)
+
+            def step():
+                plan(ones, n)
+                drawn = ops.sample_tokens(self._head(self._rows(token, table, lengths, None, 1, scratch)), u, **how)
+                token.copy_(drawn.token)
+                return drawn.logprob
+
+            graph = None
+            for i in range(1, new_tokens):
+                u.copy_(uniform[i])
+                if graph is None and 2 <= i < new_tokens - 1:            # (the first step prepares what a capture may not)
+                    graph = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(graph):
+                        held = step()
+                if graph is None:
+                    logprobs[i] = step()
+                else:
+                    graph.replay()
+                    logprobs[i] = held
+                tokens[i] = token
+            return tokens.t().tolist(), logprobs.t().tolist()
+
     def score(self, seq: int, tokens):
         """Log probability of every token of a text but its first, given those before it (sequence place `seq`, which has to be empty)."""
         if self.cache.length(seq):
@@ -254,16 +338,27 @@ class PagedDecoder:
 
 
 def main(argv=None):
-    ap = argparse.ArgumentParser(description="Greedy tokens of a random q4f16 model over a paged cache")
-    for name, value in (("layers", 4), ("hidden", 1024), ("heads", 8), ("kv-heads", 2), ("inter", 2816), ("vocab", 32000), ("tokens", 16), ("page-size", 16)):
+    ap = argparse.ArgumentParser(description="Tokens of a random q4f16 model over a paged cache")
+    for name, value in (("layers", 4), ("hidden", 1024), ("heads", 8), ("kv-heads", 2), ("inter", 2816), ("vocab", 32000), ("tokens", 16), ("page-size", 16),
+                        ("cache-bits", 16), ("top-k", 0), ("seed", 0)):
         ap.add_argument(f"--{name}", type=int, default=value)
+    for name, value in (("temperature", 0.0), ("top-p", 1.0), ("min-p", 0.0)):
+        ap.add_argument(f"--{name}", type=float, default=value, help="drawn tokens, with a temperature above 0" if name == "temperature" else None)
     a = ap.parse_args(argv)
-    cfg = PagedConfig(hidden=a.hidden, heads=a.heads, kv_heads=a.kv_heads, inter=a.inter, layers=a.layers, vocab=a.vocab, page_size=a.page_size)
+    cfg = PagedConfig(hidden=a.hidden, heads=a.heads, kv_heads=a.kv_heads, inter=a.inter, layers=a.layers, vocab=a.vocab, page_size=a.page_size,
+                      cache_bits=a.cache_bits)
     g = torch.Generator(device="cuda").manual_seed(1)
     embed = torch.randn((cfg.vocab, cfg.hidden), dtype=torch.float16, device="cuda", generator=g) * 0.02
     model = PagedDecoder(cfg, [synth_layer(cfg, i) for i in range(cfg.layers)], embed, torch.ones(cfg.hidden, dtype=torch.float16, device="cuda"), embed,
                          batch=2, max_tokens=256)
     prompts = [list(range(5, 42)), [7, 9, 11]]
+    if a.temperature > 0:
+        drawn = model.sample(prompts, a.tokens, a.temperature, a.top_k, a.top_p, a.min_p, a.seed)
+        for prompt, tokens, logprobs in zip(prompts, *drawn):
+            print(f"prompt of {len(prompt)}:")
+            for t, p in zip(tokens, logprobs):
+                print(f"  {t:6d}  log p {p:8.4f}")
+        return
     for prompt, tokens, logprobs, entropies in zip(prompts, *model.generate(prompts, a.tokens)):
         print(f"prompt of {len(prompt)}:")
         for t, p, e in zip(tokens, logprobs, entropies):
