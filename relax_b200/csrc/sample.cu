@@ -14,7 +14,8 @@
 // Passes over the row (a CTA of 512 threads, few rows over a cluster; all passes but the first out of L2):
 //   1  the maximum
 //   2  with top_k or top_p: how many entries lie in each of 2048 bins of T / 92 below the maximum (n, but from fp32)
-//   3  top_k: the bin with the border is known; its entries are put in order.  top_p: the counts times the bins' weights tell the bin but
+//   3  top_k: a list of the k largest and a few more, bounded by the threads' maxima (without pass 2) or by the bins, in order; all the rest happens
+//      on it.  Where k is more than a list holds, the bin with the border is known and its entries are put in order.  top_p: the counts times the bins' weights tell the bin but
 //      for an error in the fourth digit; the exact sum above that bin and its neighbours, and their entries in order, find the border or say
 //      on which side it lies.  Where a bin holds more entries than the list (nearly equal logits) the border is found by bisection of the keys.
 //   4  the sum of what stays, a segment a warp; then the segment in which the random number falls, a vector a thread
@@ -34,6 +35,7 @@ constexpr int kFew = 512, kMany = 256;          // threads of a CTA where there 
 constexpr int kMaxCluster = 8;
 constexpr int kBins = 2048;                     // 22 nats; counted again where that is not enough:
 constexpr int kWide = 32;                       // bins so many times as wide, 710 nats
+constexpr int kFewEnough = 600;                 // of 4 x 256 maxima 905 values, of 4 x 512 711: they fit the list
 constexpr int kAhead = 2;                       // vectors under way while one is worked on
 constexpr int kList = 1024;                     // entries of the bins around a border
 constexpr int kTableLog2 = 6, kTable = 1 << kTableLog2;                  // 2^(j / 64)
@@ -277,14 +279,16 @@ sample_tokens_kernel(const SampleParams p) {
     asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(b));
     return a;
   };
-  float m = -INFINITY;
+  float own_most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};       // of four sets of this thread's vectors
   for (int j = from + lane; j < to; j += 128) {
     uint4 v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = x.load(min(j + 32 * i, to - 1));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m = join(m, x.highest(v[i]));
+    for (int i = 0; i < 4; ++i)
+      if (j + 32 * i < to) own_most[i] = join(own_most[i], x.highest(v[i]));       // (a vector is one set's)
   }
+  float m = join(join(own_most[0], own_most[1]), join(own_most[2], own_most[3]));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = join(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (lane == 0) sm_warp[warp] = m;
@@ -454,10 +458,8 @@ sample_tokens_kernel(const SampleParams p) {
       if (n < kList) sm_own[own_turn][n] = entry_of(v, at);
     }
   };
-  // Without sums: the entries of bins [first, last], those of the counts.
-  auto gather = [&](int first, int last) {
-    const float from_bin = kBase + (float)first, to_bin = last == kBins - 1 ? INFINITY : kBase + (float)last;
-    const T reach = edge(last + 2), none = T(INFINITY);         // (a bin to spare)
+  // Without sums: the entries from `reach` on for which `also` holds.
+  auto gather_from = [&](T reach, auto also) {
     if (tid == 0) sm_count = 0;
     __syncthreads();
 #pragma unroll 1
@@ -467,14 +469,57 @@ sample_tokens_kernel(const SampleParams p) {
       for (int i = 0; i < 4; ++i) v[i] = x.load(min(j + 32 * i, to - 1));
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (j + 32 * i < to)
-          push(x.between(v[i], reach, none), x.first(j + 32 * i), [&](float v, int) {
-            const float bin = bin_of(v);
-            return bin >= from_bin && bin <= to_bin && v >= low;
-          });
+        if (j + 32 * i < to) push(x.between(v[i], reach, T(INFINITY)), x.first(j + 32 * i), also);
     }
     __syncthreads();
     return put_in_order(exchange({0., 0., sm_count, 0}));
+  };
+  // The entries of bins [first, last], those of the counts.
+  auto gather = [&](int first, int last) {
+    const float from_bin = kBase + (float)first, to_bin = last == kBins - 1 ? INFINITY : kBase + (float)last;
+    return gather_from(edge(last + 2), [&](float v, int) {               // (a bin to spare)
+      const float bin = bin_of(v);
+      return bin >= from_bin && bin <= to_bin && v >= low;
+    });
+  };
+  // The k largest, and some more: the k-th largest of the maxima that the threads have of sets of vectors bounds the k-th largest value from below.
+  // It is found to a part of the maxima's range.  Of n maxima, values from there on are about -n log(1 - k / n).
+  auto gather_few = [&](int k) {
+    float lo = INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (own_most[i] >= low) lo = fminf(lo, own_most[i]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    if (lane == 0) sm_extreme[warp].x = lo;
+    for (int i = tid; i < kBuckets; i += kThreads) sm_bucket[i] = 0;
+    if (tid == 0) sm_index = kBuckets;          // (fewer maxima than k: everything)
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) lo = fminf(lo, sm_extreme[w].x);
+    const float per = m > lo ? fminf((kBuckets - 1) / (m - lo), 1e30f) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (own_most[i] >= low) atomicAdd(&sm_bucket[(int)fminf((m - own_most[i]) * per, kBuckets - 1.f)], 1);
+    __syncthreads();
+    const int2 mine = reinterpret_cast<const int2*>(sm_bucket)[tid];
+    int upto = mine.x + mine.y;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) sm_warp_n[warp] = upto;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w)
+      if (w < warp) upto += sm_warp_n[w];
+    const int before = upto - mine.x - mine.y;
+    if (before < k && upto >= k) sm_index = 2 * tid + (before + mine.x < k);
+    __syncthreads();
+    const int bucket = sm_index;
+    return gather_from(x.up(bucket >= kBuckets - 1 || !(per > 0.f) ? low : fmaxf(m - ((float)bucket + 1.01f) / per, low)),
+                       [&](float v, int) { return v >= low; });
   };
   // Sums up to every thread's two entries, in order; the sum of all.
   auto scan = [&](const double (&w)[kList / kThreads], double& before) {
@@ -743,67 +788,71 @@ sample_tokens_kernel(const SampleParams p) {
       if (has_k && want_k < all) find_k(bin, more);
       else if (has_p && !has_k) find_p(bin, more);
     };
-    find();
-    if (bin == kBins - 1) {                     // further away than the bins reach
-      unit = kWide;
-      bins_per *= 1.f / kWide;
+    // ---- 3, top_k: a list of all that can stay --------------------------------------------------------------------------------------------
+    bool on_list = has_k && want_k <= kFewEnough / ranks && gather_few(want_k);
+    if (!on_list) {
       find();
+      if (bin == kBins - 1) {                   // further away than the bins reach
+        unit = kWide;
+        bins_per *= 1.f / kWide;
+        find();
+      }
+      on_list = has_k && want_k < all && want_k <= kList && gather(0, bin);
     }
-    u64 border_k = all_of_weight;
-    if (has_k && want_k < all) {
-      // ---- 3, top_k ----------------------------------------------------------------------------------------------------------------------
-      const int above = more;
-      if (want_k <= kList && gather(0, bin)) {
-        // All that can stay is on the list, and everybody has it.
-        int stay = min(want_k, listed);
-        double w[kEach], before_w;
+    if (on_list) {
+      // All that can stay is on the list, and everybody has it.
+      int stay = min(want_k, listed);
+      double w[kEach], before_w;
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) w[i] = tid * kEach + i < stay ? weight(value_of(sm_list[tid * kEach + i])) : 0.;
-        if (has_p) {
-          const double need = (double)want_p * scan(w, before_w);
-#pragma unroll
-          for (int i = 0; i < kEach; ++i) {
-            before_w += w[i];
-            if (tid * kEach + i < stay && before_w >= need) {
-              atomicMin(&sm_index, tid * kEach + i);
-              break;
-            }
-          }
-          __syncthreads();
-          stay = min(stay, sm_index == 0x7fffffff ? stay : sm_index + 1);
-        }
-        // those below min_p's border
-        if (tid == 0) sm_count = stay;
-        __syncthreads();
-        for (int i = tid; i < stay; i += kThreads)
-          if (sm_list[i] < border) atomicMin(&sm_count, i);
-        __syncthreads();
-        stay = max(sm_count, 1);
-        // in the order of the index
-        const float per = (float)kBuckets / p.V;
-        order(stay, [](u64 e) { return (uint32_t)e; }, [&](u64 e) { return min((int)((float)~(uint32_t)e * per), kBuckets - 1); });
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) w[i] = tid * kEach + i < stay ? weight(value_of(sm_list[tid * kEach + i])) : 0.;
-        const double whole = scan(w, before_w);
-        const float u = p.uniform[row];
-        const double goal = u > 0.f ? fmin((double)u, 1.) * whole : 0.;
+      for (int i = 0; i < kEach; ++i) w[i] = tid * kEach + i < stay ? weight(value_of(sm_list[tid * kEach + i])) : 0.;
+      if (has_p) {
+        const double need = (double)want_p * scan(w, before_w);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
           before_w += w[i];
-          if (tid * kEach + i < stay && before_w > goal) {
+          if (tid * kEach + i < stay && before_w >= need) {
             atomicMin(&sm_index, tid * kEach + i);
             break;
           }
         }
         __syncthreads();
-        if (writes) {
-          const u64 e = sm_list[min(sm_index, stay - 1)];
-          p.token[row] = (int)~(uint32_t)e;
-          if (p.logprob) p.logprob[row] = (float)log(weight(value_of(e)) / whole);
-        }
-        meet();                                 // (others may still read this CTA's part of the list)
-        return;
+        stay = min(stay, sm_index == 0x7fffffff ? stay : sm_index + 1);
       }
+      // those below min_p's border
+      if (tid == 0) sm_count = stay;
+      __syncthreads();
+      for (int i = tid; i < stay; i += kThreads)
+        if (sm_list[i] < border) atomicMin(&sm_count, i);
+      __syncthreads();
+      stay = max(sm_count, 1);
+      // in the order of the index
+      const float per = (float)kBuckets / p.V;
+      order(stay, [](u64 e) { return (uint32_t)e; }, [&](u64 e) { return min((int)((float)~(uint32_t)e * per), kBuckets - 1); });
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) w[i] = tid * kEach + i < stay ? weight(value_of(sm_list[tid * kEach + i])) : 0.;
+      const double whole = scan(w, before_w);
+      const float u = p.uniform[row];
+      const double goal = u > 0.f ? fmin((double)u, 1.) * whole : 0.;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        before_w += w[i];
+        if (tid * kEach + i < stay && before_w > goal) {
+          atomicMin(&sm_index, tid * kEach + i);
+          break;
+        }
+      }
+      __syncthreads();
+      if (writes) {
+        const u64 e = sm_list[min(sm_index, stay - 1)];
+        p.token[row] = (int)~(uint32_t)e;
+        if (p.logprob) p.logprob[row] = (float)log(weight(value_of(e)) / whole);
+      }
+      meet();                                 // (others may still read this CTA's part of the list)
+      return;
+    }
+    u64 border_k = all_of_weight;
+    if (has_k && want_k < all) {                // more than the list holds: the last one that stays, by its bin
+      const int above = more;
       if (gather(bin, bin)) border_k = sm_list[want_k - above - 1];
       else border_k = bisect(all_of_weight, (double)want_k, [](float) { return 1.; });
       __syncthreads();
