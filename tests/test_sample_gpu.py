@@ -158,3 +158,12 @@ def test_refusals(cuda_lib):
         ops.sample_tokens(x.expand(3, 100).as_strided((3, 100), (50, 1)), u)
     empty = ops.sample_tokens(x[:0], u[:0])
     assert empty.token.shape == empty.logprob.shape == (0,)
+
+
+@pytest.mark.parametrize("V", (3000, 40000, 152000))
+@pytest.mark.parametrize("top_p,min_p", ((0.95, 0.001), (0.95, 0.02), (0.5, 0.0005), (0.9, 0.15), (0.999, 1e-6), (0.3, 1.0)))
+@pytest.mark.parametrize("top_k", (0, 700, 2500))
+def test_whichever_border_is_the_higher_one(cuda_lib, V, top_p, min_p, top_k):
+    """top_p's and min_p's borders on either side of each other, and near each other, with all of top_k's ways."""
+    check(*logits_of(5, V, "fp32", seed=V + top_k), top_p=top_p, min_p=min_p, top_k=top_k)
+    check(*logits_of(3, V, "bf16", seed=V + top_k), top_p=top_p, min_p=min_p, top_k=top_k, temperature=0.4)
