@@ -20,6 +20,10 @@
 // What bounds it: HBM for long caches (131000 tokens of 8 key heads, 537 MB, 90 us: 6.0 TB/s, 0.91 of a copy; 512 sequences of 37 to 2047
 // tokens 182 us: 5.9; 64 of them, 135 MB, 31 us: 4.4); latency for short ones (32 heads at 2011, 33 MB, 13.6 us: 2 until the shares are
 // known, 7 for two or three units a warp, 4 for the joins).  Before, chunks of equal length as CTAs of their own took 157, 45 and 17.5 us.
+// Pages of 8 bits: half the bytes and as many instructions.  131000 tokens of 8 key heads, 269 MB, 60 us (4.5 TB/s); 64 ragged sequences 24; 32 heads at
+// 2011 12.6.  One unit a step and four CTAs an SM (128 registers) take as long for the long cache as two units and three CTAs, or two steps' loads
+// ahead of the products, and less for short ones (15.0, 25.6); asking L2 for units three steps ahead took 68.  With 9 to 16 rows a third CTA spills
+// (131000 tokens of 2 key heads 100 us instead of 69).
 #include <algorithm>
 #include <type_traits>
 

@@ -31,6 +31,9 @@
 // halves of N = 64 with a buffer each 523 (412 instead of 342 without the softmax).
 // Pages of 8 bits (kBytes; a translation unit of its own, paged_attn_prompt8.cu): TMA brings the codes of a block into a ring of their own, and
 // four more warps (12..15) make fp16 tiles of them, code times the scale of its 16 tokens, in the ring from which the products are made as always.
+// That is 64 KB more through shared memory for a block, beside products that read 128 bytes a clock of it: 2048 tokens of 32 heads 58 us, 512 on
+// 30000 404 with the cap, 281 without (16 bits 51, 334, 223 in the same row of calls).  With one warp for the tiles 75 and 573: 512 conversions a
+// block and lane, one after the other.
 #include <atomic>
 #include <type_traits>
 

@@ -11,14 +11,21 @@
 // exact, so that sums of equal largest logits are whole numbers).  Nine fp64 operations an entry and one a sum: the GPU has half as many fp64
 // units as fp32 ones, and a pass that took n and the exponents through whole numbers waited for the issue of 49 instructions an entry.
 //
-// Passes over the row (a CTA of 512 threads, few rows over a cluster; all passes but the first out of L2):
+// Passes over the row, out of L2 but for the first:
 //   1  the maximum
 //   2  with top_k or top_p: how many entries lie in each of 2048 bins of T / 92 below the maximum (n, but from fp32)
-//   3  top_k: a list of the k largest and a few more, bounded by the threads' maxima (without pass 2) or by the bins, in order; all the rest happens
-//      on it.  Where k is more than a list holds, the bin with the border is known and its entries are put in order.  top_p: the counts times the bins' weights tell the bin but
-//      for an error in the fourth digit; the exact sum above that bin and its neighbours, and their entries in order, find the border or say
-//      on which side it lies.  Where a bin holds more entries than the list (nearly equal logits) the border is found by bisection of the keys.
-//   4  the sum of what stays, a segment a warp; then the segment in which the random number falls, a vector a thread
+//   3  top_k: a list of the k largest and a few more, bounded by the threads' maxima (without pass 2) or by the bins, in order; all the rest
+//      happens on it.  Where k is more than a list holds, the bin with the border is known and its entries are put in order.
+//      top_p: the counts times the bins' weights tell the bin but for an error in the fourth digit; the exact sum in front of it, and its entries
+//      in order, find the border or say on which side it lies.  Where a bin holds more entries than the list (nearly equal logits) the border is
+//      found by bisection of the keys, 64 passes.
+//   4  the sum of what stays, a segment a warp (top_p's pass has it); then the segment in which the random number falls, a vector a thread
+// A row is a CTA of 512 threads, or of 256 with four on an SM where there are many rows, or a cluster of CTAs that tell each other their sums.
+//
+// What bounds it: latency for few rows (one of 32000, top_k 50 and top_p 0.9: 12.1 us; before, with all passes apart, 58); the issue of whole-number
+// and comparing instructions, which have half the rate of others, for many (512 rows of 32000 fp32, top_p and min_p: 72 us, 0.9 TB/s, of which
+// the counts' additions in shared memory take 8 and the weights 16; 2048 rows of fp16: 39 without weights, 100 with all of them, 69 with top_k 50, 200
+// with top_p).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -217,9 +224,11 @@ sample_tokens_kernel(const SampleParams p) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int ranks = gridDim.x, rank = blockIdx.x;
   const int64_t row = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
-  for (int i = tid; i < kTable * kCopies; i += kThreads) {
-    const double w = exp2((double)(i / kCopies) / kTable);
-    sm_table[i] = __hiloint2double(__double2hiint(w) - ((i / kCopies) << (20 - kTableLog2)), __double2loint(w));
+  if (tid < kTable) {
+    const double w = exp2((double)tid / kTable);
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i)
+      sm_table[tid * kCopies + i] = __hiloint2double(__double2hiint(w) - (tid << (20 - kTableLog2)), __double2loint(w));
   }
   ptx::pdl_wait();
   ptx::pdl_launch_dependents();
