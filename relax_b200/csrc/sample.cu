@@ -236,6 +236,7 @@ sample_tokens_kernel(const SampleParams p) {
   if (ranks > 1) ptx::cluster_arrive_relaxed(); // (every CTA of the cluster runs before anything is stored in it)
   auto meet = [&]() {                           // all threads of the row
     if (ranks > 1) {
+      __syncwarp();                             // (the barrier wants whole warps)
       ptx::cluster_arrive();
       ptx::cluster_wait();
     } else {
