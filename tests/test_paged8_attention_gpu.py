@@ -141,3 +141,40 @@ def test_refusals(cuda_lib):
         flat = torch.zeros((3, 2 * 16 * 128 + 8), dtype=torch.uint8, device="cuda")
         pages = flat[:, : 2 * 16 * 128].view(3, 2, 16, 128).view(torch.float8_e4m3fn)
         ops.paged_attention(**{**good, "k_pages": pages, "v_pages": pages, "k_scales": case.k_scales[:3].contiguous(), "v_scales": case.k_scales[:3].contiguous()})
+
+
+def test_pages_behind_two_billion_codes(cuda_lib):
+    """Append and attention in the last pages of a pool of 2.2e9 codes: the same bits as in a pool of their own."""
+    kv, page, dim, pages, used = 8, 128, 128, 17000, 3
+    g = torch.Generator(device="cuda").manual_seed(12)
+    qkv = torch.randn((300, (16 + 2 * kv) * dim), device="cuda", generator=g).half()
+    angle = torch.rand((400, dim // 2), device="cuda", generator=g)
+    lengths, starts = torch.tensor([300], dtype=torch.int32, device="cuda"), torch.tensor([0, 300], dtype=torch.int32, device="cuda")
+    got = []
+    for pool in (used, pages):
+        k, v = (torch.zeros((pool, kv, page, dim), dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in "kv")
+        scales = {n: torch.ones((pool, kv, page // 16), dtype=torch.float16, device="cuda") for n in ("k_scales", "v_scales")}
+        table = torch.arange(pool - used, pool, dtype=torch.int32, device="cuda").flip(0)[None].contiguous()
+        q = ops.paged_rope_append(qkv, angle.cos(), angle.sin(), k, v, table, lengths, starts=starts, **scales)
+        many = ops.paged_attention(q, k, v, table, lengths, starts=starts, max_query=300, **scales)
+        few = ops.paged_attention(q[299:].contiguous(), k, v, table, lengths, **scales)
+        got.append((q, many, few, k[-used:].view(torch.uint8).clone(), scales["v_scales"][-used:].clone()))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
+def test_calls_on_two_streams_at_once(cuda_lib):
+    """Attention with a scratch of each stream's own beside plans and sampling on the other: what each gives alone."""
+    case = Case8([1, 40], [700, 200], 8, 2, seed=13)
+    g = torch.Generator(device="cuda").manual_seed(14)
+    logits, u = torch.randn((9, 40000), device="cuda", generator=g), torch.rand(9, device="cuda", generator=g)
+    want = run(case), ops.sample_tokens(logits, u, top_p=0.9)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 3]):
+            got.append((ops.paged_attention(case.q, *case.args(), starts=case.starts, max_query=40, **case.scales()), ops.sample_tokens(logits, u, top_p=0.9)))
+    torch.cuda.synchronize()
+    for a, drawn in got:
+        assert torch.equal(a, want[0]) and torch.equal(drawn.token, want[1].token) and torch.equal(drawn.logprob, want[1].logprob)
