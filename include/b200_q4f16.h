@@ -518,8 +518,8 @@ B200_API int b200_paged_attention(const B200PagedCache* cache, const B200PagedAt
 
 /* ---- the same over pages of 8 bits ---------------------------------------------------------------
  * Pages hold e4m3 codes (strides in codes, multiples of 16), scales fp16 [pages, kv_heads, page_size / 16], one for 16 tokens of a head, all of it contiguous:
- * a value is code * scale.  The descriptor's dtype is that of the rows (q, qkv, results).  A scale is positive, of any block that a
- * row sees; what no token has reached, codes and scales, may be anything.
+ * a value is code * scale.  The descriptor's dtype is that of the rows (q, qkv, results).  A scale of any block that a row sees is
+ * positive and at most 2^7 (a value is a number of fp16); what no token has reached, codes and scales, may be anything.
  *
  * b200_paged8_rope_append: as b200_paged_rope_append, k and v rounded to the rows' type as there, then stored by their block's scale:
  *   need = the smallest power of two by which the block's new tokens are at most 448 in size, from 2^-24 to 2^7

@@ -23,8 +23,8 @@
 // A row is a CTA of 512 threads, or of 256 with four on an SM where there are many rows, or a cluster of CTAs that tell each other their sums.
 //
 // What bounds it: latency for few rows (one of 32000, top_k 50 and top_p 0.9: 12.1 us; before, with all passes apart, 58); the issue of whole-number
-// and comparing instructions, which have half the rate of others, for many (512 rows of 32000 fp32, top_p and min_p: 72 us, 0.9 TB/s, of which
-// the counts' additions in shared memory take 8 and the weights 16; 2048 rows of fp16: 39 without weights, 100 with all of them, 69 with top_k 50, 200
+// and comparing instructions, which have half the rate of others, for many (512 rows of 32000 fp32, top_p and min_p: 72 us, 0.9 TB/s; by the units'
+// rates alone the counts' additions in shared memory would be 8 and the weights' fp64 operations 10 of it; 2048 rows of fp16: 39 without weights, 100 with all of them, 69 with top_k 50, 200
 // with top_p).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
