@@ -346,19 +346,18 @@ sample_tokens_kernel(const SampleParams p) {
     return;
   }
 
-  // (a temperature so low that the next fp32 number below the maximum is out of sight counts as one that just hides it: `offset` keeps its bits)
-  const double top = m, t_eff = fmax((double)temperature, fabs(top) * 1e-11), scale = kLog2e * kTable / t_eff, offset = -top * scale;
+  const double top = m, t_eff = temperature, scale = kLog2e * kTable / t_eff;
   const char* table = reinterpret_cast<const char*>(sm_table + (lane & (kCopies - 1)));
   // The bin of a value, which only grows as the value falls, as a number above 1.5 * 2^23; its low bits count.
   constexpr float kBase = 12582912.f;
   float bins_per = fminf((float)scale, 1e30f);
   int unit = 1;                                 // n of a bin
   auto bin_of = [&](float v) { return fmaf(m - v, bins_per, kBase); };
-  // 2^((x - max) log2(e) / T) = 2^n/64 2^r/64, for values from `low` on.  (A rounding of `offset` is a factor that all weights share.)
+  // 2^((x - max) log2(e) / T) = 2^n/64 2^r/64, for values from `low` on.  The maximum is taken off first, so that its own weight is 1 to the bit.
   auto weight = [&](float v) {
     constexpr double c1 = 0.0108304246963882758, c2 = 0.000058649173078506538, c3 = 2.1173088255274404e-7;
     constexpr double kMagic = 6755399441055744.;         // 1.5 * 2^52: its sum with a number has the nearest whole one in its low bits
-    const double t = fma((double)v, scale, offset), shifted = t + kMagic, r = t - (shifted - kMagic);
+    const double d = (double)v - top, shifted = fma(d, scale, kMagic), r = fma(d, scale, kMagic - shifted);
     const int n = __double2loint(shifted);
     // (multiplications take the other pipe; the table's entries come without their own part of the exponent that n << 14 adds)
     const double of = *reinterpret_cast<const double*>(table + mul(n & (kTable - 1), kCopies * 8));
