@@ -1,14 +1,21 @@
 """Finds an importable TVM with Relax and registers the kernels' packed functions with its FFI."""
 from __future__ import annotations
 
+import os
+
 _tvm = None
 _registered = False
 
 
 def import_tvm():
-    """Returns the tvm module (the tilelang wheel bundles TVM 0.23 and puts it on sys.path)."""
+    """Returns the tvm module (the tilelang wheel bundles TVM 0.23 and puts it on sys.path).
+
+    TVM's thread pool, when first used, would bind the calling thread to half of the machine's cores.  Threads that the program starts later
+    inherit that: torch's, one for every core, would wait for one another on half of them, and a small CPU operator take a hundred times as
+    long.  So the binding is off unless TVM_BIND_THREADS says otherwise."""
     global _tvm
     if _tvm is None:
+        os.environ.setdefault("TVM_BIND_THREADS", "0")
         try:
             import tvm  # noqa: F401
         except ImportError:
