@@ -16,6 +16,7 @@ import argparse
 import dataclasses
 import math
 import operator
+import threading
 
 import numpy as np
 import torch
@@ -101,6 +102,8 @@ class PagedCache:
         self.table_host = np.full((batch, self.width), -1, np.int32)
         self.lengths_host = np.zeros(batch, np.int32)
         self.free = list(range(pages - 1, -1, -1))
+        self.held = set()                       # places of calls that keep their tables on the device
+        self._lock = threading.RLock()          # one call at a time takes pages or gives them back
 
     def length(self, seq: int) -> int:
         """Tokens of a sequence.  (A negative number names no place: it would be another name for one of the last.)"""
@@ -108,28 +111,61 @@ class PagedCache:
             raise IndexError(f"place {seq} of the cache: there are {len(self.lengths_host)}")
         return int(self.lengths_host[seq])
 
+    def _not_held(self, seq: int) -> int:
+        length = self.length(seq)
+        if seq in self.held:
+            raise ValueError(f"place {seq} of the cache is in use by a call that has not returned")
+        return length
+
     def extend(self, seq: int, tokens: int) -> None:
         """Room for `tokens` more of sequence `seq`; raises, and changes nothing, where the table or the pool has none."""
-        length = self.length(seq)
-        have, want = -(-length // self.page_size), -(-(length + tokens) // self.page_size)
-        if tokens < 0 or length + tokens > self.max_tokens:
-            raise ValueError(f"sequence {seq} of {length} tokens cannot grow by {tokens}: at most {self.max_tokens}")
-        if want - have > len(self.free):
-            raise MemoryError(f"{want - have} pages wanted, {len(self.free)} free")
-        for i in range(have, want):
-            self.table_host[seq, i] = self.free.pop()
-        self.lengths_host[seq] += tokens
+        with self._lock:
+            length = self._not_held(seq)
+            have, want = -(-length // self.page_size), -(-(length + tokens) // self.page_size)
+            if tokens < 0 or length + tokens > self.max_tokens:
+                raise ValueError(f"sequence {seq} of {length} tokens cannot grow by {tokens}: at most {self.max_tokens}")
+            if want - have > len(self.free):
+                raise MemoryError(f"{want - have} pages wanted, {len(self.free)} free")
+            for i in range(have, want):
+                self.table_host[seq, i] = self.free.pop()
+            self.lengths_host[seq] += tokens
 
     def shrink(self, seq: int, tokens: int) -> None:
         """Forgets the last `tokens` of a sequence and gives back the pages that only they were in."""
-        have = self.length(seq)
-        keep = have - tokens
-        if not 0 <= keep <= have:
-            raise ValueError(f"sequence {seq} has {have} tokens: {tokens} of them cannot be forgotten")
-        for i in range(-(-keep // self.page_size), -(-have // self.page_size)):
-            self.free.append(int(self.table_host[seq, i]))
-            self.table_host[seq, i] = -1
-        self.lengths_host[seq] = keep
+        with self._lock:
+            have = self._not_held(seq)
+            keep = have - tokens
+            if not 0 <= keep <= have:
+                raise ValueError(f"sequence {seq} has {have} tokens: {tokens} of them cannot be forgotten")
+            for i in range(-(-keep // self.page_size), -(-have // self.page_size)):
+                self.free.append(int(self.table_host[seq, i]))
+                self.table_host[seq, i] = -1
+            self.lengths_host[seq] = keep
+
+    def hold(self, tokens) -> list:
+        """Takes the places 0 .. , which have to be empty, for sequences of up to ``tokens[i]`` each, and pages for all of them, which it returns: for a
+        call whose tables are its own.  Nobody else gets the places or the pages before :meth:`give_back`.  Raises, and changes nothing, where
+        there is no room."""
+        with self._lock:
+            if any([self.length(s) for s in range(len(tokens))]) or not self.held.isdisjoint(range(len(tokens))):
+                raise ValueError("the first places of the cache are in use")
+            if max(tokens) > self.max_tokens:
+                raise ValueError(f"a sequence of {max(tokens)} tokens: at most {self.max_tokens}")
+            pages = sum(-(-n // self.page_size) for n in tokens)
+            if pages > len(self.free):
+                raise MemoryError(f"{pages} pages wanted, {len(self.free)} free")
+            taken = self.free[len(self.free) - pages:]
+            del self.free[len(self.free) - pages:]
+            self.held.update(range(len(tokens)))
+            self.lengths_host[:len(tokens)] = tokens
+            return taken
+
+    def give_back(self, places: int, pages) -> None:
+        """The places 0 .. places - 1 are empty again, and the pages free."""
+        with self._lock:
+            self.free.extend(pages)
+            self.held.difference_update(range(places))
+            self.lengths_host[:places] = 0
 
     def release(self, seq: int) -> None:
         """Gives the pages of a sequence back."""
@@ -261,8 +297,8 @@ class PagedDecoder:
         settings are those of :func:`relax_b200.ops.sample_tokens`, numbers or tensors of one for each sequence; ``uniform`` (fp32 [new_tokens,
         sequences]) gives the random numbers, else they come from `seed`.
 
-        Uses places 0 .. of the cache, which have to be empty, and leaves them so: the tables of the call are its own, on the device.  A call that
-        finds no room for all of it raises before it begins."""
+        Uses places 0 .. of the cache, which have to be empty, and leaves them so: the tables of the call are its own, on the device, over pages that
+        nobody else gets while it runs.  A call that finds no room for all of it raises before it begins."""
         n, cache = len(prompts), self.cache
         counts = [len(t) for t in prompts]
         ids = [operator.index(t) for ts in prompts for t in ts]
@@ -270,60 +306,61 @@ class PagedDecoder:
             raise ValueError("every prompt has one token at least")
         if not 0 <= min(ids) <= max(ids) < self.embed.shape[0]:
             raise ValueError(f"tokens are 0 to {self.embed.shape[0] - 1}, got {min(ids)} to {max(ids)}")
-        if any(cache.length(s) for s in range(n)):
-            raise ValueError("the first places of the cache are in use")
-        if new_tokens == 0:
-            return [[] for _ in prompts], [[] for _ in prompts]
-        longest = max(counts) + new_tokens - 1   # (the last token drawn has no keys)
-        pages = sum(-(-(c + new_tokens - 1) // cache.page_size) for c in counts)
-        if longest > cache.max_tokens:
-            raise ValueError(f"a sequence of {longest} tokens: at most {cache.max_tokens}")
-        if pages > len(cache.free):
-            raise MemoryError(f"{pages} pages wanted, {len(cache.free)} free")
-        with torch.cuda.device(self.device):
-            i32 = dict(dtype=torch.int32, device=self.device)
-            if uniform is None:
-                uniform = torch.rand((new_tokens, n), device=self.device, generator=torch.Generator(device=self.device).manual_seed(seed))
-            elif uniform.shape != (new_tokens, n) or uniform.dtype is not torch.float32 or uniform.device != self.embed.device or not uniform.is_contiguous():
-                raise ValueError(f"uniform is a contiguous fp32 tensor {(new_tokens, n)} on {self.embed.device}")
-            how = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
-            table = torch.full((n, -(-longest // cache.page_size)), -1, **i32)
-            free, free_count = torch.tensor(cache.free, **i32), torch.tensor([len(cache.free)], **i32)
-            lengths, ones = torch.zeros(n, **i32), torch.ones(n, **i32)
-            tokens, logprobs = torch.empty((new_tokens, n), **i32), torch.empty((new_tokens, n), dtype=torch.float32, device=self.device)
+        most = [c + new_tokens - 1 if new_tokens else 0 for c in counts]     # (the last token drawn has no keys)
+        pages = cache.hold(most)
+        try:
+            if new_tokens == 0:
+                return [[] for _ in prompts], [[] for _ in prompts]
+            with torch.cuda.device(self.device):
+                if uniform is None:
+                    uniform = torch.rand((new_tokens, n), device=self.device, generator=torch.Generator(device=self.device).manual_seed(seed))
+                elif uniform.shape != (new_tokens, n) or uniform.dtype is not torch.float32 or uniform.device != self.embed.device or not uniform.is_contiguous():
+                    raise ValueError(f"uniform is a contiguous fp32 tensor {(new_tokens, n)} on {self.embed.device}")
+                return self._sample(counts, ids, max(most), pages, uniform, dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p))
+        finally:
+            cache.give_back(n, pages)
 
-            def plan(counts, rows):
-                out = ops.paged_plan_buffers(n, rows, self.device)._replace(lengths=lengths, free_count=free_count)
-                return ops.paged_plan(table, lengths, counts, free, free_count, cache.page_size, rows, cache.max_tokens, out=out)
+    def _sample(self, counts, ids, longest: int, pages, uniform, how):
+        cache = self.cache
+        new_tokens, n = uniform.shape
+        i32 = dict(dtype=torch.int32, device=self.device)
+        table = torch.full((n, -(-longest // cache.page_size)), -1, **i32)
+        free, free_count = torch.tensor(pages, **i32), torch.tensor([len(pages)], **i32)
+        lengths, ones = torch.zeros(n, **i32), torch.ones(n, **i32)
+        tokens, logprobs = torch.empty((new_tokens, n), **i32), torch.empty((new_tokens, n), dtype=torch.float32, device=self.device)
 
-            # the prompts
-            p = plan(torch.tensor(counts, **i32), sum(counts))
-            h = self._rows(torch.tensor(ids, **i32), table, lengths, p.starts if max(counts) > 1 else None, max(counts))
-            drawn = ops.sample_tokens(self._head(h[p.starts[1:].long() - 1]), uniform[0], **how)
-            tokens[0], logprobs[0] = drawn.token, drawn.logprob
-            # the tokens behind them: what a step reads and writes lies where the graph expects it
-            token, u, scratch = drawn.token, torch.empty(n, dtype=torch.float32, device=self.device), ops.paged_attention_scratch(self.device)
+        def plan(counts, rows):
+            out = ops.paged_plan_buffers(n, rows, self.device)._replace(lengths=lengths, free_count=free_count)
+            return ops.paged_plan(table, lengths, counts, free, free_count, cache.page_size, rows, cache.max_tokens, out=out)
 
-            def step():
-                plan(ones, n)
-                drawn = ops.sample_tokens(self._head(self._rows(token, table, lengths, None, 1, scratch)), u, **how)
-                token.copy_(drawn.token)
-                return drawn.logprob
+        # the prompts
+        p = plan(torch.tensor(counts, **i32), sum(counts))
+        h = self._rows(torch.tensor(ids, **i32), table, lengths, p.starts if max(counts) > 1 else None, max(counts))
+        drawn = ops.sample_tokens(self._head(h[p.starts[1:].long() - 1]), uniform[0], **how)
+        tokens[0], logprobs[0] = drawn.token, drawn.logprob
+        # the tokens behind them: what a step reads and writes lies where the graph expects it
+        token, u, scratch = drawn.token, torch.empty(n, dtype=torch.float32, device=self.device), ops.paged_attention_scratch(self.device)
 
-            graph = None
-            for i in range(1, new_tokens):
-                u.copy_(uniform[i])
-                if graph is None and 2 <= i < new_tokens - 1:            # (the first step prepares what a capture may not)
-                    graph = torch.cuda.CUDAGraph()
-                    with torch.cuda.graph(graph):
-                        held = step()
-                if graph is None:
-                    logprobs[i] = step()
-                else:
-                    graph.replay()
-                    logprobs[i] = held
-                tokens[i] = token
-            return tokens.t().tolist(), logprobs.t().tolist()
+        def step():
+            plan(ones, n)
+            drawn = ops.sample_tokens(self._head(self._rows(token, table, lengths, None, 1, scratch)), u, **how)
+            token.copy_(drawn.token)
+            return drawn.logprob
+
+        graph = None
+        for i in range(1, new_tokens):
+            u.copy_(uniform[i])
+            if graph is None and 2 <= i < new_tokens - 1:            # (the first step prepares what a capture may not)
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph, capture_error_mode="thread_local"):     # (other threads may go on with their calls)
+                    held = step()
+            if graph is None:
+                logprobs[i] = step()
+            else:
+                graph.replay()
+                logprobs[i] = held
+            tokens[i] = token
+        return tokens.t().tolist(), logprobs.t().tolist()
 
     def score(self, seq: int, tokens):
         """Log probability of every token of a text but its first, given those before it (sequence place `seq`, which has to be empty)."""
