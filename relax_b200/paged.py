@@ -298,7 +298,8 @@ class PagedDecoder:
         sequences]) gives the random numbers, else they come from `seed`.
 
         Uses places 0 .. of the cache, which have to be empty, and leaves them so: the tables of the call are its own, on the device, over pages that
-        nobody else gets while it runs.  A call that finds no room for all of it raises before it begins."""
+        nobody else gets while it runs.  A call that finds no room for all of it raises before it begins; one in which a row of logits holds a NaN or
+        an infinity, so that nothing can be drawn, raises at its end."""
         n, cache = len(prompts), self.cache
         counts = [len(t) for t in prompts]
         ids = [operator.index(t) for ts in prompts for t in ts]
@@ -360,7 +361,11 @@ class PagedDecoder:
                 graph.replay()
                 logprobs[i] = held
             tokens[i] = token
-        return tokens.t().tolist(), logprobs.t().tolist()
+        tokens = tokens.t().tolist()
+        for s, of in enumerate(tokens):              # (the steps behind it went on from a token that nobody drew)
+            if -1 in of:
+                raise ValueError(f"nothing to draw for sequence {s} at its token {of.index(-1)}: its logits hold a NaN or an infinity, or exclude everything")
+        return tokens, logprobs.t().tolist()
 
     def score(self, seq: int, tokens):
         """Log probability of every token of a text but its first, given those before it (sequence place `seq`, which has to be empty)."""

@@ -60,3 +60,25 @@ def test_a_thread_beside_a_sample(cuda_lib):
     other.join()
     torch.cuda.synchronize()
     assert not errors and all(d == want for d in drawn) and all(torch.equal(g, alone) for g in got) and len(got) == 20
+
+
+@pytest.mark.parametrize("temperature", (0.0, 0.8))
+@pytest.mark.parametrize("new_tokens", (1, 2, 6))
+@pytest.mark.parametrize("bits", (8, 16))
+def test_logits_that_are_no_numbers(cuda_lib, bits, new_tokens, temperature):
+    """A token whose embedding is broken: its sequence has no token to go on with, which is said, and the cache is as before."""
+    m = model(cache_bits=bits)
+    m.embed, m.lm_head = m.embed.clone(), m.lm_head.roll(11, 0)      # (one that is whole, and says neither a prompt's last token again nor 9 behind it)
+    whole, m.embed[9] = m.embed[9].clone(), float("nan")
+    with pytest.raises(ValueError, match="sequence 1 at its token 0"):
+        m.sample([[1, 2], [3, 9, 4]], new_tokens, temperature=temperature)
+    assert len(m.cache.free) == m.cache.pages and not m.cache.lengths_host.any()
+    m.embed[9] = whole
+    m.sample([[1, 2], [3, 9, 4]], new_tokens, temperature=temperature)
+    first = m.sample([[1, 2]], 1, temperature=0.0)[0][0][0]
+    assert first not in (1, 2)
+    m.embed[first] = float("inf")                # from the second token on
+    if new_tokens > 1:
+        with pytest.raises(ValueError, match="sequence 0 at its token 1"):
+            m.sample([[1, 2]], new_tokens, temperature=0.0)
+    assert m.sample([[1, 2]], 1, temperature=0.0)[0] == [[first]]
