@@ -131,7 +131,8 @@ class PagedCache:
             self.lengths_host[seq] += tokens
 
     def shrink(self, seq: int, tokens: int) -> None:
-        """Forgets the last `tokens` of a sequence and gives back the pages that only they were in."""
+        """Forgets the last `tokens` of a sequence and gives back the pages that only they were in.  In 8 bits a block of 16 of which some are left keeps
+        the scale that the forgotten ones may have raised, and the rounding of its codes to it: 2^-10 of that scale at most."""
         with self._lock:
             have = self._not_held(seq)
             keep = have - tokens
@@ -215,7 +216,8 @@ class PagedDecoder:
 
     def forward(self, seqs, tokens, every: bool = False) -> torch.Tensor:
         """Takes `tokens[i]` (a list) as the next tokens of sequence `seqs[i]`: their keys and values go to the cache; the logits of the last
-        of each, or with `every` of all of them, come back, fp16 [rows, vocab].  A call that raises leaves the sequences as they were."""
+        of each, or with `every` of all of them, come back, fp16 [rows, vocab].  A call that raises leaves the sequences as they were: their lengths and
+        pages, and in 16 bits their keys and values.  In 8 bits it is as if the new tokens had come and been forgotten (:meth:`PagedCache.shrink`)."""
         counts = [len(t) for t in tokens]
         if len(seqs) != len(tokens) or len(set(seqs)) != len(seqs) or min(counts, default=0) < 1:
             raise ValueError("every sequence once, with one token at least")
