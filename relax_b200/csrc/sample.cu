@@ -369,7 +369,8 @@ sample_tokens_kernel(const SampleParams p) {
   u64 border = (u64)key_of(low) << 32;          // the smallest entry that stays
   const u64 all_of_weight = border;
   if (want_min > 0.f) {                         // w >= min_p: a value, rounded up to the next fp32 number
-    const double least = want_min < 1.f ? top + t_eff * log((double)want_min) : top;
+    // (an infinite temperature makes all weights 1)
+    const double least = temperature == INFINITY ? -INFINITY : want_min < 1.f ? top + t_eff * log((double)want_min) : top;
     border = max(border, (u64)key_of(__double2float_ru(least)) << 32);
   }
   int listed = 0, own_turn = 0;

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from relax_b200 import ops
-from test_sample_gpu import check
+from test_sample_gpu import check, logits_of
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +44,11 @@ def test_a_draw_among_ties(cuda_lib, V, temperature):
         got = ops.sample_tokens(x, u, temperature=temperature, **how).token.cpu()
         want = torch.tensor([math.floor(float(v) * kept) for v in u.tolist()])
         assert torch.equal(got.long(), want)
+
+
+@pytest.mark.parametrize("min_p", (0.3, 1.0, 7.0))
+@pytest.mark.parametrize("V", (50, 6001))
+def test_an_infinite_temperature_makes_all_weights_the_largest(cuda_lib, V, min_p):
+    x, u = logits_of(3, V, "fp32", seed=V)
+    for how in (dict(), dict(top_k=20), dict(top_p=0.5)):
+        check(x, u, temperature=math.inf, min_p=min_p, **how)
