@@ -519,13 +519,14 @@ B200_API int b200_paged_attention(const B200PagedCache* cache, const B200PagedAt
 /* ---- the same over pages of 8 bits ---------------------------------------------------------------
  * Pages hold e4m3 codes (strides in codes, multiples of 16), scales fp16 [pages, kv_heads, page_size / 16], one for 16 tokens of a head, all of it contiguous:
  * a value is code * scale.  The descriptor's dtype is that of the rows (q, qkv, results).  A scale of any block that a row sees is
- * positive and at most 2^7 (a value is a number of fp16); what no token has reached, codes and scales, may be anything.
+ * positive and at most 2^7 (so that no value is too large for fp16); what no token has reached, codes and scales, may be anything.
  *
  * b200_paged8_rope_append: as b200_paged_rope_append, k and v rounded to the rows' type as there, then stored by their block's scale:
  *   need = the smallest power of two by which the block's new tokens are at most 448 in size, from 2^-24 to 2^7
  *   scale = need where no earlier token is in the block, else the larger one of need and what it was; then the earlier tokens' codes are
  *   scaled anew.  Codes are rounded to nearest even; what is more than 448 * 2^7 in size becomes that, what is no finite number NaN.
- * b200_paged8_attention: as b200_paged_attention; q is taken in fp16 (of bf16 rows: up to 65504 in size), weights are rounded to fp16.
+ * b200_paged8_attention: as b200_paged_attention; q is taken in fp16 (of bf16 rows: up to 65504 in size), weights are rounded to fp16, and values are
+ *   what they are for scales that are powers of two (of others calls of many rows round code * scale to 11 bits).
  * Scratch memory as there; calls of both may share it where they are ordered. */
 typedef struct {
   void* k_scales;

@@ -46,7 +46,6 @@ __device__ __forceinline__ int power_for(float most) {
   const int e = (int)(u >> 23) - 127, power = e - 8 + ((u & 0x7fffffu) > 0x600000u);
   return most > 0.f ? min(max(power, kMinPower), kMaxPower) : kMinPower;
 }
-__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((127 + e) << 23); }
 // Two values' codes, to nearest even, at most 448 in size; NaN for what is no number.
 __device__ __forceinline__ uint32_t codes2(float lo, float hi) {
   uint16_t r;

@@ -31,8 +31,9 @@
 // halves of N = 64 with a buffer each 523 (412 instead of 342 without the softmax).
 // Pages of 8 bits (kBytes; a translation unit of its own, paged_attn_prompt8.cu): TMA brings the codes of a block into a ring of their own, and
 // four more warps (12..15) make fp16 tiles of them, code times the scale of its 16 tokens, in the ring from which the products are made as always.
+// Of scales below 2^-15 that product is no number of fp16: the tile holds more, by a power of two for 16 tokens, and their scores or weights less.
 // That is 64 KB more through shared memory for a block, beside products that read 128 bytes a clock of it: 2048 tokens of 32 heads 58 us, 512 on
-// 30000 404 with the cap, 281 without (16 bits 51, 334, 223 in the same row of calls).  With one warp for the tiles 75 and 573: 512 conversions a
+// 30000 419 with the cap, 281 without (16 bits 51, 334, 223 in the same row of calls).  With one warp for the tiles 75 and 573: 512 conversions a
 // block and lane, one after the other.
 #include <atomic>
 #include <type_traits>
@@ -61,6 +62,7 @@ constexpr int kWorks = 2;                      // work descriptors in flight
 constexpr int kKept = 64;                      // sequences whose sizes the scheduling warp keeps
 constexpr uint64_t kWaitNs = 4000000000ull;
 constexpr int kRaw = 2;                        // blocks of codes in flight
+constexpr int kLacks = 8;                      // blocks whose small scales are kept: the converting warps are at most five ahead of the rows
 // 128 x 72 + 256 x 216 = 384 x 168; 256 x 40 + 256 x 216 = 512 x 128
 constexpr int kAuxRegs = kBytes ? 40 : 72, kRowRegs = 216, kLaunchRegs = kBytes ? 128 : 168;
 __device__ int g_prompt_error = 0;
@@ -286,6 +288,7 @@ struct Smem {
   unsigned char ring[kStages][kBlockBytes];
   unsigned char raw[kBytes ? kRaw : 1][kBytes ? kBlock * D : 16];
   uint64_t raw_full[kRaw], raw_empty[kRaw], q_ready;
+  uint2 lacks[kBytes ? kLacks : 1];            // 8 bits: of keys and of values, four bits for 16 tokens (see lacking_power)
   uint64_t q_full, q_empty;
   uint64_t full[kStages], empty[kStages], ready[kReady];
   uint64_t s_full[2], p_ready[2][2], o_full[2], o_empty[2];       // [tile][half of a block]
@@ -411,6 +414,40 @@ __device__ __forceinline__ uint32_t to_half2(__half, uint32_t v) { return v; }
 __device__ __forceinline__ uint32_t to_half2(__nv_bfloat16, uint32_t v) {
   const float2 f = unpack2(__nv_bfloat16(), v);
   return pack2(__half(), f.x, f.y);
+}
+
+// 8 bits: the power of two by which a scale below 2^-15 (0 otherwise; 9 at most) is made 2^-15 to 2^-14, so that code times scale is a number of
+// fp16 for all codes.  Scores of its keys are made smaller by it, and so are the weights of its values.
+__device__ __forceinline__ int lacking_power(uint32_t half_bits) { return half_bits - 1u < 0x1ffu ? __clz(half_bits) - 22 : 0; }
+
+// A row's 128 scores, and 64 of its weights in pairs, by those powers; not in line, where they would slow the loop down that hardly ever wants them.
+__device__ __noinline__ void smaller_scores(uint32_t at, uint32_t lacks) {
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i) {
+    uint32_t x[16];
+    tmem_ld_32x32b_x16(at + 16 * i, x);
+    tmem_ld_wait();
+    const float f = power_of_two(-(int)(lacks >> 4 * i & 15u));
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * f);
+    tmem_st_32x32b_x16(at + 16 * i, x);
+  }
+  tmem_st_wait();
+}
+__device__ __noinline__ void smaller_weights(uint32_t at, uint32_t lacks) {
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {
+    uint32_t x[16];
+    tmem_ld_32x32b_x16(at + 16 * i, x);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const __half2 f = __float2half2_rn(power_of_two(-(int)(lacks >> (8 * i + 4 * (j / 8)) & 15u)));
+      const __half2 w = __hmul2(*reinterpret_cast<const __half2*>(&x[j]), f);
+      x[j] = *reinterpret_cast<const uint32_t*>(&w);
+    }
+    tmem_st_32x32b_x16(at + 16 * i, x);
+  }
 }
 
 template <typename T, int D, int kForm, bool kWide>
@@ -693,9 +730,20 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
           const int in_page = (token & ((1 << a.c.page_log2) - 1)) >> 4;
           return __ldg((lane < 8 ? a.k_scales : a.v_scales) + ((id * a.c.kv_heads + w.h) << (a.c.page_log2 - 4)) + in_page);
         };
-        __half scale = scale_at(w.u0);
+        __half next = scale_at(w.u0);
         for (int u = w.u0; ok && u < u1; ++u) {
-          const __half next = u + 1 < u1 ? scale_at(u + 1) : scale;
+          const uint32_t stored = __half_as_ushort(next);
+          const int lacks = lacking_power(stored);
+          const __half scale = __ushort_as_half((unsigned short)(stored << lacks));        // (of subnormal numbers the bits are the value)
+          if (turner == 0) {                                   // (seen by the rows behind the scores, which wait for these keys)
+            uint2 all = {0u, 0u};
+            if (__builtin_expect(__any_sync(0xffffffffu, lacks), 0)) {
+              const uint32_t bits = (uint32_t)lacks << 4 * (lane & 7);
+              all = {__reduce_or_sync(0xffffffffu, lane < 8 ? bits : 0u), __reduce_or_sync(0xffffffffu, lane >= 8 ? bits : 0u)};
+            }
+            if (lane == 0) sm.lacks[vblocks % kLacks] = all;
+          }
+          if (u + 1 < u1) next = scale_at(u + 1);
           const int from = range.unit(u) * kBlock;
           const bool whole = from + kBlock <= range.pre || (from >= range.low && from + kBlock <= range.high);
 #pragma unroll 1
@@ -756,7 +804,6 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
             }
           }
           ++vblocks;
-          scale = next;
         }
       }
     }
@@ -766,6 +813,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
     const int t = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t s_at = tmem + t * 128 + ((uint32_t)((warp & 3) * 32) << 16), o_at = s_at - t * 128 + 256 + t * D;
     uint32_t phases = 0;                         // parities: bit 0 of s_full, 1 of o_full, 2 of joined
+    uint32_t blocks = 0;                         // 8 bits: of earlier items
     bool ok = true;
     // The four warps of the tile meet; false: one of them has given up (a barrier without a limit would wait for it for ever).
     auto tile_barrier = [&]() {
@@ -797,6 +845,8 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         if (!wait(&sm.s_full[t], phases & 1, abort_flag, 12)) { ok = false; break; }
         phases ^= 1;
         tc_fence_after_sync();
+        uint2 lacks = {0u, 0u};
+        if constexpr (kBytes) lacks = sm.lacks[(blocks + (u - u0)) % kLacks];
         // First pass: the maximum, 32 columns at a time, the next ones on their way; scores that a mask changes, or a cap or a bias where
         // its short form does not hold, go back to tensor memory.  Second pass: the weights.  (What does not fit in registers comes from
         // L2 with this much shared memory, and so do the instructions of long code.)
@@ -813,9 +863,16 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         auto all_tops = [&]() { return max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]); };
         const float bias = kForm == kSloped ? -slope * (float)(at - from) : 0.f;       // of the block's first key, which lies before the row
         bool direct = whole && kForm != kGeneral && (kForm != kSloped || from + kBlock - 1 <= tile_first);
+        if (direct) tmem_ld_32x32b_x32(s_at, raw[0]);
+        if constexpr (kBytes) {
+          if (__builtin_expect(lacks.x != 0, 0)) {       // keys whose tile holds more
+            if (direct) tmem_ld_wait();
+            smaller_scores(s_at, lacks.x);
+            if (direct) tmem_ld_32x32b_x32(s_at, raw[0]);
+          }
+        }
         if (direct) {
           float lows[2] = {INFINITY, INFINITY};
-          tmem_ld_32x32b_x32(s_at, raw[0]);
 #pragma unroll 1
           for (int i = 0; i < 4; i += 2) {
 #pragma unroll
@@ -955,6 +1012,12 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
               }
               tmem_st_32x32b_x16(s_at + 16 * (i + h), packed);
             }
+            if constexpr (kBytes) {
+              if (__builtin_expect(lacks.y != 0, 0)) {   // weights of values whose tile holds more
+                tmem_st_wait();
+                smaller_weights(s_at + 16 * i, lacks.y >> 8 * i);
+              }
+            }
             tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
@@ -965,6 +1028,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         else weights(std::true_type());
       }
       if (!ok) break;
+      blocks += u1 - u0;
       // ---- the tile's result -------------------------------------------------------------------------------------------------
       const float sum = m == -INFINITY ? 0.f : (l[0] + l[1]) + (l[2] + l[3]);   // (a row that saw nothing: 2^-126 of every key)
       const bool any = w.last[t] >= 0;

@@ -155,6 +155,7 @@ struct PromptWords {
 };
 static_assert(kFewCounters * 4 + kCutTiles * 8 + sizeof(PromptWords) <= B200_PAGED_ZEROED_BYTES, "the counters");
 
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((127 + e) << 23); }
 // Four e4m3 codes (the low ones first) as fp16 values, which hold them exactly.
 __device__ __forceinline__ void e4m3_to_half4(uint32_t codes, uint32_t& lo, uint32_t& hi) {
   asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}" : "=r"(lo), "=r"(hi) : "r"(codes));
