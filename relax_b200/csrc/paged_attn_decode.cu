@@ -728,7 +728,8 @@ using namespace b200;
 extern "C" {
 
 // The counters, the maxima and sums of parts, their partial results.  The few-rows kernel has two parts a CTA at most (a tile that began before
-// its share, one that ends behind it) of 8 rows (three CTAs an SM) or 16 (two): 64 rows an SM.  The many-rows kernel has kPartsOfSlots of 256.
+// its share, one that ends behind it) of 8 rows (three CTAs an SM, four over 8 bits) or 16 (two): up to 64 rows an SM.  The many-rows kernel has
+// kPartsOfSlots of 256.
 static_assert(2 * std::max(kCtasPerSm1, kCtas8PerSm1) * 8 <= kPartsOfSlots * 256 && 2 * std::max(kCtasPerSm2, kCtas8PerSm2) * 16 <= kPartsOfSlots * 256,
               "partial results of the few-rows kernel");
 static int64_t scratch_rows() { return (int64_t)kPartsOfSlots * sm_count() * 256; }

@@ -36,7 +36,7 @@ struct PlanParams {
   long long* slots;
   int* free_count_out;
   int* status;
-  int batch, width, pool, page_log2, rows, cluster;
+  int batch, pool, page_log2, rows, cluster;
   int max_tokens;
 };
 
@@ -209,7 +209,6 @@ extern "C" int b200_paged_plan(const B200PagedPlan* a, void* stream) {
   p.free_count_out = static_cast<int*>(a->free_count_out);
   p.status = static_cast<int*>(a->status);
   p.batch = a->batch;
-  p.width = a->table_width;
   p.pool = (int)a->pages;
   p.page_log2 = a->page_size == 16 ? 4 : a->page_size == 32 ? 5 : a->page_size == 64 ? 6 : 7;
   p.rows = (int)a->rows;

@@ -17,8 +17,10 @@
 //   3  top_k: a list of the k largest and a few more, bounded by the threads' maxima (without pass 2) or by the bins, in order; all the rest
 //      happens on it.  Where k is more than a list holds, the bin with the border is known and its entries are put in order.
 //      top_p: the counts times the bins' weights tell the bin but for an error in the fourth digit; the exact sum in front of it, and its entries
-//      in order, find the border or say on which side it lies.  Where a bin holds more entries than the list (nearly equal logits) the border is
-//      found by bisection of the keys, 64 passes.
+//      in order, find the border or say on which side it lies.  Where the bin, with the neighbour that may have the border instead, holds more
+//      entries than the list, the border is found by bisection of the keys, 64 passes.  That is so for equal logits, and for some rows that
+//      are long and flat: of normal logits of size 2.5 over 152000 entries none at T = 1, one in five or more from T = 2 on (top_p 0.9); one in eight
+//      of size 1 at T = 1.  Such a row takes 0.5 ms alone, not 30 us, and 64 rows with some of them 1.2 ms, not 58 us.
 //   4  the sum of what stays, a segment a warp (top_p's pass has it); then the segment in which the random number falls, a vector a thread
 // A row is a CTA of 512 threads, or of 256 with four on an SM where there are many rows, or a cluster of CTAs that tell each other their sums.
 //
@@ -531,11 +533,11 @@ sample_tokens_kernel(const SampleParams p) {
     return gather_from(x.up(bucket >= kBuckets - 1 || !(per > 0.f) ? low : fmaxf(m - ((float)bucket + 1.01f) / per, low)),
                        [&](float v, int) { return v >= low; });
   };
-  // Sums up to every thread's two entries, in order; the sum of all.
-  auto scan = [&](const double (&w)[kList / kThreads], double& before) {
+  // Sums up to every thread's kEach entries, in order; the sum of all.
+  auto scan = [&](const double (&w)[kEach], double& before) {
     double own = 0., all = 0.;
 #pragma unroll
-    for (int i = 0; i < kList / kThreads; ++i) own += w[i];
+    for (int i = 0; i < kEach; ++i) own += w[i];
     double upto = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -1091,8 +1093,11 @@ extern "C" int b200_sample_tokens(const void* logits, int32_t dtype, int64_t str
   SampleParams p = {logits, static_cast<const float*>(uniform), static_cast<int*>(token), static_cast<float*>(logprob),
                     static_cast<const float*>(how->temperatures), static_cast<const int*>(how->top_ks), static_cast<const float*>(how->top_ps),
                     static_cast<const float*>(how->min_ps), stride, rows, (int)V, how->temperature, how->top_p, how->min_p, how->top_k};
-  // CTAs of a row: a cluster meets three to seven times, 2000 clocks each.  us for one row of 32000 with 1, 2, 4, 8 CTAs: no filter 11.0, 10.2, 8.7,
-  // 8.1; top_k 50 11.3, 12.1, 11.9, 12.4; top_p 0.9 24.2, 22.4, 19.8, 19.5.  64 such rows, top_p 0.9: 24.9, 22.7, 25.4.
+  // CTAs of a row: a cluster meets three to seven times, 2000 clocks each.  us for one row of 32000 with 1, 2, 4, 8 CTAs: no filter 13.3, 10.9, 8.2,
+  // 7.3; top_k 50 13.6, 12.6, 11.4, 12.3; top_p 0.9 27.7, 23.0, 18.9, 18.6.  64 such rows, top_p 0.9: 28.1, 23.5, 26.5, 48.5.  So each CTA gets 8000 entries
+  // at least, and the launch no more CTAs than there are SMs.  With longer rows the passes count for more than the meetings, and two CTAs share an SM:
+  // 64 rows of 128000 with 1, 2, 4 CTAs (the rule takes 4): no filter 45.9, 26.7, 23.2; top_k 50 27.4, 20.2, 22.4; top_p 0.9 81, 50, 50;
+  // 100 of them with 1, 2, 4 (the rule takes 2): 46, 40, 36; 27, 30, 35; 81, 79, 74.
   int c = 1;
   while (V / (2 * c) >= 8000 && c < kMaxCluster && rows * c * 2 <= sm_count() * (V >= 65536 ? 2 : 1)) c *= 2;
   const bool many = c == 1 && rows > 2 * sm_count();
