@@ -84,6 +84,9 @@ def rope_tables(positions: int, rotary: int, theta: float = 10000.0, scaling: di
     return tuple(torch.from_numpy((f(angle) * magnitude).astype(np.float32)).to(device).contiguous() for f in (np.cos, np.sin))
 
 
+_pool = threading.RLock()              # one call at a time takes pages of a cache or gives them back (no cache's own: caches are copied and pickled)
+
+
 class PagedCache:
     """Pages of all layers and the tables of the sequences in them: ``batch`` places for sequences, each up to ``max_tokens`` long, over
     ``pages`` pages that they share."""
@@ -103,7 +106,6 @@ class PagedCache:
         self.lengths_host = np.zeros(batch, np.int32)
         self.free = list(range(pages - 1, -1, -1))
         self.held = set()                       # places of calls that keep their tables on the device
-        self._lock = threading.RLock()          # one call at a time takes pages or gives them back
 
     def length(self, seq: int) -> int:
         """Tokens of a sequence.  (A negative number names no place: it would be another name for one of the last.)"""
@@ -119,7 +121,7 @@ class PagedCache:
 
     def extend(self, seq: int, tokens: int) -> None:
         """Room for `tokens` more of sequence `seq`; raises, and changes nothing, where the table or the pool has none."""
-        with self._lock:
+        with _pool:
             length = self._not_held(seq)
             have, want = -(-length // self.page_size), -(-(length + tokens) // self.page_size)
             if tokens < 0 or length + tokens > self.max_tokens:
@@ -133,7 +135,7 @@ class PagedCache:
     def shrink(self, seq: int, tokens: int) -> None:
         """Forgets the last `tokens` of a sequence and gives back the pages that only they were in.  In 8 bits a block of 16 of which some are left keeps
         the scale that the forgotten ones may have raised, and the rounding of its codes to it: 2^-10 of that scale at most."""
-        with self._lock:
+        with _pool:
             have = self._not_held(seq)
             keep = have - tokens
             if not 0 <= keep <= have:
@@ -147,7 +149,7 @@ class PagedCache:
         """Takes the places 0 .. , which have to be empty, for sequences of up to ``tokens[i]`` each, and pages for all of them, which it returns: for a
         call whose tables are its own.  Nobody else gets the places or the pages before :meth:`give_back`.  Raises, and changes nothing, where
         there is no room."""
-        with self._lock:
+        with _pool:
             if any([self.length(s) for s in range(len(tokens))]) or not self.held.isdisjoint(range(len(tokens))):
                 raise ValueError("the first places of the cache are in use")
             if max(tokens) > self.max_tokens:
@@ -163,7 +165,7 @@ class PagedCache:
 
     def give_back(self, places: int, pages) -> None:
         """The places 0 .. places - 1 are empty again, and the pages free."""
-        with self._lock:
+        with _pool:
             self.free.extend(pages)
             self.held.difference_update(range(places))
             self.lengths_host[:places] = 0

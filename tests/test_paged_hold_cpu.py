@@ -1,4 +1,6 @@
 """Places and pages of a call that keeps its tables on the device: nobody else gets them before it returns."""
+import copy
+import pickle
 import threading
 
 import pytest
@@ -93,3 +95,14 @@ def test_threads_share_the_pool():
     for t in threads:
         t.join()
     assert not wrong and sorted(c.free) == list(range(64)) and not c.lengths_host.any()
+
+
+@pytest.mark.parametrize("again", (copy.deepcopy, lambda c: pickle.loads(pickle.dumps(c))))
+def test_a_cache_is_copied_with_what_it_holds(again):
+    c = cache()
+    c.extend(3, 30)
+    pages = c.hold([17])
+    other = again(c)
+    assert other.free == c.free and other.held == {0} and (other.table_host == c.table_host).all()
+    other.give_back(1, pages)
+    assert c.held == {0} and c.length(0) == 17 and other.length(0) == 0 and len(other.free) == len(c.free) + 2
