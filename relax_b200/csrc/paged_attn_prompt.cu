@@ -33,7 +33,7 @@
 // four more warps (12..15) make fp16 tiles of them, code times the scale of its 16 tokens, in the ring from which the products are made as always.
 // Of scales below 2^-15 that product is no number of fp16: the tile holds more, by a power of two for 16 tokens, and their scores or weights less.
 // That is 64 KB more through shared memory for a block, beside products that read 128 bytes a clock of it: 2048 tokens of 32 heads 58 us, 512 on
-// 30000 416 with the cap, 281 without (16 bits 51, 334, 223 in the same row of calls).  With one warp for the tiles 75 and 573: 512 conversions a
+// 30000 416 with the cap, 292 without (16 bits 51, 334, 223 in the same row of calls).  With one warp for the tiles 75 and 573: 512 conversions a
 // block and lane, one after the other.
 #include <atomic>
 #include <type_traits>
