@@ -410,18 +410,18 @@ constexpr int kPlain = 0, kCapped = 1, kSloped = 2, kGeneral = 3;     // (and kW
 constexpr int kPolyOfEight = 2;
 
 // Pairs of 16-bit values to fp16; a bf16 value beyond fp16's range becomes an infinity.
-__device__ __forceinline__ uint32_t to_half2(__half, uint32_t v) { return v; }
-__device__ __forceinline__ uint32_t to_half2(__nv_bfloat16, uint32_t v) {
+[[maybe_unused]] __device__ __forceinline__ uint32_t to_half2(__half, uint32_t v) { return v; }
+[[maybe_unused]] __device__ __forceinline__ uint32_t to_half2(__nv_bfloat16, uint32_t v) {
   const float2 f = unpack2(__nv_bfloat16(), v);
   return pack2(__half(), f.x, f.y);
 }
 
 // 8 bits: the power of two by which a scale below 2^-15 (0 otherwise; 9 at most) is made 2^-15 to 2^-14, so that code times scale is a number of
 // fp16 for all codes.  Scores of its keys are made smaller by it, and so are the weights of its values.
-__device__ __forceinline__ int lacking_power(uint32_t half_bits) { return half_bits - 1u < 0x1ffu ? __clz(half_bits) - 22 : 0; }
+[[maybe_unused]] __device__ __forceinline__ int lacking_power(uint32_t half_bits) { return half_bits - 1u < 0x1ffu ? __clz(half_bits) - 22 : 0; }
 
 // A row's 128 scores, and 64 of its weights in pairs, by those powers; not in line, where they would slow the loop down that hardly ever wants them.
-__device__ __noinline__ void smaller_scores(uint32_t at, uint32_t lacks) {
+[[maybe_unused]] __device__ __noinline__ void smaller_scores(uint32_t at, uint32_t lacks) {
 #pragma unroll 1
   for (int i = 0; i < 8; ++i) {
     uint32_t x[16];
@@ -434,7 +434,7 @@ __device__ __noinline__ void smaller_scores(uint32_t at, uint32_t lacks) {
   }
   tmem_st_wait();
 }
-__device__ __noinline__ void smaller_weights(uint32_t at, uint32_t lacks) {
+[[maybe_unused]] __device__ __noinline__ void smaller_weights(uint32_t at, uint32_t lacks) {
 #pragma unroll 1
   for (int i = 0; i < 2; ++i) {
     uint32_t x[16];

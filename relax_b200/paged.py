@@ -152,7 +152,7 @@ class PagedCache:
         with _pool:
             if any([self.length(s) for s in range(len(tokens))]) or not self.held.isdisjoint(range(len(tokens))):
                 raise ValueError("the first places of the cache are in use")
-            if max(tokens) > self.max_tokens:
+            if max(tokens, default=0) > self.max_tokens:
                 raise ValueError(f"a sequence of {max(tokens)} tokens: at most {self.max_tokens}")
             pages = sum(-(-n // self.page_size) for n in tokens)
             if pages > len(self.free):
